@@ -232,6 +232,85 @@ int vbs_gfx950_linear_batch_multi(int type, uint32_t n_mat, const void *const *w
                                   float *const *y, const uint32_t *y_stride, uint32_t cols,
                                   uint32_t batch);
 
+/* ---- steps of several tokens over the cache (extension) --------------------
+ * The reference's loop takes one token at a time (src/vbs_specializer.c:353-357):
+ * ROTARY and CACHE one position, ATTENTION one query. These operators take n
+ * tokens over the same f16 caches ([layer][max_ctx][n_kv_heads * head_dim]): the
+ * chunk of a prompt, the drafted tokens of speculative decoding, and single
+ * tokens whose attention the plain op does not have. A token is stored in a
+ * slot of the cache; its position (for the rotation) may be any number. All:
+ * n <= 65535 (0: nothing is done), head_dim even and <= 256, at most 16 q heads
+ * per kv head; a row of q, k, v or out is n_heads x head_dim floats and rows lie
+ * a stride (in floats, at least a row) apart, so that the rows of a fused Q/K/V
+ * product can be given as they are. No call waits for the device. */
+
+/* Rotary positions with several axes (time, height, width): pair p (elements 2p
+ * and 2p + 1, as vbs_gfx950_rope) of every head of token i turns by
+ * pos[axis(p)][i] * theta^(-2p / head_dim), where axis x owns sections[x] pairs,
+ * in order (n_axes <= 4; the sections add up to head_dim / 2; a host array). pos
+ * is a device array [n_axes][n]. q is rotated in place; k is rotated, and k and v
+ * are stored as f16, with vbs_gfx950_cache_store's rounding, in the slots slot ..
+ * slot + n - 1 of `layer` (k itself is left as it was). q may be NULL (k and v
+ * alone), or k, v, kc and vc (q alone). Angles are formed in 64 bits, which far
+ * positions need; vbs_gfx950_rope forms them in f32, as the reference does, and
+ * differs by up to pos * 2^-23 rad: a loop takes one of the two throughout. */
+int vbs_gfx950_rope_axes(float *q, uint32_t q_stride, const float *k, const float *v,
+                         uint32_t kv_stride, const int32_t *pos, uint32_t n, uint32_t n_axes,
+                         const uint32_t *sections, uint16_t *kc, uint16_t *vc, uint32_t slot,
+                         uint32_t layer, uint32_t max_ctx, uint32_t n_q_heads,
+                         uint32_t n_kv_heads, uint32_t head_dim, float theta);
+
+/* Attention of a tree of n drafted tokens, in the slots past .. past + n - 1:
+ * row i sees every slot below past, and slot past + t where bit t % 64 of
+ * mask[i * ceil(n / 64) + t / 64] is set (a device array; a tree sets the bits of
+ * a token's ancestors and its own). out row i, per q head: sum_j w_j v_j with
+ * w = softmax(scale q.k_j) over the slots it sees, in f32 as
+ * vbs_gfx950_attention; a row that sees nothing, or whose scores are all -inf, gives
+ * 0, and what a row does not see does not reach it, infinities and NaN included. out must not overlap q. */
+int vbs_gfx950_attention_tree(const float *q, uint32_t q_stride, const uint16_t *kc,
+                              const uint16_t *vc, float *out, uint32_t out_stride, uint32_t n,
+                              uint32_t past, const uint64_t *mask, uint32_t layer,
+                              uint32_t max_ctx, uint32_t n_q_heads, uint32_t n_kv_heads,
+                              uint32_t head_dim, float scale);
+
+/* What vbs_gfx950_attention_chunk adds to plain causal attention; 0 / NULL
+ * fields are absent. Device arrays. */
+typedef struct vbs_gfx950_attn_terms {
+    float cap;             /* s = cap * tanh(s / cap) */
+    const float *slopes;   /* n_q_heads: then s = s - slopes[h] * |i - j| in slots */
+    const int32_t *docs;   /* past + n: slots of another document than the row's are not seen */
+    uint32_t prefix;       /* slots below it are seen by every row (of their document) */
+    float *mass;           /* [layer][n_kv_heads][max_ctx]: the weights added up, see below */
+} vbs_gfx950_attn_terms_t;
+
+/* Attention of n consecutive tokens in the slots past .. past + n - 1 (n = 1: one
+ * decode step): the row of slot i sees the slots j <= i, and j < prefix, of its
+ * document; s_j = scale q.k_j with the terms above (terms may be NULL), out as
+ * for the tree. With mass, the weight that each slot received is added to
+ * mass[(layer * n_kv_heads + kv head) * max_ctx + slot], summed over the rows
+ * and the q heads of the kv head in a fixed order: what vbs_gfx950_cache_evict
+ * chooses by. */
+int vbs_gfx950_attention_chunk(const float *q, uint32_t q_stride, const uint16_t *kc,
+                               const uint16_t *vc, float *out, uint32_t out_stride, uint32_t n,
+                               uint32_t past, uint32_t layer, uint32_t max_ctx,
+                               uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                               float scale, const vbs_gfx950_attn_terms_t *terms);
+
+/* Cut the first len slots of the layers layer .. layer + n_layers - 1 to budget
+ * slots, per layer and kv head: the first `first` and the last `last` stay, and of
+ * the others those of the greatest mass (the lowest slot among equals, NaN the
+ * least of all). The kept rows of K and V move, in slot order and in place, to
+ * the slots 0 .. budget - 1 of their kv head; the rows behind are left as they
+ * were. kept (device, [n_layers][n_kv_heads][budget]) receives the slots they came
+ * from, and mass_out, if not NULL (it may be mass itself), their mass, and 0 for
+ * the slots budget .. len - 1, so that tokens stored there start from 0. Each
+ * head has its own slots afterwards: distances and documents by slot
+ * (vbs_gfx950_attn_terms_t) then no longer mean the tokens' own. */
+int vbs_gfx950_cache_evict(uint16_t *kc, uint16_t *vc, const float *mass, float *mass_out,
+                           uint32_t *kept, uint32_t len, uint32_t budget, uint32_t first,
+                           uint32_t last, uint32_t layer, uint32_t n_layers, uint32_t max_ctx,
+                           uint32_t n_kv_heads, uint32_t head_dim);
+
 /* XOR checksum of a device region, as partial words, for
  * i < vbs_gfx950_checksum_partials(bytes): the region is cut into consecutive
  * spans of up to 112 KB, one per workgroup of 16 waves, and partials[16 w + v]
@@ -267,7 +346,7 @@ int vbs_gfx950_checksum_variant(const void *p, size_t bytes, uint32_t *partials,
  * largest shape before capturing. Batched Q4_0, Q4_1, Q8_0 and F16 calls take
  * memory of the graph's own while captured, at any size, which is given back
  * with the graph and its executables: such graphs may run beside each other
- * and beside any call. */
+ * and beside any call. So do vbs_gfx950_attention_tree and _chunk. */
 void *vbs_gfx950_stream(void);
 
 /* ---- graph-replayed decode step (extension) -------------------------------

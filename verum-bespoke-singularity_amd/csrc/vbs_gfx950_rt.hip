@@ -18,6 +18,7 @@
 #include "vbs_dev_common.h"
 #include "vbs_gfx950.h"
 #include "vbs_internal.h"
+#include "vbs_steps.h"
 
 // Partial results of vbs_gfx950_attention_noalloc: a fixed device array, so
 // that entry point allocates nothing. Its device address is looked up once,
@@ -760,6 +761,149 @@ int vbs_gfx950_attention_noalloc(const float *q, const uint16_t *kc, const uint1
                                    static_cast<float *>(g_rt.noalloc_scratch), layer_off, nqh,
                                    nkh, hd, scale, g_rt.stream),
                   "attention_noalloc");
+}
+
+// ---- steps of several tokens over the cache -------------------------------------
+// The arguments are checked before the device is looked at. Work is launched on the library's device, whatever device the calling thread has current.
+namespace {
+struct OnDevice {
+    int other = -1;
+    OnDevice() {
+        int cur = -1;
+        if (hipGetDevice(&cur) == hipSuccess && cur != g_rt.device && hipSetDevice(g_rt.device) == hipSuccess) other = cur;
+    }
+    ~OnDevice() {
+        if (other >= 0) (void)hipSetDevice(other);
+    }
+};
+
+// Whether the spans [a, a + na) and [b, b + nb) of bytes overlap.
+bool spans_overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
+    const uint64_t x = (uint64_t)(uintptr_t)a, y = (uint64_t)(uintptr_t)b;
+    return x < y + nb && y < x + na;
+}
+
+constexpr uint32_t kMaxStep = 65535;  // tokens of one call
+
+// The shape that the three operators of a step share; 0 with the reason set.
+int step_shape_ok(const char *who, uint32_t n, uint32_t slot, uint32_t max_ctx, uint32_t nqh, uint32_t nkh, uint32_t hd) {
+    if (nqh == 0 || nkh == 0 || hd == 0) return fail("%s: empty shape", who);
+    if (n > kMaxStep) return fail("%s: at most %u tokens per call", who, kMaxStep);
+    if ((uint64_t)slot + n > max_ctx) return fail("%s: slots %u + %u tokens > max_ctx %u", who, slot, n, max_ctx);
+    if (nqh % nkh) return fail("%s: %u q heads not a multiple of %u kv heads", who, nqh, nkh);
+    if (nqh / nkh > 16) return fail("%s: group size %u exceeds 16", who, nqh / nkh);
+    if (nkh > 65535u) return fail("%s: %u kv heads exceed 65535", who, nkh);
+    if (hd > 256 || (hd & 1u)) return fail("%s: head_dim %u must be even and <= 256", who, hd);
+    return 1;
+}
+
+// The checks and the launch of both attentions; `a` but for what `layer` offsets.
+int attention_rows(const char *who, RowsArgs a, uint32_t layer) {
+    if (!a.q || !a.kc || !a.vc || !a.out) return fail("%s: null pointer", who);
+    if (!step_shape_ok(who, a.n, a.past, a.max_ctx, a.nqh, a.nkh, a.hd)) return 0;
+    const uint64_t row = (uint64_t)a.nqh * a.hd;
+    if (a.q_stride < row || a.out_stride < row) return fail("%s: stride smaller than a row", who);
+    if (a.n == 0) return 1;
+    if (spans_overlap(a.q, 4u * ((uint64_t)(a.n - 1u) * a.q_stride + row), a.out,
+                      4u * ((uint64_t)(a.n - 1u) * a.out_stride + row)))
+        return fail("%s: out overlaps q", who);
+    a.kc += (uint64_t)layer * a.max_ctx * a.nkh * a.hd;
+    a.vc += (uint64_t)layer * a.max_ctx * a.nkh * a.hd;
+    if (a.mass) a.mass += (uint64_t)layer * a.nkh * a.max_ctx;
+    if (!ready_or_fail()) return 0;
+    const OnDevice on;
+    const std::lock_guard<std::mutex> together(g_scratch_mu);
+    void *scratch = nullptr;
+    if (const size_t bytes = rows_scratch_bytes(a)) {
+        hipError_t why = hipSuccess;
+        scratch = rt_scratch_or_captured(bytes, g_rt.stream, &why);
+        if (!scratch) return hip_ok(why, who);
+    }
+    return hip_ok(launch_rows(a, scratch, g_rt.stream), who);
+}
+}  // namespace
+
+int vbs_gfx950_rope_axes(float *q, uint32_t q_stride, const float *k, const float *v, uint32_t kv_stride,
+                         const int32_t *pos, uint32_t n, uint32_t n_axes, const uint32_t *sections,
+                         uint16_t *kc, uint16_t *vc, uint32_t slot, uint32_t layer, uint32_t max_ctx,
+                         uint32_t nqh, uint32_t nkh, uint32_t hd, float theta) {
+    const int stored = (k != nullptr) + (v != nullptr) + (kc != nullptr) + (vc != nullptr);
+    if (!pos || !sections || (stored && stored != 4) || (!q && !stored)) return fail("rope_axes: null pointer");
+    if (!step_shape_ok("rope_axes", n, stored ? slot : 0u, stored ? max_ctx : n, nqh, nkh, hd)) return 0;
+    if (n_axes == 0 || n_axes > kRopeAxes) return fail("rope_axes: %u axes (1-%u)", n_axes, kRopeAxes);
+    if (!(theta > 0.f)) return fail("rope_axes: theta must be positive");
+    if ((q && q_stride < (uint64_t)nqh * hd) || (stored && kv_stride < (uint64_t)nkh * hd))
+        return fail("rope_axes: stride smaller than a row");
+    RopeAxesArgs a{q, q_stride, k, v, kv_stride, pos, n, {}, kc, vc, nqh, nkh, hd};
+    uint64_t end = 0;
+    for (uint32_t x = 0; x < kRopeAxes; x++) {
+        end += x < n_axes ? sections[x] : 0u;
+        a.end[x] = end > hd ? hd : (uint32_t)end;
+    }
+    if (end != hd / 2u)
+        return fail("rope_axes: the sections hold %llu pairs, head_dim %u has %u", (unsigned long long)end, hd, hd / 2u);
+    if (n == 0) return 1;
+    if (stored) {
+        const uint64_t off = ((uint64_t)layer * max_ctx + slot) * nkh * hd;
+        a.kc += off;
+        a.vc += off;
+    }
+    if (!ready_or_fail()) return 0;
+    const OnDevice on;
+    return hip_ok(launch_rope_axes(a, theta, g_rt.stream), "rope_axes");
+}
+
+int vbs_gfx950_attention_tree(const float *q, uint32_t q_stride, const uint16_t *kc, const uint16_t *vc,
+                              float *out, uint32_t out_stride, uint32_t n, uint32_t past,
+                              const uint64_t *mask, uint32_t layer, uint32_t max_ctx, uint32_t nqh,
+                              uint32_t nkh, uint32_t hd, float scale) {
+    if (!mask) return fail("attention_tree: null pointer");
+    RowsArgs a{};
+    a.q = q, a.q_stride = q_stride, a.kc = kc, a.vc = vc, a.out = out, a.out_stride = out_stride;
+    a.n = n, a.past = past, a.nqh = nqh, a.nkh = nkh, a.hd = hd, a.scale = scale, a.max_ctx = max_ctx;
+    a.mask = mask;
+    a.words = (n + 63u) / 64u;
+    return attention_rows("attention_tree", a, layer);
+}
+
+int vbs_gfx950_attention_chunk(const float *q, uint32_t q_stride, const uint16_t *kc, const uint16_t *vc,
+                               float *out, uint32_t out_stride, uint32_t n, uint32_t past, uint32_t layer,
+                               uint32_t max_ctx, uint32_t nqh, uint32_t nkh, uint32_t hd, float scale,
+                               const vbs_gfx950_attn_terms_t *terms) {
+    RowsArgs a{};
+    a.q = q, a.q_stride = q_stride, a.kc = kc, a.vc = vc, a.out = out, a.out_stride = out_stride;
+    a.n = n, a.past = past, a.nqh = nqh, a.nkh = nkh, a.hd = hd, a.scale = scale, a.max_ctx = max_ctx;
+    if (terms) {
+        if (!(terms->cap >= 0.f) || isinf(terms->cap)) return fail("attention_chunk: cap must be 0 or a positive number");
+        a.cap = terms->cap;
+        a.slopes = terms->slopes;
+        a.docs = terms->docs;
+        a.mass = terms->mass;
+        const uint64_t total = (uint64_t)past + n;
+        a.prefix = terms->prefix < total ? terms->prefix : (uint32_t)total;
+    }
+    return attention_rows("attention_chunk", a, layer);
+}
+
+int vbs_gfx950_cache_evict(uint16_t *kc, uint16_t *vc, const float *mass, float *mass_out, uint32_t *kept,
+                           uint32_t len, uint32_t budget, uint32_t first, uint32_t last, uint32_t layer,
+                           uint32_t n_layers, uint32_t max_ctx, uint32_t nkh, uint32_t hd) {
+    if (!kc || !vc || !mass || !kept) return fail("cache_evict: null pointer");
+    if (len == 0 || budget == 0 || n_layers == 0 || nkh == 0 || hd == 0) return fail("cache_evict: empty shape");
+    if (len > max_ctx) return fail("cache_evict: len %u > max_ctx %u", len, max_ctx);
+    if (budget > len) return fail("cache_evict: budget %u > len %u", budget, len);
+    if ((uint64_t)first + last > budget) return fail("cache_evict: first %u + last %u > budget %u", first, last, budget);
+    if (n_layers > 65535u || nkh > 65535u) return fail("cache_evict: more than 65535 layers or kv heads");
+    if (hd > 256 || (hd & 1u)) return fail("cache_evict: head_dim %u must be even and <= 256", hd);
+    const uint64_t rows = (uint64_t)n_layers * max_ctx * nkh, before = (uint64_t)layer * max_ctx * nkh;
+    EvictArgs a{kc + before * hd, vc + before * hd, mass + before, mass_out ? mass_out + before : nullptr, kept,
+                len, budget, first, last, n_layers, max_ctx, nkh, hd};
+    if (spans_overlap(a.kc, 2u * rows * hd, a.vc, 2u * rows * hd)) return fail("cache_evict: the caches overlap");
+    if (mass_out && mass_out != mass && spans_overlap(a.mass, 4u * rows, a.mass_out, 4u * rows))
+        return fail("cache_evict: mass_out overlaps mass and is not mass");
+    if (!ready_or_fail()) return 0;
+    const OnDevice on;
+    return hip_ok(launch_evict(a, g_rt.stream), "cache_evict");
 }
 
 uint32_t vbs_gfx950_checksum_partials(size_t bytes) { return checksum_partials(bytes); }

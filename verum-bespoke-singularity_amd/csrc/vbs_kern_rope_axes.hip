@@ -1,0 +1,98 @@
+// vbs_kern_rope_axes.hip — rotary positions with several axes for n tokens, and
+// their K and V rows into the f16 cache, in one launch.
+//
+// Pair p (elements 2p, 2p + 1, as src/vbs_host_math.h:38-51) of every head of
+// token i turns by a = pos[axis(p)][i] * theta^(-2p / hd), axis(p) the axis whose
+// section of pairs holds p. q is rotated in place; k is rotated, and k and v
+// are stored with the cache's rounding (src/vbs_host_math.h:150-159).
+//
+// The angle of a far position needs more than 24 bits (position 1e6 times a
+// frequency of 1 leaves 0.06 rad of f32's spacing), so it is formed in 64 bits,
+// reduced there to [-pi/4, pi/4] and its sine and cosine are taken there too;
+// only they are rounded to f32 (half a step, 2^-24). The reference's own
+// rotation (vbs_gfx950_rope) forms its angles in f32 and so differs from this
+// one by up to position * 2^-23 rad.
+#include <math.h>
+
+#include "vbs_dev_common.h"
+#include "vbs_steps.h"
+
+namespace vbs {
+
+struct RopeFreqs {
+    double f[kRopeMaxPairs];
+};
+
+// (cos a, sin a): a = k pi/2 + r with pi/2 in two parts (53 and 53 bits; |a| up to
+// 2^31 leaves r exact to about 2^-52 * |k| * 2^-53 beyond a's own rounding), then
+// the Taylor series of sine and cosine on |r| <= pi/4, whose first dropped terms
+// are r^15 / 15! < 2.1e-14 and r^16 / 16! < 1.1e-15.
+__device__ __forceinline__ float2 cos_sin(double a) {
+    const double k = rint(a * 0.63661977236758134308);  // 2 / pi
+    double r = fma(k, -1.5707963267948965580, a);
+    r = fma(k, -6.1232339957367660359e-17, r);
+    const double z = r * r;
+    double s = 1.0 / 6227020800.0;
+    s = fma(s, z, -1.0 / 39916800.0);
+    s = fma(s, z, 1.0 / 362880.0);
+    s = fma(s, z, -1.0 / 5040.0);
+    s = fma(s, z, 1.0 / 120.0);
+    s = fma(s, z, -1.0 / 6.0);
+    s = fma(s * z, r, r);
+    double c = -1.0 / 87178291200.0;
+    c = fma(c, z, 1.0 / 479001600.0);
+    c = fma(c, z, -1.0 / 3628800.0);
+    c = fma(c, z, 1.0 / 40320.0);
+    c = fma(c, z, -1.0 / 720.0);
+    c = fma(c, z, 1.0 / 24.0);
+    c = fma(c, z, -0.5);
+    c = fma(c, z, 1.0);
+    const int quad = (int)((long long)k & 3);
+    const double cs = quad & 1 ? s : c, sn = quad & 1 ? c : s;
+    return make_float2((float)(quad == 1 || quad == 2 ? -cs : cs), (float)(quad >= 2 ? -sn : sn));
+}
+
+// grid (parts, tokens): a workgroup takes `rows` of a token's nqh + nkh heads.
+__global__ __launch_bounds__(256) void k_rope_axes(RopeAxesArgs a, RopeFreqs fr, uint32_t rows) {
+    __shared__ float2 cs[kRopeMaxPairs];
+    const uint32_t pairs = a.hd / 2u, i = blockIdx.y, t = threadIdx.x;
+    for (uint32_t p = t; p < pairs; p += 256u) {
+        uint32_t axis = 0;
+        while (p >= a.end[axis]) axis++;
+        cs[p] = cos_sin((double)a.pos[(uint64_t)axis * a.n + i] * fr.f[p]);
+    }
+    __syncthreads();
+    const uint32_t heads = (a.q ? a.nqh : 0u) + (a.k ? a.nkh : 0u), r0 = blockIdx.x * rows;
+    const uint32_t mine = min(rows, heads - r0) * pairs;
+    for (uint32_t e = t; e < mine; e += 256u) {
+        uint32_t h = r0 + e / pairs;
+        const uint32_t p = e % pairs;
+        const float2 w = cs[p];
+        if (a.q && h < a.nqh) {
+            float *x = a.q + (uint64_t)i * a.q_stride + (uint64_t)h * a.hd + 2u * p;
+            const float x0 = x[0], x1 = x[1];
+            x[0] = __fsub_rn(__fmul_rn(x0, w.x), __fmul_rn(x1, w.y));
+            x[1] = __fadd_rn(__fmul_rn(x0, w.y), __fmul_rn(x1, w.x));
+            continue;
+        }
+        if (a.q) h -= a.nqh;
+        const uint64_t from = (uint64_t)i * a.kv_stride + (uint64_t)h * a.hd + 2u * p;
+        const uint64_t to = ((uint64_t)i * a.nkh + h) * a.hd + 2u * p;
+        const float x0 = a.k[from], x1 = a.k[from + 1u];
+        a.kc[to] = vbs_f2h(__fsub_rn(__fmul_rn(x0, w.x), __fmul_rn(x1, w.y)));
+        a.kc[to + 1u] = vbs_f2h(__fadd_rn(__fmul_rn(x0, w.y), __fmul_rn(x1, w.x)));
+        a.vc[to] = vbs_f2h(a.v[from]);
+        a.vc[to + 1u] = vbs_f2h(a.v[from + 1u]);
+    }
+}
+
+hipError_t launch_rope_axes(const RopeAxesArgs &a, float theta, hipStream_t s) {
+    const uint32_t pairs = a.hd / 2u, heads = (a.q ? a.nqh : 0u) + (a.k ? a.nkh : 0u);
+    RopeFreqs fr;
+    for (uint32_t p = 0; p < pairs; p++) fr.f[p] = pow((double)theta, -2.0 * p / a.hd);
+    const uint32_t rows = 8u;
+    k_rope_axes<<<dim3((heads + rows - 1u) / rows, a.n), 256, 0, s>>>(a, fr, rows);
+    return hipGetLastError();
+}
+
+}  // namespace vbs

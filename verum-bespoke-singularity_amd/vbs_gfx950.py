@@ -128,6 +128,11 @@ class LinearJoin(C.Structure):
                 ("k_row", _P), ("kc", _P), ("vc", _P), ("kv_off", _U64)]
 
 
+class AttnTerms(C.Structure):
+    """vbs_gfx950_attn_terms_t: what vbs_gfx950_attention_chunk adds to plain causal attention."""
+    _fields_ = [("cap", _F), ("slopes", _P), ("docs", _P), ("prefix", _U32), ("mass", _P)]
+
+
 _DEVICE_SIGS = {
     "abi_version": (_I, []),
     "init": (_I, []),
@@ -154,6 +159,13 @@ _DEVICE_SIGS = {
     "cache_store": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _U32]),
     "attention": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _F]),
     "attention_noalloc": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _F]),
+    "rope_axes": (_I, [_P, _U32, _P, _P, _U32, _P, _U32, _U32, _P, _P, _P, _U32, _U32, _U32, _U32,
+                       _U32, _U32, _F]),
+    "attention_tree": (_I, [_P, _U32, _P, _P, _P, _U32, _U32, _U32, _P, _U32, _U32, _U32, _U32, _U32,
+                            _F]),
+    "attention_chunk": (_I, [_P, _U32, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _U32, _U32, _F,
+                             C.POINTER(AttnTerms)]),
+    "cache_evict": (_I, [_P, _P, _P, _P, _P] + [_U32] * 9),
     "silu_mul": (_I, [_P, _P, _P, _U32]),
     "add": (_I, [_P, _P, _P, _U32]),
     "dequant_rows": (_I, [_I, _P, _P, _U32, _U32, _P]),
@@ -327,6 +339,34 @@ class DeviceLib:
     def attention(self, q, kc, vc, out, seq_len, layer, max_ctx, nqh, nkh, hd, scale):
         self.check(self._attention(q, kc, vc, out, seq_len, layer, max_ctx, nqh, nkh, hd, scale),
                    "attention")
+
+    def rope_axes(self, q, q_stride, k, v, kv_stride, pos, n, sections, kc, vc, slot, layer, max_ctx,
+                  nqh, nkh, hd, theta):
+        """Rotate n tokens' q in place and store their rotated k, and v, in the cache slots slot ..; pos is
+        [len(sections)][n] int32 on the device. q, or k, v, kc and vc, may be 0."""
+        axes = (_U32 * len(sections))(*sections)
+        self.check(self._rope_axes(q or None, q_stride, k or None, v or None, kv_stride, pos or None, n,
+                                   len(sections), axes, kc or None, vc or None, slot, layer, max_ctx, nqh,
+                                   nkh, hd, theta), "rope_axes")
+
+    def attention_tree(self, q, q_stride, kc, vc, out, out_stride, n, past, mask, layer, max_ctx, nqh, nkh,
+                       hd, scale):
+        """Attention of n drafted tokens in the slots past ..; mask: n x ceil(n / 64) 64-bit words."""
+        self.check(self._attention_tree(q, q_stride, kc, vc, out, out_stride, n, past, mask, layer, max_ctx,
+                                        nqh, nkh, hd, scale), "attention_tree")
+
+    def attention_chunk(self, q, q_stride, kc, vc, out, out_stride, n, past, layer, max_ctx, nqh, nkh, hd,
+                        scale, cap=0.0, slopes=0, docs=0, prefix=0, mass=0):
+        """Attention of n consecutive tokens in the slots past .., with the terms of AttnTerms."""
+        terms = AttnTerms(cap, slopes or None, docs or None, prefix, mass or None)
+        self.check(self._attention_chunk(q, q_stride, kc, vc, out, out_stride, n, past, layer, max_ctx, nqh,
+                                         nkh, hd, scale, C.byref(terms)), "attention_chunk")
+
+    def cache_evict(self, kc, vc, mass, mass_out, kept, n_len, budget, first, last, layer, n_layers, max_ctx,
+                    nkh, hd):
+        """Cut n_len slots to budget, per layer and kv head, by accumulated weight (mass_out may be 0)."""
+        self.check(self._cache_evict(kc, vc, mass, mass_out or None, kept, n_len, budget, first, last, layer,
+                                     n_layers, max_ctx, nkh, hd), "cache_evict")
 
     def silu_mul(self, g, u, out, n):
         self.check(self._silu_mul(g, u, out, n), "silu_mul")
