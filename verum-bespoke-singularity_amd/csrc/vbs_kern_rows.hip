@@ -6,121 +6,536 @@
 // Row i (a token) and q head h of kv head h / group, over the slots j that the row
 // sees: s_j = scale q.k_j, capped c tanh(s_j / c), less slope_h |i - j|; m = max s_j,
 // l = sum e^(s_j - m), out = sum e^(s_j - m) v_j / l, and 0 where nothing is seen
-// (m = -inf). The weight of slot j, e^(s_j - m) / l, is summed over the rows and
+// (l = 0). The weight of slot j, e^(s_j - m) / l, is summed over the rows and
 // the q heads of its kv head into mass[j]. Rows that do not see a slot take
 // nothing from it, whatever is in its K and V.
-#include "vbs_dev_common.h"
-#include "vbs_steps.h"
+//
+// The (token, q head) pairs of a kv head are its rows, n * group of them, row r =
+// i * group + g. A workgroup takes 64 CT rows of one kv head (16 CT a wave) and a
+// range of slots, 64 (32 for head_dim above 128) at a time through LDS, on
+// v_mfma_f32_16x16x32_f16:
+// * S^T = K Q^T: A = 16 slots x 32 dims of K (the cache's f16, exact), B = 32 dims
+//   x 16 rows of q' = q 2^s, s so that the row's largest |q'| lies in [2^14, 2^15),
+//   as two f16 parts hi + lo (22 bits; the two products add up in the same f32
+//   sums). A lane then holds the scores of one row (column lane & 15) at slots
+//   16 hf + 4 (lane >> 4) + r, so the softmax needs no row-wise exchange but for the
+//   maximum.
+// * the running maximum moves only where a score passes it by more than 8 in
+//   log2: then the sums are rescaled. The weights are 2^(y - m + 7) <= 2^15, so that
+//   small ones keep their low part in f16.
+// * O^T += V^T P^T: B = P^T, the lane's own weights (hi, then lo), A = V^T with the
+//   k slots in the same order, its rows the head dims dim_of (below), so that a
+//   lane's V dims are neighbours in memory and two permutes pair its slots.
+// Each range of slots ends in m, l and acc per row; where a kv head's rows are few
+// the slots are split over several workgroups and k_rows_merge adds them up,
+// scaled to the common maximum.
+#include "vbs_rows_common.h"
 
 namespace vbs {
 
-// Whether row i (slot past + i) sees slot j.
-__device__ __forceinline__ bool row_sees(const RowsArgs &a, uint32_t i, uint32_t j) {
-    if (a.mask) {
-        if (j < a.past) return true;
-        const uint32_t t = j - a.past;
-        return (a.mask[(uint64_t)i * a.words + (t >> 6)] >> (t & 63u)) & 1u;
+// Where a lane's V words lie: HD is cut into pieces of 128, 64 and 32 dims; in a
+// piece of 16 D dims, lane column m (of 16) owns dims D m .. D m + D - 1.
+template <uint32_t HD>
+struct Pieces {
+    static constexpr uint32_t KK = HD / 32u, W = HD / 32u;  // K slices; V words (two dims) per lane
+    // the first dim, for lane column m, of word w
+    __host__ __device__ static constexpr uint32_t dim(uint32_t w, uint32_t m) {
+        const uint32_t n128 = HD / 128u, rest = HD % 128u;
+        if (w < 4u * n128) return 128u * (w / 4u) + 8u * m + 2u * (w % 4u);
+        const uint32_t b = 128u * n128, v = w - 4u * n128;
+        if (rest >= 64u && v < 2u) return b + 4u * m + 2u * v;
+        return b + (rest >= 64u ? 64u : 0u) + 2u * m;
     }
-    if (j > a.past + i && j >= a.prefix) return false;
-    return !a.docs || a.docs[j] == a.docs[a.past + i];
-}
-// The slots behind the last that row i can see.
-__device__ __forceinline__ uint32_t row_end(const RowsArgs &a, uint32_t i) {
-    if (a.mask) return a.past + a.n;
-    return max(a.past + i + 1u, a.prefix);
-}
-// The score from scale q.k.
-__device__ __forceinline__ float row_score(const RowsArgs &a, float s, float slope, uint32_t i, uint32_t j) {
-    if (a.cap > 0.f) s = a.cap * tanhf(s / a.cap);
-    const uint32_t at = a.past + i;
-    return fmaf(-slope, (float)(at > j ? at - j : j - at), s);
+};
+
+constexpr float kLazy = 8.f, kLift = 7.f;  // log2: how far a score may pass m; the weights' scale
+
+__device__ __forceinline__ uint64_t ones_below(int64_t x) {
+    return x <= 0 ? 0ull : x >= 64 ? ~0ull : (1ull << x) - 1ull;
 }
 
-// ---- every shape: a wave per row and q head, a slot per lane -----------------------
-// The scores of 64 slots at a time (f32 FMA chains in element order), a running
-// maximum and sum, then the lanes take the head's dims and walk the 64 weights.
-constexpr uint32_t kRowHd = 256;
+// The slots [p0, p0 + 64) that a row of token i sees, as bits, documents aside.
+__device__ __forceinline__ uint64_t seen_bits(const RowsArgs &a, uint32_t i, uint32_t p0, uint32_t s1) {
+    const uint64_t in = ones_below((int64_t)s1 - p0);
+    if (!a.mask) return in & ones_below((int64_t)row_end(a, i) - p0);
+    const int64_t off = (int64_t)p0 - a.past;
+    const uint64_t *row = a.mask + (uint64_t)i * a.words;
+    uint64_t v = ones_below(-off);
+    if (off >= 0) {
+        const uint64_t w = (uint64_t)off >> 6;
+        const uint32_t sh = (uint32_t)off & 63u;
+        if (w < a.words) v |= row[w] >> sh;
+        if (sh && w + 1u < a.words) v |= row[w + 1u] << (64u - sh);
+    } else if (off > -64) {
+        v |= row[0] << (uint32_t)-off;
+    }
+    return in & v;
+}
 
-__global__ __launch_bounds__(64) void k_row_any(RowsArgs a, float *__restrict__ stats) {
-    __shared__ float qs[kRowHd], ps[64];
-    const uint32_t lane = threadIdx.x, i = blockIdx.y, h = blockIdx.x, kvh = h / (a.nqh / a.nkh);
-    const float *q = a.q + (uint64_t)i * a.q_stride + (uint64_t)h * a.hd;
-    for (uint32_t d = lane; d < a.hd; d += 64u) qs[d] = q[d];
-    __syncthreads();
-    const uint64_t rstride = (uint64_t)a.nkh * a.hd, base = (uint64_t)kvh * a.hd;
-    const float slope = a.slopes ? a.slopes[h] : 0.f;
-    float m = -INFINITY, l = 0.f, acc[kRowHd / 64] = {};
-    const uint32_t end = row_end(a, i);
-    for (uint32_t j0 = 0; j0 < end; j0 += 64u) {
-        const uint32_t j = j0 + lane;
-        const bool sees = j < end && row_sees(a, i, j);
-        float s = -INFINITY;
-        if (sees) {
-            const uint16_t *k = a.kc + (uint64_t)j * rstride + base;
-            float dot = 0.f;
-            for (uint32_t d = 0; d < a.hd; d++) dot = fmaf(qs[d], h2f(k[d]), dot);
-            s = row_score(a, dot * a.scale, slope, i, j);
-        }
-        const uint64_t seen = __ballot(sees);
-        if (!seen) continue;
-        // fmaxf drops a NaN: a NaN score must come through the sum instead
-        const float mn = fmaxf(m, wave_max(s)), top = mn == -INFINITY ? 0.f : mn;
-        const float r = expf(m - top), p = sees ? expf(s - top) : 0.f;
-        l = l * r + wave_sum(p);
-        m = mn;
-        ps[lane] = p;
-        __syncthreads();
+// The q' parts of one row (column lane & 15) for lane group g: dims 32 kk + 8 g ...
+// `row` NULL: zeros. c: |scale| 2^-s, what a product of the parts is to be scaled by.
+template <uint32_t KK>
+__device__ __forceinline__ void row_parts(const float *row, uint32_t hd, bool wide, float scale, uint32_t g,
+                                          rh8 (&hi)[KK], rh8 (&lo)[KK], float &c) {
+    float x[KK][8], top = 0.f;
 #pragma unroll
-        for (uint32_t c = 0; c < kRowHd / 64u; c++) {
-            const uint32_t d = 64u * c + lane;
-            if (d >= a.hd) break;
-            float x = acc[c] * r;
-            for (uint32_t t = 0; t < 64u; t++)
-                if (seen >> t & 1u) x = fmaf(ps[t], h2f(a.vc[(uint64_t)(j0 + t) * rstride + base + d]), x);
-            acc[c] = x;
-        }
-        __syncthreads();
-    }
+    for (uint32_t kk = 0; kk < KK; kk++) {
+        const uint32_t d0 = 32u * kk + 8u * g;
+        if (row && wide && d0 < hd) {
+            const float4 u = *reinterpret_cast<const float4 *>(row + d0), v = *reinterpret_cast<const float4 *>(row + d0 + 4u);
+            x[kk][0] = u.x, x[kk][1] = u.y, x[kk][2] = u.z, x[kk][3] = u.w;
+            x[kk][4] = v.x, x[kk][5] = v.y, x[kk][6] = v.z, x[kk][7] = v.w;
+        } else {
 #pragma unroll
-    for (uint32_t c = 0; c < kRowHd / 64u; c++) {
-        const uint32_t d = 64u * c + lane;
-        if (d < a.hd) a.out[(uint64_t)i * a.out_stride + (uint64_t)h * a.hd + d] = l == 0.f ? 0.f : acc[c] / l;
+            for (uint32_t e = 0; e < 8u; e++) x[kk][e] = row && !wide && d0 + e < hd ? row[d0 + e] : 0.f;
+        }
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; e++) top = fmaxf(top, fabsf(x[kk][e]));
     }
-    if (stats && lane == 0) {
-        float *st = stats + 2u * ((uint64_t)i * a.nqh + h);
-        st[0] = m, st[1] = l;
-    }
+    top = fmaxf(top, lane_xor<16>(top));
+    top = fmaxf(top, lane_xor<32>(top));
+    int e2 = 0;
+    (void)frexpf(top, &e2);  // top < 2^e2
+    // (a row below 2^-111 scores nothing that an f32 sum keeps; 2^-sq must stay a number)
+    const int sq = top > 0.f && top < INFINITY ? (15 - e2 < 126 ? 15 - e2 : 126) : 0;
+    c = ldexpf(fabsf(scale), -sq);
+    const float sign = scale < 0.f ? -1.f : 1.f;
+#pragma unroll
+    for (uint32_t kk = 0; kk < KK; kk++)
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; e++) {
+            const float y = ldexpf(x[kk][e] * sign, sq);
+            const _Float16 h = (_Float16)y;
+            hi[kk][e] = h;
+            lo[kk][e] = (_Float16)(y - (float)h);
+        }
 }
 
-// The weights of one slot: a wave per slot and kv head, the lanes over (row, q head).
-__global__ __launch_bounds__(64) void k_mass_any(RowsArgs a, const float *__restrict__ stats) {
-    const uint32_t lane = threadIdx.x, j = blockIdx.x, kvh = blockIdx.y, group = a.nqh / a.nkh;
+// Eight cache elements of a row from element d0 on (zeros from hd on).
+__device__ __forceinline__ ru4 cache8(const uint16_t *p, uint32_t d0, uint32_t hd, bool wide) {
+    if (wide) return d0 < hd ? *reinterpret_cast<const ru4 *>(p + d0) : ru4{0u, 0u, 0u, 0u};
+    ru4 v;
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; k++) {
+        const uint32_t x = d0 + 2u * k < hd ? p[d0 + 2u * k] : 0u, y = d0 + 2u * k + 1u < hd ? p[d0 + 2u * k + 1u] : 0u;
+        v[k] = x | y << 16;
+    }
+    return v;
+}
+
+struct RowsSplit {
+    uint32_t len, n;  // slots per range (a multiple of 64), ranges
+};
+
+// How the launch's scratch is laid out: (m, l) then acc per (kv head, range, row),
+// then (m, 1 / l) per (kv head, row).
+struct RowsPart {
+    float2 *ml;
+    float *acc;
+    float2 *stats;
+};
+
+template <uint32_t HD>
+constexpr uint32_t kTile = HD > 128u ? 32u : 64u;  // slots per LDS tile
+
+template <uint32_t HD, uint32_t CT>
+__global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsPart pt, uint32_t tiles, bool wide_kv,
+                                                 bool wide_q) {
+    using P = Pieces<HD>;
+    constexpr uint32_t KK = P::KK, W = P::W, T = kTile<HD>, CPR = HD / 8u, NC = T * CPR / 256u;
+    constexpr uint32_t RS = HD * 2u + 16u;  // LDS row stride in bytes: 16 rows' chunks lie in different banks
+    __shared__ __align__(16) uint8_t kl[2][T * RS], vl[2][T * RS];
+    __shared__ int32_t dl[2][T];
+    const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u, col = lane & 15u, g = lane >> 4;
+    const uint32_t kvh = blockIdx.x % a.nkh, rest = blockIdx.x / a.nkh;
+    const uint32_t split = rest % sp.n, tile = tiles - 1u - rest / sp.n;  // (the longest rows first)
+    const uint32_t group = a.nqh / a.nkh, rows = a.n * group, row_tile = tile * 64u * CT;
+    const uint32_t end = row_end(a, (min(row_tile + 64u * CT, rows) - 1u) / group);
+    const uint32_t s0 = split * sp.len, s1 = min(s0 + sp.len, end);
+    if (s0 >= s1) return;  // (the whole workgroup; the merge counts the ranges the same way)
+    const uint32_t slots = a.past + a.n;
+
+    // ---- the wave's rows
+    const uint32_t row0 = row_tile + wave * 16u * CT;
+    const bool active = row0 < rows;
+    rh8 qh[CT][KK], ql[CT][KK];
+    float c1[CT], slope[CT];
+    uint32_t tok[CT];
+    int32_t doc[CT];
+    bool real[CT];
+#pragma unroll
+    for (uint32_t x = 0; x < CT; x++) {
+        const uint32_t r = row0 + 16u * x + col;
+        real[x] = r < rows;
+        tok[x] = real[x] ? r / group : 0u;
+        const uint32_t h = kvh * group + (real[x] ? r % group : 0u);
+        row_parts<KK>(real[x] ? a.q + (uint64_t)tok[x] * a.q_stride + (uint64_t)h * a.hd : nullptr, a.hd, wide_q, a.scale,
+                      g, qh[x], ql[x], c1[x]);
+        slope[x] = a.slopes ? a.slopes[h] : 0.f;
+        doc[x] = a.docs ? a.docs[a.past + tok[x]] : 0;
+    }
+    const bool terms = a.cap > 0.f || a.slopes;
+    // below `clear` every row of the wave sees every slot (documents aside); from `last` on, none
+    const uint32_t tok_first = min(row0, rows - 1u) / group, tok_last = (min(row0 + 16u * CT, rows) - 1u) / group;
+    const uint32_t clear = a.docs ? 0u : a.mask ? a.past : row_end(a, tok_first);
+    const uint32_t last = active ? row_end(a, tok_last) : 0u;
+
+    // ---- staging: a thread's chunks of a tile, in registers until the tile before is used
     const uint64_t rstride = (uint64_t)a.nkh * a.hd;
-    const uint16_t *k = a.kc + (uint64_t)j * rstride + (uint64_t)kvh * a.hd;
+    const uint16_t *kb = a.kc + (uint64_t)kvh * a.hd, *vb = a.vc + (uint64_t)kvh * a.hd;
+    ru4 ks[NC], vs[NC];
+    int32_t ds = 0;
+    auto fetch = [&](uint32_t p0) {
+#pragma unroll
+        for (uint32_t k = 0; k < NC; k++) {
+            const uint32_t id = t + 256u * k, r = id / CPR, d = 8u * (id % CPR);
+            // (slots behind the last repeat it: what lies there may be no number)
+            const uint64_t at = (uint64_t)min(p0 + r, slots - 1u) * rstride;
+            ks[k] = cache8(kb + at, d, a.hd, wide_kv);
+            vs[k] = cache8(vb + at, d, a.hd, wide_kv);
+        }
+        if (a.docs && t < T) ds = a.docs[min(p0 + t, slots - 1u)];
+    };
+    auto put = [&](uint32_t b) {
+#pragma unroll
+        for (uint32_t k = 0; k < NC; k++) {
+            const uint32_t id = t + 256u * k, at = id / CPR * RS + 16u * (id % CPR);
+            *reinterpret_cast<ru4 *>(&kl[b][at]) = ks[k];
+            *reinterpret_cast<ru4 *>(&vl[b][at]) = vs[k];
+        }
+        if (a.docs && t < T) dl[b][t] = ds;
+    };
+
+    float m[CT], l[CT];
+    rf4 acc[2u * W][CT];
+#pragma unroll
+    for (uint32_t x = 0; x < CT; x++) {
+        m[x] = -INFINITY, l[x] = 0.f;
+#pragma unroll
+        for (uint32_t d = 0; d < 2u * W; d++) acc[d][x] = rf4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // 32 slots from p0 on, in LDS buffer b at row `at`; vis: their bits per column tile
+    auto step = [&](uint32_t b, uint32_t at, uint32_t p0, const uint32_t (&vis)[CT], bool full) {
+        rf4 S[2][CT];
+#pragma unroll
+        for (uint32_t hf = 0; hf < 2u; hf++)
+#pragma unroll
+            for (uint32_t x = 0; x < CT; x++) S[hf][x] = rf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (uint32_t kk = 0; kk < KK; kk++) {
+            rh8 ka[2];
+#pragma unroll
+            for (uint32_t hf = 0; hf < 2u; hf++)
+                ka[hf] = *reinterpret_cast<const rh8 *>(&kl[b][(at + 16u * hf + col) * RS + 64u * kk + 16u * g]);
+#pragma unroll
+            for (uint32_t hf = 0; hf < 2u; hf++)
+#pragma unroll
+                for (uint32_t x = 0; x < CT; x++)
+                    S[hf][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[hf], qh[x][kk], S[hf][x], 0, 0, 0);
+#pragma unroll
+            for (uint32_t hf = 0; hf < 2u; hf++)
+#pragma unroll
+                for (uint32_t x = 0; x < CT; x++)
+                    S[hf][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[hf], ql[x][kk], S[hf][x], 0, 0, 0);
+        }
+        // the lane's V words: eight slots, in the order of the weights below
+        uint32_t vw[8][W];
+#pragma unroll
+        for (uint32_t j = 0; j < 8u; j++) {
+            const uint8_t *row = &vl[b][(at + 16u * (j >> 2) + 4u * g + (j & 3u)) * RS];
+#pragma unroll
+            for (uint32_t w = 0; w < W; w++) {
+                // (words of one piece are neighbours: the compiler joins the reads)
+                vw[j][w] = *reinterpret_cast<const uint32_t *>(row + 2u * P::dim(w, col));
+            }
+        }
+        // y = cm S in units of log2: the plain score, or with what the terms and the mask make of it
+        float cm[CT];
+#pragma unroll
+        for (uint32_t x = 0; x < CT; x++) cm[x] = c1[x] * kLog2e;
+        if (!full || terms) {
+#pragma unroll
+            for (uint32_t x = 0; x < CT; x++) {
+#pragma unroll
+                for (uint32_t j = 0; j < 8u; j++) {
+                    const uint32_t o = 16u * (j >> 2) + 4u * g + (j & 3u);
+                    float s = S[j >> 2][x][j & 3u] * c1[x];
+                    if (terms) s = row_score(a, s, slope[x], a.past + tok[x], p0 + o);
+                    bool sees = full || (vis[x] >> o & 1u);
+                    if (a.docs) sees = sees && dl[b][at + o] == doc[x];
+                    S[j >> 2][x][j & 3u] = sees ? s * kLog2e : -INFINITY;
+                }
+                cm[x] = 1.f;
+            }
+        }
+        float top[CT];
+        bool up = false;
+#pragma unroll
+        for (uint32_t x = 0; x < CT; x++) {
+            float v = S[0][x][0];
+#pragma unroll
+            for (uint32_t j = 1; j < 8u; j++) v = fmaxf(v, S[j >> 2][x][j & 3u]);
+            top[x] = v * cm[x];
+            up = up || top[x] > m[x] + kLazy;
+        }
+        if (__any(up)) {
+#pragma unroll
+            for (uint32_t x = 0; x < CT; x++) {
+                float v = fmaxf(top[x], lane_xor<16>(top[x]));
+                v = fmaxf(v, lane_xor<32>(v));
+                const float mn = v > m[x] + kLazy ? v : m[x];
+                const float f = mn == -INFINITY ? 1.f : exp2f(m[x] - mn);
+                m[x] = mn;
+                l[x] *= f;
+#pragma unroll
+                for (uint32_t d = 0; d < 2u * W; d++) acc[d][x] *= f;
+            }
+        }
+        rh8 ph[CT], pl[CT];
+#pragma unroll
+        for (uint32_t x = 0; x < CT; x++) {
+            const float ms = m[x] == -INFINITY ? 0.f : m[x] - kLift;
+#pragma unroll
+            for (uint32_t j = 0; j < 8u; j++) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(S[j >> 2][x][j & 3u], cm[x], -ms));
+                l[x] += p;
+                const _Float16 h = (_Float16)p;
+                ph[x][j] = h;
+                pl[x][j] = (_Float16)(p - (float)h);
+            }
+        }
+#pragma unroll
+        for (uint32_t d = 0; d < 2u * W; d++) {
+            const uint32_t sel = d & 1u ? 0x07060302u : 0x05040100u;
+            ru4 va;
+#pragma unroll
+            for (uint32_t j = 0; j < 4u; j++) va[j] = __builtin_amdgcn_perm(vw[2u * j + 1u][d >> 1], vw[2u * j][d >> 1], sel);
+#pragma unroll
+            for (uint32_t x = 0; x < CT; x++)
+                acc[d][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(rh8, va), ph[x], acc[d][x], 0, 0, 0);
+#pragma unroll
+            for (uint32_t x = 0; x < CT; x++)
+                acc[d][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(rh8, va), pl[x], acc[d][x], 0, 0, 0);
+        }
+    };
+
+    fetch(s0);
+    put(0u);
+    __syncthreads();
+    for (uint32_t p0 = s0, b = 0; p0 < s1; p0 += T, b ^= 1u) {
+        const bool more = p0 + T < s1;
+        if (more) fetch(p0 + T);
+        if (p0 < last) {
+            const bool full = p0 + T <= min(clear, s1);
+            uint64_t vis[CT];
+#pragma unroll
+            for (uint32_t x = 0; x < CT; x++) vis[x] = full ? ~0ull : real[x] ? seen_bits(a, tok[x], p0, s1) : 0ull;
+#pragma unroll
+            for (uint32_t h = 0; h < T / 32u; h++) {
+                uint32_t v[CT];
+#pragma unroll
+                for (uint32_t x = 0; x < CT; x++) v[x] = (uint32_t)(vis[x] >> (32u * h));
+                step(b, 32u * h, p0 + 32u * h, v, full);
+            }
+        }
+        if (more) {
+            put(b ^ 1u);  // (the buffer of two tiles ago: every wave left it before the last barrier)
+            __syncthreads();
+        }
+    }
+    if (!active) return;
+
+    // ---- the rows' sums: l over the four lane groups, then out (one range) or the partials
+    const uint64_t first = ((uint64_t)kvh * sp.n + split) * rows;
+#pragma unroll
+    for (uint32_t x = 0; x < CT; x++) {
+        l[x] += lane_xor<16>(l[x]);
+        l[x] += lane_xor<32>(l[x]);
+        const uint32_t r = row0 + 16u * x + col, h = kvh * group + r % group;
+        float nan = l[x] * 0.f;
+#pragma unroll
+        for (uint32_t d = 0; d < 2u * W; d++)
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; k++) nan = fmaf(acc[d][x][k], 0.f, nan);
+        const uint64_t bad = __ballot(real[x] && nan != 0.f);  // (0 times anything finite is 0)
+        const uint32_t cols = (uint32_t)(bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xFFFFu;
+        const float mo = m[x] - kLift;
+        if (real[x] && !(cols >> col & 1u)) {
+            const float inv = sp.n > 1u ? 1.f : l[x] == 0.f ? 0.f : __fdiv_rn(1.f, l[x]);
+            float *to = sp.n > 1u ? pt.acc + (first + r) * a.hd
+                                  : a.out + (uint64_t)tok[x] * a.out_stride + (uint64_t)h * a.hd;
+#pragma unroll
+            for (uint32_t w = 0; w < W; w++)
+#pragma unroll
+                for (uint32_t k = 0; k < 4u; k++) {
+                    const uint32_t d = P::dim(w, 4u * g + k);
+                    if (d < a.hd) {
+                        to[d] = acc[2u * w][x][k] * inv;
+                        to[d + 1u] = acc[2u * w + 1u][x][k] * inv;
+                    }
+                }
+            if (g == 0 && sp.n > 1u) pt.ml[first + r] = make_float2(mo, l[x]);
+            if (g == 0 && sp.n == 1u && pt.stats) pt.stats[(uint64_t)kvh * rows + r] = make_float2(mo, l[x] == 0.f ? 0.f : __fdiv_rn(1.f, l[x]));
+        }
+        // rows whose sums are not finite, one at a time (row_whole)
+        for (uint32_t c = 0; cols >> c; c++) {
+            if (!(cols >> c & 1u)) continue;
+            const uint32_t rr = row0 + 16u * x + c, i = rr / group, hh = kvh * group + rr % group;
+            float wm, wl, wa[(HD + 63u) / 64u];
+            row_whole<HD>(a, i, hh, s0, s1, lane, wm, wl, wa);
+            float *to = sp.n > 1u ? pt.acc + (first + rr) * a.hd : a.out + (uint64_t)i * a.out_stride + (uint64_t)hh * a.hd;
+#pragma unroll
+            for (uint32_t k = 0; k < (HD + 63u) / 64u; k++)
+                if (64u * k + lane < a.hd) to[64u * k + lane] = sp.n > 1u ? wa[k] : wl == 0.f ? 0.f : wa[k] / wl;
+            if (lane == 0 && sp.n > 1u) pt.ml[first + rr] = make_float2(wm, wl);
+            if (lane == 0 && sp.n == 1u && pt.stats) pt.stats[(uint64_t)kvh * rows + rr] = make_float2(wm, wl == 0.f ? 0.f : 1.f / wl);
+        }
+    }
+}
+
+// ---- the ranges of a row added up ----------------------------------------------------
+// A workgroup per (kv head, row): M = max m_c, L = sum l_c 2^(m_c - M), out = sum acc_c
+// 2^(m_c - M) / L; wave w takes the ranges w, w + 4, ..., then the waves' sums in order.
+__global__ __launch_bounds__(256) void k_rows_merge(RowsArgs a, RowsSplit sp, RowsPart pt, uint32_t tile_rows) {
+    __shared__ float2 part[4][128];
+    __shared__ float lw[4];
+    const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u, r = blockIdx.x, kvh = blockIdx.y;
+    const uint32_t group = a.nqh / a.nkh, rows = a.n * group;
+    const uint32_t end = row_end(a, (min(r / tile_rows * tile_rows + tile_rows, rows) - 1u) / group);
+    const uint32_t n = (end + sp.len - 1u) / sp.len;
+    const float2 *ml = pt.ml + (uint64_t)kvh * sp.n * rows + r;
+    const float *acc = pt.acc + ((uint64_t)kvh * sp.n * rows + r) * a.hd;
+    float M = -INFINITY;
+    for (uint32_t c = lane; c < n; c += 64u) M = fmaxf(M, ml[(uint64_t)c * rows].x);
+    M = wave_max(M);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    float2 o[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    for (uint32_t c = wave; c < n; c += 4u) {
+        const float2 v = ml[(uint64_t)c * rows];
+        const float w = exp2f(v.x - ref);
+        L = fmaf(v.y, w, L);
+#pragma unroll
+        for (uint32_t k = 0; k < 2u; k++) {
+            const uint32_t d = 2u * lane + 128u * k;
+            if (d < a.hd) {
+                const float *x = acc + (uint64_t)c * rows * a.hd + d;
+                o[k].x = fmaf(x[0], w, o[k].x);
+                o[k].y = fmaf(x[1], w, o[k].y);
+            }
+        }
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < 2u; k++) part[wave][lane + 64u * k] = o[k];
+    if (lane == 0) lw[wave] = L;
+    __syncthreads();
+    if (t >= 128u || 2u * t >= a.hd) return;
+    const float total = ((lw[0] + lw[1]) + lw[2]) + lw[3];
+    float2 s = part[0][t];
+#pragma unroll
+    for (uint32_t w = 1; w < 4u; w++) {
+        s.x += part[w][t].x;
+        s.y += part[w][t].y;
+    }
+    const float inv = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
+    float *to = a.out + (uint64_t)(r / group) * a.out_stride + (uint64_t)(kvh * group + r % group) * a.hd + 2u * t;
+    to[0] = total == 0.f ? 0.f : s.x * inv;
+    to[1] = total == 0.f ? 0.f : s.y * inv;
+    if (t == 0 && pt.stats) pt.stats[(uint64_t)kvh * rows + r] = make_float2(M, inv);
+}
+
+// ---- the weights that slots received ---------------------------------------------------
+// A wave per slot and kv head, the lanes over the rows.
+__global__ __launch_bounds__(64) void k_mass(RowsArgs a, const float2 *__restrict__ stats) {
+    const uint32_t lane = threadIdx.x, j = blockIdx.x, kvh = blockIdx.y, group = a.nqh / a.nkh, rows = a.n * group;
+    const uint16_t *k = a.kc + (uint64_t)j * a.nkh * a.hd + (uint64_t)kvh * a.hd;
     float sum = 0.f;
-    for (uint32_t e = lane; e < a.n * group; e += 64u) {
-        const uint32_t i = e / group, h = kvh * group + e % group;
+    for (uint32_t r = lane; r < rows; r += 64u) {
+        const uint32_t i = r / group, h = kvh * group + r % group;
         if (j >= row_end(a, i) || !row_sees(a, i, j)) continue;
-        const float *q = a.q + (uint64_t)i * a.q_stride + (uint64_t)h * a.hd;
-        float dot = 0.f;
-        for (uint32_t d = 0; d < a.hd; d++) dot = fmaf(q[d], h2f(k[d]), dot);
-        const float s = row_score(a, dot * a.scale, a.slopes ? a.slopes[h] : 0.f, i, j);
-        const float m = stats[2u * ((uint64_t)i * a.nqh + h)], l = stats[2u * ((uint64_t)i * a.nqh + h) + 1u];
-        if (l != 0.f) sum += expf(s - (m == -INFINITY ? 0.f : m)) / l;
+        const float s = row_score(a, row_dot(a.q + (uint64_t)i * a.q_stride + (uint64_t)h * a.hd, k, a.hd) * a.scale,
+                                  a.slopes ? a.slopes[h] : 0.f, a.past + i, j);
+        const float2 st = stats[(uint64_t)kvh * rows + r];
+        if (st.y != 0.f) sum += exp2f(s * kLog2e - (st.x == -INFINITY ? 0.f : st.x)) * st.y;
     }
     sum = wave_sum(sum);
     if (lane == 0) a.mass[(uint64_t)kvh * a.max_ctx + j] += sum;
 }
 
+// ---- launches -------------------------------------------------------------------------------
+
+struct RowsPlan {
+    uint32_t hd, ct, tiles;  // template head size, column tiles a wave, row tiles a kv head
+    RowsSplit sp;
+    size_t ml, acc, stats;  // bytes
+};
+
+static RowsPlan rows_plan(const RowsArgs &a) {
+    RowsPlan p{};
+    p.hd = a.hd <= 32u ? 32u : a.hd <= 64u ? 64u : a.hd <= 96u ? 96u : a.hd <= 128u ? 128u : 256u;
+    const uint32_t rows = a.n * (a.nqh / a.nkh), slots = a.past + a.n;
+    p.ct = rows <= 64u || p.hd > 128u ? 1u : 2u;
+    p.tiles = (rows + 64u * p.ct - 1u) / (64u * p.ct);
+    // ranges: until about 512 workgroups share the work, at least 64 slots each
+    const uint32_t most = (slots + 63u) / 64u, wgs = p.tiles * a.nkh;
+    uint32_t n = 512u / wgs;
+    n = n < 1u ? 1u : n > most ? most : n > 64u ? 64u : n;
+    p.sp.len = ((slots + n - 1u) / n + 63u) / 64u * 64u;
+    p.sp.n = (slots + p.sp.len - 1u) / p.sp.len;
+    const size_t all = (size_t)rows * a.nkh;
+    const auto round = [](size_t b) { return (b + 255u) & ~(size_t)255u; };
+    if (p.sp.n > 1u) {
+        p.ml = round(all * p.sp.n * sizeof(float2));
+        p.acc = round(all * p.sp.n * a.hd * sizeof(float));
+    }
+    if (a.mass) p.stats = round(all * sizeof(float2));
+    return p;
+}
+
 size_t rows_scratch_bytes(const RowsArgs &a) {
-    return a.mass ? (size_t)a.n * a.nqh * 2u * sizeof(float) : 0u;
+    const RowsPlan p = rows_plan(a);
+    return p.ml + p.acc + p.stats;
+}
+
+template <uint32_t HD>
+static void start_rows(const RowsArgs &a, const RowsPlan &p, const RowsPart &pt, hipStream_t s) {
+    const bool wide_kv = a.hd % 8u == 0 && (((uintptr_t)a.kc | (uintptr_t)a.vc) & 15u) == 0;
+    const bool wide_q = a.hd % 8u == 0 && a.q_stride % 4u == 0 && ((uintptr_t)a.q & 15u) == 0;
+    const uint32_t grid = p.tiles * p.sp.n * a.nkh;
+    if constexpr (HD <= 128u) {
+        if (p.ct == 2u) {
+            k_rows<HD, 2><<<grid, 256, 0, s>>>(a, p.sp, pt, p.tiles, wide_kv, wide_q);
+            return;
+        }
+    }
+    k_rows<HD, 1><<<grid, 256, 0, s>>>(a, p.sp, pt, p.tiles, wide_kv, wide_q);
 }
 
 hipError_t launch_rows(const RowsArgs &a, void *scratch, hipStream_t s) {
-    float *stats = a.mass ? static_cast<float *>(scratch) : nullptr;
-    k_row_any<<<dim3(a.nqh, a.n), 64, 0, s>>>(a, stats);
-    if (a.mass) k_mass_any<<<dim3(a.past + a.n, a.nkh), 64, 0, s>>>(a, stats);
-    return hipGetLastError();
+    const RowsPlan p = rows_plan(a);
+    uint8_t *at = static_cast<uint8_t *>(scratch);
+    RowsPart pt{};
+    if (p.sp.n > 1u) pt.ml = reinterpret_cast<float2 *>(at), pt.acc = reinterpret_cast<float *>(at + p.ml);
+    if (a.mass) pt.stats = reinterpret_cast<float2 *>(at + p.ml + p.acc);
+    switch (p.hd) {
+        case 32: start_rows<32>(a, p, pt, s); break;
+        case 64: start_rows<64>(a, p, pt, s); break;
+        case 96: start_rows<96>(a, p, pt, s); break;
+        case 128: start_rows<128>(a, p, pt, s); break;
+        default: start_rows<256>(a, p, pt, s); break;
+    }
+    hipError_t e = hipGetLastError();
+    const uint32_t rows = a.n * (a.nqh / a.nkh);
+    if (e == hipSuccess && p.sp.n > 1u) {
+        k_rows_merge<<<dim3(rows, a.nkh), 256, 0, s>>>(a, p.sp, pt, 64u * p.ct);
+        e = hipGetLastError();
+    }
+    if (e == hipSuccess && a.mass) {
+        k_mass<<<dim3(a.past + a.n, a.nkh), 64, 0, s>>>(a, pt.stats);
+        e = hipGetLastError();
+    }
+    return e;
 }
 
 }  // namespace vbs

@@ -1,0 +1,97 @@
+// vbs_rows_common.h — what the kernels of several query rows over the f16 cache
+// share (vbs_kern_rows.hip): which slots a row sees, its scores, and one row in
+// plain f32 for rows whose sums are not finite.
+#pragma once
+
+#include "vbs_dev_common.h"
+#include "vbs_steps.h"
+
+namespace vbs {
+
+constexpr float kLog2e = 1.44269504088896341f;
+
+typedef _Float16 rh8 __attribute__((ext_vector_type(8)));
+typedef float rf4 __attribute__((ext_vector_type(4)));
+typedef uint32_t ru4 __attribute__((ext_vector_type(4)));
+
+// Whether row i (slot past + i) sees slot j.
+__device__ __forceinline__ bool row_sees(const RowsArgs &a, uint32_t i, uint32_t j) {
+    if (a.mask) {
+        if (j < a.past) return true;
+        const uint32_t t = j - a.past;
+        return (a.mask[(uint64_t)i * a.words + (t >> 6)] >> (t & 63u)) & 1u;
+    }
+    if (j > a.past + i && j >= a.prefix) return false;
+    return !a.docs || a.docs[j] == a.docs[a.past + i];
+}
+// The slots behind the last that row i can see.
+__host__ __device__ __forceinline__ uint32_t row_end(const RowsArgs &a, uint32_t i) {
+    if (a.mask) return a.past + a.n;
+    const uint32_t own = a.past + i + 1u;
+    return own > a.prefix ? own : a.prefix;
+}
+
+// tanh: an odd polynomial (least relative error, fitted on |x| <= 0.6: 1.2e-8) and
+// 1 - 2 / (e^(2|x|) + 1) beyond, both within 2 F32 steps of tanh.
+__device__ __forceinline__ float tanh_any(float x) {
+    return tanhf(x);
+}
+
+// The score (natural units) from scale q.k: capped, less the distance's share.
+__device__ __forceinline__ float row_score(const RowsArgs &a, float s, float slope, uint32_t at, uint32_t j) {
+    if (a.cap > 0.f) s = a.cap * tanh_any(s / a.cap);
+    return fmaf(-slope, (float)(at > j ? at - j : j - at), s);
+}
+
+__device__ __forceinline__ float row_dot(const float *q, const uint16_t *k, uint32_t hd) {
+    float dot = 0.f;
+    for (uint32_t d = 0; d < hd; d++) dot = fmaf(q[d], h2f(k[d]), dot);
+    return dot;
+}
+
+// Row i, q head h over the slots [s0, s1), by one whole wave in f32 products: the
+// scores of 64 slots at a time, a slot per lane, a running maximum and sum, then
+// the lanes take the dims (lane + 64 c in acc[c]). For rows whose sums came out not
+// finite: an infinity in q or K meets the two f16 parts of the matrix-core path
+// as inf - inf or 0 * inf, and one in V the weight 0 of the rows that do not see
+// it. Here an unseen slot is never touched. m is in units of log2.
+template <uint32_t HD>
+__device__ __forceinline__ void row_whole(const RowsArgs &a, uint32_t i, uint32_t h, uint32_t s0, uint32_t s1,
+                                          uint32_t lane, float &m_out, float &l_out, float (&acc)[(HD + 63) / 64]) {
+    const uint32_t kvh = h / (a.nqh / a.nkh);
+    const float *q = a.q + (uint64_t)i * a.q_stride + (uint64_t)h * a.hd;
+    const uint64_t rstride = (uint64_t)a.nkh * a.hd, base = (uint64_t)kvh * a.hd;
+    const float slope = a.slopes ? a.slopes[h] : 0.f;
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (uint32_t c = 0; c < (HD + 63u) / 64u; c++) acc[c] = 0.f;
+    for (uint32_t j0 = s0; j0 < s1; j0 += 64u) {
+        const uint32_t j = j0 + lane;
+        const bool sees = j < s1 && j < row_end(a, i) && row_sees(a, i, j);
+        float y = -INFINITY;
+        if (sees)
+            y = kLog2e * row_score(a, row_dot(q, a.kc + (uint64_t)j * rstride + base, a.hd) * a.scale, slope,
+                                   a.past + i, j);
+        const uint64_t seen = __ballot(sees);
+        if (!seen) continue;
+        // (fmaxf drops a NaN: a NaN score comes through the sum instead)
+        const float mn = fmaxf(m, wave_max(y)), top = mn == -INFINITY ? 0.f : mn;
+        const float r = exp2f(m - top), p = sees ? exp2f(y - top) : 0.f;
+        l = l * r + wave_sum(p);
+        m = mn;
+#pragma unroll
+        for (uint32_t c = 0; c < (HD + 63u) / 64u; c++) {
+            const uint32_t d = 64u * c + lane;
+            float x = acc[c] * r;
+            for (uint32_t t = 0; t < 64u; t++) {
+                const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), (int)t));
+                if ((seen >> t & 1u) && d < a.hd) x = fmaf(w, h2f(a.vc[(uint64_t)(j0 + t) * rstride + base + d]), x);
+            }
+            acc[c] = x;
+        }
+    }
+    m_out = m;
+    l_out = l;
+}
+
+}  // namespace vbs
