@@ -55,7 +55,7 @@ def test_attention_refuses(lib, change, why):
 
 def test_terms_and_mask(lib):
     refused(lib, lib.attention_tree, {**ATT, "mask": 0}, "null")
-    for cap in (-1.0, float("nan"), float("inf")):
+    for cap in (-1.0, float("nan"), float("inf"), 1e-31):
         refused(lib, lib.attention_chunk, {**ATT, "cap": cap}, "cap")
 
 

@@ -874,8 +874,11 @@ int vbs_gfx950_attention_chunk(const float *q, uint32_t q_stride, const uint16_t
     a.q = q, a.q_stride = q_stride, a.kc = kc, a.vc = vc, a.out = out, a.out_stride = out_stride;
     a.n = n, a.past = past, a.nqh = nqh, a.nkh = nkh, a.hd = hd, a.scale = scale, a.max_ctx = max_ctx;
     if (terms) {
-        if (!(terms->cap >= 0.f) || isinf(terms->cap)) return fail("attention_chunk: cap must be 0 or a positive number");
-        a.cap = terms->cap;
+        const float cap = terms->cap;
+        if (!(cap >= 0.f) || isinf(cap) || (cap > 0.f && cap < 1e-30f))
+            return fail("attention_chunk: cap must be 0 or a positive number of at least 1e-30");
+        a.cap = cap;
+        a.rcap = cap > 0.f ? 1.f / cap : 0.f;
         a.slopes = terms->slopes;
         a.docs = terms->docs;
         a.mass = terms->mass;

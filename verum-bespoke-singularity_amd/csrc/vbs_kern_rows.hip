@@ -29,6 +29,7 @@
 // Each range of slots ends in m, l and acc per row; where a kv head's rows are few
 // the slots are split over several workgroups and k_rows_merge adds them up,
 // scaled to the common maximum.
+#include "vbs_lds_dma.h"
 #include "vbs_rows_common.h"
 
 namespace vbs {
@@ -98,7 +99,7 @@ __device__ __forceinline__ void row_parts(const float *row, uint32_t hd, bool wi
     (void)frexpf(top, &e2);  // top < 2^e2
     // (a row below 2^-111 scores nothing that an f32 sum keeps; 2^-sq must stay a number)
     const int sq = top > 0.f && top < INFINITY ? (15 - e2 < 126 ? 15 - e2 : 126) : 0;
-    c = ldexpf(fabsf(scale), -sq);
+    c = fmaxf(ldexpf(fabsf(scale), -sq), 0x1p-126f);  // (not 0: masked scores are -inf times it)
     const float sign = scale < 0.f ? -1.f : 1.f;
 #pragma unroll
     for (uint32_t kk = 0; kk < KK; kk++)
@@ -138,13 +139,32 @@ struct RowsPart {
 template <uint32_t HD>
 constexpr uint32_t kTile = HD > 128u ? 32u : 64u;  // slots per LDS tile
 
+// The place of 16-byte chunk c of row r in an LDS tile of HD-element rows without
+// padding (the DMA writes whole runs): so that the 16 rows of an A operand, and the
+// 16 lanes that share a row of V, lie in different banks.
+template <uint32_t HD>
+__device__ __forceinline__ uint32_t tile_chunk(uint32_t r, uint32_t c) {
+    if constexpr (HD == 96u) {
+        const uint32_t s = c + r % 12u;
+        return r * 12u + (s >= 12u ? s - 12u : s);
+    }
+    return r * (HD / 8u) + (HD >= 128u ? c ^ (r & 15u) : HD == 64u ? c ^ (r & 7u) : c ^ (r >> 2 & 3u));
+}
+// What chunk of a row stands at place s of it (tile_chunk's inverse).
+template <uint32_t HD>
+__device__ __forceinline__ uint32_t tile_place(uint32_t r, uint32_t s) {
+    if constexpr (HD == 96u) return s >= r % 12u ? s - r % 12u : s + 12u - r % 12u;
+    return HD >= 128u ? s ^ (r & 15u) : HD == 64u ? s ^ (r & 7u) : s ^ (r >> 2 & 3u);
+}
+
+static __device__ __align__(16) uint32_t rows_zero[4];  // what dims past head_dim are read as
+
 template <uint32_t HD, uint32_t CT>
 __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsPart pt, uint32_t tiles, bool wide_kv,
                                                  bool wide_q) {
     using P = Pieces<HD>;
     constexpr uint32_t KK = P::KK, W = P::W, T = kTile<HD>, CPR = HD / 8u, NC = T * CPR / 256u;
-    constexpr uint32_t RS = HD * 2u + 16u;  // LDS row stride in bytes: 16 rows' chunks lie in different banks
-    __shared__ __align__(16) uint8_t kl[2][T * RS], vl[2][T * RS];
+    __shared__ __align__(1024) uint8_t kl[2][T * HD * 2u], vl[2][T * HD * 2u];
     __shared__ int32_t dl[2][T];
     const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u, col = lane & 15u, g = lane >> 4;
     const uint32_t kvh = blockIdx.x % a.nkh, rest = blockIdx.x / a.nkh;
@@ -180,30 +200,34 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
     const uint32_t clear = a.docs ? 0u : a.mask ? a.past : row_end(a, tok_first);
     const uint32_t last = active ? row_end(a, tok_last) : 0u;
 
-    // ---- staging: a thread's chunks of a tile, in registers until the tile before is used
+    // ---- staging: tile p0 into buffer b, by LDS DMA (no registers; it arrives by the next wait) or,
+    // where rows are not whole aligned chunks, through registers
     const uint64_t rstride = (uint64_t)a.nkh * a.hd;
     const uint16_t *kb = a.kc + (uint64_t)kvh * a.hd, *vb = a.vc + (uint64_t)kvh * a.hd;
-    ru4 ks[NC], vs[NC];
     int32_t ds = 0;
-    auto fetch = [&](uint32_t p0) {
+    auto fetch = [&](uint32_t p0, uint32_t b) {
 #pragma unroll
         for (uint32_t k = 0; k < NC; k++) {
-            const uint32_t id = t + 256u * k, r = id / CPR, d = 8u * (id % CPR);
+            const uint32_t id = t + 256u * k, r = id / CPR, d = 8u * tile_place<HD>(r, id % CPR);
             // (slots behind the last repeat it: what lies there may be no number)
-            const uint64_t at = (uint64_t)min(p0 + r, slots - 1u) * rstride;
-            ks[k] = cache8(kb + at, d, a.hd, wide_kv);
-            vs[k] = cache8(vb + at, d, a.hd, wide_kv);
+            const uint64_t at = (uint64_t)min(p0 + r, slots - 1u) * rstride + d;
+            if (wide_kv) {
+                const bool in = HD == a.hd || d < a.hd;
+                const uint32_t to = 16u * (256u * k + 64u * wave);
+                dma16(in ? (const void *)(kb + at) : rows_zero, (uint32_t)(uintptr_t)&kl[b][to]);
+                dma16(in ? (const void *)(vb + at) : rows_zero, (uint32_t)(uintptr_t)&vl[b][to]);
+            } else {
+                *reinterpret_cast<ru4 *>(&kl[b][16u * id]) = cache8(kb + at - d, d, a.hd, false);
+                *reinterpret_cast<ru4 *>(&vl[b][16u * id]) = cache8(vb + at - d, d, a.hd, false);
+            }
         }
         if (a.docs && t < T) ds = a.docs[min(p0 + t, slots - 1u)];
     };
-    auto put = [&](uint32_t b) {
-#pragma unroll
-        for (uint32_t k = 0; k < NC; k++) {
-            const uint32_t id = t + 256u * k, at = id / CPR * RS + 16u * (id % CPR);
-            *reinterpret_cast<ru4 *>(&kl[b][at]) = ks[k];
-            *reinterpret_cast<ru4 *>(&vl[b][at]) = vs[k];
-        }
+    // every wave's part of the tile has arrived and every wave is done with the other buffer
+    auto arrive = [&](uint32_t b) {
         if (a.docs && t < T) dl[b][t] = ds;
+        vmcnt_le<0>();
+        __syncthreads();
     };
 
     float m[CT], l[CT];
@@ -227,7 +251,7 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
             rh8 ka[2];
 #pragma unroll
             for (uint32_t hf = 0; hf < 2u; hf++)
-                ka[hf] = *reinterpret_cast<const rh8 *>(&kl[b][(at + 16u * hf + col) * RS + 64u * kk + 16u * g]);
+                ka[hf] = *reinterpret_cast<const rh8 *>(&kl[b][16u * tile_chunk<HD>(at + 16u * hf + col, 4u * kk + g)]);
 #pragma unroll
             for (uint32_t hf = 0; hf < 2u; hf++)
 #pragma unroll
@@ -239,35 +263,70 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
                 for (uint32_t x = 0; x < CT; x++)
                     S[hf][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[hf], ql[x][kk], S[hf][x], 0, 0, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);  // (K's registers are free before V's are taken)
         // the lane's V words: eight slots, in the order of the weights below
         uint32_t vw[8][W];
 #pragma unroll
         for (uint32_t j = 0; j < 8u; j++) {
-            const uint8_t *row = &vl[b][(at + 16u * (j >> 2) + 4u * g + (j & 3u)) * RS];
+            const uint32_t r = at + 16u * (j >> 2) + 4u * g + (j & 3u);
 #pragma unroll
-            for (uint32_t w = 0; w < W; w++) {
-                // (words of one piece are neighbours: the compiler joins the reads)
-                vw[j][w] = *reinterpret_cast<const uint32_t *>(row + 2u * P::dim(w, col));
+            for (uint32_t w = 0; w < W; w++) {  // (words of one piece are neighbours: the compiler joins the reads)
+                const uint32_t d = P::dim(w, col);
+                vw[j][w] = *reinterpret_cast<const uint32_t *>(&vl[b][16u * tile_chunk<HD>(r, d / 8u) + 2u * (d % 8u)]);
             }
         }
-        // y = cm S in units of log2: the plain score, or with what the terms and the mask make of it
+        // the score in units of log2 is cm S: S the plain product, or what the terms make of it
         float cm[CT];
 #pragma unroll
         for (uint32_t x = 0; x < CT; x++) cm[x] = c1[x] * kLog2e;
-        if (!full || terms) {
+        if (terms) {
+            float unit = 1.f;
+            if (a.cap > 0.f) {
+                float far = 0.f;
 #pragma unroll
-            for (uint32_t x = 0; x < CT; x++) {
+                for (uint32_t x = 0; x < CT; x++)
+#pragma unroll
+                    for (uint32_t hf = 0; hf < 2u; hf++) {
+                        S[hf][x] *= c1[x] * a.rcap;
+#pragma unroll
+                        for (uint32_t k = 0; k < 4u; k++) far = fmaxf(far, fabsf(S[hf][x][k]));
+                    }
+                // (most scores lie well below the cap: the polynomial alone then serves the wave)
+                const bool any = __any(far >= kTanhPoly);
+#pragma unroll
+                for (uint32_t x = 0; x < CT; x++)
+#pragma unroll
+                    for (uint32_t j = 0; j < 8u; j++) {
+                        const float s = S[j >> 2][x][j & 3u];
+                        S[j >> 2][x][j & 3u] = any ? tanh_any(s) : tanh_poly(s);
+                    }
+                unit = a.cap;
+            } else {
+#pragma unroll
+                for (uint32_t x = 0; x < CT; x++) S[0][x] *= c1[x], S[1][x] *= c1[x];
+            }
+            if (a.slopes) {
+#pragma unroll
+                for (uint32_t x = 0; x < CT; x++)
+#pragma unroll
+                    for (uint32_t j = 0; j < 8u; j++)
+                        S[j >> 2][x][j & 3u] = row_far(S[j >> 2][x][j & 3u] * unit, slope[x], a.past + tok[x],
+                                                       p0 + 16u * (j >> 2) + 4u * g + (j & 3u));
+                unit = 1.f;
+            }
+#pragma unroll
+            for (uint32_t x = 0; x < CT; x++) cm[x] = unit * kLog2e;
+        }
+        if (!full) {
+#pragma unroll
+            for (uint32_t x = 0; x < CT; x++)
 #pragma unroll
                 for (uint32_t j = 0; j < 8u; j++) {
                     const uint32_t o = 16u * (j >> 2) + 4u * g + (j & 3u);
-                    float s = S[j >> 2][x][j & 3u] * c1[x];
-                    if (terms) s = row_score(a, s, slope[x], a.past + tok[x], p0 + o);
-                    bool sees = full || (vis[x] >> o & 1u);
+                    bool sees = vis[x] >> o & 1u;
                     if (a.docs) sees = sees && dl[b][at + o] == doc[x];
-                    S[j >> 2][x][j & 3u] = sees ? s * kLog2e : -INFINITY;
+                    if (!sees) S[j >> 2][x][j & 3u] = -INFINITY;
                 }
-                cm[x] = 1.f;
-            }
         }
         float top[CT];
         bool up = false;
@@ -320,18 +379,17 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
         }
     };
 
-    fetch(s0);
-    put(0u);
-    __syncthreads();
+    fetch(s0, 0u);
+    arrive(0u);
     for (uint32_t p0 = s0, b = 0; p0 < s1; p0 += T, b ^= 1u) {
         const bool more = p0 + T < s1;
-        if (more) fetch(p0 + T);
+        if (more) fetch(p0 + T, b ^ 1u);
         if (p0 < last) {
             const bool full = p0 + T <= min(clear, s1);
             uint64_t vis[CT];
 #pragma unroll
             for (uint32_t x = 0; x < CT; x++) vis[x] = full ? ~0ull : real[x] ? seen_bits(a, tok[x], p0, s1) : 0ull;
-#pragma unroll
+#pragma unroll 1
             for (uint32_t h = 0; h < T / 32u; h++) {
                 uint32_t v[CT];
 #pragma unroll
@@ -339,10 +397,7 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
                 step(b, 32u * h, p0 + 32u * h, v, full);
             }
         }
-        if (more) {
-            put(b ^ 1u);  // (the buffer of two tiles ago: every wave left it before the last barrier)
-            __syncthreads();
-        }
+        if (more) arrive(b ^ 1u);
     }
     if (!active) return;
 
@@ -446,21 +501,113 @@ __global__ __launch_bounds__(256) void k_rows_merge(RowsArgs a, RowsSplit sp, Ro
 }
 
 // ---- the weights that slots received ---------------------------------------------------
-// A wave per slot and kv head, the lanes over the rows.
-__global__ __launch_bounds__(64) void k_mass(RowsArgs a, const float2 *__restrict__ stats) {
-    const uint32_t lane = threadIdx.x, j = blockIdx.x, kvh = blockIdx.y, group = a.nqh / a.nkh, rows = a.n * group;
-    const uint16_t *k = a.kc + (uint64_t)j * a.nkh * a.hd + (uint64_t)kvh * a.hd;
-    float sum = 0.f;
-    for (uint32_t r = lane; r < rows; r += 64u) {
-        const uint32_t i = r / group, h = kvh * group + r % group;
-        if (j >= row_end(a, i) || !row_sees(a, i, j)) continue;
-        const float s = row_score(a, row_dot(a.q + (uint64_t)i * a.q_stride + (uint64_t)h * a.hd, k, a.hd) * a.scale,
-                                  a.slopes ? a.slopes[h] : 0.f, a.past + i, j);
-        const float2 st = stats[(uint64_t)kvh * rows + r];
-        if (st.y != 0.f) sum += exp2f(s * kLog2e - (st.x == -INFINITY ? 0.f : st.x)) * st.y;
+// A workgroup takes 64 (32 for head_dim above 128) slots of a kv head, their K rows as A operands in registers;
+// its waves take the row tiles of 16 in turn (S^T as above) and each lane adds up
+// 2^(y - m) / l for its slots; the 16 columns, then the waves, are summed at the end
+// in a fixed order. A slot whose sum is not finite is taken again in f32 products.
+constexpr uint32_t kMassWaves = 8;
+
+template <uint32_t HD>
+constexpr uint32_t kMassTiles = HD > 128u ? 2u : 4u;
+
+template <uint32_t HD>
+__global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, const float2 *__restrict__ stats, bool wide_kv,
+                                                          bool wide_q) {
+    constexpr uint32_t KK = HD / 32u, NT = kMassTiles<HD>, NP = 16u * NT;  // tiles of 16 slots; slots
+    __shared__ float sums[kMassWaves][NP];
+    const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u, col = lane & 15u, g = lane >> 4;
+    const uint32_t waves = blockDim.x >> 6, kvh = blockIdx.x % a.nkh, p0 = blockIdx.x / a.nkh * NP;
+    const uint32_t group = a.nqh / a.nkh, rows = a.n * group, slots = a.past + a.n;
+    const uint64_t rstride = (uint64_t)a.nkh * a.hd;
+    rh8 ka[NT][KK];
+    int32_t ds[NT][4];
+#pragma unroll
+    for (uint32_t hf = 0; hf < NT; hf++) {
+        const uint16_t *k = a.kc + (uint64_t)min(p0 + 16u * hf + col, slots - 1u) * rstride + (uint64_t)kvh * a.hd;
+#pragma unroll
+        for (uint32_t kk = 0; kk < KK; kk++)
+            ka[hf][kk] = __builtin_bit_cast(rh8, cache8(k, 32u * kk + 8u * g, a.hd, wide_kv));
+#pragma unroll
+        for (uint32_t r = 0; r < 4u; r++)
+            ds[hf][r] = a.docs ? a.docs[min(p0 + 16u * hf + 4u * g + r, slots - 1u)] : 0;
     }
-    sum = wave_sum(sum);
-    if (lane == 0) a.mass[(uint64_t)kvh * a.max_ctx + j] += sum;
+    float sum[NT][4] = {};
+    const bool terms = a.cap > 0.f || a.slopes;
+    // the rows before the first that sees p0 (without a mask or a prefix beyond it) are left out
+    const uint32_t r0 = a.mask || p0 < a.prefix || p0 <= a.past ? 0u : (p0 - a.past) * group / 16u;
+    for (uint32_t rt = r0 + wave; 16u * rt < rows; rt += waves) {
+        const uint32_t r = 16u * rt + col;
+        const bool real = r < rows;
+        const uint32_t i = real ? r / group : 0u, h = kvh * group + (real ? r % group : 0u);
+        rh8 qh[KK], ql[KK];
+        float c1;
+        const float2 st = real ? stats[(uint64_t)kvh * rows + r] : make_float2(0.f, 0.f);
+        row_parts<KK>(real ? a.q + (uint64_t)i * a.q_stride + (uint64_t)h * a.hd : nullptr, a.hd, wide_q, a.scale, g, qh,
+                      ql, c1);
+        const bool full = !a.docs && 16u * rt + 16u <= rows &&
+                          p0 + NP <= (a.mask ? a.past : row_end(a, 16u * rt / group));
+        const uint64_t vis = full ? ~0ull : real ? seen_bits(a, i, p0, slots) : 0ull;
+        const int32_t doc = a.docs ? a.docs[a.past + i] : 0;
+        const float slope = a.slopes ? a.slopes[h] : 0.f, ms = st.x == -INFINITY ? 0.f : st.x;
+#pragma unroll
+        for (uint32_t hf = 0; hf < NT; hf++) {
+            rf4 S = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (uint32_t kk = 0; kk < KK; kk++) S = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[hf][kk], qh[kk], S, 0, 0, 0);
+#pragma unroll
+            for (uint32_t kk = 0; kk < KK; kk++) S = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[hf][kk], ql[kk], S, 0, 0, 0);
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; k++) {
+                const uint32_t o = 16u * hf + 4u * g + k;
+                float y;
+                if (full && !terms) {
+                    y = fmaf(S[k], c1 * kLog2e, -ms);
+                } else {
+                    float s = S[k] * c1;
+                    if (terms) s = row_score(a, s, slope, a.past + i, p0 + o);
+                    const bool sees = (vis >> o & 1ull) && (!a.docs || ds[hf][k] == doc);
+                    y = sees ? fmaf(s, kLog2e, -ms) : -INFINITY;
+                }
+                sum[hf][k] = fmaf(__builtin_amdgcn_exp2f(y), st.y, sum[hf][k]);
+            }
+        }
+    }
+    // the 16 columns: each lane group's row of 16 lanes
+#pragma unroll
+    for (uint32_t hf = 0; hf < NT; hf++)
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; k++) {
+            float v = sum[hf][k];
+            v += bfly_partner<8>(v, lane);
+            v += bfly_partner<4>(v, lane);
+            v += bfly_partner<2>(v, lane);
+            v += bfly_partner<1>(v, lane);
+            if (col == 0) sums[wave][16u * hf + 4u * g + k] = v;
+        }
+    __syncthreads();
+    if (wave) return;
+    const uint32_t j = p0 + lane;
+    const bool in = lane < NP && j < slots;
+    float v = 0.f;
+    for (uint32_t w = 0; w < waves; w++) v += sums[w][lane % NP];
+    const uint64_t bad = __ballot(in && v * 0.f != 0.f);
+    for (uint32_t c = 0; c < 64u && bad >> c; c++) {
+        if (!(bad >> c & 1ull)) continue;
+        const uint32_t jj = p0 + c;
+        const uint16_t *k = a.kc + (uint64_t)jj * rstride + (uint64_t)kvh * a.hd;
+        float whole = 0.f;
+        for (uint32_t r = lane; r < rows; r += 64u) {
+            const uint32_t i = r / group, h = kvh * group + r % group;
+            if (jj >= row_end(a, i) || !row_sees(a, i, jj)) continue;
+            const float s = row_score(a, row_dot(a.q + (uint64_t)i * a.q_stride + (uint64_t)h * a.hd, k, a.hd) * a.scale,
+                                      a.slopes ? a.slopes[h] : 0.f, a.past + i, jj);
+            const float2 st = stats[(uint64_t)kvh * rows + r];
+            whole += exp2f(fmaf(s, kLog2e, -(st.x == -INFINITY ? 0.f : st.x))) * st.y;
+        }
+        whole = wave_sum(whole);
+        if (lane == c) v = whole;
+    }
+    if (in) a.mass[(uint64_t)kvh * a.max_ctx + j] += v;
 }
 
 // ---- launches -------------------------------------------------------------------------------
@@ -498,10 +645,17 @@ size_t rows_scratch_bytes(const RowsArgs &a) {
     return p.ml + p.acc + p.stats;
 }
 
+// Whether rows of the caches and of q may be read 16 bytes at a time.
+static bool rows_wide_kv(const RowsArgs &a) {
+    return a.hd % 8u == 0 && (((uintptr_t)a.kc | (uintptr_t)a.vc) & 15u) == 0;
+}
+static bool rows_wide_q(const RowsArgs &a) {
+    return a.hd % 8u == 0 && a.q_stride % 4u == 0 && ((uintptr_t)a.q & 15u) == 0;
+}
+
 template <uint32_t HD>
 static void start_rows(const RowsArgs &a, const RowsPlan &p, const RowsPart &pt, hipStream_t s) {
-    const bool wide_kv = a.hd % 8u == 0 && (((uintptr_t)a.kc | (uintptr_t)a.vc) & 15u) == 0;
-    const bool wide_q = a.hd % 8u == 0 && a.q_stride % 4u == 0 && ((uintptr_t)a.q & 15u) == 0;
+    const bool wide_kv = rows_wide_kv(a), wide_q = rows_wide_q(a);
     const uint32_t grid = p.tiles * p.sp.n * a.nkh;
     if constexpr (HD <= 128u) {
         if (p.ct == 2u) {
@@ -510,6 +664,14 @@ static void start_rows(const RowsArgs &a, const RowsPlan &p, const RowsPart &pt,
         }
     }
     k_rows<HD, 1><<<grid, 256, 0, s>>>(a, p.sp, pt, p.tiles, wide_kv, wide_q);
+}
+
+template <uint32_t HD>
+static void start_mass(const RowsArgs &a, const RowsPart &pt, hipStream_t s) {
+    const uint32_t tiles = (a.n * (a.nqh / a.nkh) + 15u) / 16u;
+    const uint32_t np = 16u * kMassTiles<HD>;
+    k_mass<HD><<<(a.past + a.n + np - 1u) / np * a.nkh, 64u * (tiles < kMassWaves ? tiles : kMassWaves), 0, s>>>(
+        a, pt.stats, rows_wide_kv(a), rows_wide_q(a));
 }
 
 hipError_t launch_rows(const RowsArgs &a, void *scratch, hipStream_t s) {
@@ -532,7 +694,13 @@ hipError_t launch_rows(const RowsArgs &a, void *scratch, hipStream_t s) {
         e = hipGetLastError();
     }
     if (e == hipSuccess && a.mass) {
-        k_mass<<<dim3(a.past + a.n, a.nkh), 64, 0, s>>>(a, pt.stats);
+        switch (p.hd) {
+            case 32: start_mass<32>(a, pt, s); break;
+            case 64: start_mass<64>(a, pt, s); break;
+            case 96: start_mass<96>(a, pt, s); break;
+            case 128: start_mass<128>(a, pt, s); break;
+            default: start_mass<256>(a, pt, s); break;
+        }
         e = hipGetLastError();
     }
     return e;

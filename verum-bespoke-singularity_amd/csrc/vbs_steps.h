@@ -42,7 +42,7 @@ struct RowsArgs {
     float scale;
     const uint64_t *mask;
     uint32_t words;
-    float cap;            // 0: none
+    float cap, rcap;      // 0: none; 1 / cap
     const float *slopes;  // NULL: none
     const int32_t *docs;  // NULL: none
     uint32_t prefix;
