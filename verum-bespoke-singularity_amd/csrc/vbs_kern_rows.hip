@@ -24,8 +24,7 @@
 //   log2: then the sums are rescaled. The weights are 2^(y - m + 7) <= 2^15, so that
 //   small ones keep their low part in f16.
 // * O^T += V^T P^T: B = P^T, the lane's own weights (hi, then lo), A = V^T with the
-//   k slots in the same order, its rows the head dims dim_of (below), so that a
-//   lane's V dims are neighbours in memory and two permutes pair its slots.
+//   k slots in the same order, by transposed LDS reads.
 // Each range of slots ends in m, l and acc per row; where a kv head's rows are few
 // the slots are split over several workgroups and k_rows_merge adds them up,
 // scaled to the common maximum.
@@ -34,22 +33,19 @@
 
 namespace vbs {
 
-// Where a lane's V words lie: HD is cut into pieces of 128, 64 and 32 dims; in a
-// piece of 16 D dims, lane column m (of 16) owns dims D m .. D m + D - 1.
-template <uint32_t HD>
-struct Pieces {
-    static constexpr uint32_t KK = HD / 32u, W = HD / 32u;  // K slices; V words (two dims) per lane
-    // the first dim, for lane column m, of word w
-    __host__ __device__ static constexpr uint32_t dim(uint32_t w, uint32_t m) {
-        const uint32_t n128 = HD / 128u, rest = HD % 128u;
-        if (w < 4u * n128) return 128u * (w / 4u) + 8u * m + 2u * (w % 4u);
-        const uint32_t b = 128u * n128, v = w - 4u * n128;
-        if (rest >= 64u && v < 2u) return b + 4u * m + 2u * v;
-        return b + (rest >= 64u ? 64u : 0u) + 2u * m;
-    }
-};
-
 constexpr float kLazy = 8.f, kLift = 7.f;  // log2: how far a score may pass m; the weights' scale
+
+// p - h[0] and p - h[1], the halves widened on the way (exact: h is p rounded).
+__device__ __forceinline__ float less_low(float p, rh2 h) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(p));
+    return r;
+}
+__device__ __forceinline__ float less_high(float p, rh2 h) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(p));
+    return r;
+}
 
 __device__ __forceinline__ uint64_t ones_below(int64_t x) {
     return x <= 0 ? 0ull : x >= 64 ? ~0ull : (1ull << x) - 1ull;
@@ -140,31 +136,40 @@ template <uint32_t HD>
 constexpr uint32_t kTile = HD > 128u ? 32u : 64u;  // slots per LDS tile
 
 // The place of 16-byte chunk c of row r in an LDS tile of HD-element rows without
-// padding (the DMA writes whole runs): so that the 16 rows of an A operand, and the
-// 16 lanes that share a row of V, lie in different banks.
+// padding (the DMA writes whole runs): so that the rows of an A operand of K (eight
+// at a time) and the 32-byte runs of four rows that a transposed read of V takes lie
+// in different banks. It goes by the row's last three bits alone.
 template <uint32_t HD>
-__device__ __forceinline__ uint32_t tile_chunk(uint32_t r, uint32_t c) {
+__device__ __forceinline__ uint32_t tile_place(uint32_t r, uint32_t c) {
     if constexpr (HD == 96u) {
-        const uint32_t s = c + r % 12u;
-        return r * 12u + (s >= 12u ? s - 12u : s);
+        const uint32_t s = c + 2u * (r >> 2 & 1u);
+        return s >= 12u ? s - 12u : s;
     }
-    return r * (HD / 8u) + (HD >= 128u ? c ^ (r & 15u) : HD == 64u ? c ^ (r & 7u) : c ^ (r >> 2 & 3u));
+    return c ^ 2u * (HD >= 128u ? r & 7u : HD == 64u ? r >> 1 & 3u : r >> 2 & 1u);
 }
-// What chunk of a row stands at place s of it (tile_chunk's inverse).
+// The chunk at place s of row r.
 template <uint32_t HD>
-__device__ __forceinline__ uint32_t tile_place(uint32_t r, uint32_t s) {
-    if constexpr (HD == 96u) return s >= r % 12u ? s - r % 12u : s + 12u - r % 12u;
-    return HD >= 128u ? s ^ (r & 15u) : HD == 64u ? s ^ (r & 7u) : s ^ (r >> 2 & 3u);
+__device__ __forceinline__ uint32_t tile_chunk(uint32_t r, uint32_t s) {
+    if constexpr (HD == 96u) {
+        const uint32_t o = 2u * (r >> 2 & 1u);
+        return s >= o ? s - o : s + 12u - o;
+    }
+    return tile_place<HD>(r, s);
 }
 
-static __device__ __align__(16) uint32_t rows_zero[4];  // what dims past head_dim are read as
+// Four 16-bit elements a lane, transposed within each 16 lanes: lane i receives
+// element i % 4 of what the lanes 4 e + i / 4 address, e = 0 .. 3.
+typedef short rs4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ rs4 lds_transposed(const uint8_t *p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) rs4 *)(uint32_t)(uintptr_t)p);
+}
 
 template <uint32_t HD, uint32_t CT>
 __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsPart pt, uint32_t tiles, bool wide_kv,
                                                  bool wide_q) {
-    using P = Pieces<HD>;
-    constexpr uint32_t KK = P::KK, W = P::W, T = kTile<HD>, CPR = HD / 8u, NC = T * CPR / 256u;
-    __shared__ __align__(1024) uint8_t kl[2][T * HD * 2u], vl[2][T * HD * 2u];
+    constexpr uint32_t KK = HD / 32u, DT = HD / 16u, T = kTile<HD>, CPR = HD / 8u, NC = T * CPR / 256u;
+    constexpr uint32_t RB = HD * 2u, TB = T * RB;  // bytes of a row and of a tile
+    __shared__ __align__(1024) uint8_t kv[2][2][TB];  // two buffers of K and V
     __shared__ int32_t dl[2][T];
     const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u, col = lane & 15u, g = lane >> 4;
     const uint32_t kvh = blockIdx.x % a.nkh, rest = blockIdx.x / a.nkh;
@@ -205,20 +210,36 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
     const uint64_t rstride = (uint64_t)a.nkh * a.hd;
     const uint16_t *kb = a.kc + (uint64_t)kvh * a.hd, *vb = a.vc + (uint64_t)kvh * a.hd;
     int32_t ds = 0;
-    auto fetch = [&](uint32_t p0, uint32_t b) {
+    uint32_t from[NC];  // a thread's chunks: bytes from the tile's first row
+    bool in[NC];        // (dims past head_dim stay 0)
 #pragma unroll
-        for (uint32_t k = 0; k < NC; k++) {
-            const uint32_t id = t + 256u * k, r = id / CPR, d = 8u * tile_place<HD>(r, id % CPR);
-            // (slots behind the last repeat it: what lies there may be no number)
-            const uint64_t at = (uint64_t)min(p0 + r, slots - 1u) * rstride + d;
-            if (wide_kv) {
-                const bool in = HD == a.hd || d < a.hd;
+    for (uint32_t k = 0; k < NC; k++) {
+        const uint32_t id = t + 256u * k, r = id / CPR, d = 8u * tile_chunk<HD>(r, id % CPR);
+        from[k] = (uint32_t)(2u * (r * rstride + d));
+        in[k] = d < a.hd;
+        if (!in[k])
+#pragma unroll
+            for (uint32_t b = 0; b < 4u; b++) *reinterpret_cast<ru4 *>(&kv[b >> 1][b & 1u][16u * id]) = ru4{0u, 0u, 0u, 0u};
+    }
+    auto fetch = [&](uint32_t p0, uint32_t b) {
+        if (wide_kv && p0 + T <= slots) {
+            const uint16_t *kp = kb + p0 * rstride, *vp = vb + p0 * rstride;
+#pragma unroll
+            for (uint32_t k = 0; k < NC; k++) {
                 const uint32_t to = 16u * (256u * k + 64u * wave);
-                dma16(in ? (const void *)(kb + at) : rows_zero, (uint32_t)(uintptr_t)&kl[b][to]);
-                dma16(in ? (const void *)(vb + at) : rows_zero, (uint32_t)(uintptr_t)&vl[b][to]);
-            } else {
-                *reinterpret_cast<ru4 *>(&kl[b][16u * id]) = cache8(kb + at - d, d, a.hd, false);
-                *reinterpret_cast<ru4 *>(&vl[b][16u * id]) = cache8(vb + at - d, d, a.hd, false);
+                if (HD == a.hd || in[k]) {
+                    dma16s(kp, from[k], (uint32_t)(uintptr_t)&kv[b][0][to]);
+                    dma16s(vp, from[k], (uint32_t)(uintptr_t)&kv[b][1][to]);
+                }
+            }
+        } else {
+#pragma unroll 1
+            for (uint32_t k = 0; k < NC; k++) {
+                const uint32_t id = t + 256u * k, r = id / CPR, d = 8u * tile_chunk<HD>(r, id % CPR);
+                // (slots behind the last repeat it: what lies there may be no number)
+                const uint64_t at = (uint64_t)min(p0 + r, slots - 1u) * rstride;
+                *reinterpret_cast<ru4 *>(&kv[b][0][16u * id]) = cache8(kb + at, d, a.hd, wide_kv);
+                *reinterpret_cast<ru4 *>(&kv[b][1][16u * id]) = cache8(vb + at, d, a.hd, wide_kv);
             }
         }
         if (a.docs && t < T) ds = a.docs[min(p0 + t, slots - 1u)];
@@ -229,17 +250,29 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
         vmcnt_le<0>();
         __syncthreads();
     };
+    // where the lane reads: its chunk of K per slice (row `col` of a 16-row tile), and per 16 dims its part of
+    // the transposed V read: slot 4 g + col / 4, dims 4 (col % 4) ..
+    constexpr uint32_t NV = DT < 8u ? DT : 8u;  // (dims from 128 on lie 256 bytes on)
+    uint32_t kat[KK < 4u ? KK : 4u], vat[NV];
+#pragma unroll
+    for (uint32_t kk = 0; kk < KK && kk < 4u; kk++) kat[kk] = col * RB + 16u * tile_place<HD>(col, 4u * kk + g);
+#pragma unroll
+    for (uint32_t d = 0; d < NV; d++) {
+        const uint32_t r = 4u * g + (col >> 2);
+        vat[d] = TB + r * RB + 16u * tile_place<HD>(r, 2u * d + (col >> 1 & 1u)) + 8u * (col & 1u);
+    }
 
     float m[CT], l[CT];
-    rf4 acc[2u * W][CT];
+    rf4 acc[DT][CT];
 #pragma unroll
     for (uint32_t x = 0; x < CT; x++) {
         m[x] = -INFINITY, l[x] = 0.f;
 #pragma unroll
-        for (uint32_t d = 0; d < 2u * W; d++) acc[d][x] = rf4{0.f, 0.f, 0.f, 0.f};
+        for (uint32_t d = 0; d < DT; d++) acc[d][x] = rf4{0.f, 0.f, 0.f, 0.f};
     }
 
     // 32 slots from p0 on, in LDS buffer b at row `at`; vis: their bits per column tile
+    const uint8_t *const lds = &kv[0][0][0];
     auto step = [&](uint32_t b, uint32_t at, uint32_t p0, const uint32_t (&vis)[CT], bool full) {
         rf4 S[2][CT];
 #pragma unroll
@@ -251,7 +284,7 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
             rh8 ka[2];
 #pragma unroll
             for (uint32_t hf = 0; hf < 2u; hf++)
-                ka[hf] = *reinterpret_cast<const rh8 *>(&kl[b][16u * tile_chunk<HD>(at + 16u * hf + col, 4u * kk + g)]);
+                ka[hf] = *reinterpret_cast<const rh8 *>(lds + kat[kk & 3u] + 256u * (kk >> 2) + (at + 16u * hf) * RB);
 #pragma unroll
             for (uint32_t hf = 0; hf < 2u; hf++)
 #pragma unroll
@@ -262,18 +295,6 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
 #pragma unroll
                 for (uint32_t x = 0; x < CT; x++)
                     S[hf][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[hf], ql[x][kk], S[hf][x], 0, 0, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);  // (K's registers are free before V's are taken)
-        // the lane's V words: eight slots, in the order of the weights below
-        uint32_t vw[8][W];
-#pragma unroll
-        for (uint32_t j = 0; j < 8u; j++) {
-            const uint32_t r = at + 16u * (j >> 2) + 4u * g + (j & 3u);
-#pragma unroll
-            for (uint32_t w = 0; w < W; w++) {  // (words of one piece are neighbours: the compiler joins the reads)
-                const uint32_t d = P::dim(w, col);
-                vw[j][w] = *reinterpret_cast<const uint32_t *>(&vl[b][16u * tile_chunk<HD>(r, d / 8u) + 2u * (d % 8u)]);
-            }
         }
         // the score in units of log2 is cm S: S the plain product, or what the terms make of it
         float cm[CT];
@@ -292,14 +313,17 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
                         for (uint32_t k = 0; k < 4u; k++) far = fmaxf(far, fabsf(S[hf][x][k]));
                     }
                 // (most scores lie well below the cap: the polynomial alone then serves the wave)
-                const bool any = __any(far >= kTanhPoly);
+                if (__any(far >= kTanhPoly)) {
 #pragma unroll
-                for (uint32_t x = 0; x < CT; x++)
+                    for (uint32_t x = 0; x < CT; x++)
 #pragma unroll
-                    for (uint32_t j = 0; j < 8u; j++) {
-                        const float s = S[j >> 2][x][j & 3u];
-                        S[j >> 2][x][j & 3u] = any ? tanh_any(s) : tanh_poly(s);
-                    }
+                        for (uint32_t j = 0; j < 8u; j++) S[j >> 2][x][j & 3u] = tanh_any(S[j >> 2][x][j & 3u]);
+                } else {
+#pragma unroll
+                    for (uint32_t x = 0; x < CT; x++)
+#pragma unroll
+                        for (uint32_t j = 0; j < 8u; j++) S[j >> 2][x][j & 3u] = tanh_poly(S[j >> 2][x][j & 3u]);
+                }
                 unit = a.cap;
             } else {
 #pragma unroll
@@ -348,7 +372,7 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
                 m[x] = mn;
                 l[x] *= f;
 #pragma unroll
-                for (uint32_t d = 0; d < 2u * W; d++) acc[d][x] *= f;
+                for (uint32_t d = 0; d < DT; d++) acc[d][x] *= f;
             }
         }
         rh8 ph[CT], pl[CT];
@@ -356,26 +380,28 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
         for (uint32_t x = 0; x < CT; x++) {
             const float ms = m[x] == -INFINITY ? 0.f : m[x] - kLift;
 #pragma unroll
-            for (uint32_t j = 0; j < 8u; j++) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(S[j >> 2][x][j & 3u], cm[x], -ms));
-                l[x] += p;
-                const _Float16 h = (_Float16)p;
-                ph[x][j] = h;
-                pl[x][j] = (_Float16)(p - (float)h);
+            for (uint32_t j = 0; j < 8u; j += 2u) {
+                rf2 p;
+                p[0] = __builtin_amdgcn_exp2f(fmaf(S[j >> 2][x][j & 3u], cm[x], -ms));
+                p[1] = __builtin_amdgcn_exp2f(fmaf(S[j >> 2][x][(j & 3u) + 1u], cm[x], -ms));
+                l[x] += p[0];
+                l[x] += p[1];
+                const rh2 h = __builtin_convertvector(p, rh2);
+                const rf2 r = {less_low(p[0], h), less_high(p[1], h)};
+                const rh2 q = __builtin_convertvector(r, rh2);
+                ph[x][j] = h[0], ph[x][j + 1u] = h[1];
+                pl[x][j] = q[0], pl[x][j + 1u] = q[1];
             }
         }
 #pragma unroll
-        for (uint32_t d = 0; d < 2u * W; d++) {
-            const uint32_t sel = d & 1u ? 0x07060302u : 0x05040100u;
-            ru4 va;
+        for (uint32_t d = 0; d < DT; d++) {
+            const uint8_t *v = lds + vat[d & 7u] + 256u * (d >> 3) + at * RB;
+            const rs4 v0 = lds_transposed(v), v1 = lds_transposed(v + 16u * RB);
+            const rh8 va = __builtin_bit_cast(rh8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-            for (uint32_t j = 0; j < 4u; j++) va[j] = __builtin_amdgcn_perm(vw[2u * j + 1u][d >> 1], vw[2u * j][d >> 1], sel);
+            for (uint32_t x = 0; x < CT; x++) acc[d][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[x], acc[d][x], 0, 0, 0);
 #pragma unroll
-            for (uint32_t x = 0; x < CT; x++)
-                acc[d][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(rh8, va), ph[x], acc[d][x], 0, 0, 0);
-#pragma unroll
-            for (uint32_t x = 0; x < CT; x++)
-                acc[d][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(rh8, va), pl[x], acc[d][x], 0, 0, 0);
+            for (uint32_t x = 0; x < CT; x++) acc[d][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[x], acc[d][x], 0, 0, 0);
         }
     };
 
@@ -389,7 +415,7 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
             uint64_t vis[CT];
 #pragma unroll
             for (uint32_t x = 0; x < CT; x++) vis[x] = full ? ~0ull : real[x] ? seen_bits(a, tok[x], p0, s1) : 0ull;
-#pragma unroll 1
+#pragma unroll
             for (uint32_t h = 0; h < T / 32u; h++) {
                 uint32_t v[CT];
 #pragma unroll
@@ -398,11 +424,17 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
             }
         }
         if (more) arrive(b ^ 1u);
+        const uint32_t on = b ? 0u - 2u * TB : 2u * TB;  // (the other buffer)
+#pragma unroll
+        for (uint32_t kk = 0; kk < KK && kk < 4u; kk++) kat[kk] += on;
+#pragma unroll
+        for (uint32_t d = 0; d < NV; d++) vat[d] += on;
     }
     if (!active) return;
 
     // ---- the rows' sums: l over the four lane groups, then out (one range) or the partials
     const uint64_t first = ((uint64_t)kvh * sp.n + split) * rows;
+    const bool wide_to = a.hd % 4u == 0 && (sp.n > 1u || (a.out_stride % 4u == 0 && ((uintptr_t)a.out & 15u) == 0));
 #pragma unroll
     for (uint32_t x = 0; x < CT; x++) {
         l[x] += lane_xor<16>(l[x]);
@@ -410,7 +442,7 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
         const uint32_t r = row0 + 16u * x + col, h = kvh * group + r % group;
         float nan = l[x] * 0.f;
 #pragma unroll
-        for (uint32_t d = 0; d < 2u * W; d++)
+        for (uint32_t d = 0; d < DT; d++)
 #pragma unroll
             for (uint32_t k = 0; k < 4u; k++) nan = fmaf(acc[d][x][k], 0.f, nan);
         const uint64_t bad = __ballot(real[x] && nan != 0.f);  // (0 times anything finite is 0)
@@ -421,15 +453,16 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
             float *to = sp.n > 1u ? pt.acc + (first + r) * a.hd
                                   : a.out + (uint64_t)tok[x] * a.out_stride + (uint64_t)h * a.hd;
 #pragma unroll
-            for (uint32_t w = 0; w < W; w++)
+            for (uint32_t d = 0; d < DT; d++) {
+                const uint32_t d0 = 16u * d + 4u * g;
+                if (wide_to && d0 < a.hd) {
+                    *reinterpret_cast<rf4 *>(to + d0) = acc[d][x] * inv;
+                } else if (!wide_to) {
 #pragma unroll
-                for (uint32_t k = 0; k < 4u; k++) {
-                    const uint32_t d = P::dim(w, 4u * g + k);
-                    if (d < a.hd) {
-                        to[d] = acc[2u * w][x][k] * inv;
-                        to[d + 1u] = acc[2u * w + 1u][x][k] * inv;
-                    }
+                    for (uint32_t k = 0; k < 4u; k++)
+                        if (d0 + k < a.hd) to[d0 + k] = acc[d][x][k] * inv;
                 }
+            }
             if (g == 0 && sp.n > 1u) pt.ml[first + r] = make_float2(mo, l[x]);
             if (g == 0 && sp.n == 1u && pt.stats) pt.stats[(uint64_t)kvh * rows + r] = make_float2(mo, l[x] == 0.f ? 0.f : __fdiv_rn(1.f, l[x]));
         }

@@ -11,6 +11,8 @@ namespace vbs {
 constexpr float kLog2e = 1.44269504088896341f;
 
 typedef _Float16 rh8 __attribute__((ext_vector_type(8)));
+typedef _Float16 rh2 __attribute__((ext_vector_type(2)));
+typedef float rf2 __attribute__((ext_vector_type(2)));
 typedef float rf4 __attribute__((ext_vector_type(4)));
 typedef uint32_t ru4 __attribute__((ext_vector_type(4)));
 
