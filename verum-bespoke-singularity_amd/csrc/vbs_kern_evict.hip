@@ -19,7 +19,8 @@
 
 namespace vbs {
 
-constexpr uint32_t kSelThreads = 1024, kSelWaves = kSelThreads / 64;
+constexpr uint32_t kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelBins = 2048;
+constexpr uint32_t kSelKeys = 8, kSelRun = kSelThreads * kSelKeys;  // slots a thread and a workgroup hold at once
 
 // The order of weights as unsigned numbers: -0 as 0, NaN below everything.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -28,8 +29,29 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
+// Inclusive sum over the lanes up to each.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t lane) {
+#pragma unroll
+    for (uint32_t o = 1; o < 64u; o <<= 1) {
+        const uint32_t x = __shfl_up(v, o, 64);
+        if (lane >= o) v += x;
+    }
+    return v;
+}
+// The sum of the waves' entries before `wave`, and of all.
+__device__ __forceinline__ uint2 waves_before(const uint32_t *waves, uint32_t wave) {
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (uint32_t v = 0; v < kSelWaves; v++) {
+        const uint32_t x = waves[v];
+        if (v < wave) before += x;
+        all += x;
+    }
+    return make_uint2(before, all);
+}
+
 __global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
-    __shared__ uint32_t hist[256], waves[2][kSelWaves], s_prefix, s_need;
+    __shared__ uint32_t hist[kSelBins], waves[2][kSelWaves], s_bin, s_need, s_count;
     const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u, h = blockIdx.x, l = blockIdx.y;
     const float *mass = a.mass + ((uint64_t)l * a.nkh + h) * a.max_ctx;
     float *mass_out = a.mass_out ? a.mass_out + ((uint64_t)l * a.nkh + h) * a.max_ctx : nullptr;
@@ -37,109 +59,160 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
     const uint32_t lo = a.first, hi = a.len - a.last;  // the slots that are chosen among
     uint32_t need = a.budget - a.first - a.last;       // as many of them
 
-    // the key of the need-th greatest, eight bits a pass; `need` becomes how many of
-    // that key are taken
-    uint32_t prefix = 0;
-    if (need > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (t < 256u) hist[t] = 0;
-            __syncthreads();
-            for (uint32_t j = lo + t; j < hi; j += kSelThreads) {
-                const uint32_t key = weight_key(mass[j]);
-                if (shift == 24 || key >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&hist[key >> shift & 255u], 1u);
-            }
-            __syncthreads();
-            if (t == 0) {
-                uint32_t b = 255u, n = need;
-                while (b > 0u && hist[b] < n) n -= hist[b--];
-                s_prefix = prefix | b << shift;
-                s_need = n;
-            }
-            __syncthreads();
-            prefix = s_prefix;
-            need = s_need;
-        }
-    }
-    const bool any = a.budget > a.first + a.last;
+    // a run of kSelRun slots in registers, 64 kSelKeys in a row to each wave; the weights stay
+    // there if one run holds them all
+    const uint32_t runs = (a.len + kSelRun - 1u) / kSelRun;
+    float w[kSelKeys];
+    auto slot = [&](uint32_t run, uint32_t k) { return run * kSelRun + (wave * kSelKeys + k) * 64u + lane; };
+    auto load = [&](uint32_t run) {
+#pragma unroll
+        for (uint32_t k = 0; k < kSelKeys; k++) w[k] = slot(run, k) < a.len ? mass[slot(run, k)] : 0.f;
+    };
+    load(0u);
 
-    // one ordered pass: ties of the last key in slot order, kept slots in slot order
+    // the first bits of the key of the need-th greatest, up to 11 a pass: every key with
+    // greater bits is kept, and `need` of those that share them (all, once `whole`)
+    uint32_t prefix = 0, bits = 0;
+    bool whole = false;
+    for (uint32_t pass = 0; pass < 3u && need > 0u && !whole; pass++) {
+        const uint32_t width = pass < 2u ? 11u : 10u, shift = 32u - bits - width;
+        for (uint32_t i = t; i < kSelBins; i += kSelThreads) hist[i] = 0;
+        __syncthreads();
+        for (uint32_t run = 0; run < runs; run++) {
+            if (runs > 1u) load(run);
+#pragma unroll
+            for (uint32_t k = 0; k < kSelKeys; k++) {
+                const uint32_t j = slot(run, k), key = weight_key(w[k]);
+                if (j >= lo && j < hi && (bits == 0u || key >> (32u - bits) == prefix))
+                    atomicAdd(&hist[key >> shift & ((1u << width) - 1u)], 1u);
+            }
+        }
+        __syncthreads();
+        // thread t takes the bins 2 t and 2 t + 1 counted from the greatest
+        const uint32_t top = kSelBins - 1u - 2u * t, n0 = hist[top], n1 = hist[top - 1u];
+        const uint32_t sum = wave_scan(n0 + n1, lane);
+        if (lane == 63u) waves[0][wave] = sum;
+        __syncthreads();
+        const uint32_t before = waves_before(waves[0], wave).x + sum - n0 - n1;
+        if (before < need && need <= before + n0 + n1) {  // (one thread)
+            const bool first = need <= before + n0;
+            s_bin = first ? top : top - 1u;
+            s_need = need - before - (first ? 0u : n0);
+            s_count = first ? n0 : n1;
+        }
+        __syncthreads();
+        prefix = prefix << width | s_bin;
+        bits += width;
+        need = s_need;
+        whole = need == s_count;
+    }
+    const bool any = bits > 0u;
+    const uint32_t down = 32u - bits;
+
+    // ordered passes over the runs: ties of the last key in slot order, kept slots in slot order
     uint32_t ties0 = 0, kept0 = 0;
-    for (uint32_t j0 = 0; j0 < a.len; j0 += kSelThreads) {
-        const uint32_t j = j0 + t;
-        const float w = j < a.len ? mass[j] : 0.f;
-        const uint32_t key = weight_key(w);
-        const bool open = j >= lo && j < hi, tie = any && open && key == prefix;
-        const uint64_t tb = __ballot(tie), below = (1ull << lane) - 1ull;
-        if (lane == 0) waves[0][wave] = (uint32_t)__popcll(tb);
-        __syncthreads();
-        uint32_t before = ties0;
-        for (uint32_t v = 0; v < kSelWaves; v++) {
-            if (v < wave) before += waves[0][v];
-            ties0 += waves[0][v];
+    for (uint32_t run = 0; run < runs; run++) {
+        if (runs > 1u) load(run);  // (what earlier runs wrote lies below this run's slots)
+        uint32_t tie = 0, keep = 0, n = 0;  // bits per key; the wave's count
+#pragma unroll
+        for (uint32_t k = 0; k < kSelKeys; k++) {
+            const uint32_t j = slot(run, k), head = any ? weight_key(w[k]) >> down : 0u;
+            const bool open = j >= lo && j < hi;
+            if (any && open && head == prefix) tie |= 1u << k;
+            if (j < a.len && (!open || (any && head > prefix))) keep |= 1u << k;
         }
-        before += (uint32_t)__popcll(tb & below);
-        const bool keep = j < a.len && (!open || (any && (key > prefix || (tie && before < need))));
-        const uint64_t kb = __ballot(keep);
-        if (lane == 0) waves[1][wave] = (uint32_t)__popcll(kb);
-        __syncthreads();
-        uint32_t at = kept0;
-        for (uint32_t v = 0; v < kSelWaves; v++) {
-            if (v < wave) at += waves[1][v];
-            kept0 += waves[1][v];
+        if (whole) {
+            keep |= tie;
+        } else if (any) {
+#pragma unroll
+            for (uint32_t k = 0; k < kSelKeys; k++) n += (uint32_t)__popcll(__ballot(tie >> k & 1u));
+            if (lane == 0) waves[0][wave] = n;
+            __syncthreads();
+            const uint2 b = waves_before(waves[0], wave);
+            uint32_t at = ties0 + b.x;
+            ties0 += b.y;
+#pragma unroll
+            for (uint32_t k = 0; k < kSelKeys; k++) {
+                const uint64_t m = __ballot(tie >> k & 1u);
+                if ((tie >> k & 1u) && at + (uint32_t)__popcll(m & ((1ull << lane) - 1ull)) < need) keep |= 1u << k;
+                at += (uint32_t)__popcll(m);
+            }
         }
-        at += (uint32_t)__popcll(kb & below);
-        if (keep) {
-            kept[at] = j;
-            if (mass_out) mass_out[at] = w;  // (at <= j: read above, or by an earlier pass)
+        n = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < kSelKeys; k++) n += (uint32_t)__popcll(__ballot(keep >> k & 1u));
+        if (lane == 0) waves[1][wave] = n;
+        __syncthreads();  // (every weight of this run is in a register)
+        const uint2 b = waves_before(waves[1], wave);
+        uint32_t at = kept0 + b.x;
+        kept0 += b.y;
+#pragma unroll
+        for (uint32_t k = 0; k < kSelKeys; k++) {
+            const uint64_t m = __ballot(keep >> k & 1u);
+            if (keep >> k & 1u) {
+                const uint32_t to = at + (uint32_t)__popcll(m & ((1ull << lane) - 1ull));
+                kept[to] = slot(run, k);
+                if (mass_out) mass_out[to] = w[k];  // (to <= the slot)
+            }
+            at += (uint32_t)__popcll(m);
         }
+        if (runs > 1u) __syncthreads();  // (the counts are read before the next run's)
     }
     __syncthreads();
     if (mass_out)
         for (uint32_t j = a.budget + t; j < a.len; j += kSelThreads) mass_out[j] = 0.f;
 }
 
-// A slice: `lanes` units of type U of one head's rows. Threads: (row, unit).
-constexpr uint32_t kMoveThreads = 512, kMoveDepth = 4;
+// A slice: `lanes` units of type U of one head's rows, of K or of V. Threads: (row, unit).
+// Workgroups whose slices share rows follow each other by the number of XCDs, so
+// that they run on one, which then has the rows' other bytes in its L2.
+constexpr uint32_t kMoveThreads = 512, kMoveDepth = 4, kXcds = 8;
+typedef uint32_t eu4 __attribute__((ext_vector_type(4)));
 
 template <class U>
 __global__ __launch_bounds__(kMoveThreads) void k_evict_move(EvictArgs a, uint32_t lanes, uint32_t slices) {
     const uint32_t t = threadIdx.x, rows = kMoveThreads / lanes, row = t / lanes;
-    const uint32_t slice = blockIdx.x % slices, h = blockIdx.x / slices;
+    const uint32_t slice = blockIdx.x / kXcds % slices, unit = blockIdx.x / (kXcds * slices) * kXcds + blockIdx.x % kXcds;
+    if (unit >= 2u * a.nkh * a.n_layers) return;  // (the grid is whole groups of kXcds units)
+    const uint32_t lh = unit >> 1, l = lh / a.nkh, h = lh % a.nkh;
     const uint32_t units = a.hd * 2u / (uint32_t)sizeof(U), u = slice * lanes + t % lanes;
-    const uint32_t *kept = a.kept + ((uint64_t)blockIdx.y * a.nkh + h) * a.budget;
-    U *c = reinterpret_cast<U *>(blockIdx.z ? a.vc : a.kc) + ((uint64_t)blockIdx.y * a.max_ctx * a.nkh + h) * units + u;
+    const uint32_t *kept = a.kept + (uint64_t)lh * a.budget;
+    U *c = reinterpret_cast<U *>(unit & 1u ? a.vc : a.kc) + ((uint64_t)l * a.max_ctx * a.nkh + h) * units + u;
     const uint64_t stride = (uint64_t)a.nkh * units;
-    const bool mine = row < rows && u < units;
-    U v[2][kMoveDepth];
-    uint32_t from[2][kMoveDepth];
-    auto load = [&](uint32_t b, U(&x)[kMoveDepth], uint32_t(&f)[kMoveDepth]) {
+    const uint32_t budget = row < rows && u < units ? a.budget : 0u;  // (threads past the slice have nothing)
+    // the slots of the batch to write, of the one whose rows are on their way and of the one behind it
+    uint32_t fa[kMoveDepth], fb[kMoveDepth], fc[kMoveDepth];
+    U v0[kMoveDepth], v1[kMoveDepth];
+    auto place = [&](uint32_t b, uint32_t k) { return (b * kMoveDepth + k) * rows + row; };
+    auto ids = [&](uint32_t b, uint32_t(&f)[kMoveDepth]) {
 #pragma unroll
-        for (uint32_t k = 0; k < kMoveDepth; k++) {
-            const uint32_t i = (b * kMoveDepth + k) * rows + row;
-            f[k] = mine && i < a.budget ? kept[i] : i;
-            if (f[k] != i) x[k] = c[f[k] * stride];
-        }
+        for (uint32_t k = 0; k < kMoveDepth; k++) f[k] = place(b, k) < budget ? kept[place(b, k)] : place(b, k);
     };
-    auto store = [&](uint32_t b, const U(&x)[kMoveDepth], const uint32_t(&f)[kMoveDepth]) {
+    auto load = [&](uint32_t b, U(&x)[kMoveDepth]) {
 #pragma unroll
-        for (uint32_t k = 0; k < kMoveDepth; k++) {
-            const uint32_t i = (b * kMoveDepth + k) * rows + row;
-            if (f[k] != i) c[i * stride] = x[k];
-        }
+        for (uint32_t k = 0; k < kMoveDepth; k++)
+            if (fb[k] != place(b, k)) x[k] = c[fb[k] * stride];
     };
     const uint32_t per = kMoveDepth * rows, batches = (a.budget + per - 1u) / per;
-    load(0u, v[0], from[0]);
-    for (uint32_t b = 0; b < batches; b += 2u) {
+    // every row of the batch at hand has arrived, in every wave, before the first is written;
+    // the next batch's rows lie above every place of it
+    auto turn = [&](uint32_t b, const U(&x)[kMoveDepth], U(&y)[kMoveDepth]) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
 #pragma unroll
-        for (uint32_t o = 0; o < 2u; o++) {
-            if (b + o >= batches) break;
-            // every row of this batch has arrived, in every wave, before the first is written
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            // the next batch's rows lie above every place of this one
-            if (b + o + 1u < batches) load(b + o + 1u, v[1u - o], from[1u - o]);
-            store(b + o, v[o], from[o]);
-        }
+        for (uint32_t k = 0; k < kMoveDepth; k++) fa[k] = fb[k], fb[k] = fc[k];
+        if (b + 1u < batches) load(b + 1u, y);
+        ids(b + 2u, fc);
+#pragma unroll
+        for (uint32_t k = 0; k < kMoveDepth; k++)
+            if (fa[k] != place(b, k)) c[place(b, k) * stride] = x[k];
+    };
+    ids(0u, fb);
+    load(0u, v0);
+    ids(1u, fc);
+    for (uint32_t b = 0; b < batches; b += 2u) {
+        turn(b, v0, v1);
+        if (b + 1u < batches) turn(b + 1u, v1, v0);
     }
 }
 
@@ -148,11 +221,16 @@ hipError_t launch_evict(const EvictArgs &a, hipStream_t s) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const bool wide = a.hd % 8u == 0 && (((uintptr_t)a.kc | (uintptr_t)a.vc) & 15u) == 0;
-    const uint32_t units = wide ? a.hd / 8u : a.hd, want = wide ? 4u : 32u;
-    const uint32_t lanes = units < want ? units : want, slices = (units + lanes - 1u) / lanes;
-    const dim3 grid(a.nkh * slices, a.n_layers, 2);
+    // Whole rows a workgroup where that gives a workgroup per CU (32 layers of 8 heads of 128, 8192
+    // slots to 4096: 223 us, 4.8 TB/s read and written; half rows 253, quarters 303, eighths 335), else
+    // narrower slices, down to 32 bytes (one such layer, 2049 to 1024: 3.5 us; whole rows 11.2).
+    const uint32_t units = wide ? a.hd / 8u : a.hd, pairs = 2u * a.nkh * a.n_layers, least = wide ? 2u : 16u;
+    uint32_t lanes = units;
+    while (lanes > least && pairs * ((units + lanes - 1u) / lanes) < 256u) lanes = (lanes + 1u) / 2u;
+    const uint32_t slices = (units + lanes - 1u) / lanes;
+    const uint32_t grid = (pairs + kXcds - 1u) / kXcds * kXcds * slices;
     if (wide)
-        k_evict_move<uint4><<<grid, kMoveThreads, 0, s>>>(a, lanes, slices);
+        k_evict_move<eu4><<<grid, kMoveThreads, 0, s>>>(a, lanes, slices);
     else
         k_evict_move<uint16_t><<<grid, kMoveThreads, 0, s>>>(a, lanes, slices);
     return hipGetLastError();

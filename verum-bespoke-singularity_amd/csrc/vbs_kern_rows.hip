@@ -132,6 +132,9 @@ struct RowsPart {
     float2 *stats;
 };
 
+// Floats from one partial row to the next.
+__host__ __device__ __forceinline__ uint32_t part_stride(uint32_t hd) { return (hd + 3u) / 4u * 4u; }
+
 template <uint32_t HD>
 constexpr uint32_t kTile = HD > 128u ? 32u : 64u;  // slots per LDS tile
 
@@ -164,116 +167,65 @@ __device__ __forceinline__ rs4 lds_transposed(const uint8_t *p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) rs4 *)(uint32_t)(uintptr_t)p);
 }
 
+// The rows of one wave: CT column tiles of 16, their q' parts and their running sums.
 template <uint32_t HD, uint32_t CT>
-__global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsPart pt, uint32_t tiles, bool wide_kv,
-                                                 bool wide_q) {
-    constexpr uint32_t KK = HD / 32u, DT = HD / 16u, T = kTile<HD>, CPR = HD / 8u, NC = T * CPR / 256u;
-    constexpr uint32_t RB = HD * 2u, TB = T * RB;  // bytes of a row and of a tile
-    __shared__ __align__(1024) uint8_t kv[2][2][TB];  // two buffers of K and V
-    __shared__ int32_t dl[2][T];
-    const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u, col = lane & 15u, g = lane >> 4;
-    const uint32_t kvh = blockIdx.x % a.nkh, rest = blockIdx.x / a.nkh;
-    const uint32_t split = rest % sp.n, tile = tiles - 1u - rest / sp.n;  // (the longest rows first)
-    const uint32_t group = a.nqh / a.nkh, rows = a.n * group, row_tile = tile * 64u * CT;
-    const uint32_t end = row_end(a, (min(row_tile + 64u * CT, rows) - 1u) / group);
-    const uint32_t s0 = split * sp.len, s1 = min(s0 + sp.len, end);
-    if (s0 >= s1) return;  // (the whole workgroup; the merge counts the ranges the same way)
-    const uint32_t slots = a.past + a.n;
-
-    // ---- the wave's rows
-    const uint32_t row0 = row_tile + wave * 16u * CT;
-    const bool active = row0 < rows;
+struct RowTiles {
+    static constexpr uint32_t KK = HD / 32u, DT = HD / 16u, RB = HD * 2u;
+    static constexpr uint32_t NK = KK < 4u ? KK : 4u, NV = DT < 8u ? DT : 8u;  // (dims from 128 on lie 256 bytes on)
     rh8 qh[CT][KK], ql[CT][KK];
-    float c1[CT], slope[CT];
+    float c1[CT], slope[CT], m[CT], l[CT];
     uint32_t tok[CT];
     int32_t doc[CT];
     bool real[CT];
-#pragma unroll
-    for (uint32_t x = 0; x < CT; x++) {
-        const uint32_t r = row0 + 16u * x + col;
-        real[x] = r < rows;
-        tok[x] = real[x] ? r / group : 0u;
-        const uint32_t h = kvh * group + (real[x] ? r % group : 0u);
-        row_parts<KK>(real[x] ? a.q + (uint64_t)tok[x] * a.q_stride + (uint64_t)h * a.hd : nullptr, a.hd, wide_q, a.scale,
-                      g, qh[x], ql[x], c1[x]);
-        slope[x] = a.slopes ? a.slopes[h] : 0.f;
-        doc[x] = a.docs ? a.docs[a.past + tok[x]] : 0;
-    }
-    const bool terms = a.cap > 0.f || a.slopes;
-    // below `clear` every row of the wave sees every slot (documents aside); from `last` on, none
-    const uint32_t tok_first = min(row0, rows - 1u) / group, tok_last = (min(row0 + 16u * CT, rows) - 1u) / group;
-    const uint32_t clear = a.docs ? 0u : a.mask ? a.past : row_end(a, tok_first);
-    const uint32_t last = active ? row_end(a, tok_last) : 0u;
-
-    // ---- staging: tile p0 into buffer b, by LDS DMA (no registers; it arrives by the next wait) or,
-    // where rows are not whole aligned chunks, through registers
-    const uint64_t rstride = (uint64_t)a.nkh * a.hd;
-    const uint16_t *kb = a.kc + (uint64_t)kvh * a.hd, *vb = a.vc + (uint64_t)kvh * a.hd;
-    int32_t ds = 0;
-    uint32_t from[NC];  // a thread's chunks: bytes from the tile's first row
-    bool in[NC];        // (dims past head_dim stay 0)
-#pragma unroll
-    for (uint32_t k = 0; k < NC; k++) {
-        const uint32_t id = t + 256u * k, r = id / CPR, d = 8u * tile_chunk<HD>(r, id % CPR);
-        from[k] = (uint32_t)(2u * (r * rstride + d));
-        in[k] = d < a.hd;
-        if (!in[k])
-#pragma unroll
-            for (uint32_t b = 0; b < 4u; b++) *reinterpret_cast<ru4 *>(&kv[b >> 1][b & 1u][16u * id]) = ru4{0u, 0u, 0u, 0u};
-    }
-    auto fetch = [&](uint32_t p0, uint32_t b) {
-        if (wide_kv && p0 + T <= slots) {
-            const uint16_t *kp = kb + p0 * rstride, *vp = vb + p0 * rstride;
-#pragma unroll
-            for (uint32_t k = 0; k < NC; k++) {
-                const uint32_t to = 16u * (256u * k + 64u * wave);
-                if (HD == a.hd || in[k]) {
-                    dma16s(kp, from[k], (uint32_t)(uintptr_t)&kv[b][0][to]);
-                    dma16s(vp, from[k], (uint32_t)(uintptr_t)&kv[b][1][to]);
-                }
-            }
-        } else {
-#pragma unroll 1
-            for (uint32_t k = 0; k < NC; k++) {
-                const uint32_t id = t + 256u * k, r = id / CPR, d = 8u * tile_chunk<HD>(r, id % CPR);
-                // (slots behind the last repeat it: what lies there may be no number)
-                const uint64_t at = (uint64_t)min(p0 + r, slots - 1u) * rstride;
-                *reinterpret_cast<ru4 *>(&kv[b][0][16u * id]) = cache8(kb + at, d, a.hd, wide_kv);
-                *reinterpret_cast<ru4 *>(&kv[b][1][16u * id]) = cache8(vb + at, d, a.hd, wide_kv);
-            }
-        }
-        if (a.docs && t < T) ds = a.docs[min(p0 + t, slots - 1u)];
-    };
-    // every wave's part of the tile has arrived and every wave is done with the other buffer
-    auto arrive = [&](uint32_t b) {
-        if (a.docs && t < T) dl[b][t] = ds;
-        vmcnt_le<0>();
-        __syncthreads();
-    };
-    // where the lane reads: its chunk of K per slice (row `col` of a 16-row tile), and per 16 dims its part of
-    // the transposed V read: slot 4 g + col / 4, dims 4 (col % 4) ..
-    constexpr uint32_t NV = DT < 8u ? DT : 8u;  // (dims from 128 on lie 256 bytes on)
-    uint32_t kat[KK < 4u ? KK : 4u], vat[NV];
-#pragma unroll
-    for (uint32_t kk = 0; kk < KK && kk < 4u; kk++) kat[kk] = col * RB + 16u * tile_place<HD>(col, 4u * kk + g);
-#pragma unroll
-    for (uint32_t d = 0; d < NV; d++) {
-        const uint32_t r = 4u * g + (col >> 2);
-        vat[d] = TB + r * RB + 16u * tile_place<HD>(r, 2u * d + (col >> 1 & 1u)) + 8u * (col & 1u);
-    }
-
-    float m[CT], l[CT];
     rf4 acc[DT][CT];
+    uint32_t kat[NK], vat[NV];  // where the lane reads in LDS, from a tile's first byte of K
+    // below `clear` every row sees every slot (documents aside); from `last` on, none
+    uint32_t clear, last;
+
+    // v_at: from a tile's first byte of K to its first of V
+    __device__ __forceinline__ void init(const RowsArgs &a, uint32_t kvh, uint32_t row0, bool wide_q, uint32_t lane,
+                                         uint32_t v_at) {
+        const uint32_t col = lane & 15u, g = lane >> 4, group = a.nqh / a.nkh, rows = a.n * group;
 #pragma unroll
-    for (uint32_t x = 0; x < CT; x++) {
-        m[x] = -INFINITY, l[x] = 0.f;
+        for (uint32_t x = 0; x < CT; x++) {
+            const uint32_t r = row0 + 16u * x + col;
+            real[x] = r < rows;
+            tok[x] = real[x] ? r / group : 0u;
+            const uint32_t h = kvh * group + (real[x] ? r % group : 0u);
+            row_parts<KK>(real[x] ? a.q + (uint64_t)tok[x] * a.q_stride + (uint64_t)h * a.hd : nullptr, a.hd, wide_q,
+                          a.scale, g, qh[x], ql[x], c1[x]);
+            slope[x] = a.slopes ? a.slopes[h] : 0.f;
+            doc[x] = a.docs ? a.docs[a.past + tok[x]] : 0;
+            m[x] = -INFINITY, l[x] = 0.f;
 #pragma unroll
-        for (uint32_t d = 0; d < DT; d++) acc[d][x] = rf4{0.f, 0.f, 0.f, 0.f};
+            for (uint32_t d = 0; d < DT; d++) acc[d][x] = rf4{0.f, 0.f, 0.f, 0.f};
+        }
+        clear = a.docs ? 0u : a.mask ? a.past : row_end(a, min(row0, rows - 1u) / group);
+        last = row0 < rows ? row_end(a, (min(row0 + 16u * CT, rows) - 1u) / group) : 0u;
+        // its chunk of K per slice (row `col` of a 16-row tile), and per 16 dims its part of the
+        // transposed V read: slot 4 g + col / 4, dims 4 (col % 4) ..
+#pragma unroll
+        for (uint32_t kk = 0; kk < NK; kk++) kat[kk] = col * RB + 16u * tile_place<HD>(col, 4u * kk + g);
+#pragma unroll
+        for (uint32_t d = 0; d < NV; d++) {
+            const uint32_t r = 4u * g + (col >> 2);
+            vat[d] = v_at + r * RB + 16u * tile_place<HD>(r, 2u * d + (col >> 1 & 1u)) + 8u * (col & 1u);
+        }
     }
 
-    // 32 slots from p0 on, in LDS buffer b at row `at`; vis: their bits per column tile
-    const uint8_t *const lds = &kv[0][0][0];
-    auto step = [&](uint32_t b, uint32_t at, uint32_t p0, const uint32_t (&vis)[CT], bool full) {
+    __device__ __forceinline__ void turn(uint32_t by) {  // on to another buffer
+#pragma unroll
+        for (uint32_t kk = 0; kk < NK; kk++) kat[kk] += by;
+#pragma unroll
+        for (uint32_t d = 0; d < NV; d++) vat[d] += by;
+    }
+
+    // 32 slots from p0 on, in LDS from row `at` of the tile; full: every row sees them all, else vis
+    // holds their bits per column tile and docs (or NULL) their documents
+    __device__ __forceinline__ void step(const RowsArgs &a, const uint8_t *lds, uint32_t at, uint32_t p0,
+                                         const uint32_t (&vis)[CT], bool full, const int32_t *docs, uint32_t lane) {
+        const uint32_t g = lane >> 4;
+        const bool terms = a.cap > 0.f || a.slopes;
         rf4 S[2][CT];
 #pragma unroll
         for (uint32_t hf = 0; hf < 2u; hf++)
@@ -348,7 +300,7 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
                 for (uint32_t j = 0; j < 8u; j++) {
                     const uint32_t o = 16u * (j >> 2) + 4u * g + (j & 3u);
                     bool sees = vis[x] >> o & 1u;
-                    if (a.docs) sees = sees && dl[b][at + o] == doc[x];
+                    if (docs) sees = sees && docs[o] == doc[x];
                     if (!sees) S[j >> 2][x][j & 3u] = -INFINITY;
                 }
         }
@@ -403,6 +355,116 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
 #pragma unroll
             for (uint32_t x = 0; x < CT; x++) acc[d][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[x], acc[d][x], 0, 0, 0);
         }
+    }
+
+    // l over the four lane groups of a row
+    __device__ __forceinline__ void sum_l() {
+#pragma unroll
+        for (uint32_t x = 0; x < CT; x++) {
+            l[x] += lane_xor<16>(l[x]);
+            l[x] += lane_xor<32>(l[x]);
+        }
+    }
+};
+
+// Where the results of row r of kv head kvh over range `split` go: the partials, or
+// (one range) out, divided by l, and what the mass needs.
+struct RowsTo {
+    float *acc;
+    float2 *ml;     // NULL: out
+    float2 *stats;  // NULL: not wanted
+    __device__ __forceinline__ RowsTo(const RowsArgs &a, const RowsSplit &sp, const RowsPart &pt, uint32_t kvh,
+                                      uint32_t split, uint32_t r) {
+        const uint32_t group = a.nqh / a.nkh, rows = a.n * group;
+        const uint64_t at = ((uint64_t)kvh * sp.n + split) * rows + r;
+        ml = sp.n > 1u ? pt.ml + at : nullptr;
+        acc = sp.n > 1u ? pt.acc + at * part_stride(a.hd)
+                        : a.out + (uint64_t)(r / group) * a.out_stride + (uint64_t)(kvh * group + r % group) * a.hd;
+        stats = sp.n == 1u && pt.stats ? pt.stats + (uint64_t)kvh * rows + r : nullptr;
+    }
+    __device__ __forceinline__ float scale(float l) const { return ml ? 1.f : l == 0.f ? 0.f : __fdiv_rn(1.f, l); }
+    __device__ __forceinline__ void put_ml(float m, float l) const {
+        if (ml) *ml = make_float2(m, l);
+        if (stats) *stats = make_float2(m, l == 0.f ? 0.f : __fdiv_rn(1.f, l));
+    }
+};
+// The row again in f32 products, by a whole wave (row_whole), to the same place.
+template <uint32_t HD>
+__device__ __forceinline__ void row_again(const RowsArgs &a, const RowsSplit &sp, const RowsPart &pt, uint32_t kvh,
+                                          uint32_t split, uint32_t r, uint32_t s0, uint32_t s1, uint32_t lane) {
+    const uint32_t group = a.nqh / a.nkh;
+    float m, l, o[(HD + 63u) / 64u];
+    row_whole<HD>(a, r / group, kvh * group + r % group, s0, s1, lane, m, l, o);
+    const RowsTo to(a, sp, pt, kvh, split, r);
+#pragma unroll
+    for (uint32_t k = 0; k < (HD + 63u) / 64u; k++)
+        if (64u * k + lane < a.hd) to.acc[64u * k + lane] = to.ml ? o[k] : l == 0.f ? 0.f : o[k] / l;
+    if (lane == 0) to.put_ml(m, l);
+}
+
+// ---- many rows: four waves with rows of their own, slots through two shared buffers ------
+template <uint32_t HD, uint32_t CT>
+__global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsPart pt, uint32_t tiles, bool wide_kv,
+                                                 bool wide_q) {
+    constexpr uint32_t DT = HD / 16u, T = kTile<HD>, CPR = HD / 8u, NC = T * CPR / 256u;
+    constexpr uint32_t RB = HD * 2u, TB = T * RB;  // bytes of a row and of a tile
+    __shared__ __align__(1024) uint8_t kv[2][2][TB];  // two buffers of K and V
+    __shared__ int32_t dl[2][T];
+    const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u, col = lane & 15u, g = lane >> 4;
+    const uint32_t kvh = blockIdx.x % a.nkh, rest = blockIdx.x / a.nkh;
+    const uint32_t split = rest % sp.n, tile = tiles - 1u - rest / sp.n;  // (the longest rows first)
+    const uint32_t group = a.nqh / a.nkh, rows = a.n * group, row_tile = tile * 64u * CT;
+    const uint32_t end = row_end(a, (min(row_tile + 64u * CT, rows) - 1u) / group);
+    const uint32_t s0 = split * sp.len, s1 = min(s0 + sp.len, end);
+    if (s0 >= s1) return;  // (the whole workgroup; the merge counts the ranges the same way)
+    const uint32_t slots = a.past + a.n, row0 = row_tile + wave * 16u * CT;
+    RowTiles<HD, CT> R;
+    R.init(a, kvh, row0, wide_q, lane, TB);
+
+    // ---- staging: tile p0 into buffer b, by LDS DMA (no registers; it arrives by the next wait) or,
+    // where rows are not whole aligned chunks, through registers
+    const uint64_t rstride = (uint64_t)a.nkh * a.hd;
+    const uint16_t *kb = a.kc + (uint64_t)kvh * a.hd, *vb = a.vc + (uint64_t)kvh * a.hd;
+    int32_t ds = 0;
+    uint32_t from[NC];  // a thread's chunks: bytes from the tile's first row
+    bool in[NC];        // (dims past head_dim stay 0)
+#pragma unroll
+    for (uint32_t k = 0; k < NC; k++) {
+        const uint32_t id = t + 256u * k, r = id / CPR, d = 8u * tile_chunk<HD>(r, id % CPR);
+        from[k] = (uint32_t)(2u * (r * rstride + d));
+        in[k] = d < a.hd;
+        if (!in[k])
+#pragma unroll
+            for (uint32_t b = 0; b < 4u; b++) *reinterpret_cast<ru4 *>(&kv[b >> 1][b & 1u][16u * id]) = ru4{0u, 0u, 0u, 0u};
+    }
+    auto fetch = [&](uint32_t p0, uint32_t b) {
+        if (wide_kv && p0 + T <= slots) {
+            const uint16_t *kp = kb + p0 * rstride, *vp = vb + p0 * rstride;
+#pragma unroll
+            for (uint32_t k = 0; k < NC; k++) {
+                const uint32_t to = 16u * (256u * k + 64u * wave);
+                if (HD == a.hd || in[k]) {
+                    dma16s(kp, from[k], (uint32_t)(uintptr_t)&kv[b][0][to]);
+                    dma16s(vp, from[k], (uint32_t)(uintptr_t)&kv[b][1][to]);
+                }
+            }
+        } else {
+#pragma unroll 1
+            for (uint32_t k = 0; k < NC; k++) {
+                const uint32_t id = t + 256u * k, r = id / CPR, d = 8u * tile_chunk<HD>(r, id % CPR);
+                // (slots behind the last repeat it: what lies there may be no number)
+                const uint64_t at = (uint64_t)min(p0 + r, slots - 1u) * rstride;
+                *reinterpret_cast<ru4 *>(&kv[b][0][16u * id]) = cache8(kb + at, d, a.hd, wide_kv);
+                *reinterpret_cast<ru4 *>(&kv[b][1][16u * id]) = cache8(vb + at, d, a.hd, wide_kv);
+            }
+        }
+        if (a.docs && t < T) ds = a.docs[min(p0 + t, slots - 1u)];
+    };
+    // every wave's part of the tile has arrived and every wave is done with the other buffer
+    auto arrive = [&](uint32_t b) {
+        if (a.docs && t < T) dl[b][t] = ds;
+        vmcnt_le<0>();
+        __syncthreads();
     };
 
     fetch(s0, 0u);
@@ -410,127 +472,216 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
     for (uint32_t p0 = s0, b = 0; p0 < s1; p0 += T, b ^= 1u) {
         const bool more = p0 + T < s1;
         if (more) fetch(p0 + T, b ^ 1u);
-        if (p0 < last) {
-            const bool full = p0 + T <= min(clear, s1);
+        if (p0 < R.last) {
+            const bool full = p0 + T <= min(R.clear, s1);
             uint64_t vis[CT];
 #pragma unroll
-            for (uint32_t x = 0; x < CT; x++) vis[x] = full ? ~0ull : real[x] ? seen_bits(a, tok[x], p0, s1) : 0ull;
+            for (uint32_t x = 0; x < CT; x++) vis[x] = full ? ~0ull : R.real[x] ? seen_bits(a, R.tok[x], p0, s1) : 0ull;
 #pragma unroll
             for (uint32_t h = 0; h < T / 32u; h++) {
                 uint32_t v[CT];
 #pragma unroll
                 for (uint32_t x = 0; x < CT; x++) v[x] = (uint32_t)(vis[x] >> (32u * h));
-                step(b, 32u * h, p0 + 32u * h, v, full);
+                R.step(a, &kv[0][0][0], 32u * h, p0 + 32u * h, v, full, a.docs ? &dl[b][32u * h] : nullptr, lane);
             }
         }
         if (more) arrive(b ^ 1u);
-        const uint32_t on = b ? 0u - 2u * TB : 2u * TB;  // (the other buffer)
-#pragma unroll
-        for (uint32_t kk = 0; kk < KK && kk < 4u; kk++) kat[kk] += on;
-#pragma unroll
-        for (uint32_t d = 0; d < NV; d++) vat[d] += on;
+        R.turn(b ? 0u - 2u * TB : 2u * TB);
     }
-    if (!active) return;
+    if (row0 >= rows) return;
 
-    // ---- the rows' sums: l over the four lane groups, then out (one range) or the partials
-    const uint64_t first = ((uint64_t)kvh * sp.n + split) * rows;
-    const bool wide_to = a.hd % 4u == 0 && (sp.n > 1u || (a.out_stride % 4u == 0 && ((uintptr_t)a.out & 15u) == 0));
+    // ---- the rows' sums
+    R.sum_l();
+    const bool wide_to = a.hd % 4u == 0 && (a.out_stride % 4u == 0 && ((uintptr_t)a.out & 15u) == 0);
 #pragma unroll
     for (uint32_t x = 0; x < CT; x++) {
-        l[x] += lane_xor<16>(l[x]);
-        l[x] += lane_xor<32>(l[x]);
-        const uint32_t r = row0 + 16u * x + col, h = kvh * group + r % group;
-        float nan = l[x] * 0.f;
+        float nan = R.l[x] * 0.f;
 #pragma unroll
         for (uint32_t d = 0; d < DT; d++)
 #pragma unroll
-            for (uint32_t k = 0; k < 4u; k++) nan = fmaf(acc[d][x][k], 0.f, nan);
-        const uint64_t bad = __ballot(real[x] && nan != 0.f);  // (0 times anything finite is 0)
+            for (uint32_t k = 0; k < 4u; k++) nan = fmaf(R.acc[d][x][k], 0.f, nan);
+        const uint64_t bad = __ballot(R.real[x] && nan != 0.f);  // (0 times anything finite is 0)
         const uint32_t cols = (uint32_t)(bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xFFFFu;
-        const float mo = m[x] - kLift;
-        if (real[x] && !(cols >> col & 1u)) {
-            const float inv = sp.n > 1u ? 1.f : l[x] == 0.f ? 0.f : __fdiv_rn(1.f, l[x]);
-            float *to = sp.n > 1u ? pt.acc + (first + r) * a.hd
-                                  : a.out + (uint64_t)tok[x] * a.out_stride + (uint64_t)h * a.hd;
+        if (R.real[x] && !(cols >> col & 1u)) {
+            const RowsTo to(a, sp, pt, kvh, split, row0 + 16u * x + col);
+            const float inv = to.scale(R.l[x]);
 #pragma unroll
             for (uint32_t d = 0; d < DT; d++) {
                 const uint32_t d0 = 16u * d + 4u * g;
-                if (wide_to && d0 < a.hd) {
-                    *reinterpret_cast<rf4 *>(to + d0) = acc[d][x] * inv;
-                } else if (!wide_to) {
+                if (to.ml || wide_to) {  // (the partials' rows are whole float4s)
+                    if (d0 < a.hd) *reinterpret_cast<rf4 *>(to.acc + d0) = R.acc[d][x] * inv;
+                } else {
 #pragma unroll
                     for (uint32_t k = 0; k < 4u; k++)
-                        if (d0 + k < a.hd) to[d0 + k] = acc[d][x][k] * inv;
+                        if (d0 + k < a.hd) to.acc[d0 + k] = R.acc[d][x][k] * inv;
                 }
             }
-            if (g == 0 && sp.n > 1u) pt.ml[first + r] = make_float2(mo, l[x]);
-            if (g == 0 && sp.n == 1u && pt.stats) pt.stats[(uint64_t)kvh * rows + r] = make_float2(mo, l[x] == 0.f ? 0.f : __fdiv_rn(1.f, l[x]));
+            if (g == 0) to.put_ml(R.m[x] - kLift, R.l[x]);
         }
-        // rows whose sums are not finite, one at a time (row_whole)
-        for (uint32_t c = 0; cols >> c; c++) {
-            if (!(cols >> c & 1u)) continue;
-            const uint32_t rr = row0 + 16u * x + c, i = rr / group, hh = kvh * group + rr % group;
-            float wm, wl, wa[(HD + 63u) / 64u];
-            row_whole<HD>(a, i, hh, s0, s1, lane, wm, wl, wa);
-            float *to = sp.n > 1u ? pt.acc + (first + rr) * a.hd : a.out + (uint64_t)i * a.out_stride + (uint64_t)hh * a.hd;
-#pragma unroll
-            for (uint32_t k = 0; k < (HD + 63u) / 64u; k++)
-                if (64u * k + lane < a.hd) to[64u * k + lane] = sp.n > 1u ? wa[k] : wl == 0.f ? 0.f : wa[k] / wl;
-            if (lane == 0 && sp.n > 1u) pt.ml[first + rr] = make_float2(wm, wl);
-            if (lane == 0 && sp.n == 1u && pt.stats) pt.stats[(uint64_t)kvh * rows + rr] = make_float2(wm, wl == 0.f ? 0.f : 1.f / wl);
-        }
+        // rows whose sums are not finite, one at a time
+        for (uint32_t c = 0; cols >> c; c++)
+            if (cols >> c & 1u) row_again<HD>(a, sp, pt, kvh, split, row0 + 16u * x + c, s0, s1, lane);
     }
 }
 
-// ---- the ranges of a row added up ----------------------------------------------------
-// A workgroup per (kv head, row): M = max m_c, L = sum l_c 2^(m_c - M), out = sum acc_c
-// 2^(m_c - M) / L; wave w takes the ranges w, w + 4, ..., then the waves' sums in order.
-__global__ __launch_bounds__(256) void k_rows_merge(RowsArgs a, RowsSplit sp, RowsPart pt, uint32_t tile_rows) {
-    __shared__ float2 part[4][128];
-    __shared__ float lw[4];
-    const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u, r = blockIdx.x, kvh = blockIdx.y;
-    const uint32_t group = a.nqh / a.nkh, rows = a.n * group;
-    const uint32_t end = row_end(a, (min(r / tile_rows * tile_rows + tile_rows, rows) - 1u) / group);
-    const uint32_t n = (end + sp.len - 1u) / sp.len;
-    const float2 *ml = pt.ml + (uint64_t)kvh * sp.n * rows + r;
-    const float *acc = pt.acc + ((uint64_t)kvh * sp.n * rows + r) * a.hd;
-    float M = -INFINITY;
-    for (uint32_t c = lane; c < n; c += 64u) M = fmaxf(M, ml[(uint64_t)c * rows].x);
-    M = wave_max(M);
-    const float ref = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
-    float2 o[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-    for (uint32_t c = wave; c < n; c += 4u) {
-        const float2 v = ml[(uint64_t)c * rows];
-        const float w = exp2f(v.x - ref);
-        L = fmaf(v.y, w, L);
+// ---- few rows: four waves with the same 16 CT rows, each with slots of its own ---------------
+// A wave takes the 32-slot tiles wave, wave + 4, ... of the range, in an LDS buffer of its own (no barrier
+// until the end), then the waves' sums are added in LDS.
+template <uint32_t HD, uint32_t CT>
+__global__ __launch_bounds__(256, 2) void k_rows_few(RowsArgs a, RowsSplit sp, RowsPart pt, bool wide_q) {
+    constexpr uint32_t DT = HD / 16u, T = 32u, CPR = HD / 8u, NC = T * CPR / 64u, RB = HD * 2u, TB = T * RB;
+    constexpr uint32_t RS = HD + 4u;  // floats of a row's sums in LDS (the rows of a store in different banks)
+    constexpr uint32_t OWN = 2u * TB > 16u * CT * RS * 4u ? 2u * TB : 16u * CT * RS * 4u;
+    __shared__ __align__(1024) uint8_t kv[4][OWN];
+    __shared__ float2 mls[4][16u * CT];
+    __shared__ uint32_t bad[16u * CT];
+    const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63u, col = lane & 15u, g = lane >> 4;
+    const uint32_t kvh = blockIdx.x % a.nkh, rest = blockIdx.x / a.nkh, split = rest % sp.n, row0 = rest / sp.n * 16u * CT;
+    const uint32_t group = a.nqh / a.nkh, rows = a.n * group, slots = a.past + a.n;
+    const uint32_t end = row_end(a, (min(row0 + 16u * CT, rows) - 1u) / group);
+    const uint32_t s0 = split * sp.len, s1 = min(s0 + sp.len, end);
+    if (s0 >= s1) return;  // (the whole workgroup)
+    uint8_t *const own = &kv[wave][0];
+    const uint64_t rstride = (uint64_t)a.nkh * a.hd;
+    const uint16_t *kb = a.kc + (uint64_t)kvh * a.hd, *vb = a.vc + (uint64_t)kvh * a.hd;
 #pragma unroll
-        for (uint32_t k = 0; k < 2u; k++) {
-            const uint32_t d = 2u * lane + 128u * k;
-            if (d < a.hd) {
-                const float *x = acc + (uint64_t)c * rows * a.hd + d;
-                o[k].x = fmaf(x[0], w, o[k].x);
-                o[k].y = fmaf(x[1], w, o[k].y);
+    for (uint32_t k = 0; k < NC; k++) {  // (dims past head_dim stay 0)
+        const uint32_t id = lane + 64u * k, r = id / CPR;
+        if (8u * tile_chunk<HD>(r, id % CPR) < a.hd) continue;
+        *reinterpret_cast<ru4 *>(own + 16u * id) = ru4{0u, 0u, 0u, 0u};
+        *reinterpret_cast<ru4 *>(own + TB + 16u * id) = ru4{0u, 0u, 0u, 0u};
+    }
+    auto fetch = [&](uint32_t p0) {
+        const uint16_t *kp = kb + p0 * rstride, *vp = vb + p0 * rstride;
+        const uint32_t most = min(slots - p0, T) - 1u;  // (slots behind the last repeat it)
+#pragma unroll
+        for (uint32_t k = 0; k < NC; k++) {
+            const uint32_t id = lane + 64u * k, r = id / CPR, d = 8u * tile_chunk<HD>(r, id % CPR);
+            const uint32_t from = (uint32_t)(2u * (min(r, most) * rstride + d));
+            if (HD == a.hd || d < a.hd) {
+                dma16s(kp, from, (uint32_t)(uintptr_t)(own + 1024u * k));
+                dma16s(vp, from, (uint32_t)(uintptr_t)(own + TB + 1024u * k));
             }
         }
-    }
+    };
+    uint32_t p0 = s0 + T * wave;
+    if (p0 < s1) fetch(p0);
+    RowTiles<HD, CT> R;
+    R.init(a, kvh, row0, wide_q, lane, TB);
+    while (p0 < s1) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (p0 < R.last) {
+            const bool full = p0 + T <= min(R.clear, s1);
+            uint32_t vis[CT];
 #pragma unroll
-    for (uint32_t k = 0; k < 2u; k++) part[wave][lane + 64u * k] = o[k];
-    if (lane == 0) lw[wave] = L;
+            for (uint32_t x = 0; x < CT; x++) vis[x] = full ? ~0u : R.real[x] ? (uint32_t)seen_bits(a, R.tok[x], p0, s1) : 0u;
+            R.step(a, own, 0u, p0, vis, full, a.docs ? a.docs + p0 : nullptr, lane);
+        }
+        p0 += 4u * T;
+        if (p0 >= s1) break;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the tile has been read)
+        fetch(p0);
+    }
+    // ---- the waves' sums: M = max m_w, sum acc_w 2^(m_w - M), in the order of the waves
+    R.sum_l();
+    float *const sums = reinterpret_cast<float *>(own);
+#pragma unroll
+    for (uint32_t x = 0; x < CT; x++) {
+#pragma unroll
+        for (uint32_t d = 0; d < DT; d++)
+            *reinterpret_cast<rf4 *>(sums + (16u * x + col) * RS + 16u * d + 4u * g) = R.acc[d][x];
+        if (g == 0) mls[wave][16u * x + col] = make_float2(R.m[x], R.l[x]);
+    }
+    if (t < 16u * CT) bad[t] = 0;
     __syncthreads();
-    if (t >= 128u || 2u * t >= a.hd) return;
-    const float total = ((lw[0] + lw[1]) + lw[2]) + lw[3];
-    float2 s = part[0][t];
+    const bool wide_to = a.hd % 4u == 0 && a.out_stride % 4u == 0 && ((uintptr_t)a.out & 15u) == 0;
+    for (uint32_t e = t; e < 16u * CT * (HD / 4u); e += 256u) {
+        const uint32_t r = e / (HD / 4u), d0 = 4u * (e % (HD / 4u));
+        if (row0 + r >= rows || d0 >= a.hd) continue;
+        float M = -INFINITY, l = 0.f;
 #pragma unroll
-    for (uint32_t w = 1; w < 4u; w++) {
-        s.x += part[w][t].x;
-        s.y += part[w][t].y;
+        for (uint32_t w = 0; w < 4u; w++) M = fmaxf(M, mls[w][r].x);
+        const float ref = M == -INFINITY ? 0.f : M;
+        rf4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (uint32_t w = 0; w < 4u; w++) {
+            const float2 v = mls[w][r];
+            const float f = exp2f(v.x - ref);
+            l = fmaf(v.y, f, l);
+            o += *reinterpret_cast<const rf4 *>(reinterpret_cast<const float *>(&kv[w][0]) + r * RS + d0) * f;
+        }
+        const RowsTo to(a, sp, pt, kvh, split, row0 + r);
+        const float inv = to.scale(l);
+        const float nan = fmaf(o[0], 0.f, fmaf(o[1], 0.f, fmaf(o[2], 0.f, fmaf(o[3], 0.f, l * 0.f))));
+        if (nan != 0.f) bad[r] = 1u;
+        o *= inv;
+        if (to.ml || wide_to) {
+            *reinterpret_cast<rf4 *>(to.acc + d0) = o;
+        } else {
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; k++)
+                if (d0 + k < a.hd) to.acc[d0 + k] = o[k];
+        }
+        if (d0 == 0) to.put_ml(M - kLift, l);
     }
-    const float inv = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
-    float *to = a.out + (uint64_t)(r / group) * a.out_stride + (uint64_t)(kvh * group + r % group) * a.hd + 2u * t;
-    to[0] = total == 0.f ? 0.f : s.x * inv;
-    to[1] = total == 0.f ? 0.f : s.y * inv;
-    if (t == 0 && pt.stats) pt.stats[(uint64_t)kvh * rows + r] = make_float2(M, inv);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (a row that is taken again is written after this)
+    __syncthreads();
+    for (uint32_t r = wave; r < 16u * CT; r += 4u)
+        if (bad[r]) row_again<HD>(a, sp, pt, kvh, split, row0 + r, s0, s1, lane);
+}
+
+// ---- the ranges of a row added up ----------------------------------------------------
+// TPR threads per row: M = max m_c, L = sum l_c 2^(m_c - M), out = sum acc_c 2^(m_c - M) / L. Every wave holds the
+// weights of the ranges in its lanes; lane groups of a row's float4s take the ranges in turn, eight at a time in
+// flight, and the groups are added in order.
+constexpr uint32_t kMostRanges = 128;
+
+template <uint32_t TPR>
+__global__ __launch_bounds__(256) void k_rows_merge(RowsArgs a, RowsSplit sp, RowsPart pt, uint32_t tile_rows, uint32_t width) {
+    __shared__ rf4 part[256];
+    const uint32_t t = threadIdx.x, lane = t & 63u, in = t % TPR, kvh = blockIdx.y;
+    const uint32_t group = a.nqh / a.nkh, rows = a.n * group, r = min(blockIdx.x * (256u / TPR) + t / TPR, rows - 1u);
+    const uint32_t end = row_end(a, (min(r / tile_rows * tile_rows + tile_rows, rows) - 1u) / group);
+    const uint32_t n = (end + sp.len - 1u) / sp.len;
+    const uint32_t q = in % width, grp = in / width, groups = TPR / width, ps = part_stride(a.hd);
+    const float2 *ml = pt.ml + (uint64_t)kvh * sp.n * rows + r;
+    const float *acc = pt.acc + ((uint64_t)kvh * sp.n * rows + r) * ps + 4u * q;
+    const bool mine = 4u * q < a.hd;
+    rf4 v[8];
+    auto load = [&](uint32_t c0) {
+#pragma unroll
+        for (uint32_t k = 0; k < 8u; k++) {
+            const uint32_t c = c0 + k * groups;
+            v[k] = mine && c < n ? *reinterpret_cast<const rf4 *>(acc + (uint64_t)c * rows * ps) : rf4{0.f, 0.f, 0.f, 0.f};
+        }
+    };
+    load(grp);
+    const float2 none = make_float2(-INFINITY, 0.f);
+    const float2 x0 = lane < n ? ml[(uint64_t)lane * rows] : none;
+    const float2 x1 = lane + 64u < n ? ml[(uint64_t)(lane + 64u) * rows] : none;
+    const float M = wave_max(fmaxf(x0.x, x1.x)), ref = M == -INFINITY ? 0.f : M;
+    const float w0 = exp2f(x0.x - ref), w1 = exp2f(x1.x - ref);
+    const float L = wave_sum(fmaf(x0.y, w0, x1.y * w1));
+    rf4 o = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t c0 = grp; c0 < n + grp; c0 += 8u * groups) {  // (the same count in every lane)
+        if (c0 != grp) load(c0);
+#pragma unroll
+        for (uint32_t k = 0; k < 8u; k++) {
+            const uint32_t c = c0 + k * groups;
+            const float f0 = __shfl(w0, (int)(c & 63u), 64), f1 = __shfl(w1, (int)(c & 63u), 64);
+            if (c < n) o += v[k] * (c < 64u ? f0 : f1);
+        }
+    }
+    part[t] = o;
+    __syncthreads();
+    if (grp || !mine || blockIdx.x * (256u / TPR) + t / TPR >= rows) return;
+    for (uint32_t k = 1; k < groups; k++) o += part[t + k * width];
+    const float inv = L == 0.f ? 0.f : __fdiv_rn(1.f, L);
+    float *to = a.out + (uint64_t)(r / group) * a.out_stride + (uint64_t)(kvh * group + r % group) * a.hd + 4u * q;
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; k++)
+        if (4u * q + k < a.hd) to[k] = L == 0.f ? 0.f : o[k] * inv;
+    if (q == 0 && pt.stats) pt.stats[(uint64_t)kvh * rows + r] = make_float2(M, inv);
 }
 
 // ---- the weights that slots received ---------------------------------------------------
@@ -647,27 +798,38 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, const floa
 
 struct RowsPlan {
     uint32_t hd, ct, tiles;  // template head size, column tiles a wave, row tiles a kv head
+    bool few;
     RowsSplit sp;
     size_t ml, acc, stats;  // bytes
 };
+
+// Whether rows of the caches and of q may be read 16 bytes at a time.
+static bool rows_wide_kv(const RowsArgs &a) {
+    return a.hd % 8u == 0 && (((uintptr_t)a.kc | (uintptr_t)a.vc) & 15u) == 0;
+}
+static bool rows_wide_q(const RowsArgs &a) {
+    return a.hd % 8u == 0 && a.q_stride % 4u == 0 && ((uintptr_t)a.q & 15u) == 0;
+}
 
 static RowsPlan rows_plan(const RowsArgs &a) {
     RowsPlan p{};
     p.hd = a.hd <= 32u ? 32u : a.hd <= 64u ? 64u : a.hd <= 96u ? 96u : a.hd <= 128u ? 128u : 256u;
     const uint32_t rows = a.n * (a.nqh / a.nkh), slots = a.past + a.n;
-    p.ct = rows <= 64u || p.hd > 128u ? 1u : 2u;
-    p.tiles = (rows + 64u * p.ct - 1u) / (64u * p.ct);
-    // ranges: until about 512 workgroups share the work, at least 64 slots each
-    const uint32_t most = (slots + 63u) / 64u, wgs = p.tiles * a.nkh;
+    p.few = rows <= 16u && rows_wide_kv(a);
+    p.ct = p.few || rows <= 64u || p.hd > 128u ? 1u : 2u;
+    const uint32_t tile_rows = (p.few ? 16u : 64u) * p.ct;
+    p.tiles = (rows + tile_rows - 1u) / tile_rows;
+    // ranges: until about 512 workgroups share the work, at least a tile a wave or workgroup each
+    const uint32_t least = p.few ? 128u : 64u, most = (slots + least - 1u) / least, wgs = p.tiles * a.nkh;
     uint32_t n = 512u / wgs;
-    n = n < 1u ? 1u : n > most ? most : n > 64u ? 64u : n;
-    p.sp.len = ((slots + n - 1u) / n + 63u) / 64u * 64u;
+    n = n < 1u ? 1u : n > most ? most : n > kMostRanges ? kMostRanges : n;
+    p.sp.len = ((slots + n - 1u) / n + least - 1u) / least * least;
     p.sp.n = (slots + p.sp.len - 1u) / p.sp.len;
     const size_t all = (size_t)rows * a.nkh;
     const auto round = [](size_t b) { return (b + 255u) & ~(size_t)255u; };
     if (p.sp.n > 1u) {
         p.ml = round(all * p.sp.n * sizeof(float2));
-        p.acc = round(all * p.sp.n * a.hd * sizeof(float));
+        p.acc = round(all * p.sp.n * part_stride(a.hd) * sizeof(float));
     }
     if (a.mass) p.stats = round(all * sizeof(float2));
     return p;
@@ -678,18 +840,14 @@ size_t rows_scratch_bytes(const RowsArgs &a) {
     return p.ml + p.acc + p.stats;
 }
 
-// Whether rows of the caches and of q may be read 16 bytes at a time.
-static bool rows_wide_kv(const RowsArgs &a) {
-    return a.hd % 8u == 0 && (((uintptr_t)a.kc | (uintptr_t)a.vc) & 15u) == 0;
-}
-static bool rows_wide_q(const RowsArgs &a) {
-    return a.hd % 8u == 0 && a.q_stride % 4u == 0 && ((uintptr_t)a.q & 15u) == 0;
-}
-
 template <uint32_t HD>
 static void start_rows(const RowsArgs &a, const RowsPlan &p, const RowsPart &pt, hipStream_t s) {
     const bool wide_kv = rows_wide_kv(a), wide_q = rows_wide_q(a);
     const uint32_t grid = p.tiles * p.sp.n * a.nkh;
+    if (p.few) {
+        k_rows_few<HD, 1><<<grid, 256, 0, s>>>(a, p.sp, pt, wide_q);
+        return;
+    }
     if constexpr (HD <= 128u) {
         if (p.ct == 2u) {
             k_rows<HD, 2><<<grid, 256, 0, s>>>(a, p.sp, pt, p.tiles, wide_kv, wide_q);
@@ -723,7 +881,13 @@ hipError_t launch_rows(const RowsArgs &a, void *scratch, hipStream_t s) {
     hipError_t e = hipGetLastError();
     const uint32_t rows = a.n * (a.nqh / a.nkh);
     if (e == hipSuccess && p.sp.n > 1u) {
-        k_rows_merge<<<dim3(rows, a.nkh), 256, 0, s>>>(a, p.sp, pt, 64u * p.ct);
+        const uint32_t tile_rows = (p.few ? 16u : 64u) * p.ct;
+        const uint32_t width = a.hd <= 32u ? 8u : a.hd <= 64u ? 16u : a.hd <= 128u ? 32u : 64u;  // float4s of a row
+        // a wave per row where its lanes hold every range in one round of loads
+        if (p.sp.n <= 8u * (64u / width))
+            k_rows_merge<64><<<dim3((rows + 3u) / 4u, a.nkh), 256, 0, s>>>(a, p.sp, pt, tile_rows, width);
+        else
+            k_rows_merge<256><<<dim3(rows, a.nkh), 256, 0, s>>>(a, p.sp, pt, tile_rows, width);
         e = hipGetLastError();
     }
     if (e == hipSuccess && a.mass) {
