@@ -11,8 +11,8 @@
 // nothing from it, whatever is in its K and V.
 //
 // The (token, q head) pairs of a kv head are its rows, n * group of them, row r =
-// i * group + g. A workgroup takes 64 CT rows of one kv head (16 CT a wave) and a
-// range of slots, 64 (32 for head_dim above 128) at a time through LDS, on
+// i * group + g. A workgroup takes 64 rows of one kv head (16 a wave) and a range of
+// slots, 64 (32 for head_dim above 128) at a time through LDS, on
 // v_mfma_f32_16x16x32_f16:
 // * S^T = K Q^T: A = 16 slots x 32 dims of K (the cache's f16, exact), B = 32 dims
 //   x 16 rows of q' = q 2^s, s so that the row's largest |q'| lies in [2^14, 2^15),
@@ -69,44 +69,85 @@ __device__ __forceinline__ uint64_t seen_bits(const RowsArgs &a, uint32_t i, uin
     return in & v;
 }
 
-// The q' parts of one row (column lane & 15) for lane group g: dims 32 kk + 8 g ...
-// `row` NULL: zeros. c: |scale| 2^-s, what a product of the parts is to be scaled by.
+// One row of q (column lane & 15), lane group g's part: dims 32 kk + 8 g ..
 template <uint32_t KK>
-__device__ __forceinline__ void row_parts(const float *row, uint32_t hd, bool wide, float scale, uint32_t g,
-                                          rh8 (&hi)[KK], rh8 (&lo)[KK], float &c) {
-    float x[KK][8], top = 0.f;
+struct RowQ {
+    float x[KK][8];
+    // `row` NULL: zeros
+    __device__ __forceinline__ void load(const float *row, uint32_t hd, bool wide, uint32_t g) {
 #pragma unroll
-    for (uint32_t kk = 0; kk < KK; kk++) {
-        const uint32_t d0 = 32u * kk + 8u * g;
-        if (row && wide && d0 < hd) {
-            const float4 u = *reinterpret_cast<const float4 *>(row + d0), v = *reinterpret_cast<const float4 *>(row + d0 + 4u);
-            x[kk][0] = u.x, x[kk][1] = u.y, x[kk][2] = u.z, x[kk][3] = u.w;
-            x[kk][4] = v.x, x[kk][5] = v.y, x[kk][6] = v.z, x[kk][7] = v.w;
-        } else {
+        for (uint32_t kk = 0; kk < KK; kk++) {
+            const uint32_t d0 = 32u * kk + 8u * g;
+            if (row && wide && d0 < hd) {
+                const rf4 u = *reinterpret_cast<const rf4 *>(row + d0), v = *reinterpret_cast<const rf4 *>(row + d0 + 4u);
 #pragma unroll
-            for (uint32_t e = 0; e < 8u; e++) x[kk][e] = row && !wide && d0 + e < hd ? row[d0 + e] : 0.f;
+                for (uint32_t e = 0; e < 4u; e++) x[kk][e] = u[e], x[kk][4u + e] = v[e];
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < 8u; e++) x[kk][e] = row && !wide && d0 + e < hd ? row[d0 + e] : 0.f;
+            }
         }
-#pragma unroll
-        for (uint32_t e = 0; e < 8u; e++) top = fmaxf(top, fabsf(x[kk][e]));
     }
-    top = fmaxf(top, lane_xor<16>(top));
-    top = fmaxf(top, lane_xor<32>(top));
-    int e2 = 0;
-    (void)frexpf(top, &e2);  // top < 2^e2
-    // (a row below 2^-111 scores nothing that an f32 sum keeps; 2^-sq must stay a number)
-    const int sq = top > 0.f && top < INFINITY ? (15 - e2 < 126 ? 15 - e2 : 126) : 0;
-    c = fmaxf(ldexpf(fabsf(scale), -sq), 0x1p-126f);  // (not 0: masked scores are -inf times it)
-    const float sign = scale < 0.f ? -1.f : 1.f;
+    // its parts, and c: |scale| 2^-s, what a product of the parts is to be scaled by
+    __device__ __forceinline__ void split(float scale, rh8 (&hi)[KK], rh8 (&lo)[KK], float &c) const {
+        float top = 0.f;
 #pragma unroll
-    for (uint32_t kk = 0; kk < KK; kk++)
+        for (uint32_t kk = 0; kk < KK; kk++)
 #pragma unroll
-        for (uint32_t e = 0; e < 8u; e++) {
-            const float y = ldexpf(x[kk][e] * sign, sq);
-            const _Float16 h = (_Float16)y;
-            hi[kk][e] = h;
-            lo[kk][e] = (_Float16)(y - (float)h);
+            for (uint32_t e = 0; e < 8u; e++) top = fmaxf(top, fabsf(x[kk][e]));
+        top = fmaxf(top, lane_xor<16>(top));
+        top = fmaxf(top, lane_xor<32>(top));
+        int e2 = 0;
+        (void)frexpf(top, &e2);  // top < 2^e2
+        // (a row below 2^-111 scores nothing that an f32 sum keeps; 2^-sq must stay a number)
+        const int sq = top > 0.f && top < INFINITY ? (15 - e2 < 126 ? 15 - e2 : 126) : 0;
+        c = fmaxf(ldexpf(fabsf(scale), -sq), 0x1p-126f);  // (not 0: masked scores are -inf times it)
+        const float sign = scale < 0.f ? -1.f : 1.f;
+#pragma unroll
+        for (uint32_t kk = 0; kk < KK; kk++)
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; e += 2u) {
+                const rf2 y = {ldexpf(x[kk][e] * sign, sq), ldexpf(x[kk][e + 1u] * sign, sq)};
+                const rh2 h = __builtin_convertvector(y, rh2);
+                const rf2 r = {less_low(y[0], h), less_high(y[1], h)};
+                const rh2 q = __builtin_convertvector(r, rh2);
+                hi[kk][e] = h[0], hi[kk][e + 1u] = h[1];
+                lo[kk][e] = q[0], lo[kk][e + 1u] = q[1];
+            }
+    }
+};
+
+// The documents of the tokens i0 .. i1 lie in [lo, hi]: slots of others are not looked at.
+struct DocRange {
+    int32_t lo, hi;
+    __device__ __forceinline__ DocRange(const RowsArgs &a, uint32_t i0, uint32_t i1, uint32_t lane) {
+        lo = 0x7FFFFFFF, hi = -0x7FFFFFFF - 1;
+        if (!a.docs) return;
+        for (uint32_t i = i0 + lane; i <= i1; i += 64u) {
+            const int32_t d = a.docs[a.past + i];
+            lo = min(lo, d), hi = max(hi, d);
         }
-}
+#pragma unroll
+        for (int o = 32; o; o >>= 1) lo = min(lo, __shfl_xor(lo, o, 64)), hi = max(hi, __shfl_xor(hi, o, 64));
+    }
+    // The first tile of T slots from p on (p a tile's first slot, up to s1) that holds a slot of the range; s1
+    // if none does. 256 slots are looked at in one round of loads.
+    template <uint32_t T>
+    __device__ __forceinline__ uint32_t next(const RowsArgs &a, uint32_t p, uint32_t s1, uint32_t lane) const {
+        if (!a.docs) return p;
+        for (; p < s1; p += 256u) {
+            int32_t d[4];
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; k++) d[k] = a.docs[min(p + 64u * k + lane, s1 - 1u)];
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; k++) {
+                const uint64_t in = __ballot(p + 64u * k + lane < s1 && d[k] >= lo && d[k] <= hi);
+                if (in) return p + 64u * k + (uint32_t)(__ffsll((unsigned long long)in) - 1) / T * T;
+            }
+        }
+        return s1;
+    }
+};
 
 // Eight cache elements of a row from element d0 on (zeros from hd on).
 __device__ __forceinline__ ru4 cache8(const uint16_t *p, uint32_t d0, uint32_t hd, bool wide) {
@@ -167,18 +208,21 @@ __device__ __forceinline__ rs4 lds_transposed(const uint8_t *p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) rs4 *)(uint32_t)(uintptr_t)p);
 }
 
-// The rows of one wave: CT column tiles of 16, their q' parts and their running sums.
-template <uint32_t HD, uint32_t CT>
-struct RowTiles {
+// Sixteen rows of a wave (one a column): their q' parts and their running sums.
+template <uint32_t HD>
+struct RowTile {
     static constexpr uint32_t KK = HD / 32u, DT = HD / 16u, RB = HD * 2u;
-    static constexpr uint32_t NK = KK < 4u ? KK : 4u, NV = DT < 8u ? DT : 8u;  // (dims from 128 on lie 256 bytes on)
-    rh8 qh[CT][KK], ql[CT][KK];
-    float c1[CT], slope[CT], m[CT], l[CT];
-    uint32_t tok[CT];
-    int32_t doc[CT];
-    bool real[CT];
-    rf4 acc[DT][CT];
-    uint32_t kat[NK], vat[NV];  // where the lane reads in LDS, from a tile's first byte of K
+    // where the lane reads in LDS, from a tile's first byte of K: where places are xors, one address
+    // each for K and V and the slice or dim tile xored in, else (96) one per slice and dim tile
+    static constexpr bool XOR = HD != 96u;
+    static constexpr uint32_t NK = XOR ? 1u : KK, NV = XOR ? 1u : DT;
+    rh8 qh[KK], ql[KK];
+    float c1, slope, m, l;
+    uint32_t tok;
+    int32_t doc;
+    bool real;
+    rf4 acc[DT];
+    uint32_t kat[NK], vat[NV];
     // below `clear` every row sees every slot (documents aside); from `last` on, none
     uint32_t clear, last;
 
@@ -186,22 +230,20 @@ struct RowTiles {
     __device__ __forceinline__ void init(const RowsArgs &a, uint32_t kvh, uint32_t row0, bool wide_q, uint32_t lane,
                                          uint32_t v_at) {
         const uint32_t col = lane & 15u, g = lane >> 4, group = a.nqh / a.nkh, rows = a.n * group;
+        const uint32_t r = row0 + col;
+        real = r < rows;
+        tok = real ? r / group : 0u;
+        const uint32_t h = kvh * group + (real ? r % group : 0u);
+        RowQ<KK> x;
+        x.load(real ? a.q + (uint64_t)tok * a.q_stride + (uint64_t)h * a.hd : nullptr, a.hd, wide_q, g);
+        slope = a.slopes ? a.slopes[h] : 0.f;
+        doc = a.docs ? a.docs[a.past + tok] : 0;
+        x.split(a.scale, qh, ql, c1);
+        m = -INFINITY, l = 0.f;
 #pragma unroll
-        for (uint32_t x = 0; x < CT; x++) {
-            const uint32_t r = row0 + 16u * x + col;
-            real[x] = r < rows;
-            tok[x] = real[x] ? r / group : 0u;
-            const uint32_t h = kvh * group + (real[x] ? r % group : 0u);
-            row_parts<KK>(real[x] ? a.q + (uint64_t)tok[x] * a.q_stride + (uint64_t)h * a.hd : nullptr, a.hd, wide_q,
-                          a.scale, g, qh[x], ql[x], c1[x]);
-            slope[x] = a.slopes ? a.slopes[h] : 0.f;
-            doc[x] = a.docs ? a.docs[a.past + tok[x]] : 0;
-            m[x] = -INFINITY, l[x] = 0.f;
-#pragma unroll
-            for (uint32_t d = 0; d < DT; d++) acc[d][x] = rf4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (uint32_t d = 0; d < DT; d++) acc[d] = rf4{0.f, 0.f, 0.f, 0.f};
         clear = a.docs ? 0u : a.mask ? a.past : row_end(a, min(row0, rows - 1u) / group);
-        last = row0 < rows ? row_end(a, (min(row0 + 16u * CT, rows) - 1u) / group) : 0u;
+        last = row0 < rows ? row_end(a, (min(row0 + 16u, rows) - 1u) / group) : 0u;
         // its chunk of K per slice (row `col` of a 16-row tile), and per 16 dims its part of the
         // transposed V read: slot 4 g + col / 4, dims 4 (col % 4) ..
 #pragma unroll
@@ -213,6 +255,14 @@ struct RowTiles {
         }
     }
 
+    // (dims from 128 on lie 256 bytes on)
+    __device__ __forceinline__ uint32_t k_at(uint32_t kk) const {
+        return XOR ? (kat[0] ^ 64u * (kk & 3u)) + 256u * (kk >> 2) : kat[XOR ? 0u : kk];
+    }
+    __device__ __forceinline__ uint32_t v_at(uint32_t d) const {
+        return XOR ? (vat[0] ^ 32u * (d & 7u)) + 256u * (d >> 3) : vat[XOR ? 0u : d];
+    }
+
     __device__ __forceinline__ void turn(uint32_t by) {  // on to another buffer
 #pragma unroll
         for (uint32_t kk = 0; kk < NK; kk++) kat[kk] += by;
@@ -221,149 +271,120 @@ struct RowTiles {
     }
 
     // 32 slots from p0 on, in LDS from row `at` of the tile; full: every row sees them all, else vis
-    // holds their bits per column tile and docs (or NULL) their documents
-    __device__ __forceinline__ void step(const RowsArgs &a, const uint8_t *lds, uint32_t at, uint32_t p0,
-                                         const uint32_t (&vis)[CT], bool full, const int32_t *docs, uint32_t lane) {
+    // holds their bits and docs (or NULL) their documents
+    __device__ __forceinline__ void step(const RowsArgs &a, const uint8_t *lds, uint32_t at, uint32_t p0, uint32_t vis,
+                                         bool full, const int32_t *docs, uint32_t lane) {
         const uint32_t g = lane >> 4;
-        const bool terms = a.cap > 0.f || a.slopes;
-        rf4 S[2][CT];
+        rf4 S[2] = {rf4{0.f, 0.f, 0.f, 0.f}, rf4{0.f, 0.f, 0.f, 0.f}};
+        // (each slice's K is read while the one before it is multiplied, V two dim tiles ahead: left to itself the
+        // compiler waits for every read in turn)
+        rh8 ka[2][2], va[3];
+        auto read_k = [&](uint32_t kk) {
 #pragma unroll
-        for (uint32_t hf = 0; hf < 2u; hf++)
-#pragma unroll
-            for (uint32_t x = 0; x < CT; x++) S[hf][x] = rf4{0.f, 0.f, 0.f, 0.f};
+            for (uint32_t hf = 0; hf < 2u; hf++)
+                ka[kk & 1u][hf] = *reinterpret_cast<const rh8 *>(lds + k_at(kk) + (at + 16u * hf) * RB);
+        };
+        auto read_v = [&](uint32_t d) {
+            const uint8_t *v = lds + v_at(d) + at * RB;
+            const rs4 v0 = lds_transposed(v), v1 = lds_transposed(v + 16u * RB);
+            va[d % 3u] = __builtin_bit_cast(rh8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        read_k(0u);
 #pragma unroll
         for (uint32_t kk = 0; kk < KK; kk++) {
-            rh8 ka[2];
+            if (kk + 1u < KK) read_k(kk + 1u);
+            if (kk + 1u == KK) read_v(0u), read_v(1u);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (uint32_t hf = 0; hf < 2u; hf++)
-                ka[hf] = *reinterpret_cast<const rh8 *>(lds + kat[kk & 3u] + 256u * (kk >> 2) + (at + 16u * hf) * RB);
+                S[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[kk & 1u][hf], qh[kk], S[hf], 0, 0, 0);
 #pragma unroll
             for (uint32_t hf = 0; hf < 2u; hf++)
-#pragma unroll
-                for (uint32_t x = 0; x < CT; x++)
-                    S[hf][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[hf], qh[x][kk], S[hf][x], 0, 0, 0);
-#pragma unroll
-            for (uint32_t hf = 0; hf < 2u; hf++)
-#pragma unroll
-                for (uint32_t x = 0; x < CT; x++)
-                    S[hf][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[hf], ql[x][kk], S[hf][x], 0, 0, 0);
+                S[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[kk & 1u][hf], ql[kk], S[hf], 0, 0, 0);
         }
         // the score in units of log2 is cm S: S the plain product, or what the terms make of it
-        float cm[CT];
-#pragma unroll
-        for (uint32_t x = 0; x < CT; x++) cm[x] = c1[x] * kLog2e;
-        if (terms) {
+        float cm = c1 * kLog2e;
+        if (a.cap > 0.f || a.slopes) {
             float unit = 1.f;
             if (a.cap > 0.f) {
                 float far = 0.f;
 #pragma unroll
-                for (uint32_t x = 0; x < CT; x++)
+                for (uint32_t hf = 0; hf < 2u; hf++) {
+                    S[hf] *= c1 * a.rcap;
 #pragma unroll
-                    for (uint32_t hf = 0; hf < 2u; hf++) {
-                        S[hf][x] *= c1[x] * a.rcap;
-#pragma unroll
-                        for (uint32_t k = 0; k < 4u; k++) far = fmaxf(far, fabsf(S[hf][x][k]));
-                    }
+                    for (uint32_t k = 0; k < 4u; k++) far = fmaxf(far, fabsf(S[hf][k]));
+                }
                 // (most scores lie well below the cap: the polynomial alone then serves the wave)
                 if (__any(far >= kTanhPoly)) {
 #pragma unroll
-                    for (uint32_t x = 0; x < CT; x++)
-#pragma unroll
-                        for (uint32_t j = 0; j < 8u; j++) S[j >> 2][x][j & 3u] = tanh_any(S[j >> 2][x][j & 3u]);
+                    for (uint32_t j = 0; j < 8u; j++) S[j >> 2][j & 3u] = tanh_any(S[j >> 2][j & 3u]);
                 } else {
 #pragma unroll
-                    for (uint32_t x = 0; x < CT; x++)
-#pragma unroll
-                        for (uint32_t j = 0; j < 8u; j++) S[j >> 2][x][j & 3u] = tanh_poly(S[j >> 2][x][j & 3u]);
+                    for (uint32_t j = 0; j < 8u; j++) S[j >> 2][j & 3u] = tanh_poly(S[j >> 2][j & 3u]);
                 }
                 unit = a.cap;
             } else {
-#pragma unroll
-                for (uint32_t x = 0; x < CT; x++) S[0][x] *= c1[x], S[1][x] *= c1[x];
+                S[0] *= c1, S[1] *= c1;
             }
             if (a.slopes) {
 #pragma unroll
-                for (uint32_t x = 0; x < CT; x++)
-#pragma unroll
-                    for (uint32_t j = 0; j < 8u; j++)
-                        S[j >> 2][x][j & 3u] = row_far(S[j >> 2][x][j & 3u] * unit, slope[x], a.past + tok[x],
-                                                       p0 + 16u * (j >> 2) + 4u * g + (j & 3u));
+                for (uint32_t j = 0; j < 8u; j++)
+                    S[j >> 2][j & 3u] = row_far(S[j >> 2][j & 3u] * unit, slope, a.past + tok,
+                                                p0 + 16u * (j >> 2) + 4u * g + (j & 3u));
                 unit = 1.f;
             }
-#pragma unroll
-            for (uint32_t x = 0; x < CT; x++) cm[x] = unit * kLog2e;
+            cm = unit * kLog2e;
         }
         if (!full) {
 #pragma unroll
-            for (uint32_t x = 0; x < CT; x++)
-#pragma unroll
-                for (uint32_t j = 0; j < 8u; j++) {
-                    const uint32_t o = 16u * (j >> 2) + 4u * g + (j & 3u);
-                    bool sees = vis[x] >> o & 1u;
-                    if (docs) sees = sees && docs[o] == doc[x];
-                    if (!sees) S[j >> 2][x][j & 3u] = -INFINITY;
-                }
-        }
-        float top[CT];
-        bool up = false;
-#pragma unroll
-        for (uint32_t x = 0; x < CT; x++) {
-            float v = S[0][x][0];
-#pragma unroll
-            for (uint32_t j = 1; j < 8u; j++) v = fmaxf(v, S[j >> 2][x][j & 3u]);
-            top[x] = v * cm[x];
-            up = up || top[x] > m[x] + kLazy;
-        }
-        if (__any(up)) {
-#pragma unroll
-            for (uint32_t x = 0; x < CT; x++) {
-                float v = fmaxf(top[x], lane_xor<16>(top[x]));
-                v = fmaxf(v, lane_xor<32>(v));
-                const float mn = v > m[x] + kLazy ? v : m[x];
-                const float f = mn == -INFINITY ? 1.f : exp2f(m[x] - mn);
-                m[x] = mn;
-                l[x] *= f;
-#pragma unroll
-                for (uint32_t d = 0; d < DT; d++) acc[d][x] *= f;
+            for (uint32_t j = 0; j < 8u; j++) {
+                const uint32_t o = 16u * (j >> 2) + 4u * g + (j & 3u);
+                bool sees = vis >> o & 1u;
+                if (docs) sees = sees && docs[o] == doc;
+                if (!sees) S[j >> 2][j & 3u] = -INFINITY;
             }
         }
-        rh8 ph[CT], pl[CT];
+        float top = S[0][0];
 #pragma unroll
-        for (uint32_t x = 0; x < CT; x++) {
-            const float ms = m[x] == -INFINITY ? 0.f : m[x] - kLift;
+        for (uint32_t j = 1; j < 8u; j++) top = fmaxf(top, S[j >> 2][j & 3u]);
+        top *= cm;
+        if (__any(top > m + kLazy)) {
+            top = fmaxf(top, lane_xor<16>(top));
+            top = fmaxf(top, lane_xor<32>(top));
+            const float mn = top > m + kLazy ? top : m, f = mn == -INFINITY ? 1.f : exp2f(m - mn);
+            m = mn;
+            l *= f;
 #pragma unroll
-            for (uint32_t j = 0; j < 8u; j += 2u) {
-                rf2 p;
-                p[0] = __builtin_amdgcn_exp2f(fmaf(S[j >> 2][x][j & 3u], cm[x], -ms));
-                p[1] = __builtin_amdgcn_exp2f(fmaf(S[j >> 2][x][(j & 3u) + 1u], cm[x], -ms));
-                l[x] += p[0];
-                l[x] += p[1];
-                const rh2 h = __builtin_convertvector(p, rh2);
-                const rf2 r = {less_low(p[0], h), less_high(p[1], h)};
-                const rh2 q = __builtin_convertvector(r, rh2);
-                ph[x][j] = h[0], ph[x][j + 1u] = h[1];
-                pl[x][j] = q[0], pl[x][j + 1u] = q[1];
-            }
+            for (uint32_t d = 0; d < DT; d++) acc[d] *= f;
+        }
+        rh8 ph, pl;
+        const float ms = m == -INFINITY ? 0.f : m - kLift;
+#pragma unroll
+        for (uint32_t j = 0; j < 8u; j += 2u) {
+            rf2 p;
+            p[0] = __builtin_amdgcn_exp2f(fmaf(S[j >> 2][j & 3u], cm, -ms));
+            p[1] = __builtin_amdgcn_exp2f(fmaf(S[j >> 2][(j & 3u) + 1u], cm, -ms));
+            l += p[0];
+            l += p[1];
+            const rh2 h = __builtin_convertvector(p, rh2);
+            const rf2 r = {less_low(p[0], h), less_high(p[1], h)};
+            const rh2 q = __builtin_convertvector(r, rh2);
+            ph[j] = h[0], ph[j + 1u] = h[1];
+            pl[j] = q[0], pl[j + 1u] = q[1];
         }
 #pragma unroll
         for (uint32_t d = 0; d < DT; d++) {
-            const uint8_t *v = lds + vat[d & 7u] + 256u * (d >> 3) + at * RB;
-            const rs4 v0 = lds_transposed(v), v1 = lds_transposed(v + 16u * RB);
-            const rh8 va = __builtin_bit_cast(rh8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-            for (uint32_t x = 0; x < CT; x++) acc[d][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[x], acc[d][x], 0, 0, 0);
-#pragma unroll
-            for (uint32_t x = 0; x < CT; x++) acc[d][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[x], acc[d][x], 0, 0, 0);
+            if (d + 2u < DT) read_v(d + 2u);
+            __builtin_amdgcn_sched_barrier(0);
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[d % 3u], ph, acc[d], 0, 0, 0);
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[d % 3u], pl, acc[d], 0, 0, 0);
         }
     }
 
     // l over the four lane groups of a row
     __device__ __forceinline__ void sum_l() {
-#pragma unroll
-        for (uint32_t x = 0; x < CT; x++) {
-            l[x] += lane_xor<16>(l[x]);
-            l[x] += lane_xor<32>(l[x]);
-        }
+        l += lane_xor<16>(l);
+        l += lane_xor<32>(l);
     }
 };
 
@@ -403,7 +424,7 @@ __device__ __forceinline__ void row_again(const RowsArgs &a, const RowsSplit &sp
 }
 
 // ---- many rows: four waves with rows of their own, slots through two shared buffers ------
-template <uint32_t HD, uint32_t CT>
+template <uint32_t HD>
 __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsPart pt, uint32_t tiles, bool wide_kv,
                                                  bool wide_q) {
     constexpr uint32_t DT = HD / 16u, T = kTile<HD>, CPR = HD / 8u, NC = T * CPR / 256u;
@@ -413,12 +434,12 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
     const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u, col = lane & 15u, g = lane >> 4;
     const uint32_t kvh = blockIdx.x % a.nkh, rest = blockIdx.x / a.nkh;
     const uint32_t split = rest % sp.n, tile = tiles - 1u - rest / sp.n;  // (the longest rows first)
-    const uint32_t group = a.nqh / a.nkh, rows = a.n * group, row_tile = tile * 64u * CT;
-    const uint32_t end = row_end(a, (min(row_tile + 64u * CT, rows) - 1u) / group);
+    const uint32_t group = a.nqh / a.nkh, rows = a.n * group, row_tile = tile * 64u;
+    const uint32_t end = row_end(a, (min(row_tile + 64u, rows) - 1u) / group);
     const uint32_t s0 = split * sp.len, s1 = min(s0 + sp.len, end);
     if (s0 >= s1) return;  // (the whole workgroup; the merge counts the ranges the same way)
-    const uint32_t slots = a.past + a.n, row0 = row_tile + wave * 16u * CT;
-    RowTiles<HD, CT> R;
+    const uint32_t slots = a.past + a.n, row0 = row_tile + wave * 16u;
+    RowTile<HD> R;
     R.init(a, kvh, row0, wide_q, lane, TB);
 
     // ---- staging: tile p0 into buffer b, by LDS DMA (no registers; it arrives by the next wait) or,
@@ -467,78 +488,75 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
         __syncthreads();
     };
 
-    fetch(s0, 0u);
-    arrive(0u);
-    for (uint32_t p0 = s0, b = 0; p0 < s1; p0 += T, b ^= 1u) {
-        const bool more = p0 + T < s1;
-        if (more) fetch(p0 + T, b ^ 1u);
+    const DocRange of(a, row_tile / group, (min(row_tile + 64u, rows) - 1u) / group, lane);
+    uint32_t p0 = of.next<T>(a, s0, s1, lane);
+    if (p0 < s1) {
+        fetch(p0, 0u);
+        arrive(0u);
+    }
+    for (uint32_t b = 0; p0 < s1; b ^= 1u) {
+        const uint32_t p1 = of.next<T>(a, p0 + T, s1, lane);
+        if (p1 < s1) fetch(p1, b ^ 1u);
         if (p0 < R.last) {
             const bool full = p0 + T <= min(R.clear, s1);
-            uint64_t vis[CT];
+            const uint64_t vis = full ? ~0ull : R.real ? seen_bits(a, R.tok, p0, s1) : 0ull;
 #pragma unroll
-            for (uint32_t x = 0; x < CT; x++) vis[x] = full ? ~0ull : R.real[x] ? seen_bits(a, R.tok[x], p0, s1) : 0ull;
-#pragma unroll
-            for (uint32_t h = 0; h < T / 32u; h++) {
-                uint32_t v[CT];
-#pragma unroll
-                for (uint32_t x = 0; x < CT; x++) v[x] = (uint32_t)(vis[x] >> (32u * h));
-                R.step(a, &kv[0][0][0], 32u * h, p0 + 32u * h, v, full, a.docs ? &dl[b][32u * h] : nullptr, lane);
-            }
+            for (uint32_t h = 0; h < T / 32u; h++)
+                R.step(a, &kv[0][0][0], 32u * h, p0 + 32u * h, (uint32_t)(vis >> (32u * h)), full,
+                       a.docs ? &dl[b][32u * h] : nullptr, lane);
         }
-        if (more) arrive(b ^ 1u);
+        if (p1 < s1) arrive(b ^ 1u);
         R.turn(b ? 0u - 2u * TB : 2u * TB);
+        p0 = p1;
     }
     if (row0 >= rows) return;
 
     // ---- the rows' sums
     R.sum_l();
     const bool wide_to = a.hd % 4u == 0 && (a.out_stride % 4u == 0 && ((uintptr_t)a.out & 15u) == 0);
+    float nan = R.l * 0.f;
 #pragma unroll
-    for (uint32_t x = 0; x < CT; x++) {
-        float nan = R.l[x] * 0.f;
+    for (uint32_t d = 0; d < DT; d++)
 #pragma unroll
-        for (uint32_t d = 0; d < DT; d++)
+        for (uint32_t k = 0; k < 4u; k++) nan = fmaf(R.acc[d][k], 0.f, nan);
+    const uint64_t bad = __ballot(R.real && nan != 0.f);  // (0 times anything finite is 0)
+    const uint32_t cols = (uint32_t)(bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xFFFFu;
+    if (R.real && !(cols >> col & 1u)) {
+        const RowsTo to(a, sp, pt, kvh, split, row0 + col);
+        const float inv = to.scale(R.l);
 #pragma unroll
-            for (uint32_t k = 0; k < 4u; k++) nan = fmaf(R.acc[d][x][k], 0.f, nan);
-        const uint64_t bad = __ballot(R.real[x] && nan != 0.f);  // (0 times anything finite is 0)
-        const uint32_t cols = (uint32_t)(bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xFFFFu;
-        if (R.real[x] && !(cols >> col & 1u)) {
-            const RowsTo to(a, sp, pt, kvh, split, row0 + 16u * x + col);
-            const float inv = to.scale(R.l[x]);
+        for (uint32_t d = 0; d < DT; d++) {
+            const uint32_t d0 = 16u * d + 4u * g;
+            if (to.ml || wide_to) {  // (the partials' rows are whole float4s)
+                if (d0 < a.hd) *reinterpret_cast<rf4 *>(to.acc + d0) = R.acc[d] * inv;
+            } else {
 #pragma unroll
-            for (uint32_t d = 0; d < DT; d++) {
-                const uint32_t d0 = 16u * d + 4u * g;
-                if (to.ml || wide_to) {  // (the partials' rows are whole float4s)
-                    if (d0 < a.hd) *reinterpret_cast<rf4 *>(to.acc + d0) = R.acc[d][x] * inv;
-                } else {
-#pragma unroll
-                    for (uint32_t k = 0; k < 4u; k++)
-                        if (d0 + k < a.hd) to.acc[d0 + k] = R.acc[d][x][k] * inv;
-                }
+                for (uint32_t k = 0; k < 4u; k++)
+                    if (d0 + k < a.hd) to.acc[d0 + k] = R.acc[d][k] * inv;
             }
-            if (g == 0) to.put_ml(R.m[x] - kLift, R.l[x]);
         }
-        // rows whose sums are not finite, one at a time
-        for (uint32_t c = 0; cols >> c; c++)
-            if (cols >> c & 1u) row_again<HD>(a, sp, pt, kvh, split, row0 + 16u * x + c, s0, s1, lane);
+        if (g == 0) to.put_ml(R.m - kLift, R.l);
     }
+    // rows whose sums are not finite, one at a time
+    for (uint32_t c = 0; cols >> c; c++)
+        if (cols >> c & 1u) row_again<HD>(a, sp, pt, kvh, split, row0 + c, s0, s1, lane);
 }
 
-// ---- few rows: four waves with the same 16 CT rows, each with slots of its own ---------------
+// ---- few rows: four waves with the same 16 rows, each with slots of its own ---------------
 // A wave takes the 32-slot tiles wave, wave + 4, ... of the range, in an LDS buffer of its own (no barrier
 // until the end), then the waves' sums are added in LDS.
-template <uint32_t HD, uint32_t CT>
+template <uint32_t HD>
 __global__ __launch_bounds__(256, 2) void k_rows_few(RowsArgs a, RowsSplit sp, RowsPart pt, bool wide_q) {
     constexpr uint32_t DT = HD / 16u, T = 32u, CPR = HD / 8u, NC = T * CPR / 64u, RB = HD * 2u, TB = T * RB;
     constexpr uint32_t RS = HD + 4u;  // floats of a row's sums in LDS (the rows of a store in different banks)
-    constexpr uint32_t OWN = 2u * TB > 16u * CT * RS * 4u ? 2u * TB : 16u * CT * RS * 4u;
+    constexpr uint32_t OWN = 2u * TB > 16u * RS * 4u ? 2u * TB : 16u * RS * 4u;
     __shared__ __align__(1024) uint8_t kv[4][OWN];
-    __shared__ float2 mls[4][16u * CT];
-    __shared__ uint32_t bad[16u * CT];
+    __shared__ float2 mls[4][16u];
+    __shared__ uint32_t bad[16u];
     const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63u, col = lane & 15u, g = lane >> 4;
-    const uint32_t kvh = blockIdx.x % a.nkh, rest = blockIdx.x / a.nkh, split = rest % sp.n, row0 = rest / sp.n * 16u * CT;
+    const uint32_t kvh = blockIdx.x % a.nkh, rest = blockIdx.x / a.nkh, split = rest % sp.n, row0 = rest / sp.n * 16u;
     const uint32_t group = a.nqh / a.nkh, rows = a.n * group, slots = a.past + a.n;
-    const uint32_t end = row_end(a, (min(row0 + 16u * CT, rows) - 1u) / group);
+    const uint32_t end = row_end(a, (min(row0 + 16u, rows) - 1u) / group);
     const uint32_t s0 = split * sp.len, s1 = min(s0 + sp.len, end);
     if (s0 >= s1) return;  // (the whole workgroup)
     uint8_t *const own = &kv[wave][0];
@@ -564,20 +582,29 @@ __global__ __launch_bounds__(256, 2) void k_rows_few(RowsArgs a, RowsSplit sp, R
             }
         }
     };
-    uint32_t p0 = s0 + T * wave;
+    const DocRange of(a, row0 / group, (min(row0 + 16u, rows) - 1u) / group, lane);
+    // (the wave's next tile, past those without a slot of the rows' documents)
+    auto next = [&](uint32_t p) {
+        if (a.docs)
+            while (p < s1) {
+                const int32_t d = a.docs[min(p + (lane & 31u), s1 - 1u)];
+                if (__any(d >= of.lo && d <= of.hi)) break;
+                p += 4u * T;
+            }
+        return p;
+    };
+    uint32_t p0 = next(s0 + T * wave);
     if (p0 < s1) fetch(p0);
-    RowTiles<HD, CT> R;
+    RowTile<HD> R;
     R.init(a, kvh, row0, wide_q, lane, TB);
     while (p0 < s1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if (p0 < R.last) {
             const bool full = p0 + T <= min(R.clear, s1);
-            uint32_t vis[CT];
-#pragma unroll
-            for (uint32_t x = 0; x < CT; x++) vis[x] = full ? ~0u : R.real[x] ? (uint32_t)seen_bits(a, R.tok[x], p0, s1) : 0u;
+            const uint32_t vis = full ? ~0u : R.real ? (uint32_t)seen_bits(a, R.tok, p0, s1) : 0u;
             R.step(a, own, 0u, p0, vis, full, a.docs ? a.docs + p0 : nullptr, lane);
         }
-        p0 += 4u * T;
+        p0 = next(p0 + 4u * T);
         if (p0 >= s1) break;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the tile has been read)
         fetch(p0);
@@ -586,16 +613,12 @@ __global__ __launch_bounds__(256, 2) void k_rows_few(RowsArgs a, RowsSplit sp, R
     R.sum_l();
     float *const sums = reinterpret_cast<float *>(own);
 #pragma unroll
-    for (uint32_t x = 0; x < CT; x++) {
-#pragma unroll
-        for (uint32_t d = 0; d < DT; d++)
-            *reinterpret_cast<rf4 *>(sums + (16u * x + col) * RS + 16u * d + 4u * g) = R.acc[d][x];
-        if (g == 0) mls[wave][16u * x + col] = make_float2(R.m[x], R.l[x]);
-    }
-    if (t < 16u * CT) bad[t] = 0;
+    for (uint32_t d = 0; d < DT; d++) *reinterpret_cast<rf4 *>(sums + col * RS + 16u * d + 4u * g) = R.acc[d];
+    if (g == 0) mls[wave][col] = make_float2(R.m, R.l);
+    if (t < 16u) bad[t] = 0;
     __syncthreads();
     const bool wide_to = a.hd % 4u == 0 && a.out_stride % 4u == 0 && ((uintptr_t)a.out & 15u) == 0;
-    for (uint32_t e = t; e < 16u * CT * (HD / 4u); e += 256u) {
+    for (uint32_t e = t; e < 16u * (HD / 4u); e += 256u) {
         const uint32_t r = e / (HD / 4u), d0 = 4u * (e % (HD / 4u));
         if (row0 + r >= rows || d0 >= a.hd) continue;
         float M = -INFINITY, l = 0.f;
@@ -626,7 +649,7 @@ __global__ __launch_bounds__(256, 2) void k_rows_few(RowsArgs a, RowsSplit sp, R
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (a row that is taken again is written after this)
     __syncthreads();
-    for (uint32_t r = wave; r < 16u * CT; r += 4u)
+    for (uint32_t r = wave; r < 16u; r += 4u)
         if (bad[r]) row_again<HD>(a, sp, pt, kvh, split, row0 + r, s0, s1, lane);
 }
 
@@ -689,18 +712,22 @@ __global__ __launch_bounds__(256) void k_rows_merge(RowsArgs a, RowsSplit sp, Ro
 // its waves take the row tiles of 16 in turn (S^T as above) and each lane adds up
 // 2^(y - m) / l for its slots; the 16 columns, then the waves, are summed at the end
 // in a fixed order. A slot whose sum is not finite is taken again in f32 products.
+// Where slots are few, the rows are split over `parts` workgroups and k_mass_add sums
+// what they leave in `part`.
 constexpr uint32_t kMassWaves = 8;
 
 template <uint32_t HD>
 constexpr uint32_t kMassTiles = HD > 128u ? 2u : 4u;
 
 template <uint32_t HD>
-__global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, const float2 *__restrict__ stats, bool wide_kv,
+__global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, const float2 *__restrict__ stats,
+                                                          float *__restrict__ part, uint32_t parts, bool wide_kv,
                                                           bool wide_q) {
     constexpr uint32_t KK = HD / 32u, NT = kMassTiles<HD>, NP = 16u * NT;  // tiles of 16 slots; slots
     __shared__ float sums[kMassWaves][NP];
     const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u, col = lane & 15u, g = lane >> 4;
-    const uint32_t waves = blockDim.x >> 6, kvh = blockIdx.x % a.nkh, p0 = blockIdx.x / a.nkh * NP;
+    const uint32_t waves = blockDim.x >> 6, kvh = blockIdx.x % a.nkh, rest = blockIdx.x / a.nkh;
+    const uint32_t mine = rest % parts, p0 = rest / parts * NP;
     const uint32_t group = a.nqh / a.nkh, rows = a.n * group, slots = a.past + a.n;
     const uint64_t rstride = (uint64_t)a.nkh * a.hd;
     rh8 ka[NT][KK];
@@ -717,21 +744,39 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, const floa
     }
     float sum[NT][4] = {};
     const bool terms = a.cap > 0.f || a.slopes;
-    // the rows before the first that sees p0 (without a mask or a prefix beyond it) are left out
-    const uint32_t r0 = a.mask || p0 < a.prefix || p0 <= a.past ? 0u : (p0 - a.past) * group / 16u;
-    for (uint32_t rt = r0 + wave; 16u * rt < rows; rt += waves) {
+    int32_t lo = 0, hi = 0;  // the slots' documents
+    if (a.docs) {
+        const int32_t d = a.docs[min(p0 + lane % NP, slots - 1u)];
+        lo = hi = d;
+#pragma unroll
+        for (int o = 32; o; o >>= 1) lo = min(lo, __shfl_xor(lo, o, 64)), hi = max(hi, __shfl_xor(hi, o, 64));
+    }
+    // this part's row tiles; those before the first that sees p0 (without a mask or a prefix beyond it) are left out
+    const uint32_t first = a.mask || p0 < a.prefix || p0 <= a.past ? 0u : (p0 - a.past) * group / 16u;
+    const uint32_t all = (rows + 15u) / 16u, per = (all - min(first, all) + parts - 1u) / parts;
+    const uint32_t t0 = first + mine * per, t1 = min(t0 + per, all);
+    RowQ<KK> x;  // (the next tile's rows are on their way while one is worked on)
+    auto fetch = [&](uint32_t rt) {
+        const uint32_t r = 16u * rt + col;
+        x.load(rt < t1 && r < rows ? a.q + (uint64_t)(r / group) * a.q_stride + (uint64_t)(kvh * group + r % group) * a.hd
+                                   : nullptr,
+               a.hd, wide_q, g);
+    };
+    fetch(t0 + wave);
+    for (uint32_t rt = t0 + wave; rt < t1; rt += waves) {
         const uint32_t r = 16u * rt + col;
         const bool real = r < rows;
         const uint32_t i = real ? r / group : 0u, h = kvh * group + (real ? r % group : 0u);
+        const float2 st = real ? stats[(uint64_t)kvh * rows + r] : make_float2(0.f, 0.f);
         rh8 qh[KK], ql[KK];
         float c1;
-        const float2 st = real ? stats[(uint64_t)kvh * rows + r] : make_float2(0.f, 0.f);
-        row_parts<KK>(real ? a.q + (uint64_t)i * a.q_stride + (uint64_t)h * a.hd : nullptr, a.hd, wide_q, a.scale, g, qh,
-                      ql, c1);
+        x.split(a.scale, qh, ql, c1);
+        fetch(rt + waves);
         const bool full = !a.docs && 16u * rt + 16u <= rows &&
                           p0 + NP <= (a.mask ? a.past : row_end(a, 16u * rt / group));
         const uint64_t vis = full ? ~0ull : real ? seen_bits(a, i, p0, slots) : 0ull;
         const int32_t doc = a.docs ? a.docs[a.past + i] : 0;
+        if (a.docs && !__any(doc >= lo && doc <= hi)) continue;
         const float slope = a.slopes ? a.slopes[h] : 0.f, ms = st.x == -INFINITY ? 0.f : st.x;
 #pragma unroll
         for (uint32_t hf = 0; hf < NT; hf++) {
@@ -780,7 +825,7 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, const floa
         const uint32_t jj = p0 + c;
         const uint16_t *k = a.kc + (uint64_t)jj * rstride + (uint64_t)kvh * a.hd;
         float whole = 0.f;
-        for (uint32_t r = lane; r < rows; r += 64u) {
+        for (uint32_t r = 16u * t0 + lane; r < min(16u * t1, rows); r += 64u) {
             const uint32_t i = r / group, h = kvh * group + r % group;
             if (jj >= row_end(a, i) || !row_sees(a, i, jj)) continue;
             const float s = row_score(a, row_dot(a.q + (uint64_t)i * a.q_stride + (uint64_t)h * a.hd, k, a.hd) * a.scale,
@@ -791,16 +836,36 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, const floa
         whole = wave_sum(whole);
         if (lane == c) v = whole;
     }
-    if (in) a.mass[(uint64_t)kvh * a.max_ctx + j] += v;
+    if (!in) return;
+    if (parts > 1u)
+        part[((uint64_t)mine * a.nkh + kvh) * slots + j] = v;
+    else
+        a.mass[(uint64_t)kvh * a.max_ctx + j] += v;
 }
+
+__global__ __launch_bounds__(256) void k_mass_add(RowsArgs a, const float *__restrict__ part, uint32_t parts) {
+    const uint32_t j = blockIdx.x * 256u + threadIdx.x, kvh = blockIdx.y, slots = a.past + a.n;
+    if (j >= slots) return;
+    float v = 0.f;
+    for (uint32_t c = 0; c < parts; c += 8u) {
+        float x[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8u; k++) x[k] = c + k < parts ? part[((uint64_t)(c + k) * a.nkh + kvh) * slots + j] : 0.f;
+#pragma unroll
+        for (uint32_t k = 0; k < 8u; k++) v += x[k];
+    }
+    a.mass[(uint64_t)kvh * a.max_ctx + j] += v;
+}
+
 
 // ---- launches -------------------------------------------------------------------------------
 
 struct RowsPlan {
-    uint32_t hd, ct, tiles;  // template head size, column tiles a wave, row tiles a kv head
+    uint32_t hd, tiles;  // template head size, row tiles a kv head
     bool few;
     RowsSplit sp;
-    size_t ml, acc, stats;  // bytes
+    uint32_t parts;               // of the rows, for the mass
+    size_t ml, acc, stats, mass;  // bytes
 };
 
 // Whether rows of the caches and of q may be read 16 bytes at a time.
@@ -816,8 +881,7 @@ static RowsPlan rows_plan(const RowsArgs &a) {
     p.hd = a.hd <= 32u ? 32u : a.hd <= 64u ? 64u : a.hd <= 96u ? 96u : a.hd <= 128u ? 128u : 256u;
     const uint32_t rows = a.n * (a.nqh / a.nkh), slots = a.past + a.n;
     p.few = rows <= 16u && rows_wide_kv(a);
-    p.ct = p.few || rows <= 64u || p.hd > 128u ? 1u : 2u;
-    const uint32_t tile_rows = (p.few ? 16u : 64u) * p.ct;
+    const uint32_t tile_rows = p.few ? 16u : 64u;
     p.tiles = (rows + tile_rows - 1u) / tile_rows;
     // ranges: until about 512 workgroups share the work, at least a tile a wave or workgroup each
     const uint32_t least = p.few ? 128u : 64u, most = (slots + least - 1u) / least, wgs = p.tiles * a.nkh;
@@ -831,13 +895,20 @@ static RowsPlan rows_plan(const RowsArgs &a) {
         p.ml = round(all * p.sp.n * sizeof(float2));
         p.acc = round(all * p.sp.n * part_stride(a.hd) * sizeof(float));
     }
-    if (a.mass) p.stats = round(all * sizeof(float2));
+    if (a.mass) {
+        p.stats = round(all * sizeof(float2));
+        // about 512 workgroups of eight waves, at least a row tile a wave
+        const uint32_t np = p.hd > 128u ? 32u : 64u, blocks = (slots + np - 1u) / np * a.nkh, waves = (rows + 127u) / 128u;
+        p.parts = blocks >= 512u ? 1u : 512u / blocks;
+        p.parts = p.parts < waves ? p.parts : waves;
+        if (p.parts > 1u) p.mass = round((size_t)p.parts * a.nkh * slots * sizeof(float));
+    }
     return p;
 }
 
 size_t rows_scratch_bytes(const RowsArgs &a) {
     const RowsPlan p = rows_plan(a);
-    return p.ml + p.acc + p.stats;
+    return p.ml + p.acc + p.stats + p.mass;
 }
 
 template <uint32_t HD>
@@ -845,24 +916,17 @@ static void start_rows(const RowsArgs &a, const RowsPlan &p, const RowsPart &pt,
     const bool wide_kv = rows_wide_kv(a), wide_q = rows_wide_q(a);
     const uint32_t grid = p.tiles * p.sp.n * a.nkh;
     if (p.few) {
-        k_rows_few<HD, 1><<<grid, 256, 0, s>>>(a, p.sp, pt, wide_q);
+        k_rows_few<HD><<<grid, 256, 0, s>>>(a, p.sp, pt, wide_q);
         return;
     }
-    if constexpr (HD <= 128u) {
-        if (p.ct == 2u) {
-            k_rows<HD, 2><<<grid, 256, 0, s>>>(a, p.sp, pt, p.tiles, wide_kv, wide_q);
-            return;
-        }
-    }
-    k_rows<HD, 1><<<grid, 256, 0, s>>>(a, p.sp, pt, p.tiles, wide_kv, wide_q);
+    k_rows<HD><<<grid, 256, 0, s>>>(a, p.sp, pt, p.tiles, wide_kv, wide_q);
 }
 
 template <uint32_t HD>
-static void start_mass(const RowsArgs &a, const RowsPart &pt, hipStream_t s) {
-    const uint32_t tiles = (a.n * (a.nqh / a.nkh) + 15u) / 16u;
-    const uint32_t np = 16u * kMassTiles<HD>;
-    k_mass<HD><<<(a.past + a.n + np - 1u) / np * a.nkh, 64u * (tiles < kMassWaves ? tiles : kMassWaves), 0, s>>>(
-        a, pt.stats, rows_wide_kv(a), rows_wide_q(a));
+static void start_mass(const RowsArgs &a, const RowsPlan &p, const RowsPart &pt, float *part, hipStream_t s) {
+    const uint32_t tiles = (a.n * (a.nqh / a.nkh) + 15u) / 16u, np = 16u * kMassTiles<HD>;
+    k_mass<HD><<<(a.past + a.n + np - 1u) / np * a.nkh * p.parts, 64u * (tiles < kMassWaves ? tiles : kMassWaves), 0, s>>>(
+        a, pt.stats, part, p.parts, rows_wide_kv(a), rows_wide_q(a));
 }
 
 hipError_t launch_rows(const RowsArgs &a, void *scratch, hipStream_t s) {
@@ -881,7 +945,7 @@ hipError_t launch_rows(const RowsArgs &a, void *scratch, hipStream_t s) {
     hipError_t e = hipGetLastError();
     const uint32_t rows = a.n * (a.nqh / a.nkh);
     if (e == hipSuccess && p.sp.n > 1u) {
-        const uint32_t tile_rows = (p.few ? 16u : 64u) * p.ct;
+        const uint32_t tile_rows = p.few ? 16u : 64u;
         const uint32_t width = a.hd <= 32u ? 8u : a.hd <= 64u ? 16u : a.hd <= 128u ? 32u : 64u;  // float4s of a row
         // a wave per row where its lanes hold every range in one round of loads
         if (p.sp.n <= 8u * (64u / width))
@@ -891,14 +955,18 @@ hipError_t launch_rows(const RowsArgs &a, void *scratch, hipStream_t s) {
         e = hipGetLastError();
     }
     if (e == hipSuccess && a.mass) {
+        float *part = reinterpret_cast<float *>(at + p.ml + p.acc + p.stats);
         switch (p.hd) {
-            case 32: start_mass<32>(a, pt, s); break;
-            case 64: start_mass<64>(a, pt, s); break;
-            case 96: start_mass<96>(a, pt, s); break;
-            case 128: start_mass<128>(a, pt, s); break;
-            default: start_mass<256>(a, pt, s); break;
+            case 32: start_mass<32>(a, p, pt, part, s); break;
+            case 64: start_mass<64>(a, p, pt, part, s); break;
+            case 96: start_mass<96>(a, p, pt, part, s); break;
+            case 128: start_mass<128>(a, p, pt, part, s); break;
+            default: start_mass<256>(a, p, pt, part, s); break;
         }
         e = hipGetLastError();
+        if (e == hipSuccess && p.parts > 1u)
+            k_mass_add<<<dim3((a.past + a.n + 255u) / 256u, a.nkh), 256, 0, s>>>(a, part, p.parts);
+        if (e == hipSuccess) e = hipGetLastError();
     }
     return e;
 }
