@@ -226,16 +226,21 @@ struct RowTile {
     // below `clear` every row sees every slot (documents aside); from `last` on, none
     uint32_t clear, last;
 
+    // what is read of q (its loads are to be under way before the first tile's, behind which they would wait)
+    __device__ __forceinline__ static void load(const RowsArgs &a, uint32_t kvh, uint32_t row0, bool wide_q, uint32_t lane,
+                                                RowQ<KK> &x) {
+        const uint32_t group = a.nqh / a.nkh, r = row0 + (lane & 15u);
+        x.load(r < a.n * group ? a.q + (uint64_t)(r / group) * a.q_stride + (uint64_t)(kvh * group + r % group) * a.hd : nullptr,
+               a.hd, wide_q, lane >> 4);
+    }
     // v_at: from a tile's first byte of K to its first of V
-    __device__ __forceinline__ void init(const RowsArgs &a, uint32_t kvh, uint32_t row0, bool wide_q, uint32_t lane,
+    __device__ __forceinline__ void init(const RowsArgs &a, uint32_t kvh, uint32_t row0, const RowQ<KK> &x, uint32_t lane,
                                          uint32_t v_at) {
         const uint32_t col = lane & 15u, g = lane >> 4, group = a.nqh / a.nkh, rows = a.n * group;
         const uint32_t r = row0 + col;
         real = r < rows;
         tok = real ? r / group : 0u;
         const uint32_t h = kvh * group + (real ? r % group : 0u);
-        RowQ<KK> x;
-        x.load(real ? a.q + (uint64_t)tok * a.q_stride + (uint64_t)h * a.hd : nullptr, a.hd, wide_q, g);
         slope = a.slopes ? a.slopes[h] : 0.f;
         doc = a.docs ? a.docs[a.past + tok] : 0;
         x.split(a.scale, qh, ql, c1);
@@ -270,37 +275,45 @@ struct RowTile {
         for (uint32_t d = 0; d < NV; d++) vat[d] += by;
     }
 
-    // 32 slots from p0 on, in LDS from row `at` of the tile; full: every row sees them all, else vis
-    // holds their bits and docs (or NULL) their documents
-    __device__ __forceinline__ void step(const RowsArgs &a, const uint8_t *lds, uint32_t at, uint32_t p0, uint32_t vis,
-                                         bool full, const int32_t *docs, uint32_t lane) {
+    // 32 NH slots from p0 on, in LDS; full: every row sees them all, else vis holds their bits and docs (or NULL)
+    // their documents. Slot 16 hf + 4 g + k is element S[hf][k].
+    template <uint32_t NH>
+    __device__ __forceinline__ void step(const RowsArgs &a, const uint8_t *lds, uint32_t p0, uint64_t vis, bool full,
+                                         const int32_t *docs, uint32_t lane) {
+        constexpr uint32_t NS = 2u * NH, ND = DT < 4u ? DT : DT % 4u ? 2u : 4u;  // 16-slot tiles; dim tiles at a time
         const uint32_t g = lane >> 4;
-        rf4 S[2] = {rf4{0.f, 0.f, 0.f, 0.f}, rf4{0.f, 0.f, 0.f, 0.f}};
-        // (each slice's K is read while the one before it is multiplied, V two dim tiles ahead: left to itself the
-        // compiler waits for every read in turn)
-        rh8 ka[2][2], va[3];
+        // A product waits for the one before it into the same sums: the tiles are taken in turn, the high parts
+        // then the low, so that four products lie between. Each slice's K is read while the one before it is
+        // multiplied, and V a group of dim tiles ahead: left to itself the compiler waits for every read in turn.
+        rf4 S[NS];
+        rh8 ka[2][NS], va[2][ND];
+#pragma unroll
+        for (uint32_t i = 0; i < NS; i++) S[i] = rf4{0.f, 0.f, 0.f, 0.f};
         auto read_k = [&](uint32_t kk) {
 #pragma unroll
-            for (uint32_t hf = 0; hf < 2u; hf++)
-                ka[kk & 1u][hf] = *reinterpret_cast<const rh8 *>(lds + k_at(kk) + (at + 16u * hf) * RB);
+            for (uint32_t i = 0; i < NS; i++) ka[kk & 1u][i] = *reinterpret_cast<const rh8 *>(lds + k_at(kk) + 16u * i * RB);
         };
-        auto read_v = [&](uint32_t d) {
-            const uint8_t *v = lds + v_at(d) + at * RB;
-            const rs4 v0 = lds_transposed(v), v1 = lds_transposed(v + 16u * RB);
-            va[d % 3u] = __builtin_bit_cast(rh8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        // group u of V: ND dim tiles of half u % NH
+        auto read_v = [&](uint32_t u) {
+#pragma unroll
+            for (uint32_t d = 0; d < ND; d++) {
+                const uint8_t *v = lds + v_at(u / NH * ND + d) + u % NH * 32u * RB;
+                const rs4 v0 = lds_transposed(v), v1 = lds_transposed(v + 16u * RB);
+                va[u & 1u][d] = __builtin_bit_cast(rh8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+            }
         };
         read_k(0u);
 #pragma unroll
         for (uint32_t kk = 0; kk < KK; kk++) {
-            if (kk + 1u < KK) read_k(kk + 1u);
-            if (kk + 1u == KK) read_v(0u), read_v(1u);
+            if (kk + 1u < KK)
+                read_k(kk + 1u);
+            else
+                read_v(0u);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (uint32_t hf = 0; hf < 2u; hf++)
-                S[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[kk & 1u][hf], qh[kk], S[hf], 0, 0, 0);
+            for (uint32_t i = 0; i < NS; i++) S[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[kk & 1u][i], qh[kk], S[i], 0, 0, 0);
 #pragma unroll
-            for (uint32_t hf = 0; hf < 2u; hf++)
-                S[hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[kk & 1u][hf], ql[kk], S[hf], 0, 0, 0);
+            for (uint32_t i = 0; i < NS; i++) S[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[kk & 1u][i], ql[kk], S[i], 0, 0, 0);
         }
         // the score in units of log2 is cm S: S the plain product, or what the terms make of it
         float cm = c1 * kLog2e;
@@ -309,44 +322,52 @@ struct RowTile {
             if (a.cap > 0.f) {
                 float far = 0.f;
 #pragma unroll
-                for (uint32_t hf = 0; hf < 2u; hf++) {
-                    S[hf] *= c1 * a.rcap;
+                for (uint32_t i = 0; i < NS; i++) {
+                    S[i] *= c1 * a.rcap;
 #pragma unroll
-                    for (uint32_t k = 0; k < 4u; k++) far = fmaxf(far, fabsf(S[hf][k]));
+                    for (uint32_t k = 0; k < 4u; k++) far = fmaxf(far, fabsf(S[i][k]));
                 }
                 // (most scores lie well below the cap: the polynomial alone then serves the wave)
                 if (__any(far >= kTanhPoly)) {
 #pragma unroll
-                    for (uint32_t j = 0; j < 8u; j++) S[j >> 2][j & 3u] = tanh_any(S[j >> 2][j & 3u]);
+                    for (uint32_t i = 0; i < NS; i++)
+#pragma unroll
+                        for (uint32_t k = 0; k < 4u; k++) S[i][k] = tanh_any(S[i][k]);
                 } else {
 #pragma unroll
-                    for (uint32_t j = 0; j < 8u; j++) S[j >> 2][j & 3u] = tanh_poly(S[j >> 2][j & 3u]);
+                    for (uint32_t i = 0; i < NS; i++)
+#pragma unroll
+                        for (uint32_t k = 0; k < 4u; k++) S[i][k] = tanh_poly(S[i][k]);
                 }
                 unit = a.cap;
             } else {
-                S[0] *= c1, S[1] *= c1;
+#pragma unroll
+                for (uint32_t i = 0; i < NS; i++) S[i] *= c1;
             }
             if (a.slopes) {
 #pragma unroll
-                for (uint32_t j = 0; j < 8u; j++)
-                    S[j >> 2][j & 3u] = row_far(S[j >> 2][j & 3u] * unit, slope, a.past + tok,
-                                                p0 + 16u * (j >> 2) + 4u * g + (j & 3u));
+                for (uint32_t i = 0; i < NS; i++)
+#pragma unroll
+                    for (uint32_t k = 0; k < 4u; k++)
+                        S[i][k] = row_far(S[i][k] * unit, slope, a.past + tok, p0 + 16u * i + 4u * g + k);
                 unit = 1.f;
             }
             cm = unit * kLog2e;
         }
         if (!full) {
 #pragma unroll
-            for (uint32_t j = 0; j < 8u; j++) {
-                const uint32_t o = 16u * (j >> 2) + 4u * g + (j & 3u);
-                bool sees = vis >> o & 1u;
-                if (docs) sees = sees && docs[o] == doc;
-                if (!sees) S[j >> 2][j & 3u] = -INFINITY;
-            }
-        }
-        float top = S[0][0];
+            for (uint32_t i = 0; i < NS; i++)
 #pragma unroll
-        for (uint32_t j = 1; j < 8u; j++) top = fmaxf(top, S[j >> 2][j & 3u]);
+                for (uint32_t k = 0; k < 4u; k++) {
+                    const uint32_t o = 16u * i + 4u * g + k;
+                    bool sees = vis >> o & 1ull;
+                    if (docs) sees = sees && docs[o] == doc;
+                    if (!sees) S[i][k] = -INFINITY;
+                }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (uint32_t i = 0; i < NS; i++) top = fmaxf(top, fmaxf(fmaxf(S[i][0], S[i][1]), fmaxf(S[i][2], S[i][3])));
         top *= cm;
         if (__any(top > m + kLazy)) {
             top = fmaxf(top, lane_xor<16>(top));
@@ -357,27 +378,36 @@ struct RowTile {
 #pragma unroll
             for (uint32_t d = 0; d < DT; d++) acc[d] *= f;
         }
-        rh8 ph, pl;
+        rh8 ph[NH], pl[NH];
         const float ms = m == -INFINITY ? 0.f : m - kLift;
+        float sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (uint32_t j = 0; j < 8u; j += 2u) {
+        for (uint32_t j = 0; j < 8u * NH; j += 2u) {
+            const uint32_t i = j >> 2, k = j & 3u, e = j & 7u;
             rf2 p;
-            p[0] = __builtin_amdgcn_exp2f(fmaf(S[j >> 2][j & 3u], cm, -ms));
-            p[1] = __builtin_amdgcn_exp2f(fmaf(S[j >> 2][(j & 3u) + 1u], cm, -ms));
-            l += p[0];
-            l += p[1];
+            p[0] = __builtin_amdgcn_exp2f(fmaf(S[i][k], cm, -ms));
+            p[1] = __builtin_amdgcn_exp2f(fmaf(S[i][k + 1u], cm, -ms));
+            sum[0] += p[0];
+            sum[1] += p[1];
             const rh2 h = __builtin_convertvector(p, rh2);
             const rf2 r = {less_low(p[0], h), less_high(p[1], h)};
             const rh2 q = __builtin_convertvector(r, rh2);
-            ph[j] = h[0], ph[j + 1u] = h[1];
-            pl[j] = q[0], pl[j + 1u] = q[1];
+            ph[j >> 3][e] = h[0], ph[j >> 3][e + 1u] = h[1];
+            pl[j >> 3][e] = q[0], pl[j >> 3][e + 1u] = q[1];
         }
+        l += sum[0] + sum[1];
 #pragma unroll
-        for (uint32_t d = 0; d < DT; d++) {
-            if (d + 2u < DT) read_v(d + 2u);
+        for (uint32_t u = 0; u < DT / ND * NH; u++) {
+            if (u + 1u < DT / ND * NH) read_v(u + 1u);
             __builtin_amdgcn_sched_barrier(0);
-            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[d % 3u], ph, acc[d], 0, 0, 0);
-            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[d % 3u], pl, acc[d], 0, 0, 0);
+#pragma unroll
+            for (uint32_t d = 0; d < ND; d++)
+                acc[u / NH * ND + d] =
+                    __builtin_amdgcn_mfma_f32_16x16x32_f16(va[u & 1u][d], ph[u % NH], acc[u / NH * ND + d], 0, 0, 0);
+#pragma unroll
+            for (uint32_t d = 0; d < ND; d++)
+                acc[u / NH * ND + d] =
+                    __builtin_amdgcn_mfma_f32_16x16x32_f16(va[u & 1u][d], pl[u % NH], acc[u / NH * ND + d], 0, 0, 0);
         }
     }
 
@@ -439,9 +469,6 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
     const uint32_t s0 = split * sp.len, s1 = min(s0 + sp.len, end);
     if (s0 >= s1) return;  // (the whole workgroup; the merge counts the ranges the same way)
     const uint32_t slots = a.past + a.n, row0 = row_tile + wave * 16u;
-    RowTile<HD> R;
-    R.init(a, kvh, row0, wide_q, lane, TB);
-
     // ---- staging: tile p0 into buffer b, by LDS DMA (no registers; it arrives by the next wait) or,
     // where rows are not whole aligned chunks, through registers
     const uint64_t rstride = (uint64_t)a.nkh * a.hd;
@@ -490,20 +517,19 @@ __global__ __launch_bounds__(256, 2) void k_rows(RowsArgs a, RowsSplit sp, RowsP
 
     const DocRange of(a, row_tile / group, (min(row_tile + 64u, rows) - 1u) / group, lane);
     uint32_t p0 = of.next<T>(a, s0, s1, lane);
-    if (p0 < s1) {
-        fetch(p0, 0u);
-        arrive(0u);
-    }
+    RowQ<HD / 32u> x;
+    RowTile<HD>::load(a, kvh, row0, wide_q, lane, x);
+    if (p0 < s1) fetch(p0, 0u);
+    RowTile<HD> R;
+    R.init(a, kvh, row0, x, lane, TB);
+    if (p0 < s1) arrive(0u);
     for (uint32_t b = 0; p0 < s1; b ^= 1u) {
         const uint32_t p1 = of.next<T>(a, p0 + T, s1, lane);
         if (p1 < s1) fetch(p1, b ^ 1u);
         if (p0 < R.last) {
             const bool full = p0 + T <= min(R.clear, s1);
             const uint64_t vis = full ? ~0ull : R.real ? seen_bits(a, R.tok, p0, s1) : 0ull;
-#pragma unroll
-            for (uint32_t h = 0; h < T / 32u; h++)
-                R.step(a, &kv[0][0][0], 32u * h, p0 + 32u * h, (uint32_t)(vis >> (32u * h)), full,
-                       a.docs ? &dl[b][32u * h] : nullptr, lane);
+            R.template step<T / 32u>(a, &kv[0][0][0], p0, vis, full, a.docs ? dl[b] : nullptr, lane);
         }
         if (p1 < s1) arrive(b ^ 1u);
         R.turn(b ? 0u - 2u * TB : 2u * TB);
@@ -594,15 +620,17 @@ __global__ __launch_bounds__(256, 2) void k_rows_few(RowsArgs a, RowsSplit sp, R
         return p;
     };
     uint32_t p0 = next(s0 + T * wave);
+    RowQ<HD / 32u> x;
+    RowTile<HD>::load(a, kvh, row0, wide_q, lane, x);
     if (p0 < s1) fetch(p0);
     RowTile<HD> R;
-    R.init(a, kvh, row0, wide_q, lane, TB);
+    R.init(a, kvh, row0, x, lane, TB);
     while (p0 < s1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if (p0 < R.last) {
             const bool full = p0 + T <= min(R.clear, s1);
-            const uint32_t vis = full ? ~0u : R.real ? (uint32_t)seen_bits(a, R.tok, p0, s1) : 0u;
-            R.step(a, own, 0u, p0, vis, full, a.docs ? a.docs + p0 : nullptr, lane);
+            const uint64_t vis = full ? ~0ull : R.real ? seen_bits(a, R.tok, p0, s1) : 0ull;
+            R.template step<1u>(a, own, p0, vis, full, a.docs ? a.docs + p0 : nullptr, lane);
         }
         p0 = next(p0 + 4u * T);
         if (p0 >= s1) break;
