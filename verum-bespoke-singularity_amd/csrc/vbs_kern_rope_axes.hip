@@ -88,8 +88,15 @@ __global__ __launch_bounds__(256) void k_rope_axes(RopeAxesArgs a, RopeFreqs fr,
 
 hipError_t launch_rope_axes(const RopeAxesArgs &a, float theta, hipStream_t s) {
     const uint32_t pairs = a.hd / 2u, heads = (a.q ? a.nqh : 0u) + (a.k ? a.nkh : 0u);
-    RopeFreqs fr;
-    for (uint32_t p = 0; p < pairs; p++) fr.f[p] = pow((double)theta, -2.0 * p / a.hd);
+    // (kept from one call to the next: 64 powers take about 2 us of a call's 10)
+    static thread_local RopeFreqs fr;
+    static thread_local float fr_theta = 0.f;
+    static thread_local uint32_t fr_hd = 0;
+    if (fr_theta != theta || fr_hd != a.hd) {
+        for (uint32_t p = 0; p < pairs; p++) fr.f[p] = pow((double)theta, -2.0 * p / a.hd);
+        fr_theta = theta;
+        fr_hd = a.hd;
+    }
     const uint32_t rows = 8u;
     k_rope_axes<<<dim3((heads + rows - 1u) / rows, a.n), 256, 0, s>>>(a, fr, rows);
     return hipGetLastError();

@@ -162,7 +162,7 @@ __device__ __forceinline__ ru4 cache8(const uint16_t *p, uint32_t d0, uint32_t h
 }
 
 struct RowsSplit {
-    uint32_t len, n;  // slots per range (a multiple of 64), ranges
+    uint32_t len, n;  // slots per range (a multiple of 128), ranges
 };
 
 // How the launch's scratch is laid out: (m, l) then acc per (kv head, range, row),
@@ -911,11 +911,14 @@ static RowsPlan rows_plan(const RowsArgs &a) {
     p.few = rows <= 16u && rows_wide_kv(a);
     const uint32_t tile_rows = p.few ? 16u : 64u;
     p.tiles = (rows + tile_rows - 1u) / tile_rows;
-    // ranges: until about 512 workgroups share the work, at least a tile a wave or workgroup each
-    const uint32_t least = p.few ? 128u : 64u, most = (slots + least - 1u) / least, wgs = p.tiles * a.nkh;
+    // Ranges: until about 512 workgroups share the work. A range is at least a tile a wave (few) or two tiles of a
+    // workgroup (16 tokens over 2048 slots, 32/8 heads of 128: 11.5 us, one tile 14.5), and 1024 slots where half
+    // the CUs have a workgroup already (777 tokens in documents, 16 heads of 64: 22 us whole, 22 and the merge's 10
+    // in two ranges).
+    const uint32_t wgs = p.tiles * a.nkh, least = !p.few && wgs >= 128u ? 1024u : 128u, most = (slots + least - 1u) / least;
     uint32_t n = 512u / wgs;
     n = n < 1u ? 1u : n > most ? most : n > kMostRanges ? kMostRanges : n;
-    p.sp.len = ((slots + n - 1u) / n + least - 1u) / least * least;
+    p.sp.len = ((slots + n - 1u) / n + 127u) / 128u * 128u;
     p.sp.n = (slots + p.sp.len - 1u) / p.sp.len;
     const size_t all = (size_t)rows * a.nkh;
     const auto round = [](size_t b) { return (b + 255u) & ~(size_t)255u; };
