@@ -239,7 +239,7 @@ int vbs_gfx950_linear_batch_multi(int type, uint32_t n_mat, const void *const *w
  * chunk of a prompt, the drafted tokens of speculative decoding, and single
  * tokens whose attention the plain op does not have. A token is stored in a
  * slot of the cache; its position (for the rotation) may be any number. All:
- * n <= 65535 (0: nothing is done), head_dim even and <= 256, at most 16 q heads
+ * n <= 65535 (0: nothing is done), at most 2^31 slots, head_dim even and <= 256, at most 16 q heads
  * per kv head; a row of q, k, v or out is n_heads x head_dim floats and rows lie
  * a stride (in floats, at least a row) apart, so that the rows of a fused Q/K/V
  * product can be given as they are. No call waits for the device. */

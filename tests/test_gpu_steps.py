@@ -557,3 +557,113 @@ def test_nothing_to_do(dev, mem):
     dev.attention_tree(s.pq, s.qs, s.pk, s.pv, s.po, s.os, 0, 3, mask, 0, s.max_ctx, 2, 1, 32, 1.0)
     dev.attention_chunk(s.pq, s.qs, s.pk, s.pv, s.po, s.os, 0, 4, 0, s.max_ctx, 2, 1, 32, 1.0)
     assert np.array_equal(dev.download(s.po, s.out0.shape, np.float32), s.out0)
+
+
+# ---- few rows (at most 16 of a kv head) and the mass, where they go their own ways ---------------------------
+
+FEW = [(1, 500, 4, 1, 256), (2, 70, 16, 2, 256), (16, 40, 1, 1, 128), (1, 3000, 16, 1, 64), (4, 1000, 4, 1, 96),
+       (1, 127, 2, 1, 32), (3, 333, 10, 2, 80), (1, 0, 16, 1, 128), (5, 4100, 3, 1, 40)]
+
+
+@pytest.mark.parametrize("shape", FEW, ids=["-".join(map(str, s)) for s in FEW])
+@pytest.mark.parametrize("docs", [False, True])
+def test_few_rows(dev, mem, shape, docs):
+    n, past, nqh, nkh, hd = shape
+    rng = np.random.default_rng(past)
+    s = Step(rng, mem, dev, *shape, out_pad=2, q_pad=4)
+    ids = rng.integers(-1, 2, past + n).astype(np.int32) if docs else None
+    mass0 = rng.random((s.layers, nkh, s.max_ctx)).astype(np.float32)
+    slopes = np.linspace(0.5, 0.01, nqh).astype(np.float32)
+    want, w, tol, wtol = s.want(R.sees_chunk(n, past, 0, ids), cap=8.0, slopes=slopes)
+    close(s.chunk(cap=8.0, slopes=slopes, mass=mass0, **({"docs": ids} if docs else {})), want, tol)
+    add, off = R.mass(w, wtol, nkh)
+    got = dev.download(s.pm, mass0.shape, np.float32).astype(np.float64)
+    exp, full = mass0.astype(np.float64), np.zeros_like(got)
+    exp[1, :, :past + n] += add
+    full[1, :, :past + n] = off + 2 * R.F32 * exp[1, :, :past + n]
+    close(got, exp, full)
+
+
+@pytest.mark.parametrize("n,past,nqh,nkh,hd", [(2, 90, 4, 2, 128), (3, 200, 2, 1, 64), (60, 90, 4, 2, 128),
+                                               (200, 30, 8, 1, 80), (40, 10, 2, 1, 6)])
+@pytest.mark.parametrize("bad", [NAN16, INF16, INF16 | 0x8000])
+def test_mass_with_values_that_are_not_finite(dev, mem, n, past, nqh, nkh, hd, bad):
+    """K and V of unseen slots spoil no weight; a seen slot whose score is -inf weighs 0 and leaves the others' alone."""
+    rng = np.random.default_rng(n)
+    docs = (np.arange(past + n) % 5 == 0).astype(np.int32)
+    docs[past:] = 0  # every row is of document 0
+    s = Step(rng, mem, dev, n, past, nqh, nkh, hd)
+    s.kc[1, :past][docs[:past] == 1] = bad
+    s.vc[1, :past][docs[:past] == 1] = bad
+    s.kc[1, 7] = 0
+    s.kc[1, 7, :, 0] = INF16 | 0x8000  # q is positive there: -inf
+    s.q[:, 0::hd] = np.abs(s.q[:, 0::hd]) + 0.1
+    mass0 = np.zeros((2, nkh, s.max_ctx), np.float32)
+    want, w, tol, wtol = s.want(R.sees_chunk(n, past, 0, docs))
+    close(s.chunk(docs=docs, mass=mass0), want, tol)
+    add, off = R.mass(w, wtol, nkh)
+    got = dev.download(s.pm, mass0.shape, np.float32).astype(np.float64)
+    assert np.isfinite(got).all() and (got[1, :, 7] == 0).all() and (got[1, :, :past][:, docs[:past] == 1] == 0).all()
+    close(got[1, :, :past + n], add, off)
+    assert (got[0] == 0).all() and (got[:, :, past + n:] == 0).all()
+
+
+@pytest.mark.parametrize("n,past,hd", [(2, 60, 128), (50, 60, 64), (20, 20, 10)])
+@pytest.mark.parametrize("scale", [0.0, -0.25, 1e-30, 3.0])
+def test_scales(dev, mem, n, past, hd, scale):
+    rng = np.random.default_rng(n)
+    s = Step(rng, mem, dev, n, past, 4, 2, hd)
+    s.scale = float(np.float32(scale))
+    docs = (np.arange(past + n) % 2).astype(np.int32)
+    want, _, tol, _ = s.want(R.sees_chunk(n, past, 0, docs))
+    close(s.chunk(docs=docs), want, tol)
+
+
+@pytest.mark.parametrize("n,past,nqh,nkh,hd", [(200, 1500, 4, 2, 64), (70, 900, 2, 2, 256), (1, 1500, 8, 2, 128),
+                                               (300, 700, 3, 1, 96)])
+@pytest.mark.parametrize("order", ["runs", "mixed", "far"])
+def test_documents_over_many_tiles(dev, mem, n, past, nqh, nkh, hd, order):
+    """Runs of documents (most tiles hold none of a row's), documents in any order, and the largest and least ids."""
+    rng = np.random.default_rng(past)
+    total = past + n
+    docs = np.repeat(np.arange(total), rng.integers(1, 200, total))[:total].astype(np.int32)
+    if order == "mixed":
+        docs = rng.permutation(docs).astype(np.int32)
+    if order == "far":
+        docs = np.where(docs % 2 == 0, np.int32(2**31 - 1), np.int32(-2**31)).astype(np.int32)
+    s = Step(rng, mem, dev, n, past, nqh, nkh, hd)
+    prefix = past + 3
+    want, w, tol, wtol = s.want(R.sees_chunk(n, past, prefix, docs))
+    mass0 = np.zeros((2, nkh, s.max_ctx), np.float32)
+    close(s.chunk(docs=docs, prefix=prefix, mass=mass0), want, tol)
+    add, off = R.mass(w, wtol, nkh)
+    close(dev.download(s.pm, mass0.shape, np.float32)[1, :, :total].astype(np.float64), add, off)
+
+
+@pytest.mark.parametrize("n,past,nqh,nkh,hd", [(1, 200, 8, 2, 128), (2, 77, 2, 2, 64), (70, 33, 2, 1, 96)])
+def test_unaligned_few_and_many(dev, mem, n, past, nqh, nkh, hd):
+    rng = np.random.default_rng(hd)
+    s = Step(rng, mem, dev, n, past, nqh, nkh, hd, shift=3, q_pad=1, out_pad=3)
+    mass0 = np.zeros((2, nkh, s.max_ctx), np.float32)
+    want, w, tol, wtol = s.want(R.sees_chunk(n, past), cap=3.0)
+    close(s.chunk(cap=3.0, mass=mass0), want, tol)
+    add, off = R.mass(w, wtol, nkh)
+    close(dev.download(s.pm, mass0.shape, np.float32)[1, :, :past + n].astype(np.float64), add, off)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+def test_seen_infinities_in_few_rows(dev, mem, hd):
+    """As test_values_that_are_not_finite_and_seen, at one and two rows of a kv head."""
+    rng = np.random.default_rng(hd)
+    s = Step(rng, mem, dev, 2, 300, 2, 1, hd)
+    s.vc[1, 3, 0, 1] = INF16
+    s.kc[1, 5] = 0
+    s.kc[1, 5, 0, 0] = INF16 | 0x8000
+    s.q[:, 0::hd] = np.abs(s.q[:, 0::hd]) + 0.1
+    s.q[1, hd + 1] = np.nan
+    want, _, tol, _ = s.want(R.sees_chunk(2, 300))
+    got = s.chunk()
+    assert np.isnan(got[1, 1]).all() and np.isposinf(got[0, :, 1]).all() and np.isposinf(got[1, 0, 1])
+    got[1, 1] = want[1, 1] = 0
+    tol[1, 1] = 0
+    close(got, want, np.where(np.isnan(tol), 0, tol))

@@ -42,7 +42,7 @@ ATT = dict(q=P, q_stride=256, kc=P, vc=P, out=P2, out_stride=256, n=4, past=10, 
 ATT_BAD = [
     (dict(q=0), "null"), (dict(kc=0), "null"), (dict(vc=0), "null"), (dict(out=0), "null"), (dict(nqh=0), "empty"),
     (dict(nkh=0), "empty"), (dict(hd=0), "empty"), (dict(n=65536, max_ctx=BIG), "65535"), (dict(past=13), "max_ctx"),
-    (dict(past=BIG), "max_ctx"), (dict(nqh=3), "multiple"), (dict(nqh=34), "group"), (dict(hd=65), "even"),
+    (dict(past=BIG), "max_ctx"), (dict(past=1 << 31, max_ctx=BIG), "2.31"), (dict(nqh=3), "multiple"), (dict(nqh=34), "group"), (dict(hd=65), "even"),
     (dict(hd=258), "256"), (dict(q_stride=255), "stride"), (dict(out_stride=255), "stride"), (dict(out=P), "overlaps"),
     (dict(out=P + 4 * 1023), "overlaps"), (dict(out=P - 4), "overlaps")]
 
@@ -66,7 +66,7 @@ EV = dict(kc=P, vc=P2, mass=P, mass_out=P2, kept=P, n_len=100, budget=50, first=
 @pytest.mark.parametrize("change,why", [
     (dict(kc=0), "null"), (dict(vc=0), "null"), (dict(mass=0), "null"), (dict(kept=0), "null"), (dict(n_len=0), "empty"),
     (dict(budget=0), "empty"), (dict(n_layers=0), "empty"), (dict(nkh=0), "empty"), (dict(hd=0), "empty"),
-    (dict(n_len=129), "max_ctx"), (dict(budget=101), "budget"), (dict(first=43), "budget"), (dict(last=BIG), "budget"),
+    (dict(n_len=129), "max_ctx"), (dict(n_len=(1 << 31) + 1, max_ctx=BIG), "2.31"), (dict(budget=101), "budget"), (dict(first=43), "budget"), (dict(last=BIG), "budget"),
     (dict(n_layers=65536), "65535"), (dict(hd=7), "even"), (dict(hd=512), "256"), (dict(vc=P), "overlap"),
     (dict(vc=P + 2 * 2 * 128 * 2 * 64 - 2), "overlap"), (dict(mass_out=P + 4), "overlaps")])
 def test_evict_refuses(lib, change, why):

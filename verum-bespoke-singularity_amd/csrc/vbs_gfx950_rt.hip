@@ -783,13 +783,15 @@ bool spans_overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
     return x < y + nb && y < x + na;
 }
 
-constexpr uint32_t kMaxStep = 65535;  // tokens of one call
+constexpr uint32_t kMaxStep = 65535;         // tokens of one call
+constexpr uint64_t kMaxSlots = 1ull << 31;   // slots that one call looks at
 
 // The shape that the three operators of a step share; 0 with the reason set.
 int step_shape_ok(const char *who, uint32_t n, uint32_t slot, uint32_t max_ctx, uint32_t nqh, uint32_t nkh, uint32_t hd) {
     if (nqh == 0 || nkh == 0 || hd == 0) return fail("%s: empty shape", who);
     if (n > kMaxStep) return fail("%s: at most %u tokens per call", who, kMaxStep);
     if ((uint64_t)slot + n > max_ctx) return fail("%s: slots %u + %u tokens > max_ctx %u", who, slot, n, max_ctx);
+    if ((uint64_t)slot + n > kMaxSlots) return fail("%s: at most 2^31 slots", who);
     if (nqh % nkh) return fail("%s: %u q heads not a multiple of %u kv heads", who, nqh, nkh);
     if (nqh / nkh > 16) return fail("%s: group size %u exceeds 16", who, nqh / nkh);
     if (nkh > 65535u) return fail("%s: %u kv heads exceed 65535", who, nkh);
@@ -894,6 +896,7 @@ int vbs_gfx950_cache_evict(uint16_t *kc, uint16_t *vc, const float *mass, float 
     if (!kc || !vc || !mass || !kept) return fail("cache_evict: null pointer");
     if (len == 0 || budget == 0 || n_layers == 0 || nkh == 0 || hd == 0) return fail("cache_evict: empty shape");
     if (len > max_ctx) return fail("cache_evict: len %u > max_ctx %u", len, max_ctx);
+    if (len > kMaxSlots) return fail("cache_evict: at most 2^31 slots");
     if (budget > len) return fail("cache_evict: budget %u > len %u", budget, len);
     if ((uint64_t)first + last > budget) return fail("cache_evict: first %u + last %u > budget %u", first, last, budget);
     if (n_layers > 65535u || nkh > 65535u) return fail("cache_evict: more than 65535 layers or kv heads");

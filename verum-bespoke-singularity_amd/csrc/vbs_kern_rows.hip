@@ -166,11 +166,13 @@ struct RowsSplit {
 };
 
 // How the launch's scratch is laid out: (m, l) then acc per (kv head, range, row),
-// then (m, 1 / l) per (kv head, row).
+// then (m, 1 / l) per (kv head, row), then what the mass needs.
+__host__ __device__ __forceinline__ uint64_t score_stride(uint32_t slots) { return ((uint64_t)slots + 31u) / 32u * 32u; }
 struct RowsPart {
     float2 *ml;
     float *acc;
     float2 *stats;
+    float *scores;  // few rows with a mass: (kv head, row, score_stride(slots)), else NULL
 };
 
 // Floats from one partial row to the next.
@@ -276,10 +278,11 @@ struct RowTile {
     }
 
     // 32 NH slots from p0 on, in LDS; full: every row sees them all, else vis holds their bits and docs (or NULL)
-    // their documents. Slot 16 hf + 4 g + k is element S[hf][k].
+    // their documents. Slot 16 i + 4 g + k is element S[i][k]. `scores` (or NULL): where the row's scores of these
+    // slots go, in units of log2.
     template <uint32_t NH>
     __device__ __forceinline__ void step(const RowsArgs &a, const uint8_t *lds, uint32_t p0, uint64_t vis, bool full,
-                                         const int32_t *docs, uint32_t lane) {
+                                         const int32_t *docs, uint32_t lane, float *scores = nullptr) {
         constexpr uint32_t NS = 2u * NH, ND = DT < 4u ? DT : DT % 4u ? 2u : 4u;  // 16-slot tiles; dim tiles at a time
         const uint32_t g = lane >> 4;
         // A product waits for the one before it into the same sums: the tiles are taken in turn, the high parts
@@ -365,6 +368,9 @@ struct RowTile {
                     if (!sees) S[i][k] = -INFINITY;
                 }
         }
+        if (scores && real)
+#pragma unroll
+            for (uint32_t i = 0; i < NS; i++) *reinterpret_cast<rf4 *>(scores + 16u * i + 4u * g) = S[i] * cm;
         float top = -INFINITY;
 #pragma unroll
         for (uint32_t i = 0; i < NS; i++) top = fmaxf(top, fmaxf(fmaxf(S[i][0], S[i][1]), fmaxf(S[i][2], S[i][3])));
@@ -445,7 +451,8 @@ __device__ __forceinline__ void row_again(const RowsArgs &a, const RowsSplit &sp
                                           uint32_t split, uint32_t r, uint32_t s0, uint32_t s1, uint32_t lane) {
     const uint32_t group = a.nqh / a.nkh;
     float m, l, o[(HD + 63u) / 64u];
-    row_whole<HD>(a, r / group, kvh * group + r % group, s0, s1, lane, m, l, o);
+    row_whole<HD>(a, r / group, kvh * group + r % group, s0, s1, lane, m, l, o,
+                  pt.scores ? pt.scores + ((uint64_t)kvh * a.n * group + r) * score_stride(a.past + a.n) : nullptr);
     const RowsTo to(a, sp, pt, kvh, split, r);
 #pragma unroll
     for (uint32_t k = 0; k < (HD + 63u) / 64u; k++)
@@ -630,7 +637,8 @@ __global__ __launch_bounds__(256, 2) void k_rows_few(RowsArgs a, RowsSplit sp, R
         if (p0 < R.last) {
             const bool full = p0 + T <= min(R.clear, s1);
             const uint64_t vis = full ? ~0ull : R.real ? seen_bits(a, R.tok, p0, s1) : 0ull;
-            R.template step<1u>(a, own, p0, vis, full, a.docs ? a.docs + p0 : nullptr, lane);
+            R.template step<1u>(a, own, p0, vis, full, a.docs ? a.docs + p0 : nullptr, lane,
+                                pt.scores ? pt.scores + ((uint64_t)kvh * rows + row0 + col) * score_stride(slots) + p0 : nullptr);
         }
         p0 = next(p0 + 4u * T);
         if (p0 >= s1) break;
@@ -741,7 +749,9 @@ __global__ __launch_bounds__(256) void k_rows_merge(RowsArgs a, RowsSplit sp, Ro
 // 2^(y - m) / l for its slots; the 16 columns, then the waves, are summed at the end
 // in a fixed order. A slot whose sum is not finite is taken again in f32 products.
 // Where slots are few, the rows are split over `parts` workgroups and k_mass_add sums
-// what they leave in `part`.
+// what they leave in `part`. At most 16 rows leave their scores on the way instead, and
+// k_mass_few adds up their weights without a second product (one token over 2047 slots,
+// 32/8 heads of 128: @@).
 constexpr uint32_t kMassWaves = 8;
 
 template <uint32_t HD>
@@ -871,6 +881,23 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, const floa
         a.mass[(uint64_t)kvh * a.max_ctx + j] += v;
 }
 
+// Few rows: their scores are there (k_rows_few), a thread takes a slot.
+__global__ __launch_bounds__(256) void k_mass_few(RowsArgs a, RowsPart pt) {
+    const uint32_t j = blockIdx.x * 256u + threadIdx.x, kvh = blockIdx.y, slots = a.past + a.n, group = a.nqh / a.nkh;
+    if (j >= slots) return;
+    const float *y = pt.scores + (uint64_t)kvh * a.n * group * score_stride(slots) + j;
+    const float2 *stats = pt.stats + (uint64_t)kvh * a.n * group;
+    float v = 0.f;
+    for (uint32_t i = 0; i < a.n; i++) {
+        if (j >= row_end(a, i) || !row_sees(a, i, j)) continue;  // (its scores may not have been written)
+        for (uint32_t r = i * group; r < (i + 1u) * group; r++) {
+            const float2 st = stats[r];
+            v = fmaf(__builtin_amdgcn_exp2f(y[r * score_stride(slots)] - (st.x == -INFINITY ? 0.f : st.x)), st.y, v);
+        }
+    }
+    a.mass[(uint64_t)kvh * a.max_ctx + j] += v;
+}
+
 __global__ __launch_bounds__(256) void k_mass_add(RowsArgs a, const float *__restrict__ part, uint32_t parts) {
     const uint32_t j = blockIdx.x * 256u + threadIdx.x, kvh = blockIdx.y, slots = a.past + a.n;
     if (j >= slots) return;
@@ -893,7 +920,7 @@ struct RowsPlan {
     bool few;
     RowsSplit sp;
     uint32_t parts;               // of the rows, for the mass
-    size_t ml, acc, stats, mass;  // bytes
+    size_t ml, acc, stats, mass;  // bytes (mass: the scores of few rows, or the parts' sums)
 };
 
 // Whether rows of the caches and of q may be read 16 bytes at a time.
@@ -928,6 +955,10 @@ static RowsPlan rows_plan(const RowsArgs &a) {
     }
     if (a.mass) {
         p.stats = round(all * sizeof(float2));
+        if (p.few) {
+            p.mass = round(all * score_stride(slots) * sizeof(float));
+            return p;
+        }
         // about 512 workgroups of eight waves, at least a row tile a wave
         const uint32_t np = p.hd > 128u ? 32u : 64u, blocks = (slots + np - 1u) / np * a.nkh, waves = (rows + 127u) / 128u;
         p.parts = blocks >= 512u ? 1u : 512u / blocks;
@@ -966,6 +997,7 @@ hipError_t launch_rows(const RowsArgs &a, void *scratch, hipStream_t s) {
     RowsPart pt{};
     if (p.sp.n > 1u) pt.ml = reinterpret_cast<float2 *>(at), pt.acc = reinterpret_cast<float *>(at + p.ml);
     if (a.mass) pt.stats = reinterpret_cast<float2 *>(at + p.ml + p.acc);
+    if (a.mass && p.few) pt.scores = reinterpret_cast<float *>(at + p.ml + p.acc + p.stats);
     switch (p.hd) {
         case 32: start_rows<32>(a, p, pt, s); break;
         case 64: start_rows<64>(a, p, pt, s); break;
@@ -985,7 +1017,10 @@ hipError_t launch_rows(const RowsArgs &a, void *scratch, hipStream_t s) {
             k_rows_merge<256><<<dim3(rows, a.nkh), 256, 0, s>>>(a, p.sp, pt, tile_rows, width);
         e = hipGetLastError();
     }
-    if (e == hipSuccess && a.mass) {
+    if (e == hipSuccess && a.mass && p.few) {
+        k_mass_few<<<dim3((a.past + a.n + 255u) / 256u, a.nkh), 256, 0, s>>>(a, pt);
+        e = hipGetLastError();
+    } else if (e == hipSuccess && a.mass) {
         float *part = reinterpret_cast<float *>(at + p.ml + p.acc + p.stats);
         switch (p.hd) {
             case 32: start_mass<32>(a, p, pt, part, s); break;

@@ -73,10 +73,12 @@ __device__ __forceinline__ float row_dot(const float *q, const uint16_t *k, uint
 // the lanes take the dims (lane + 64 c in acc[c]). For rows whose sums came out not
 // finite: an infinity in q or K meets the two f16 parts of the matrix-core path
 // as inf - inf or 0 * inf, and one in V the weight 0 of the rows that do not see
-// it. Here an unseen slot is never touched. m is in units of log2.
+// it. Here an unseen slot is never touched. m is in units of log2, as the scores of the
+// slots it sees, that go to scores[j] (if not NULL).
 template <uint32_t HD>
 __device__ __forceinline__ void row_whole(const RowsArgs &a, uint32_t i, uint32_t h, uint32_t s0, uint32_t s1,
-                                          uint32_t lane, float &m_out, float &l_out, float (&acc)[(HD + 63) / 64]) {
+                                          uint32_t lane, float &m_out, float &l_out, float (&acc)[(HD + 63) / 64],
+                                          float *scores = nullptr) {
     const uint32_t kvh = h / (a.nqh / a.nkh);
     const float *q = a.q + (uint64_t)i * a.q_stride + (uint64_t)h * a.hd;
     const uint64_t rstride = (uint64_t)a.nkh * a.hd, base = (uint64_t)kvh * a.hd;
@@ -91,6 +93,7 @@ __device__ __forceinline__ void row_whole(const RowsArgs &a, uint32_t i, uint32_
         if (sees)
             y = kLog2e * row_score(a, row_dot(q, a.kc + (uint64_t)j * rstride + base, a.hd) * a.scale, slope,
                                    a.past + i, j);
+        if (scores && sees) scores[j] = y;
         const uint64_t seen = __ballot(sees);
         if (!seen) continue;
         // (fmaxf drops a NaN: a NaN score comes through the sum instead)
