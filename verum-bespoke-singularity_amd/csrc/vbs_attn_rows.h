@@ -1,5 +1,5 @@
-// vbs_rows_common.h — what the kernels of several query rows over the f16 cache
-// share (vbs_kern_rows.hip): which slots a row sees, its scores, and one row in
+// vbs_attn_rows.h — what the kernels of several query rows over the f16 cache
+// share (vbs_kern_attn_rows.hip): which slots a row sees, its scores, and one row in
 // plain f32 for rows whose sums are not finite.
 #pragma once
 

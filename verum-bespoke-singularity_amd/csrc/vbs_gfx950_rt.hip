@@ -816,12 +816,12 @@ int attention_rows(const char *who, RowsArgs a, uint32_t layer) {
     const OnDevice on;
     const std::lock_guard<std::mutex> together(g_scratch_mu);
     void *scratch = nullptr;
-    if (const size_t bytes = rows_scratch_bytes(a)) {
+    if (const size_t bytes = attn_rows_scratch_bytes(a)) {
         hipError_t why = hipSuccess;
         scratch = rt_scratch_or_captured(bytes, g_rt.stream, &why);
         if (!scratch) return hip_ok(why, who);
     }
-    return hip_ok(launch_rows(a, scratch, g_rt.stream), who);
+    return hip_ok(launch_attn_rows(a, scratch, g_rt.stream), who);
 }
 }  // namespace
 

@@ -49,9 +49,9 @@ struct RowsArgs {
     float *mass;  // at the layer's first row of max_ctx floats per kv head, or NULL
     uint32_t max_ctx;
 };
-size_t rows_scratch_bytes(const RowsArgs &a);
-// `scratch`: rows_scratch_bytes(a) of device memory (may be NULL if that is 0).
-hipError_t launch_rows(const RowsArgs &a, void *scratch, hipStream_t s);
+size_t attn_rows_scratch_bytes(const RowsArgs &a);
+// `scratch`: attn_rows_scratch_bytes(a) of device memory (may be NULL if that is 0).
+hipError_t launch_attn_rows(const RowsArgs &a, void *scratch, hipStream_t s);
 
 struct EvictArgs {
     uint16_t *kc, *vc;  // at the first layer
