@@ -667,3 +667,90 @@ def test_seen_infinities_in_few_rows(dev, mem, hd):
     got[1, 1] = want[1, 1] = 0
     tol[1, 1] = 0
     close(got, want, np.where(np.isnan(tol), 0, tol))
+
+
+@pytest.mark.parametrize("length,budget,first,last", [(8193, 8192, 0, 1), (20001, 9000, 3, 100), (16384, 1, 0, 0),
+                                                      (24600, 24599, 5, 7)])
+@pytest.mark.parametrize("values", ["spread", "ties"])
+def test_evict_longer_than_a_run(dev, mem, length, budget, first, last, values):
+    """More slots than a workgroup holds at once: selection and order over several runs, the mass in place."""
+    rng = np.random.default_rng(length)
+    nkh, hd = 2, 16
+    kc, vc = f16_bits(rng, 1, length, nkh, hd), f16_bits(rng, 1, length, nkh, hd)
+    m = np.exp(2 * rng.standard_normal((1, nkh, length))).astype(np.float32)
+    if values == "ties":
+        m = rng.integers(0, 2, m.shape).astype(np.float32)
+    pk, pv, pm, kept = mem.up(kc), mem.up(vc), mem.up(m), mem.zeros(nkh * budget, np.uint32)
+    dev.cache_evict(pk, pv, pm, pm, kept, length, budget, first, last, 0, 1, length, nkh, hd)
+    got, gk, gv = dev.download(kept, (nkh, budget), np.uint32), dev.download(pk, kc.shape, np.uint16), dev.download(pv, vc.shape, np.uint16)
+    gm = dev.download(pm, m.shape, np.float32)
+    for h in range(nkh):
+        slots = R.evict(m[0, h], length, budget, first, last)
+        assert np.array_equal(got[h], slots)
+        assert np.array_equal(gk[0, :budget, h], kc[0, slots, h]) and np.array_equal(gv[0, :budget, h], vc[0, slots, h])
+        assert np.array_equal(gk[0, budget:, h], kc[0, budget:, h])
+        assert np.array_equal(gm[0, h, :budget], m[0, h, slots]) and (gm[0, h, budget:] == 0).all()
+
+
+def test_a_captured_step_and_two_graphs_at_once(dev, mem):
+    """A whole step (rotation and store, attention with weights, eviction) replayed from one graph; and graphs of
+    attentions that use scratch replayed on two streams at once: each has memory of its own."""
+    rng = np.random.default_rng(21)
+    hip, stream = V.Hip(), dev.stream()
+    n, past, nqh, nkh, hd, sec = 20, 230, 8, 2, 64, (32,)
+    total, kvd = past + n, nkh * hd
+    kc, vc = f16_bits(rng, total, nkh, hd), f16_bits(rng, total, nkh, hd)
+    q, k, v = (rng.standard_normal((n, w)).astype(np.float32) for w in (nqh * hd, kvd, kvd))
+    m = rng.random((nkh, total)).astype(np.float32)
+    arrays = [kc, vc, q, m, np.zeros((n, nqh * hd), np.float32), np.zeros((nkh, 100), np.uint32)]
+    ptrs = [mem.up(a) for a in arrays]
+    pkc, pvc, pq, pm, po, pkept = ptrs
+    pk, pv, pp = mem.up(k), mem.up(v), mem.up(np.arange(n, dtype=np.int32) + past)
+
+    def step():
+        dev.rope_axes(pq, nqh * hd, pk, pv, kvd, pp, n, sec, pkc, pvc, past, 0, total, nqh, nkh, hd, 10000.0)
+        dev.attention_chunk(pq, nqh * hd, pkc, pvc, po, nqh * hd, n, past, 0, total, nqh, nkh, hd, 0.125, mass=pm)
+        dev.cache_evict(pkc, pvc, pm, pm, pkept, total, 100, 4, 30, 0, 1, total, nkh, hd)
+
+    graph = hip.capture(stream, step)
+    results = []
+    try:
+        for i in range(4):
+            for p, a in zip(ptrs, arrays):
+                dev.write(p, a)
+            step() if i % 2 == 0 else hip.launch(graph, stream)
+            dev.sync()
+            results.append([dev.download(p, a.shape, a.dtype) for p, a in zip(ptrs, arrays)])
+        for r in results[1:]:
+            for a, b in zip(r, results[0]):
+                assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
+    finally:
+        hip.destroy(graph)
+
+    other = C.c_void_p()
+    assert hip.h.hipStreamCreateWithFlags(C.byref(other), 1) == 0
+    graphs, steps = [], []
+    try:
+        for n, past, nqh, nkh, hd in ((1, 6000, 16, 2, 128), (30, 900, 8, 2, 64)):
+            s = Step(rng, mem, dev, n, past, nqh, nkh, hd)
+            want = s.chunk(cap=7.0)
+            shape = (s.layer, s.max_ctx, nqh, nkh, hd, s.scale)
+
+            def call(s=s, shape=shape):
+                for _ in range(8):
+                    dev.attention_chunk(s.pq, s.qs, s.pk, s.pv, s.po, s.os, s.n, s.past, *shape, cap=7.0)
+            graphs.append(hip.capture(stream, call))
+            steps.append((s, want))
+        for _ in range(5):
+            for s, _ in steps:
+                dev.write(s.po, s.out0)
+            hip.launch(graphs[0], stream)
+            hip.launch(graphs[1], other.value)
+            assert hip.h.hipStreamSynchronize(other) == 0
+            dev.sync()
+            for s, want in steps:
+                assert np.array_equal(s.got(), want)
+    finally:
+        for g in graphs:
+            hip.destroy(g)
+        hip.h.hipStreamDestroy(other)
