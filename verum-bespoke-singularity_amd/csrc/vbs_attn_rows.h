@@ -55,7 +55,7 @@ __device__ __forceinline__ float tanh_any(float x) {
 
 // The score (natural units) from scale q.k: capped, less the distance's share.
 __device__ __forceinline__ float row_far(float s, float slope, uint32_t at, uint32_t j) {
-    return fmaf(-slope, (float)(at > j ? at - j : j - at), s);
+    return fmaf(-slope, fabsf((float)(int32_t)(at - j)), s);  // (slots are at most 2^31)
 }
 __device__ __forceinline__ float row_score(const RowsArgs &a, float s, float slope, uint32_t at, uint32_t j) {
     if (a.cap > 0.f) s = a.cap * tanh_any(s * a.rcap);

@@ -133,30 +133,47 @@ struct RowQ {
 // The documents of the tokens i0 .. i1 lie in [lo, hi]: slots of others are not looked at.
 struct DocRange {
     int32_t lo, hi;
-    __device__ __forceinline__ DocRange(const RowsArgs &a, uint32_t i0, uint32_t i1, uint32_t lane) {
-        lo = 0x7FFFFFFF, hi = -0x7FFFFFFF - 1;
+    // which of the four runs of 64 slots from `win` on (a multiple of 64) hold a slot of the range
+    uint32_t win, runs;
+
+    // (the first window's documents are asked for with the tokens': one round trip)
+    __device__ __forceinline__ DocRange(const RowsArgs &a, uint32_t i0, uint32_t i1, uint32_t s0, uint32_t s1, uint32_t lane) {
+        lo = 0x7FFFFFFF, hi = -0x7FFFFFFF - 1, win = s0, runs = 0;
         if (!a.docs) return;
+        int32_t d[4];
+        read(a, s0, s1, lane, d);
         for (uint32_t i = i0 + lane; i <= i1; i += 64u) {
-            const int32_t d = a.docs[a.past + i];
-            lo = min(lo, d), hi = max(hi, d);
+            const int32_t own = a.docs[a.past + i];
+            lo = min(lo, own), hi = max(hi, own);
         }
 #pragma unroll
         for (int o = 32; o; o >>= 1) lo = min(lo, __shfl_xor(lo, o, 64)), hi = max(hi, __shfl_xor(hi, o, 64));
+        look(s0, s1, lane, d);
     }
-    // The first tile of T slots from p on (p a tile's first slot, up to s1) that holds a slot of the range; s1
-    // if none does. 256 slots are looked at in one round of loads.
-    template <uint32_t T>
-    __device__ __forceinline__ uint32_t next(const RowsArgs &a, uint32_t p, uint32_t s1, uint32_t lane) const {
+    __device__ __forceinline__ static void read(const RowsArgs &a, uint32_t p, uint32_t s1, uint32_t lane, int32_t (&d)[4]) {
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; k++) d[k] = a.docs[min(p + 64u * k + lane, s1 - 1u)];
+    }
+    __device__ __forceinline__ void look(uint32_t p, uint32_t s1, uint32_t lane, const int32_t (&d)[4]) {
+        win = p, runs = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; k++)
+            if (__any(p + 64u * k + lane < s1 && d[k] >= lo && d[k] <= hi)) runs |= 1u << k;
+    }
+    // The first slot from p on (a multiple of 32) whose run of 64 holds a slot of the range, a multiple of 64 unless it
+    // is p itself; s1 if there is none. Slots are looked at 256 in one round of loads.
+    __device__ __forceinline__ uint32_t next(const RowsArgs &a, uint32_t p, uint32_t s1, uint32_t lane) {
         if (!a.docs) return p;
-        for (; p < s1; p += 256u) {
-            int32_t d[4];
-#pragma unroll
-            for (uint32_t k = 0; k < 4u; k++) d[k] = a.docs[min(p + 64u * k + lane, s1 - 1u)];
-#pragma unroll
-            for (uint32_t k = 0; k < 4u; k++) {
-                const uint64_t in = __ballot(p + 64u * k + lane < s1 && d[k] >= lo && d[k] <= hi);
-                if (in) return p + 64u * k + (uint32_t)(__ffsll((unsigned long long)in) - 1) / T * T;
+        while (p < s1) {
+            if (p - win >= 256u) {
+                int32_t d[4];
+                read(a, p / 64u * 64u, s1, lane, d);
+                look(p / 64u * 64u, s1, lane, d);
             }
+            const uint32_t k = (p - win) / 64u, left = runs >> k;
+            if (left & 1u) return p;
+            if (left) return win + 64u * (k + (uint32_t)__builtin_ctz(left));
+            p = win + 256u;
         }
         return s1;
     }
@@ -293,7 +310,7 @@ struct RowTile {
     // 32 NH slots from p0 on, in LDS; full: every row sees them all, else vis holds their bits and docs (or NULL)
     // their documents. Slot 16 i + 4 g + k is element S[i][k]. `scores` (or NULL): where the row's scores of these
     // slots go, in units of log2.
-    template <uint32_t NH>
+    template <uint32_t NH, bool DOCS_LDS>
     __device__ __forceinline__ void step(const RowsArgs &a, const uint8_t *lds, uint32_t p0, uint64_t vis, bool full,
                                          const int32_t *docs, uint32_t lane, float *scores = nullptr) {
         constexpr uint32_t NS = 2u * NH, ND = DT < 4u ? DT : DT % 4u ? 2u : 4u;  // 16-slot tiles; dim tiles at a time
@@ -372,14 +389,18 @@ struct RowTile {
         }
         if (!full) {
 #pragma unroll
-            for (uint32_t i = 0; i < NS; i++)
+            for (uint32_t i = 0; i < NS; i++) {
+                typedef int32_t ri4 __attribute__((ext_vector_type(4)));
+                ri4 d = {doc, doc, doc, doc};
+                if (docs && DOCS_LDS) d = *reinterpret_cast<const ri4 *>(docs + 16u * i + 4u * g);
 #pragma unroll
                 for (uint32_t k = 0; k < 4u; k++) {
                     const uint32_t o = 16u * i + 4u * g + k;
-                    bool sees = vis >> o & 1ull;
-                    if (docs) sees = sees && docs[o] == doc;
-                    if (!sees) S[i][k] = -INFINITY;
+                    const bool in = vis >> o & 1ull;
+                    if (docs && !DOCS_LDS && in) d[k] = docs[o];  // (behind the last slot there is none)
+                    S[i][k] = in & (d[k] == doc) ? S[i][k] : -INFINITY;
                 }
+            }
         }
         if (scores && real)
 #pragma unroll
@@ -480,7 +501,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(RowsArgs a, RowsSplit sp, 
     constexpr uint32_t DT = HD / 16u, T = kTile<HD>, CPR = HD / 8u, NC = T * CPR / 256u;
     constexpr uint32_t RB = HD * 2u, TB = T * RB;  // bytes of a row and of a tile
     __shared__ __align__(1024) uint8_t kv[2][2][TB];  // two buffers of K and V
-    __shared__ int32_t dl[2][T];
+    __shared__ __align__(16) int32_t dl[2][T];
     const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u, col = lane & 15u, g = lane >> 4;
     const uint32_t kvh = blockIdx.x % a.nkh, rest = blockIdx.x / a.nkh;
     const uint32_t split = rest % sp.n, tile = tiles - 1u - rest / sp.n;  // (the longest rows first)
@@ -535,8 +556,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(RowsArgs a, RowsSplit sp, 
         __syncthreads();
     };
 
-    const DocRange of(a, row_tile / group, (min(row_tile + 64u, rows) - 1u) / group, lane);
-    uint32_t p0 = of.next<T>(a, s0, s1, lane);
+    DocRange of(a, row_tile / group, (min(row_tile + 64u, rows) - 1u) / group, s0, s1, lane);
+    uint32_t p0 = of.next(a, s0, s1, lane);
     RowQ<HD / 32u> x;
     RowTile<HD>::load(a, kvh, row0, wide_q, lane, x);
     if (p0 < s1) fetch(p0, 0u);
@@ -544,12 +565,12 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(RowsArgs a, RowsSplit sp, 
     R.init(a, kvh, row0, x, lane, TB);
     if (p0 < s1) arrive(0u);
     for (uint32_t b = 0; p0 < s1; b ^= 1u) {
-        const uint32_t p1 = of.next<T>(a, p0 + T, s1, lane);
+        const uint32_t p1 = of.next(a, p0 + T, s1, lane);
         if (p1 < s1) fetch(p1, b ^ 1u);
         if (p0 < R.last) {
             const bool full = p0 + T <= min(R.clear, s1);
             const uint64_t vis = full ? ~0ull : R.real ? seen_bits(a, R.tok, p0, s1) : 0ull;
-            R.template step<T / 32u>(a, &kv[0][0][0], p0, vis, full, a.docs ? dl[b] : nullptr, lane);
+            R.template step<T / 32u, true>(a, &kv[0][0][0], p0, vis, full, a.docs ? dl[b] : nullptr, lane);
         }
         if (p1 < s1) arrive(b ^ 1u);
         R.turn(b ? 0u - 2u * TB : 2u * TB);
@@ -631,7 +652,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_few(RowsArgs a, RowsSplit sp, R
             }
         }
     };
-    const DocRange of(a, row0 / group, (min(row0 + 16u, rows) - 1u) / group, lane);
+    const DocRange of(a, row0 / group, (min(row0 + 16u, rows) - 1u) / group, s0, s1, lane);
     // (the wave's next tile, past those without a slot of the rows' documents)
     auto next = [&](uint32_t p) {
         if (a.docs)
@@ -653,7 +674,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_few(RowsArgs a, RowsSplit sp, R
         if (p0 < R.last) {
             const bool full = p0 + T <= min(R.clear, s1);
             const uint64_t vis = full ? ~0ull : R.real ? seen_bits(a, R.tok, p0, s1) : 0ull;
-            R.template step<1u>(a, own, p0, vis, full, a.docs ? a.docs + p0 : nullptr, lane,
+            R.template step<1u, false>(a, own, p0, vis, full, a.docs ? a.docs + p0 : nullptr, lane,
                                 pt.scores ? pt.scores + ((uint64_t)kvh * rows + row0 + col) * score_stride(slots) + p0 : nullptr);
         }
         p0 = next(p0 + 4u * T);
@@ -951,6 +972,8 @@ static RowsPlan rows_plan(const RowsArgs &a) {
     RowsPlan p{};
     p.hd = a.hd <= 32u ? 32u : a.hd <= 64u ? 64u : a.hd <= 96u ? 96u : a.hd <= 128u ? 128u : 256u;
     const uint32_t rows = a.n * (a.nqh / a.nkh), slots = a.past + a.n;
+    // (up to 64 rows the two kernels are within 15% of each other either way, the few-row one ahead over short
+    // contexts: 32 rows over 500 slots 10.9 and 12.5 us, over 2048 13.8 and 12.2)
     p.few = rows <= 16u && rows_wide_kv(a);
     const uint32_t tile_rows = p.few ? 16u : 64u;
     p.tiles = (rows + tile_rows - 1u) / tile_rows;
@@ -975,9 +998,10 @@ static RowsPlan rows_plan(const RowsArgs &a) {
             p.mass = round(all * score_stride(slots) * sizeof(float));
             return p;
         }
-        // about 512 workgroups of eight waves, at least a row tile a wave
+        // about 256 workgroups of eight waves, at least a row tile a wave (2560 rows over 643 slots, 2 kv heads of 80:
+        // 12.1 us under the tracer; 512 workgroups 15.0, 128 16.4)
         const uint32_t np = p.hd > 128u ? 32u : 64u, blocks = (slots + np - 1u) / np * a.nkh, waves = (rows + 127u) / 128u;
-        p.parts = blocks >= 512u ? 1u : 512u / blocks;
+        p.parts = blocks >= 256u ? 1u : 256u / blocks;
         p.parts = p.parts < waves ? p.parts : waves;
         if (p.parts > 1u) p.mass = round((size_t)p.parts * a.nkh * slots * sizeof(float));
     }
