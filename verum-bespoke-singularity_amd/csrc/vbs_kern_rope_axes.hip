@@ -52,37 +52,51 @@ __device__ __forceinline__ float2 cos_sin(double a) {
     return make_float2((float)(quad == 1 || quad == 2 ? -cs : cs), (float)(quad >= 2 ? -sn : sn));
 }
 
-// grid (parts, tokens): a workgroup takes `rows` of a token's nqh + nkh heads.
-__global__ __launch_bounds__(256) void k_rope_axes(RopeAxesArgs a, RopeFreqs fr, uint32_t rows) {
+// grid (parts, tokens): a workgroup takes kRopeRows of a token's nqh + nkh heads; what it rotates is on its way while
+// the angles are formed.
+constexpr uint32_t kRopeRows = 8, kRopeMine = kRopeRows * kRopeMaxPairs / 256u;
+
+__global__ __launch_bounds__(256) void k_rope_axes(RopeAxesArgs a, RopeFreqs fr) {
     __shared__ float2 cs[kRopeMaxPairs];
     const uint32_t pairs = a.hd / 2u, i = blockIdx.y, t = threadIdx.x;
-    for (uint32_t p = t; p < pairs; p += 256u) {
+    const uint32_t heads = (a.q ? a.nqh : 0u) + (a.k ? a.nkh : 0u), r0 = blockIdx.x * kRopeRows;
+    const uint32_t mine = min(kRopeRows, heads - r0) * pairs, nq = a.q ? a.nqh : 0u;
+    float x0[kRopeMine], x1[kRopeMine], v0[kRopeMine], v1[kRopeMine];
+#pragma unroll
+    for (uint32_t n = 0; n < kRopeMine; n++) {
+        const uint32_t e = t + 256u * n, h = r0 + e / pairs, d = 2u * (e % pairs);
+        if (e >= mine) break;
+        const float *x = h < nq ? a.q + (uint64_t)i * a.q_stride + (uint64_t)h * a.hd + d
+                                : a.k + (uint64_t)i * a.kv_stride + (uint64_t)(h - nq) * a.hd + d;
+        x0[n] = x[0], x1[n] = x[1];
+        if (h >= nq) {
+            const float *v = a.v + (uint64_t)i * a.kv_stride + (uint64_t)(h - nq) * a.hd + d;
+            v0[n] = v[0], v1[n] = v[1];
+        }
+    }
+    if (t < pairs) {
         uint32_t axis = 0;
-        while (p >= a.end[axis]) axis++;
-        cs[p] = cos_sin((double)a.pos[(uint64_t)axis * a.n + i] * fr.f[p]);
+        while (t >= a.end[axis]) axis++;
+        cs[t] = cos_sin((double)a.pos[(uint64_t)axis * a.n + i] * fr.f[t]);
     }
     __syncthreads();
-    const uint32_t heads = (a.q ? a.nqh : 0u) + (a.k ? a.nkh : 0u), r0 = blockIdx.x * rows;
-    const uint32_t mine = min(rows, heads - r0) * pairs;
-    for (uint32_t e = t; e < mine; e += 256u) {
-        uint32_t h = r0 + e / pairs;
-        const uint32_t p = e % pairs;
+#pragma unroll
+    for (uint32_t n = 0; n < kRopeMine; n++) {
+        const uint32_t e = t + 256u * n, h = r0 + e / pairs, p = e % pairs;
+        if (e >= mine) break;
         const float2 w = cs[p];
-        if (a.q && h < a.nqh) {
+        const float y0 = __fsub_rn(__fmul_rn(x0[n], w.x), __fmul_rn(x1[n], w.y));
+        const float y1 = __fadd_rn(__fmul_rn(x0[n], w.y), __fmul_rn(x1[n], w.x));
+        if (h < nq) {
             float *x = a.q + (uint64_t)i * a.q_stride + (uint64_t)h * a.hd + 2u * p;
-            const float x0 = x[0], x1 = x[1];
-            x[0] = __fsub_rn(__fmul_rn(x0, w.x), __fmul_rn(x1, w.y));
-            x[1] = __fadd_rn(__fmul_rn(x0, w.y), __fmul_rn(x1, w.x));
+            x[0] = y0, x[1] = y1;
             continue;
         }
-        if (a.q) h -= a.nqh;
-        const uint64_t from = (uint64_t)i * a.kv_stride + (uint64_t)h * a.hd + 2u * p;
-        const uint64_t to = ((uint64_t)i * a.nkh + h) * a.hd + 2u * p;
-        const float x0 = a.k[from], x1 = a.k[from + 1u];
-        a.kc[to] = vbs_f2h(__fsub_rn(__fmul_rn(x0, w.x), __fmul_rn(x1, w.y)));
-        a.kc[to + 1u] = vbs_f2h(__fadd_rn(__fmul_rn(x0, w.y), __fmul_rn(x1, w.x)));
-        a.vc[to] = vbs_f2h(a.v[from]);
-        a.vc[to + 1u] = vbs_f2h(a.v[from + 1u]);
+        const uint64_t to = ((uint64_t)i * a.nkh + (h - nq)) * a.hd + 2u * p;
+        a.kc[to] = vbs_f2h(y0);
+        a.kc[to + 1u] = vbs_f2h(y1);
+        a.vc[to] = vbs_f2h(v0[n]);
+        a.vc[to + 1u] = vbs_f2h(v1[n]);
     }
 }
 
@@ -97,8 +111,7 @@ hipError_t launch_rope_axes(const RopeAxesArgs &a, float theta, hipStream_t s) {
         fr_theta = theta;
         fr_hd = a.hd;
     }
-    const uint32_t rows = 8u;
-    k_rope_axes<<<dim3((heads + rows - 1u) / rows, a.n), 256, 0, s>>>(a, fr, rows);
+    k_rope_axes<<<dim3((heads + kRopeRows - 1u) / kRopeRows, a.n), 256, 0, s>>>(a, fr);
     return hipGetLastError();
 }
 

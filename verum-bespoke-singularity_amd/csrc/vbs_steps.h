@@ -12,7 +12,7 @@
 namespace vbs {
 
 constexpr uint32_t kRopeAxes = 4;       // position axes of one call
-constexpr uint32_t kRopeMaxPairs = 256;  // head_dim 512, as vbs_gfx950_rope
+constexpr uint32_t kRopeMaxPairs = 128;  // head_dim 256, as the attentions
 
 struct RopeAxesArgs {
     float *q;  // NULL: k and v alone
