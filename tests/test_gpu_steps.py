@@ -754,3 +754,23 @@ def test_a_captured_step_and_two_graphs_at_once(dev, mem):
         for g in graphs:
             hip.destroy(g)
         hip.h.hipStreamDestroy(other)
+
+
+@pytest.mark.parametrize("docs", [False, True])
+def test_mass_of_more_rows_than_a_wave_looks_through_at_once(dev, mem, docs):
+    """8800 rows of a kv head in one workgroup's share. The heads of a kv head ask the same, so one of them stands
+    for all in the oracle, and the bound of a sum counts every row."""
+    n, past, nqh, nkh, hd, group = 1100, 0, 128, 16, 32, 8
+    rng = np.random.default_rng(n)
+    s = Step(rng, mem, dev, n, past, nqh, nkh, hd)
+    one = s.q.reshape(n, nkh, group, hd)[:, :, :1].copy()
+    s.q = np.ascontiguousarray(np.broadcast_to(one, (n, nkh, group, hd))).reshape(n, nqh * hd)
+    ids = np.repeat(np.arange(n), rng.integers(1, 60, n))[:n].astype(np.int32) if docs else None
+    want, w, tol, wtol = R.attend(one[:, :, 0].astype(np.float64), R.half(s.kc[1, :n]), R.half(s.vc[1, :n]),
+                                  R.sees_chunk(n, past, 0, ids), s.scale, past)
+    mass0 = np.zeros((2, nkh, s.max_ctx), np.float32)
+    got = s.chunk(mass=mass0, **({"docs": ids} if docs else {}))
+    close(got, np.repeat(want, group, 1), np.repeat(tol, group, 1))
+    add = group * w.sum(0)
+    off = group * wtol.sum(0) + add * (n * group + 2) * R.F32
+    close(dev.download(s.pm, mass0.shape, np.float32)[1, :, :n].astype(np.float64), add, off)

@@ -203,6 +203,10 @@ struct RowsPart {
     float *acc;
     float2 *stats;
     float *scores;  // few rows with a mass: (kv head, row, score_stride(slots)), else NULL
+    // many rows with a mass: the parts of q as the matrix cores take them (kv head, 16-row tile, slice of 32 dims,
+    // lane; 16 bytes of the high part, then 16 of the low) and the rows' c, else NULL
+    ru4 *qparts;
+    float *qc;
 };
 
 // Floats from one partial row to the next.
@@ -313,7 +317,8 @@ struct RowTile {
     template <uint32_t NH, bool DOCS_LDS>
     __device__ __forceinline__ void step(const RowsArgs &a, const uint8_t *lds, uint32_t p0, uint64_t vis, bool full,
                                          const int32_t *docs, uint32_t lane, float *scores = nullptr) {
-        constexpr uint32_t NS = 2u * NH, ND = DT < 4u ? DT : DT % 4u ? 2u : 4u;  // 16-slot tiles; dim tiles at a time
+        // 16-slot tiles; dim tiles at a time (two at head_dim 256, where four leave 37 registers in memory)
+        constexpr uint32_t NS = 2u * NH, ND = DT < 4u ? DT : DT % 4u || DT > 8u ? 2u : 4u;
         const uint32_t g = lane >> 4;
         // A product waits for the one before it into the same sums: the tiles are taken in turn, the high parts
         // then the low, so that four products lie between. Each slice's K is read while the one before it is
@@ -563,6 +568,16 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(RowsArgs a, RowsSplit sp, 
     if (p0 < s1) fetch(p0, 0u);
     RowTile<HD> R;
     R.init(a, kvh, row0, x, lane, TB);
+    if (pt.qparts && split == 0u && row0 < rows) {  // (the mass multiplies them again)
+        const uint64_t rt = (uint64_t)kvh * ((rows + 15u) / 16u) + row0 / 16u;
+        ru4 *to = pt.qparts + (rt * (HD / 32u) * 64u + lane) * 2u;
+#pragma unroll
+        for (uint32_t kk = 0; kk < HD / 32u; kk++) {
+            to[128u * kk] = __builtin_bit_cast(ru4, R.qh[kk]);
+            to[128u * kk + 1u] = __builtin_bit_cast(ru4, R.ql[kk]);
+        }
+        if (g == 0) pt.qc[rt * 16u + col] = R.c1;
+    }
     if (p0 < s1) arrive(0u);
     for (uint32_t b = 0; p0 < s1; b ^= 1u) {
         const uint32_t p1 = of.next(a, p0 + T, s1, lane);
@@ -785,6 +800,8 @@ __global__ __launch_bounds__(256) void k_attn_rows_merge(RowsArgs a, RowsSplit s
 // its waves take the row tiles of 16 in turn (S^T as above) and each lane adds up
 // 2^(y - m) / l for its slots; the 16 columns, then the waves, are summed at the end
 // in a fixed order. A slot whose sum is not finite is taken again in f32 products.
+// q's parts come from k_attn_rows, as the matrix cores take them: splitting q again for every 64 slots costs more
+// than the products (1024 tokens over 5120 slots, 32/8 heads of 128: 269 us under the tracer, 166 from the parts).
 // Where slots are few, the rows are split over `parts` workgroups and k_mass_add sums
 // what they leave in `part`. At most 16 rows leave their scores on the way instead, and
 // k_mass_few adds up their weights without a second product (one token over 2047 slots,
@@ -795,9 +812,8 @@ template <uint32_t HD>
 constexpr uint32_t kMassTiles = HD > 128u ? 2u : 4u;
 
 template <uint32_t HD>
-__global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, const float2 *__restrict__ stats,
-                                                          float *__restrict__ part, uint32_t parts, bool wide_kv,
-                                                          bool wide_q) {
+__global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, RowsPart pt, float *__restrict__ part, uint32_t parts,
+                                                          bool wide_kv) {
     constexpr uint32_t KK = HD / 32u, NT = kMassTiles<HD>, NP = 16u * NT;  // tiles of 16 slots; slots
     __shared__ float sums[kMassWaves][NP];
     const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u, col = lane & 15u, g = lane >> 4;
@@ -805,17 +821,18 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, const floa
     const uint32_t mine = rest % parts, p0 = rest / parts * NP;
     const uint32_t group = a.nqh / a.nkh, rows = a.n * group, slots = a.past + a.n;
     const uint64_t rstride = (uint64_t)a.nkh * a.hd;
+    const float2 *stats = pt.stats + (uint64_t)kvh * rows;
     rh8 ka[NT][KK];
     int32_t ds[NT][4];
 #pragma unroll
-    for (uint32_t hf = 0; hf < NT; hf++) {
-        const uint16_t *k = a.kc + (uint64_t)min(p0 + 16u * hf + col, slots - 1u) * rstride + (uint64_t)kvh * a.hd;
+    for (uint32_t i = 0; i < NT; i++) {
+        const uint16_t *k = a.kc + (uint64_t)min(p0 + 16u * i + col, slots - 1u) * rstride + (uint64_t)kvh * a.hd;
 #pragma unroll
         for (uint32_t kk = 0; kk < KK; kk++)
-            ka[hf][kk] = __builtin_bit_cast(rh8, cache8(k, 32u * kk + 8u * g, a.hd, wide_kv));
+            ka[i][kk] = __builtin_bit_cast(rh8, cache8(k, 32u * kk + 8u * g, a.hd, wide_kv));
 #pragma unroll
         for (uint32_t r = 0; r < 4u; r++)
-            ds[hf][r] = a.docs ? a.docs[min(p0 + 16u * hf + 4u * g + r, slots - 1u)] : 0;
+            ds[i][r] = a.docs ? a.docs[min(p0 + 16u * i + 4u * g + r, slots - 1u)] : 0;
     }
     float sum[NT][4] = {};
     const bool terms = a.cap > 0.f || a.slopes;
@@ -827,66 +844,86 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, const floa
         for (int o = 32; o; o >>= 1) lo = min(lo, __shfl_xor(lo, o, 64)), hi = max(hi, __shfl_xor(hi, o, 64));
     }
     // this part's row tiles; those before the first that sees p0 (without a mask or a prefix beyond it) are left out
-    const uint32_t first = a.mask || p0 < a.prefix || p0 <= a.past ? 0u : (p0 - a.past) * group / 16u;
-    const uint32_t all = (rows + 15u) / 16u, per = (all - min(first, all) + parts - 1u) / parts;
-    const uint32_t t0 = first + mine * per, t1 = min(t0 + per, all);
-    RowQ<KK> x;  // (the next tile's rows are on their way while one is worked on)
+    const uint32_t all = (rows + 15u) / 16u;
+    const uint32_t first = min(a.mask || p0 < a.prefix || p0 <= a.past ? 0u : (p0 - a.past) * group / 16u, all);
+    const uint32_t per = (all - first + parts - 1u) / parts, t0 = first + mine * per, t1 = min(t0 + per, all);
+    // The wave's tiles are t0 + wave, + waves, ...; 64 of them at a time, a tile to a lane, are looked through for a
+    // document of the slots', and the next one's q is on its way while one is worked on.
+    ru4 qn[KK][2];
     auto fetch = [&](uint32_t rt) {
-        const uint32_t r = 16u * rt + col;
-        x.load(rt < t1 && r < rows ? a.q + (uint64_t)(r / group) * a.q_stride + (uint64_t)(kvh * group + r % group) * a.hd
-                                   : nullptr,
-               a.hd, wide_q, g);
+        const ru4 *from = pt.qparts + (((uint64_t)kvh * all + rt) * KK * 64u + lane) * 2u;
+#pragma unroll
+        for (uint32_t kk = 0; kk < KK; kk++) qn[kk][0] = from[128u * kk], qn[kk][1] = from[128u * kk + 1u];
     };
-    fetch(t0 + wave);
-    for (uint32_t rt = t0 + wave; rt < t1; rt += waves) {
-        const uint32_t r = 16u * rt + col;
-        const bool real = r < rows;
-        const uint32_t i = real ? r / group : 0u, h = kvh * group + (real ? r % group : 0u);
-        const float2 st = real ? stats[(uint64_t)kvh * rows + r] : make_float2(0.f, 0.f);
-        rh8 qh[KK], ql[KK];
-        float c1;
-        x.split(a.scale, qh, ql, c1);
-        fetch(rt + waves);
-        const bool full = !a.docs && 16u * rt + 16u <= rows &&
-                          p0 + NP <= (a.mask ? a.past : row_end(a, 16u * rt / group));
-        const uint64_t vis = full ? ~0ull : real ? seen_bits(a, i, p0, slots) : 0ull;
-        const int32_t doc = a.docs ? a.docs[a.past + i] : 0;
-        if (a.docs && !__any(doc >= lo && doc <= hi)) continue;
-        const float slope = a.slopes ? a.slopes[h] : 0.f, ms = st.x == -INFINITY ? 0.f : st.x;
-#pragma unroll
-        for (uint32_t hf = 0; hf < NT; hf++) {
-            rf4 S = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (uint32_t kk = 0; kk < KK; kk++) S = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[hf][kk], qh[kk], S, 0, 0, 0);
-#pragma unroll
-            for (uint32_t kk = 0; kk < KK; kk++) S = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[hf][kk], ql[kk], S, 0, 0, 0);
-#pragma unroll
-            for (uint32_t k = 0; k < 4u; k++) {
-                const uint32_t o = 16u * hf + 4u * g + k;
-                float y;
-                if (full && !terms) {
-                    y = fmaf(S[k], c1 * kLog2e, -ms);
-                } else {
-                    float s = S[k] * c1;
-                    if (terms) s = row_score(a, s, slope, a.past + i, p0 + o);
-                    const bool sees = (vis >> o & 1ull) && (!a.docs || ds[hf][k] == doc);
-                    y = sees ? fmaf(s, kLog2e, -ms) : -INFINITY;
-                }
-                sum[hf][k] = fmaf(__builtin_amdgcn_exp2f(y), st.y, sum[hf][k]);
+    for (uint32_t base = t0 + wave; base < t1; base += 64u * waves) {
+        const uint32_t lt = base + lane * waves;
+        bool need = lt < t1;
+        if (a.docs && need) {
+            need = false;
+            for (uint32_t i = 16u * lt / group; i <= (min(16u * lt + 16u, rows) - 1u) / group; i++) {
+                const int32_t d = a.docs[a.past + i];
+                need = need || (d >= lo && d <= hi);
             }
+        }
+        uint64_t left = __ballot(need);
+        if (left) fetch(base + (uint32_t)__builtin_ctzll(left) * waves);
+        while (left) {
+            const uint32_t rt = base + (uint32_t)__builtin_ctzll(left) * waves;
+            left &= left - 1ull;
+            const uint32_t r = 16u * rt + col;
+            const bool real = r < rows;
+            const uint32_t i = real ? r / group : 0u, h = kvh * group + (real ? r % group : 0u);
+            const float2 st = real ? stats[r] : make_float2(0.f, 0.f);
+            const float c1 = pt.qc[((uint64_t)kvh * all + rt) * 16u + col];
+            rh8 qh[KK], ql[KK];
+#pragma unroll
+            for (uint32_t kk = 0; kk < KK; kk++)
+                qh[kk] = __builtin_bit_cast(rh8, qn[kk][0]), ql[kk] = __builtin_bit_cast(rh8, qn[kk][1]);
+            if (left) fetch(base + (uint32_t)__builtin_ctzll(left) * waves);
+            const bool full = !a.docs && 16u * rt + 16u <= rows &&
+                              p0 + NP <= (a.mask ? a.past : row_end(a, 16u * rt / group));
+            const uint64_t vis = full ? ~0ull : real ? seen_bits(a, i, p0, slots) : 0ull;
+            const int32_t doc = a.docs ? a.docs[a.past + i] : 0;
+            const float slope = a.slopes ? a.slopes[h] : 0.f, ms = st.x == -INFINITY ? 0.f : st.x;
+            rf4 S[NT];
+#pragma unroll
+            for (uint32_t j = 0; j < NT; j++) S[j] = rf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (uint32_t kk = 0; kk < KK; kk++)
+#pragma unroll
+                for (uint32_t v = 0; v < 2u; v++)
+#pragma unroll
+                    for (uint32_t j = 0; j < NT; j++)
+                        S[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[j][kk], v ? ql[kk] : qh[kk], S[j], 0, 0, 0);
+#pragma unroll
+            for (uint32_t j = 0; j < NT; j++)
+#pragma unroll
+                for (uint32_t k = 0; k < 4u; k++) {
+                    const uint32_t o = 16u * j + 4u * g + k;
+                    float y;
+                    if (full && !terms) {
+                        y = fmaf(S[j][k], c1 * kLog2e, -ms);
+                    } else {
+                        float s = S[j][k] * c1;
+                        if (terms) s = row_score(a, s, slope, a.past + i, p0 + o);
+                        const bool sees = (vis >> o & 1ull) & (ds[j][k] == doc);  // (0 == 0 without documents)
+                        y = sees ? fmaf(s, kLog2e, -ms) : -INFINITY;
+                    }
+                    sum[j][k] = fmaf(__builtin_amdgcn_exp2f(y), st.y, sum[j][k]);
+                }
         }
     }
     // the 16 columns: each lane group's row of 16 lanes
 #pragma unroll
-    for (uint32_t hf = 0; hf < NT; hf++)
+    for (uint32_t j = 0; j < NT; j++)
 #pragma unroll
         for (uint32_t k = 0; k < 4u; k++) {
-            float v = sum[hf][k];
+            float v = sum[j][k];
             v += bfly_partner<8>(v, lane);
             v += bfly_partner<4>(v, lane);
             v += bfly_partner<2>(v, lane);
             v += bfly_partner<1>(v, lane);
-            if (col == 0) sums[wave][16u * hf + 4u * g + k] = v;
+            if (col == 0) sums[wave][16u * j + 4u * g + k] = v;
         }
     __syncthreads();
     if (wave) return;
@@ -905,7 +942,7 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, const floa
             if (jj >= row_end(a, i) || !row_sees(a, i, jj)) continue;
             const float s = row_score(a, row_dot(a.q + (uint64_t)i * a.q_stride + (uint64_t)h * a.hd, k, a.hd) * a.scale,
                                       a.slopes ? a.slopes[h] : 0.f, a.past + i, jj);
-            const float2 st = stats[(uint64_t)kvh * rows + r];
+            const float2 st = stats[r];
             whole += exp2f(fmaf(s, kLog2e, -(st.x == -INFINITY ? 0.f : st.x))) * st.y;
         }
         whole = wave_sum(whole);
@@ -957,7 +994,7 @@ struct RowsPlan {
     bool few;
     RowsSplit sp;
     uint32_t parts;               // of the rows, for the mass
-    size_t ml, acc, stats, mass;  // bytes (mass: the scores of few rows, or the parts' sums)
+    size_t ml, acc, stats, mass, qparts, qc;  // bytes (mass: the scores of few rows, or the parts' sums)
 };
 
 // Whether rows of the caches and of q may be read 16 bytes at a time.
@@ -978,10 +1015,14 @@ static RowsPlan rows_plan(const RowsArgs &a) {
     const uint32_t tile_rows = p.few ? 16u : 64u;
     p.tiles = (rows + tile_rows - 1u) / tile_rows;
     // Ranges: until about 512 workgroups share the work. A range is at least a tile a wave (few) or two tiles of a
-    // workgroup (16 tokens over 2048 slots, 32/8 heads of 128: 11.5 us, one tile 14.5), and 1024 slots where half
-    // the CUs have a workgroup already (777 tokens in documents, 16 heads of 64: 22 us whole, 22 and the merge's 10
-    // in two ranges).
-    const uint32_t wgs = p.tiles * a.nkh, least = !p.few && wgs >= 128u ? 1024u : 128u, most = (slots + least - 1u) / least;
+    // workgroup (16 tokens over 2048 slots, 32/8 heads of 128: 11.5 us, one tile 14.5), and, where half the CUs have a
+    // workgroup already, so many slots that sharing their products is worth the merge: 1024 at heads of 64 (777 tokens
+    // in documents, 16 heads: 22 us whole, 22 and the merge's 10 in two ranges), 512 at 128 (2010 tokens, 4 heads, in
+    // documents: 52 us in ranges of 1024, 40 in ranges of 512), 256 at 256 (1024 tokens over 2048 slots, 8/1 heads: 95
+    // and 66; 130 tokens over 536 slots, 64/8 heads: 46 whole, 45 in two).
+    const uint32_t wgs = p.tiles * a.nkh;
+    const uint32_t least = p.few || wgs < 128u ? 128u : p.hd <= 64u ? 1024u : 65536u / p.hd / 128u * 128u;
+    const uint32_t most = (slots + least - 1u) / least;
     uint32_t n = 512u / wgs;
     n = n < 1u ? 1u : n > most ? most : n > kMostRanges ? kMostRanges : n;
     p.sp.len = ((slots + n - 1u) / n + 127u) / 128u * 128u;
@@ -1004,13 +1045,16 @@ static RowsPlan rows_plan(const RowsArgs &a) {
         p.parts = blocks >= 256u ? 1u : 256u / blocks;
         p.parts = p.parts < waves ? p.parts : waves;
         if (p.parts > 1u) p.mass = round((size_t)p.parts * a.nkh * slots * sizeof(float));
+        const size_t tiles = (size_t)((rows + 15u) / 16u) * a.nkh;
+        p.qparts = round(tiles * p.hd * 64u);
+        p.qc = round(tiles * 16u * sizeof(float));
     }
     return p;
 }
 
 size_t attn_rows_scratch_bytes(const RowsArgs &a) {
     const RowsPlan p = rows_plan(a);
-    return p.ml + p.acc + p.stats + p.mass;
+    return p.ml + p.acc + p.stats + p.mass + p.qparts + p.qc;
 }
 
 template <uint32_t HD>
@@ -1028,7 +1072,7 @@ template <uint32_t HD>
 static void start_mass(const RowsArgs &a, const RowsPlan &p, const RowsPart &pt, float *part, hipStream_t s) {
     const uint32_t tiles = (a.n * (a.nqh / a.nkh) + 15u) / 16u, np = 16u * kMassTiles<HD>;
     k_mass<HD><<<(a.past + a.n + np - 1u) / np * a.nkh * p.parts, 64u * (tiles < kMassWaves ? tiles : kMassWaves), 0, s>>>(
-        a, pt.stats, part, p.parts, rows_wide_kv(a), rows_wide_q(a));
+        a, pt, part, p.parts, rows_wide_kv(a));
 }
 
 hipError_t launch_attn_rows(const RowsArgs &a, void *scratch, hipStream_t s) {
@@ -1037,7 +1081,12 @@ hipError_t launch_attn_rows(const RowsArgs &a, void *scratch, hipStream_t s) {
     RowsPart pt{};
     if (p.sp.n > 1u) pt.ml = reinterpret_cast<float2 *>(at), pt.acc = reinterpret_cast<float *>(at + p.ml);
     if (a.mass) pt.stats = reinterpret_cast<float2 *>(at + p.ml + p.acc);
-    if (a.mass && p.few) pt.scores = reinterpret_cast<float *>(at + p.ml + p.acc + p.stats);
+    float *const mass = reinterpret_cast<float *>(at + p.ml + p.acc + p.stats);
+    if (a.mass && p.few) pt.scores = mass;
+    if (a.mass && !p.few) {
+        pt.qparts = reinterpret_cast<ru4 *>(at + p.ml + p.acc + p.stats + p.mass);
+        pt.qc = reinterpret_cast<float *>(at + p.ml + p.acc + p.stats + p.mass + p.qparts);
+    }
     switch (p.hd) {
         case 32: start_rows<32>(a, p, pt, s); break;
         case 64: start_rows<64>(a, p, pt, s); break;
@@ -1061,17 +1110,16 @@ hipError_t launch_attn_rows(const RowsArgs &a, void *scratch, hipStream_t s) {
         k_mass_few<<<dim3((a.past + a.n + 255u) / 256u, a.nkh), 256, 0, s>>>(a, pt);
         e = hipGetLastError();
     } else if (e == hipSuccess && a.mass) {
-        float *part = reinterpret_cast<float *>(at + p.ml + p.acc + p.stats);
         switch (p.hd) {
-            case 32: start_mass<32>(a, p, pt, part, s); break;
-            case 64: start_mass<64>(a, p, pt, part, s); break;
-            case 96: start_mass<96>(a, p, pt, part, s); break;
-            case 128: start_mass<128>(a, p, pt, part, s); break;
-            default: start_mass<256>(a, p, pt, part, s); break;
+            case 32: start_mass<32>(a, p, pt, mass, s); break;
+            case 64: start_mass<64>(a, p, pt, mass, s); break;
+            case 96: start_mass<96>(a, p, pt, mass, s); break;
+            case 128: start_mass<128>(a, p, pt, mass, s); break;
+            default: start_mass<256>(a, p, pt, mass, s); break;
         }
         e = hipGetLastError();
         if (e == hipSuccess && p.parts > 1u)
-            k_mass_add<<<dim3((a.past + a.n + 255u) / 256u, a.nkh), 256, 0, s>>>(a, part, p.parts);
+            k_mass_add<<<dim3((a.past + a.n + 255u) / 256u, a.nkh), 256, 0, s>>>(a, mass, p.parts);
         if (e == hipSuccess) e = hipGetLastError();
     }
     return e;
