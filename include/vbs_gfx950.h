@@ -240,7 +240,8 @@ int vbs_gfx950_linear_batch_multi(int type, uint32_t n_mat, const void *const *w
  * tokens whose attention the plain op does not have. A token is stored in a
  * slot of the cache; its position (for the rotation) may be any number. All:
  * n <= 65535 (0: nothing is done), at most 2^31 slots, head_dim even and <= 256, at most 16 q heads
- * per kv head; a row of q, k, v or out is n_heads x head_dim floats and rows lie
+ * per kv head, at most 2^28 rows (tokens x q heads) of an attention; a row of q, k, v or out is
+ * n_heads x head_dim floats and rows lie
  * a stride (in floats, at least a row) apart, so that the rows of a fused Q/K/V
  * product can be given as they are. No call waits for the device. */
 
@@ -289,7 +290,7 @@ typedef struct vbs_gfx950_attn_terms {
  * for the tree. With mass, the weight that each slot received is added to
  * mass[(layer * n_kv_heads + kv head) * max_ctx + slot], summed over the rows
  * and the q heads of the kv head in a fixed order: what vbs_gfx950_cache_evict
- * chooses by. */
+ * chooses by (for at most 2^27 slots x kv heads). */
 int vbs_gfx950_attention_chunk(const float *q, uint32_t q_stride, const uint16_t *kc,
                                const uint16_t *vc, float *out, uint32_t out_stride, uint32_t n,
                                uint32_t past, uint32_t layer, uint32_t max_ctx,
@@ -305,7 +306,8 @@ int vbs_gfx950_attention_chunk(const float *q, uint32_t q_stride, const uint16_t
  * from, and mass_out, if not NULL (it may be mass itself), their mass, and 0 for
  * the slots budget .. len - 1, so that tokens stored there start from 0. Each
  * head has its own slots afterwards: distances and documents by slot
- * (vbs_gfx950_attn_terms_t) then no longer mean the tokens' own. */
+ * (vbs_gfx950_attn_terms_t) then no longer mean the tokens' own. At most 2^20
+ * layers x kv heads. */
 int vbs_gfx950_cache_evict(uint16_t *kc, uint16_t *vc, const float *mass, float *mass_out,
                            uint32_t *kept, uint32_t len, uint32_t budget, uint32_t first,
                            uint32_t last, uint32_t layer, uint32_t n_layers, uint32_t max_ctx,

@@ -91,3 +91,12 @@ def test_reference_helpers():
     nan = float("nan")
     assert list(R.evict(np.array([9.0, 1, nan, 1, -np.inf, 2, 0]), 7, 5, 1, 1)) == [0, 1, 3, 5, 6]
     assert list(R.evict(np.array([nan, -np.inf, nan]), 3, 2, 0, 0)) == [0, 1]
+
+
+def test_sizes_beyond_a_launch(lib):
+    """Shapes whose launches would pass 2^32 threads of a dimension."""
+    wide = dict(n=65535, nqh=4112, nkh=257, hd=2, q_stride=8224, out_stride=8224, past=0, max_ctx=65535, out=1 << 50)
+    refused(lib, lib.attention_chunk, {**ATT, **wide}, "2.28")
+    refused(lib, lib.attention_tree, {**ATT, "mask": P2, **wide}, "2.28")
+    refused(lib, lib.attention_chunk, {**ATT, "past": 1 << 26, "max_ctx": BIG, "mass": P}, "2.27")
+    refused(lib, lib.cache_evict, {**EV, "n_layers": 4097, "nkh": 256}, "2.20")

@@ -785,6 +785,10 @@ bool spans_overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
 
 constexpr uint32_t kMaxStep = 65535;         // tokens of one call
 constexpr uint64_t kMaxSlots = 1ull << 31;   // slots that one call looks at
+// (below, what keeps every launch under 2^32 threads a dimension)
+constexpr uint64_t kMaxStepRows = 1ull << 28;  // tokens x q heads of an attention
+constexpr uint64_t kMaxMass = 1ull << 27;      // slots x kv heads of an attention with a mass
+constexpr uint64_t kMaxEvict = 1ull << 20;     // layers x kv heads of an eviction
 
 // The shape that the three operators of a step share; 0 with the reason set.
 int step_shape_ok(const char *who, uint32_t n, uint32_t slot, uint32_t max_ctx, uint32_t nqh, uint32_t nkh, uint32_t hd) {
@@ -803,6 +807,8 @@ int step_shape_ok(const char *who, uint32_t n, uint32_t slot, uint32_t max_ctx, 
 int attention_rows(const char *who, RowsArgs a, uint32_t layer) {
     if (!a.q || !a.kc || !a.vc || !a.out) return fail("%s: null pointer", who);
     if (!step_shape_ok(who, a.n, a.past, a.max_ctx, a.nqh, a.nkh, a.hd)) return 0;
+    if ((uint64_t)a.n * a.nqh > kMaxStepRows) return fail("%s: more than 2^28 tokens x q heads", who);
+    if (a.mass && ((uint64_t)a.past + a.n) * a.nkh > kMaxMass) return fail("%s: a mass of more than 2^27 slots x kv heads", who);
     const uint64_t row = (uint64_t)a.nqh * a.hd;
     if (a.q_stride < row || a.out_stride < row) return fail("%s: stride smaller than a row", who);
     if (a.n == 0) return 1;
@@ -900,6 +906,7 @@ int vbs_gfx950_cache_evict(uint16_t *kc, uint16_t *vc, const float *mass, float 
     if (budget > len) return fail("cache_evict: budget %u > len %u", budget, len);
     if ((uint64_t)first + last > budget) return fail("cache_evict: first %u + last %u > budget %u", first, last, budget);
     if (n_layers > 65535u || nkh > 65535u) return fail("cache_evict: more than 65535 layers or kv heads");
+    if ((uint64_t)n_layers * nkh > kMaxEvict) return fail("cache_evict: more than 2^20 layers x kv heads");
     if (hd > 256 || (hd & 1u)) return fail("cache_evict: head_dim %u must be even and <= 256", hd);
     const uint64_t rows = (uint64_t)n_layers * max_ctx * nkh, before = (uint64_t)layer * max_ctx * nkh;
     EvictArgs a{kc + before * hd, vc + before * hd, mass + before, mass_out ? mass_out + before : nullptr, kept,
