@@ -3,10 +3,11 @@
 //
 // Per layer and kv head: the first and the last slots stay, and of those between
 // the ones of the greatest weight (the lowest slot among equals; a NaN counts
-// as the lowest weight there is). Two launches: k_evict_select writes the kept
+// as the lowest weight there is). k_evict_select writes the kept
 // slots in order (one workgroup per layer and head: the weight of the last slot
 // taken by a radix selection over the 32-bit order of floats, then one ordered
-// pass), k_evict_move moves their K and V rows to the front.
+// pass), k_evict_move moves their K and V rows to the front; k_evict does both for
+// few heads of few slots.
 //
 // The move is in place. A kept slot never moves up (its new place is the number
 // of kept slots before it), so rows taken in ascending order are safe as long as
@@ -20,7 +21,7 @@
 namespace vbs {
 
 constexpr uint32_t kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelBins = 2048;
-constexpr uint32_t kSelKeys = 8, kSelRun = kSelThreads * kSelKeys;  // slots a thread and a workgroup hold at once
+constexpr uint32_t kSelKeys = 8, kSelRun = kSelThreads * kSelKeys;  // most slots a thread and a workgroup hold at once
 
 // The order of weights as unsigned numbers: -0 as 0, NaN below everything.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -29,13 +30,15 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// Inclusive sum over the lanes up to each.
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t lane) {
-#pragma unroll
-    for (uint32_t o = 1; o < 64u; o <<= 1) {
-        const uint32_t x = __shfl_up(v, o, 64);
-        if (lane >= o) v += x;
-    }
+// Inclusive sum over the lanes up to each: within the rows of 16 lanes, then the rows before added (DPP row_shr and
+// row_bcast; lanes without a source add 0). The whole wave must be active.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);  // lane 15 of rows 0, 2 to rows 1, 3
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);  // lane 31 to rows 2, 3
     return v;
 }
 // The sum of the waves' entries before `wave`, and of all.
@@ -50,23 +53,29 @@ __device__ __forceinline__ uint2 waves_before(const uint32_t *waves, uint32_t wa
     return make_uint2(before, all);
 }
 
-__global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
+// The selection of one layer and head by a workgroup: put(place, slot, weight) for every kept slot.
+template <uint32_t KEYS, class Put>
+__device__ __forceinline__ void evict_select(const EvictArgs &a, const float *mass, Put put) {
     __shared__ uint32_t hist[kSelBins], waves[2][kSelWaves], s_bin, s_need, s_count;
-    const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u, h = blockIdx.x, l = blockIdx.y;
-    const float *mass = a.mass + ((uint64_t)l * a.nkh + h) * a.max_ctx;
-    float *mass_out = a.mass_out ? a.mass_out + ((uint64_t)l * a.nkh + h) * a.max_ctx : nullptr;
-    uint32_t *kept = a.kept + ((uint64_t)l * a.nkh + h) * a.budget;
+    const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u;
     const uint32_t lo = a.first, hi = a.len - a.last;  // the slots that are chosen among
     uint32_t need = a.budget - a.first - a.last;       // as many of them
 
-    // a run of kSelRun slots in registers, 64 kSelKeys in a row to each wave; the weights stay
-    // there if one run holds them all
-    const uint32_t runs = (a.len + kSelRun - 1u) / kSelRun;
-    float w[kSelKeys];
-    auto slot = [&](uint32_t run, uint32_t k) { return run * kSelRun + (wave * kSelKeys + k) * 64u + lane; };
+    // a run of slots in registers, 64 KEYS in a row to each wave; the weights stay there if one run holds them all
+    constexpr uint32_t RUN = kSelThreads * KEYS;
+    const uint32_t runs = (a.len + RUN - 1u) / RUN;
+    float w[KEYS];
+    uint32_t key[KEYS], is_open = 0;  // (bits of the slots that are chosen among)
+    auto slot = [&](uint32_t run, uint32_t k) { return run * RUN + (wave * KEYS + k) * 64u + lane; };
     auto load = [&](uint32_t run) {
+        is_open = 0;
 #pragma unroll
-        for (uint32_t k = 0; k < kSelKeys; k++) w[k] = slot(run, k) < a.len ? mass[slot(run, k)] : 0.f;
+        for (uint32_t k = 0; k < KEYS; k++) w[k] = slot(run, k) < a.len ? mass[slot(run, k)] : 0.f;
+#pragma unroll
+        for (uint32_t k = 0; k < KEYS; k++) {
+            key[k] = weight_key(w[k]);
+            is_open |= (slot(run, k) >= lo && slot(run, k) < hi ? 1u : 0u) << k;
+        }
     };
     load(0u);
 
@@ -81,16 +90,14 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
         for (uint32_t run = 0; run < runs; run++) {
             if (runs > 1u) load(run);
 #pragma unroll
-            for (uint32_t k = 0; k < kSelKeys; k++) {
-                const uint32_t j = slot(run, k), key = weight_key(w[k]);
-                if (j >= lo && j < hi && (bits == 0u || key >> (32u - bits) == prefix))
-                    atomicAdd(&hist[key >> shift & ((1u << width) - 1u)], 1u);
-            }
+            for (uint32_t k = 0; k < KEYS; k++)
+                if ((is_open >> k & 1u) && (bits == 0u || key[k] >> (32u - bits) == prefix))
+                    atomicAdd(&hist[key[k] >> shift & ((1u << width) - 1u)], 1u);
         }
         __syncthreads();
         // thread t takes the bins 2 t and 2 t + 1 counted from the greatest
         const uint32_t top = kSelBins - 1u - 2u * t, n0 = hist[top], n1 = hist[top - 1u];
-        const uint32_t sum = wave_scan(n0 + n1, lane);
+        const uint32_t sum = wave_scan(n0 + n1);
         if (lane == 63u) waves[0][wave] = sum;
         __syncthreads();
         const uint32_t before = waves_before(waves[0], wave).x + sum - n0 - n1;
@@ -115,24 +122,24 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
         if (runs > 1u) load(run);  // (what earlier runs wrote lies below this run's slots)
         uint32_t tie = 0, keep = 0, n = 0;  // bits per key; the wave's count
 #pragma unroll
-        for (uint32_t k = 0; k < kSelKeys; k++) {
-            const uint32_t j = slot(run, k), head = any ? weight_key(w[k]) >> down : 0u;
-            const bool open = j >= lo && j < hi;
+        for (uint32_t k = 0; k < KEYS; k++) {
+            const uint32_t head = any ? key[k] >> down : 0u;
+            const bool open = is_open >> k & 1u;
             if (any && open && head == prefix) tie |= 1u << k;
-            if (j < a.len && (!open || (any && head > prefix))) keep |= 1u << k;
+            if (slot(run, k) < a.len && (!open || (any && head > prefix))) keep |= 1u << k;
         }
         if (whole) {
             keep |= tie;
         } else if (any) {
 #pragma unroll
-            for (uint32_t k = 0; k < kSelKeys; k++) n += (uint32_t)__popcll(__ballot(tie >> k & 1u));
+            for (uint32_t k = 0; k < KEYS; k++) n += (uint32_t)__popcll(__ballot(tie >> k & 1u));
             if (lane == 0) waves[0][wave] = n;
             __syncthreads();
             const uint2 b = waves_before(waves[0], wave);
             uint32_t at = ties0 + b.x;
             ties0 += b.y;
 #pragma unroll
-            for (uint32_t k = 0; k < kSelKeys; k++) {
+            for (uint32_t k = 0; k < KEYS; k++) {
                 const uint64_t m = __ballot(tie >> k & 1u);
                 if ((tie >> k & 1u) && at + (uint32_t)__popcll(m & ((1ull << lane) - 1ull)) < need) keep |= 1u << k;
                 at += (uint32_t)__popcll(m);
@@ -140,27 +147,37 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
         }
         n = 0;
 #pragma unroll
-        for (uint32_t k = 0; k < kSelKeys; k++) n += (uint32_t)__popcll(__ballot(keep >> k & 1u));
+        for (uint32_t k = 0; k < KEYS; k++) n += (uint32_t)__popcll(__ballot(keep >> k & 1u));
         if (lane == 0) waves[1][wave] = n;
         __syncthreads();  // (every weight of this run is in a register)
         const uint2 b = waves_before(waves[1], wave);
         uint32_t at = kept0 + b.x;
         kept0 += b.y;
 #pragma unroll
-        for (uint32_t k = 0; k < kSelKeys; k++) {
+        for (uint32_t k = 0; k < KEYS; k++) {
             const uint64_t m = __ballot(keep >> k & 1u);
             if (keep >> k & 1u) {
                 const uint32_t to = at + (uint32_t)__popcll(m & ((1ull << lane) - 1ull));
-                kept[to] = slot(run, k);
-                if (mass_out) mass_out[to] = w[k];  // (to <= the slot)
+                put(to, slot(run, k), w[k]);  // (to <= the slot)
             }
             at += (uint32_t)__popcll(m);
         }
         if (runs > 1u) __syncthreads();  // (the counts are read before the next run's)
     }
     __syncthreads();
+}
+
+template <uint32_t KEYS>
+__global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
+    const uint64_t lh = (uint64_t)blockIdx.y * a.nkh + blockIdx.x;
+    float *mass_out = a.mass_out ? a.mass_out + lh * a.max_ctx : nullptr;
+    uint32_t *kept = a.kept + lh * a.budget;
+    evict_select<KEYS>(a, a.mass + lh * a.max_ctx, [&](uint32_t to, uint32_t slot, float w) {
+        kept[to] = slot;
+        if (mass_out) mass_out[to] = w;
+    });
     if (mass_out)
-        for (uint32_t j = a.budget + t; j < a.len; j += kSelThreads) mass_out[j] = 0.f;
+        for (uint32_t j = a.budget + threadIdx.x; j < a.len; j += kSelThreads) mass_out[j] = 0.f;
 }
 
 // A slice: `lanes` units of type U of one head's rows, of K or of V. Threads: (row, unit).
@@ -169,14 +186,19 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_select(EvictArgs a) {
 constexpr uint32_t kMoveThreads = 512, kMoveDepth = 4, kXcds = 8;
 typedef uint32_t eu4 __attribute__((ext_vector_type(4)));
 
-template <class U>
-__global__ __launch_bounds__(kMoveThreads) void k_evict_move(EvictArgs a, uint32_t lanes, uint32_t slices) {
-    const uint32_t t = threadIdx.x, rows = kMoveThreads / lanes, row = t / lanes;
-    const uint32_t slice = blockIdx.x / kXcds % slices, unit = blockIdx.x / (kXcds * slices) * kXcds + blockIdx.x % kXcds;
-    if (unit >= 2u * a.nkh * a.n_layers) return;  // (the grid is whole groups of kXcds units)
-    const uint32_t lh = unit >> 1, l = lh / a.nkh, h = lh % a.nkh;
-    const uint32_t units = a.hd * 2u / (uint32_t)sizeof(U), u = slice * lanes + t % lanes;
-    const uint32_t *kept = a.kept + (uint64_t)lh * a.budget;
+struct MoveOf {  // whose rows this workgroup moves: the unit (layer, head, K or V) and the slice of them
+    uint32_t unit, slice;
+    bool any;
+    __device__ MoveOf(const EvictArgs &a, uint32_t slices)
+        : unit(blockIdx.x / (kXcds * slices) * kXcds + blockIdx.x % kXcds), slice(blockIdx.x / kXcds % slices),
+          any(unit < 2u * a.nkh * a.n_layers) {}  // (the grid is whole groups of kXcds units)
+};
+
+template <class U, uint32_t THREADS, class Id>
+__device__ __forceinline__ void evict_move(const EvictArgs &a, MoveOf of, uint32_t lanes, const Id *kept) {
+    const uint32_t t = threadIdx.x, rows = THREADS / lanes, row = t / lanes, unit = of.unit;
+    const uint32_t l = (unit >> 1) / a.nkh, h = (unit >> 1) % a.nkh;
+    const uint32_t units = a.hd * 2u / (uint32_t)sizeof(U), u = of.slice * lanes + t % lanes;
     U *c = reinterpret_cast<U *>(unit & 1u ? a.vc : a.kc) + ((uint64_t)l * a.max_ctx * a.nkh + h) * units + u;
     const uint64_t stride = (uint64_t)a.nkh * units;
     const uint32_t budget = row < rows && u < units ? a.budget : 0u;  // (threads past the slice have nothing)
@@ -216,10 +238,34 @@ __global__ __launch_bounds__(kMoveThreads) void k_evict_move(EvictArgs a, uint32
     }
 }
 
+template <class U>
+__global__ __launch_bounds__(kMoveThreads) void k_evict_move(EvictArgs a, uint32_t lanes, uint32_t slices) {
+    const MoveOf of(a, slices);
+    if (of.any) evict_move<U, kMoveThreads>(a, of, lanes, a.kept + (uint64_t)(of.unit >> 1) * a.budget);
+}
+
+// Both in one launch, where a run holds every slot: each workgroup of a head selects for itself, and one of them
+// writes what the caller gets. Not where mass_out is mass, which the others may still have to read.
+template <class U, uint32_t KEYS>
+__global__ __launch_bounds__(kSelThreads) void k_evict(EvictArgs a, uint32_t lanes, uint32_t slices) {
+    __shared__ uint16_t ids[kSelThreads * KEYS];
+    const MoveOf of(a, slices);
+    if (!of.any) return;
+    const uint64_t lh = of.unit >> 1;
+    const bool tells = !(of.unit & 1u) && of.slice == 0u;
+    float *mass_out = tells && a.mass_out ? a.mass_out + lh * a.max_ctx : nullptr;
+    uint32_t *kept = a.kept + lh * a.budget;
+    evict_select<KEYS>(a, a.mass + lh * a.max_ctx, [&](uint32_t to, uint32_t slot, float w) {
+        ids[to] = (uint16_t)slot;
+        if (tells) kept[to] = slot;
+        if (mass_out) mass_out[to] = w;
+    });
+    if (mass_out)
+        for (uint32_t j = a.budget + threadIdx.x; j < a.len; j += kSelThreads) mass_out[j] = 0.f;
+    evict_move<U, kSelThreads>(a, of, lanes, ids);
+}
+
 hipError_t launch_evict(const EvictArgs &a, hipStream_t s) {
-    k_evict_select<<<dim3(a.nkh, a.n_layers), kSelThreads, 0, s>>>(a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
     const bool wide = a.hd % 8u == 0 && (((uintptr_t)a.kc | (uintptr_t)a.vc) & 15u) == 0;
     // Whole rows a workgroup where that gives a workgroup per CU (32 layers of 8 heads of 128, 8192
     // slots to 4096: 223 us, 4.8 TB/s read and written; half rows 253, quarters 303, eighths 335), else
@@ -229,6 +275,28 @@ hipError_t launch_evict(const EvictArgs &a, hipStream_t s) {
     while (lanes > least && pairs * ((units + lanes - 1u) / lanes) < 256u) lanes = (lanes + 1u) / 2u;
     const uint32_t slices = (units + lanes - 1u) / lanes;
     const uint32_t grid = (pairs + kXcds - 1u) / kXcds * kXcds * slices;
+    // Four slots a thread where they hold every slot: the code is read anew by every launch and is shorter (2049 slots:
+    // the selection 9.2 us under the tracer with eight, 6.7 with four). One launch for up to two workgroups per CU
+    // (2049 to 1024 of 8 heads 8.7 us, two launches 10.0; 32 layers of 8192 to 4096 229 and 236); with more, selecting
+    // for K and for V costs more than a launch.
+    const bool small = a.len <= kSelThreads * 4u;
+    if (a.len <= kSelRun && a.mass_out != a.mass && grid <= 512u) {
+        if (small && wide)
+            k_evict<eu4, 4><<<grid, kSelThreads, 0, s>>>(a, lanes, slices);
+        else if (wide)
+            k_evict<eu4, 8><<<grid, kSelThreads, 0, s>>>(a, lanes, slices);
+        else if (small)
+            k_evict<uint16_t, 4><<<grid, kSelThreads, 0, s>>>(a, lanes, slices);
+        else
+            k_evict<uint16_t, 8><<<grid, kSelThreads, 0, s>>>(a, lanes, slices);
+        return hipGetLastError();
+    }
+    if (small)
+        k_evict_select<4><<<dim3(a.nkh, a.n_layers), kSelThreads, 0, s>>>(a);
+    else
+        k_evict_select<8><<<dim3(a.nkh, a.n_layers), kSelThreads, 0, s>>>(a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
     if (wide)
         k_evict_move<eu4><<<grid, kMoveThreads, 0, s>>>(a, lanes, slices);
     else
