@@ -16,6 +16,12 @@ typedef float rf2 __attribute__((ext_vector_type(2)));
 typedef float rf4 __attribute__((ext_vector_type(4)));
 typedef uint32_t ru4 __attribute__((ext_vector_type(4)));
 
+// r / group, the token of row r of a kv head: r + 1/2 is exact, at least 1/2 / group from where the quotient turns, and
+// the two roundings lose less than 2^20 / group * 2^-23 (rows are fewer than 2^20).
+__device__ __forceinline__ uint32_t row_token(const RowsArgs &a, uint32_t r) {
+    return (uint32_t)(((float)r + 0.5f) * a.rgroup);
+}
+
 // Whether row i (slot past + i) sees slot j.
 __device__ __forceinline__ bool row_sees(const RowsArgs &a, uint32_t i, uint32_t j) {
     if (a.mask) {
@@ -79,7 +85,7 @@ template <uint32_t HD>
 __device__ __forceinline__ void row_whole(const RowsArgs &a, uint32_t i, uint32_t h, uint32_t s0, uint32_t s1,
                                           uint32_t lane, float &m_out, float &l_out, float (&acc)[(HD + 63) / 64],
                                           float *scores = nullptr) {
-    const uint32_t kvh = h / (a.nqh / a.nkh);
+    const uint32_t kvh = h / a.group;
     const float *q = a.q + (uint64_t)i * a.q_stride + (uint64_t)h * a.hd;
     const uint64_t rstride = (uint64_t)a.nkh * a.hd, base = (uint64_t)kvh * a.hd;
     const float slope = a.slopes ? a.slopes[h] : 0.f;

@@ -815,6 +815,8 @@ int attention_rows(const char *who, RowsArgs a, uint32_t layer) {
     if (spans_overlap(a.q, 4u * ((uint64_t)(a.n - 1u) * a.q_stride + row), a.out,
                       4u * ((uint64_t)(a.n - 1u) * a.out_stride + row)))
         return fail("%s: out overlaps q", who);
+    a.group = a.nqh / a.nkh;
+    a.rgroup = 1.f / (float)a.group;
     a.kc += (uint64_t)layer * a.max_ctx * a.nkh * a.hd;
     a.vc += (uint64_t)layer * a.max_ctx * a.nkh * a.hd;
     if (a.mass) a.mass += (uint64_t)layer * a.nkh * a.max_ctx;

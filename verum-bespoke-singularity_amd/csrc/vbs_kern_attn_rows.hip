@@ -265,26 +265,26 @@ struct RowTile {
     // what is read of q (its loads are to be under way before the first tile's, behind which they would wait)
     __device__ __forceinline__ static void load(const RowsArgs &a, uint32_t kvh, uint32_t row0, bool wide_q, uint32_t lane,
                                                 RowQ<KK> &x) {
-        const uint32_t group = a.nqh / a.nkh, r = row0 + (lane & 15u);
-        x.load(r < a.n * group ? a.q + (uint64_t)(r / group) * a.q_stride + (uint64_t)(kvh * group + r % group) * a.hd : nullptr,
+        const uint32_t group = a.group, r = row0 + (lane & 15u), i = row_token(a, r);
+        x.load(r < a.n * group ? a.q + (uint64_t)i * a.q_stride + (uint64_t)(kvh * group + r - i * group) * a.hd : nullptr,
                a.hd, wide_q, lane >> 4);
     }
     // v_at: from a tile's first byte of K to its first of V
     __device__ __forceinline__ void init(const RowsArgs &a, uint32_t kvh, uint32_t row0, const RowQ<KK> &x, uint32_t lane,
                                          uint32_t v_at) {
-        const uint32_t col = lane & 15u, g = lane >> 4, group = a.nqh / a.nkh, rows = a.n * group;
+        const uint32_t col = lane & 15u, g = lane >> 4, group = a.group, rows = a.n * group;
         const uint32_t r = row0 + col;
         real = r < rows;
-        tok = real ? r / group : 0u;
-        const uint32_t h = kvh * group + (real ? r % group : 0u);
+        tok = real ? row_token(a, r) : 0u;
+        const uint32_t h = kvh * group + (real ? r - tok * group : 0u);
         slope = a.slopes ? a.slopes[h] : 0.f;
         doc = a.docs ? a.docs[a.past + tok] : 0;
         x.split(a.scale, qh, ql, c1);
         m = -INFINITY, l = 0.f;
 #pragma unroll
         for (uint32_t d = 0; d < DT; d++) acc[d] = rf4{0.f, 0.f, 0.f, 0.f};
-        clear = a.docs ? 0u : a.mask ? a.past : row_end(a, min(row0, rows - 1u) / group);
-        last = row0 < rows ? row_end(a, (min(row0 + 16u, rows) - 1u) / group) : 0u;
+        clear = a.docs ? 0u : a.mask ? a.past : row_end(a, row_token(a, min(row0, rows - 1u)));
+        last = row0 < rows ? row_end(a, row_token(a, min(row0 + 16u, rows) - 1u)) : 0u;
         // its chunk of K per slice (row `col` of a 16-row tile), and per 16 dims its part of the
         // transposed V read: slot 4 g + col / 4, dims 4 (col % 4) ..
 #pragma unroll
@@ -471,11 +471,12 @@ struct RowsTo {
     float2 *stats;  // NULL: not wanted
     __device__ __forceinline__ RowsTo(const RowsArgs &a, const RowsSplit &sp, const RowsPart &pt, uint32_t kvh,
                                       uint32_t split, uint32_t r) {
-        const uint32_t group = a.nqh / a.nkh, rows = a.n * group;
+        const uint32_t group = a.group, rows = a.n * group;
+        const uint32_t i = row_token(a, r);
         const uint64_t at = ((uint64_t)kvh * sp.n + split) * rows + r;
         ml = sp.n > 1u ? pt.ml + at : nullptr;
         acc = sp.n > 1u ? pt.acc + at * part_stride(a.hd)
-                        : a.out + (uint64_t)(r / group) * a.out_stride + (uint64_t)(kvh * group + r % group) * a.hd;
+                        : a.out + (uint64_t)i * a.out_stride + (uint64_t)(kvh * group + r - i * group) * a.hd;
         stats = sp.n == 1u && pt.stats ? pt.stats + (uint64_t)kvh * rows + r : nullptr;
     }
     __device__ __forceinline__ float scale(float l) const { return ml ? 1.f : l == 0.f ? 0.f : __fdiv_rn(1.f, l); }
@@ -488,9 +489,9 @@ struct RowsTo {
 template <uint32_t HD>
 __device__ __forceinline__ void row_again(const RowsArgs &a, const RowsSplit &sp, const RowsPart &pt, uint32_t kvh,
                                           uint32_t split, uint32_t r, uint32_t s0, uint32_t s1, uint32_t lane) {
-    const uint32_t group = a.nqh / a.nkh;
+    const uint32_t group = a.group, i = row_token(a, r);
     float m, l, o[(HD + 63u) / 64u];
-    row_whole<HD>(a, r / group, kvh * group + r % group, s0, s1, lane, m, l, o,
+    row_whole<HD>(a, i, kvh * group + r - i * group, s0, s1, lane, m, l, o,
                   pt.scores ? pt.scores + ((uint64_t)kvh * a.n * group + r) * score_stride(a.past + a.n) : nullptr);
     const RowsTo to(a, sp, pt, kvh, split, r);
 #pragma unroll
@@ -501,17 +502,16 @@ __device__ __forceinline__ void row_again(const RowsArgs &a, const RowsSplit &sp
 
 // ---- many rows: four waves with rows of their own, slots through two shared buffers ------
 template <uint32_t HD>
-__global__ __launch_bounds__(256, 2) void k_attn_rows(RowsArgs a, RowsSplit sp, RowsPart pt, uint32_t tiles, bool wide_kv,
+__global__ __launch_bounds__(256, 2) void k_attn_rows(RowsArgs a, RowsSplit sp, RowsPart pt, bool wide_kv,
                                                  bool wide_q) {
     constexpr uint32_t DT = HD / 16u, T = kTile<HD>, CPR = HD / 8u, NC = T * CPR / 256u;
     constexpr uint32_t RB = HD * 2u, TB = T * RB;  // bytes of a row and of a tile
     __shared__ __align__(1024) uint8_t kv[2][2][TB];  // two buffers of K and V
     __shared__ __align__(16) int32_t dl[2][T];
     const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u, col = lane & 15u, g = lane >> 4;
-    const uint32_t kvh = blockIdx.x % a.nkh, rest = blockIdx.x / a.nkh;
-    const uint32_t split = rest % sp.n, tile = tiles - 1u - rest / sp.n;  // (the longest rows first)
-    const uint32_t group = a.nqh / a.nkh, rows = a.n * group, row_tile = tile * 64u;
-    const uint32_t end = row_end(a, (min(row_tile + 64u, rows) - 1u) / group);
+    const uint32_t kvh = blockIdx.x, split = blockIdx.y, tile = gridDim.z - 1u - blockIdx.z;  // (the longest rows first)
+    const uint32_t group = a.group, rows = a.n * group, row_tile = tile * 64u;
+    const uint32_t end = row_end(a, row_token(a, min(row_tile + 64u, rows) - 1u));
     const uint32_t s0 = split * sp.len, s1 = min(s0 + sp.len, end);
     if (s0 >= s1) return;  // (the whole workgroup; the merge counts the ranges the same way)
     const uint32_t slots = a.past + a.n, row0 = row_tile + wave * 16u;
@@ -561,7 +561,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(RowsArgs a, RowsSplit sp, 
         __syncthreads();
     };
 
-    DocRange of(a, row_tile / group, (min(row_tile + 64u, rows) - 1u) / group, s0, s1, lane);
+    DocRange of(a, row_token(a, row_tile), row_token(a, min(row_tile + 64u, rows) - 1u), s0, s1, lane);
     uint32_t p0 = of.next(a, s0, s1, lane);
     RowQ<HD / 32u> x;
     RowTile<HD>::load(a, kvh, row0, wide_q, lane, x);
@@ -639,9 +639,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_few(RowsArgs a, RowsSplit sp, R
     __shared__ float2 mls[4][16u];
     __shared__ uint32_t bad[16u];
     const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63u, col = lane & 15u, g = lane >> 4;
-    const uint32_t kvh = blockIdx.x % a.nkh, rest = blockIdx.x / a.nkh, split = rest % sp.n, row0 = rest / sp.n * 16u;
-    const uint32_t group = a.nqh / a.nkh, rows = a.n * group, slots = a.past + a.n;
-    const uint32_t end = row_end(a, (min(row0 + 16u, rows) - 1u) / group);
+    const uint32_t kvh = blockIdx.x, split = blockIdx.y, row0 = 16u * blockIdx.z;
+    const uint32_t group = a.group, rows = a.n * group, slots = a.past + a.n;
+    const uint32_t end = row_end(a, row_token(a, min(row0 + 16u, rows) - 1u));
     const uint32_t s0 = split * sp.len, s1 = min(s0 + sp.len, end);
     if (s0 >= s1) return;  // (the whole workgroup)
     uint8_t *const own = &kv[wave][0];
@@ -667,7 +667,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_few(RowsArgs a, RowsSplit sp, R
             }
         }
     };
-    const DocRange of(a, row0 / group, (min(row0 + 16u, rows) - 1u) / group, s0, s1, lane);
+    const DocRange of(a, row_token(a, row0), row_token(a, min(row0 + 16u, rows) - 1u), s0, s1, lane);
     // (the wave's next tile, past those without a slot of the rows' documents)
     auto next = [&](uint32_t p) {
         if (a.docs)
@@ -748,47 +748,56 @@ __global__ __launch_bounds__(256, 2) void k_attn_few(RowsArgs a, RowsSplit sp, R
 constexpr uint32_t kMostRanges = 128;
 
 template <uint32_t TPR>
-__global__ __launch_bounds__(256) void k_attn_rows_merge(RowsArgs a, RowsSplit sp, RowsPart pt, uint32_t tile_rows, uint32_t width) {
+__global__ __launch_bounds__(256) void k_attn_rows_merge(RowsArgs a, RowsSplit sp, RowsPart pt, uint32_t tile_bits, uint32_t width_bits) {
     __shared__ rf4 part[256];
     const uint32_t t = threadIdx.x, lane = t & 63u, in = t % TPR, kvh = blockIdx.y;
-    const uint32_t group = a.nqh / a.nkh, rows = a.n * group, r = min(blockIdx.x * (256u / TPR) + t / TPR, rows - 1u);
-    const uint32_t end = row_end(a, (min(r / tile_rows * tile_rows + tile_rows, rows) - 1u) / group);
-    const uint32_t n = (end + sp.len - 1u) / sp.len;
-    const uint32_t q = in % width, grp = in / width, groups = TPR / width, ps = part_stride(a.hd);
+    const uint32_t group = a.group, rows = a.n * group, r = min(blockIdx.x * (256u / TPR) + t / TPR, rows - 1u);
+    const uint32_t end = row_end(a, row_token(a, min((r >> tile_bits) + 1u << tile_bits, rows) - 1u)), i = row_token(a, r);
+    const uint32_t width = 1u << width_bits, q = in & (width - 1u), grp = in >> width_bits, groups = TPR >> width_bits;
+    const uint32_t ps = part_stride(a.hd);
+    auto has = [&](uint32_t c) { return c < sp.n && c * sp.len < end; };  // (sp.n ranges pass the last slot by less than one)
     const float2 *ml = pt.ml + (uint64_t)kvh * sp.n * rows + r;
-    const float *acc = pt.acc + ((uint64_t)kvh * sp.n * rows + r) * ps + 4u * q;
+    const float *acc = pt.acc + ((uint64_t)kvh * sp.n * rows + r) * ps + min(4u * q, ps - 4u);
     const bool mine = 4u * q < a.hd;
     rf4 v[8];
-    auto load = [&](uint32_t c0) {
+    auto load = [&](uint32_t c0) {  // (range 0, which every row has, for one that is not there)
 #pragma unroll
         for (uint32_t k = 0; k < 8u; k++) {
             const uint32_t c = c0 + k * groups;
-            v[k] = mine && c < n ? *reinterpret_cast<const rf4 *>(acc + (uint64_t)c * rows * ps) : rf4{0.f, 0.f, 0.f, 0.f};
+            v[k] = *reinterpret_cast<const rf4 *>(acc + (uint64_t)((has(c) ? c : 0u) * rows) * ps);
         }
     };
     load(grp);
-    const float2 none = make_float2(-INFINITY, 0.f);
-    const float2 x0 = lane < n ? ml[(uint64_t)lane * rows] : none;
-    const float2 x1 = lane + 64u < n ? ml[(uint64_t)(lane + 64u) * rows] : none;
-    const float M = wave_max(fmaxf(x0.x, x1.x)), ref = M == -INFINITY ? 0.f : M;
-    const float w0 = exp2f(x0.x - ref), w1 = exp2f(x1.x - ref);
-    const float L = wave_sum(fmaf(x0.y, w0, x1.y * w1));
+    const float2 y0 = ml[(has(lane) ? lane : 0u) * rows], y1 = ml[(has(lane + 64u) ? lane + 64u : 0u) * rows];
+    const float m0 = has(lane) ? y0.x : -INFINITY, m1 = has(lane + 64u) ? y1.x : -INFINITY;
+    const float M = wave_max(fmaxf(m0, m1)), ref = M == -INFINITY ? 0.f : M;
+    const float w0 = exp2f(m0 - ref), w1 = exp2f(m1 - ref);
+    const float L = wave_sum(fmaf(has(lane) ? y0.y : 0.f, w0, (has(lane + 64u) ? y1.y : 0.f) * w1));
     rf4 o = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t c0 = grp; c0 < n + grp; c0 += 8u * groups) {  // (the same count in every lane)
-        if (c0 != grp) load(c0);
+    for (uint32_t c0 = grp;;) {  // (the same rounds in every lane)
 #pragma unroll
         for (uint32_t k = 0; k < 8u; k++) {
             const uint32_t c = c0 + k * groups;
-            const float f0 = __shfl(w0, (int)(c & 63u), 64), f1 = __shfl(w1, (int)(c & 63u), 64);
-            if (c < n) o += v[k] * (c < 64u ? f0 : f1);
+            float f = __shfl(w0, (int)(c & 63u), 64);
+            if (TPR > 64u) {  // (a wave per row takes at most 64 ranges)
+                const float f1 = __shfl(w1, (int)(c & 63u), 64);
+                f = c < 64u ? f : f1;
+            }
+            const rf4 sum = o + v[k] * f;
+            const bool is = has(c);
+#pragma unroll
+            for (uint32_t x = 0; x < 4u; x++) o[x] = is ? sum[x] : o[x];
         }
+        c0 += 8u * groups;
+        if (c0 - grp >= sp.n) break;
+        load(c0);
     }
     part[t] = o;
     __syncthreads();
     if (grp || !mine || blockIdx.x * (256u / TPR) + t / TPR >= rows) return;
     for (uint32_t k = 1; k < groups; k++) o += part[t + k * width];
     const float inv = L == 0.f ? 0.f : __fdiv_rn(1.f, L);
-    float *to = a.out + (uint64_t)(r / group) * a.out_stride + (uint64_t)(kvh * group + r % group) * a.hd + 4u * q;
+    float *to = a.out + (uint64_t)i * a.out_stride + (uint64_t)(kvh * group + r - i * group) * a.hd + 4u * q;
 #pragma unroll
     for (uint32_t k = 0; k < 4u; k++)
         if (4u * q + k < a.hd) to[k] = L == 0.f ? 0.f : o[k] * inv;
@@ -819,7 +828,7 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, RowsPart p
     const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u, col = lane & 15u, g = lane >> 4;
     const uint32_t waves = blockDim.x >> 6, kvh = blockIdx.x % a.nkh, rest = blockIdx.x / a.nkh;
     const uint32_t mine = rest % parts, p0 = rest / parts * NP;
-    const uint32_t group = a.nqh / a.nkh, rows = a.n * group, slots = a.past + a.n;
+    const uint32_t group = a.group, rows = a.n * group, slots = a.past + a.n;
     const uint64_t rstride = (uint64_t)a.nkh * a.hd;
     const float2 *stats = pt.stats + (uint64_t)kvh * rows;
     rh8 ka[NT][KK];
@@ -860,7 +869,7 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, RowsPart p
         bool need = lt < t1;
         if (a.docs && need) {
             need = false;
-            for (uint32_t i = 16u * lt / group; i <= (min(16u * lt + 16u, rows) - 1u) / group; i++) {
+            for (uint32_t i = row_token(a, 16u * lt); i <= row_token(a, min(16u * lt + 16u, rows) - 1u); i++) {
                 const int32_t d = a.docs[a.past + i];
                 need = need || (d >= lo && d <= hi);
             }
@@ -872,7 +881,7 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, RowsPart p
             left &= left - 1ull;
             const uint32_t r = 16u * rt + col;
             const bool real = r < rows;
-            const uint32_t i = real ? r / group : 0u, h = kvh * group + (real ? r % group : 0u);
+            const uint32_t i = real ? row_token(a, r) : 0u, h = kvh * group + (real ? r - i * group : 0u);
             const float2 st = real ? stats[r] : make_float2(0.f, 0.f);
             const float c1 = pt.qc[((uint64_t)kvh * all + rt) * 16u + col];
             rh8 qh[KK], ql[KK];
@@ -881,7 +890,7 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, RowsPart p
                 qh[kk] = __builtin_bit_cast(rh8, qn[kk][0]), ql[kk] = __builtin_bit_cast(rh8, qn[kk][1]);
             if (left) fetch(base + (uint32_t)__builtin_ctzll(left) * waves);
             const bool full = !a.docs && 16u * rt + 16u <= rows &&
-                              p0 + NP <= (a.mask ? a.past : row_end(a, 16u * rt / group));
+                              p0 + NP <= (a.mask ? a.past : row_end(a, row_token(a, 16u * rt)));
             const uint64_t vis = full ? ~0ull : real ? seen_bits(a, i, p0, slots) : 0ull;
             const int32_t doc = a.docs ? a.docs[a.past + i] : 0;
             const float slope = a.slopes ? a.slopes[h] : 0.f, ms = st.x == -INFINITY ? 0.f : st.x;
@@ -938,7 +947,7 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, RowsPart p
         const uint16_t *k = a.kc + (uint64_t)jj * rstride + (uint64_t)kvh * a.hd;
         float whole = 0.f;
         for (uint32_t r = 16u * t0 + lane; r < min(16u * t1, rows); r += 64u) {
-            const uint32_t i = r / group, h = kvh * group + r % group;
+            const uint32_t i = row_token(a, r), h = kvh * group + r - i * group;
             if (jj >= row_end(a, i) || !row_sees(a, i, jj)) continue;
             const float s = row_score(a, row_dot(a.q + (uint64_t)i * a.q_stride + (uint64_t)h * a.hd, k, a.hd) * a.scale,
                                       a.slopes ? a.slopes[h] : 0.f, a.past + i, jj);
@@ -957,7 +966,7 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, RowsPart p
 
 // Few rows: their scores are there (k_attn_few), a thread takes a slot.
 __global__ __launch_bounds__(256) void k_mass_few(RowsArgs a, RowsPart pt) {
-    const uint32_t j = blockIdx.x * 256u + threadIdx.x, kvh = blockIdx.y, slots = a.past + a.n, group = a.nqh / a.nkh;
+    const uint32_t j = blockIdx.x * 256u + threadIdx.x, kvh = blockIdx.y, slots = a.past + a.n, group = a.group;
     if (j >= slots) return;
     const float *y = pt.scores + (uint64_t)kvh * a.n * group * score_stride(slots) + j;
     const float2 *stats = pt.stats + (uint64_t)kvh * a.n * group;
@@ -1008,7 +1017,7 @@ static bool rows_wide_q(const RowsArgs &a) {
 static RowsPlan rows_plan(const RowsArgs &a) {
     RowsPlan p{};
     p.hd = a.hd <= 32u ? 32u : a.hd <= 64u ? 64u : a.hd <= 96u ? 96u : a.hd <= 128u ? 128u : 256u;
-    const uint32_t rows = a.n * (a.nqh / a.nkh), slots = a.past + a.n;
+    const uint32_t rows = a.n * a.group, slots = a.past + a.n;
     // (up to 64 rows the two kernels are within 15% of each other either way, the few-row one ahead over short
     // contexts: 32 rows over 500 slots 10.9 and 12.5 us, over 2048 13.8 and 12.2)
     p.few = rows <= 16u && rows_wide_kv(a);
@@ -1060,17 +1069,17 @@ size_t attn_rows_scratch_bytes(const RowsArgs &a) {
 template <uint32_t HD>
 static void start_rows(const RowsArgs &a, const RowsPlan &p, const RowsPart &pt, hipStream_t s) {
     const bool wide_kv = rows_wide_kv(a), wide_q = rows_wide_q(a);
-    const uint32_t grid = p.tiles * p.sp.n * a.nkh;
+    const dim3 grid(a.nkh, p.sp.n, p.tiles);
     if (p.few) {
         k_attn_few<HD><<<grid, 256, 0, s>>>(a, p.sp, pt, wide_q);
         return;
     }
-    k_attn_rows<HD><<<grid, 256, 0, s>>>(a, p.sp, pt, p.tiles, wide_kv, wide_q);
+    k_attn_rows<HD><<<grid, 256, 0, s>>>(a, p.sp, pt, wide_kv, wide_q);
 }
 
 template <uint32_t HD>
 static void start_mass(const RowsArgs &a, const RowsPlan &p, const RowsPart &pt, float *part, hipStream_t s) {
-    const uint32_t tiles = (a.n * (a.nqh / a.nkh) + 15u) / 16u, np = 16u * kMassTiles<HD>;
+    const uint32_t tiles = (a.n * a.group + 15u) / 16u, np = 16u * kMassTiles<HD>;
     k_mass<HD><<<(a.past + a.n + np - 1u) / np * a.nkh * p.parts, 64u * (tiles < kMassWaves ? tiles : kMassWaves), 0, s>>>(
         a, pt, part, p.parts, rows_wide_kv(a));
 }
@@ -1095,15 +1104,15 @@ hipError_t launch_attn_rows(const RowsArgs &a, void *scratch, hipStream_t s) {
         default: start_rows<256>(a, p, pt, s); break;
     }
     hipError_t e = hipGetLastError();
-    const uint32_t rows = a.n * (a.nqh / a.nkh);
+    const uint32_t rows = a.n * a.group;
     if (e == hipSuccess && p.sp.n > 1u) {
-        const uint32_t tile_rows = p.few ? 16u : 64u;
-        const uint32_t width = a.hd <= 32u ? 8u : a.hd <= 64u ? 16u : a.hd <= 128u ? 32u : 64u;  // float4s of a row
+        const uint32_t tile_bits = p.few ? 4u : 6u;
+        const uint32_t width_bits = a.hd <= 32u ? 3u : a.hd <= 64u ? 4u : a.hd <= 128u ? 5u : 6u;  // float4s of a row
         // a wave per row where its lanes hold every range in one round of loads
-        if (p.sp.n <= 8u * (64u / width))
-            k_attn_rows_merge<64><<<dim3((rows + 3u) / 4u, a.nkh), 256, 0, s>>>(a, p.sp, pt, tile_rows, width);
+        if (p.sp.n <= 8u * (64u >> width_bits))
+            k_attn_rows_merge<64><<<dim3((rows + 3u) / 4u, a.nkh), 256, 0, s>>>(a, p.sp, pt, tile_bits, width_bits);
         else
-            k_attn_rows_merge<256><<<dim3(rows, a.nkh), 256, 0, s>>>(a, p.sp, pt, tile_rows, width);
+            k_attn_rows_merge<256><<<dim3(rows, a.nkh), 256, 0, s>>>(a, p.sp, pt, tile_bits, width_bits);
         e = hipGetLastError();
     }
     if (e == hipSuccess && a.mass && p.few) {

@@ -39,6 +39,8 @@ struct RowsArgs {
     float *out;
     uint32_t out_stride;
     uint32_t n, past, nqh, nkh, hd;
+    uint32_t group;  // nqh / nkh
+    float rgroup;    // 1 / group
     float scale;
     const uint64_t *mask;
     uint32_t words;
