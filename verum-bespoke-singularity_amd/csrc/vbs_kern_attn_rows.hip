@@ -40,7 +40,7 @@
 // spill), three waves a SIMD 667, a ring of four tiles 581, V transposed by permutes
 // instead of by the LDS read 857.
 // Short ones: launches and one round trip to memory each; 16 tokens over 2048 slots
-// 11 + 4.5 us under the tracer.
+// 10.7 + 4.3 us under the tracer.
 #include "vbs_lds_dma.h"
 #include "vbs_attn_rows.h"
 
@@ -628,7 +628,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(RowsArgs a, RowsSplit sp, 
 // A wave takes the 32-slot tiles wave, wave + 4, ... of the range, in an LDS buffer of its own (no barrier
 // until the end), then the waves' sums are added in LDS. At most 16 rows a kv head: single tokens and the
 // smallest drafts, that read the cache once and compute little. One token over 8192 slots, 64/8 heads of 128,
-// capped: 10.8 us under the tracer and the merge's 4.1 (33.6 MB: 6.9 us at the rate of a copy); on the kernel
+// capped: 11.7 us under the tracer and the merge's 3.9 (33.6 MB: 6.9 us at the rate of a copy); on the kernel
 // above, whose other three waves then have no rows, 13.7.
 template <uint32_t HD>
 __global__ __launch_bounds__(256, 2) void k_attn_few(RowsArgs a, RowsSplit sp, RowsPart pt, bool wide_q) {

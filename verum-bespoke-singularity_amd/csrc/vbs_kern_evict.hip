@@ -275,8 +275,8 @@ hipError_t launch_evict(const EvictArgs &a, hipStream_t s) {
     while (lanes > least && pairs * ((units + lanes - 1u) / lanes) < 256u) lanes = (lanes + 1u) / 2u;
     const uint32_t slices = (units + lanes - 1u) / lanes;
     const uint32_t grid = (pairs + kXcds - 1u) / kXcds * kXcds * slices;
-    // Four slots a thread where they hold every slot: the code is read anew by every launch and is shorter (2049 slots:
-    // the selection 9.2 us under the tracer with eight, 6.7 with four). One launch for up to two workgroups per CU
+    // Four slots a thread where they hold every slot: every pass is half as long (2049 slots: the selection 9.2 us under
+    // the tracer with eight, 6.7 with four). One launch for up to two workgroups per CU
     // (2049 to 1024 of 8 heads 8.7 us, two launches 10.0; 32 layers of 8192 to 4096 229 and 236); with more, selecting
     // for K and for V costs more than a launch.
     const bool small = a.len <= kSelThreads * 4u;
