@@ -774,3 +774,31 @@ def test_mass_of_more_rows_than_a_wave_looks_through_at_once(dev, mem, docs):
     add = group * w.sum(0)
     off = group * wtol.sum(0) + add * (n * group + 2) * R.F32
     close(dev.download(s.pm, mass0.shape, np.float32)[1, :, :n].astype(np.float64), add, off)
+
+
+@pytest.mark.parametrize("layers,length,budget,nkh,hd", [(33, 2100, 1050, 8, 16), (33, 600, 300, 8, 16), (33, 4100, 2060, 8, 16)])
+@pytest.mark.parametrize("place", ["same", "other", "none"])
+def test_evict_of_many_heads(dev, mem, layers, length, budget, nkh, hd, place):
+    """264 heads: more workgroups than two a CU, the mass in place, in another array, or left as it is."""
+    rng = np.random.default_rng(length)
+    first, last, max_ctx = 4, 30, length + 2
+    mass = rng.integers(0, 1 << 16, (layers, nkh, max_ctx)).astype(np.float32)  # (some equal)
+    kc, vc = (rng.integers(0, 1 << 16, (layers, max_ctx, nkh, hd)).astype(np.uint16) for _ in range(2))
+    pk, pv, pm = mem.up(kc), mem.up(vc), mem.up(mass)
+    po = {"same": pm, "other": mem.up(np.full_like(mass, 3.0)), "none": 0}[place]
+    pt = mem.up(np.zeros((layers, nkh, budget), np.uint32))
+    dev.cache_evict(pk, pv, pm, po, pt, length, budget, first, last, 0, layers, max_ctx, nkh, hd)
+    kept = dev.download(pt, (layers, nkh, budget), np.uint32).astype(np.int64)
+    gk, gv = dev.download(pk, kc.shape, np.uint16), dev.download(pv, vc.shape, np.uint16)
+    gm = dev.download(po or pm, mass.shape, np.float32)
+    for l in range(layers):
+        for h in range(nkh):
+            want = R.evict(mass[l, h], length, budget, first, last)
+            assert np.array_equal(kept[l, h], want)
+            assert np.array_equal(gk[l, :budget, h], kc[l, want, h]) and np.array_equal(gv[l, :budget, h], vc[l, want, h])
+            if po:
+                assert np.array_equal(gm[l, h, :budget], mass[l, h, want]) and not gm[l, h, budget:length].any()
+    assert np.array_equal(gk[:, budget:], kc[:, budget:]) and np.array_equal(gv[:, budget:], vc[:, budget:])
+    assert np.array_equal(gm[..., length:], mass[..., length:] if place != "other" else np.full_like(gm[..., length:], 3.0))
+    if not po:
+        assert np.array_equal(gm, mass)

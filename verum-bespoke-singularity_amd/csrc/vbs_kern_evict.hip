@@ -6,8 +6,8 @@
 // as the lowest weight there is). k_evict_select writes the kept
 // slots in order (one workgroup per layer and head: the weight of the last slot
 // taken by a radix selection over the 32-bit order of floats, then one ordered
-// pass), k_evict_move moves their K and V rows to the front; k_evict does both for
-// few heads of few slots.
+// pass), k_evict_move moves their K and V rows to the front; k_evict does both, for
+// few heads or long moves.
 //
 // The move is in place. A kept slot never moves up (its new place is the number
 // of kept slots before it), so rows taken in ascending order are safe as long as
@@ -276,11 +276,12 @@ hipError_t launch_evict(const EvictArgs &a, hipStream_t s) {
     const uint32_t slices = (units + lanes - 1u) / lanes;
     const uint32_t grid = (pairs + kXcds - 1u) / kXcds * kXcds * slices;
     // Four slots a thread where they hold every slot: every pass is half as long (2049 slots: the selection 9.2 us under
-    // the tracer with eight, 6.7 with four). One launch for up to two workgroups per CU
-    // (2049 to 1024 of 8 heads 8.7 us, two launches 10.0; 32 layers of 8192 to 4096 229 and 236); with more, selecting
-    // for K and for V costs more than a launch.
-    const bool small = a.len <= kSelThreads * 4u;
-    if (a.len <= kSelRun && a.mass_out != a.mass && grid <= 512u) {
+    // the tracer with eight, 6.7 with four). One launch for up to two workgroups per CU (2049 to 1024 of 8 heads 8.7 us,
+    // two launches 10.0; 32 layers of 8192 to 4096 229 and 236), or where the move is long beside the selection, which
+    // one launch does for K and for V (64 layers of 8 heads, 4096 to 2048: 232 and 241; but 8192 to 256 57 and 50, 1024
+    // to 512 53 and 50, 128 layers of 512 to 256 59 and 39).
+    const bool small = a.len <= kSelThreads * 4u, one = grid <= 512u || (a.budget >= 1024u && a.len / 2u <= a.budget);
+    if (a.len <= kSelRun && a.mass_out != a.mass && one) {
         if (small && wide)
             k_evict<eu4, 4><<<grid, kSelThreads, 0, s>>>(a, lanes, slices);
         else if (wide)
