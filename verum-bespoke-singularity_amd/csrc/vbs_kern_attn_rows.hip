@@ -1023,7 +1023,8 @@ static RowsPlan rows_plan(const RowsArgs &a) {
     p.few = rows <= 16u && rows_wide_kv(a);
     const uint32_t tile_rows = p.few ? 16u : 64u;
     p.tiles = (rows + tile_rows - 1u) / tile_rows;
-    // Ranges: until about 512 workgroups share the work. A range is at least a tile a wave (few) or two tiles of a
+    // Ranges: until about 512 workgroups, two a CU, share the work (64 tokens over 8255 slots, 64/8 heads of 128: 47 us;
+    // until 256 59, until 768 54). A range is at least a tile a wave (few) or two tiles of a
     // workgroup (16 tokens over 2048 slots, 32/8 heads of 128: 11.5 us, one tile 14.5), and, where half the CUs have a
     // workgroup already, so many slots that sharing their products is worth the merge: 1024 at heads of 64 (777 tokens
     // in documents, 16 heads: 22 us whole, 22 and the merge's 10 in two ranges), 512 at 128 (2010 tokens, 4 heads, in
