@@ -1,0 +1,87 @@
+"""Attention of several tokens (vbs_gfx950_attention_chunk, _attention_tree) where scores, caps or weights are far from
+the usual: finite caches, so that the matrix-core path itself is seen. Against the formulas in 64 bits (steps_ref.py),
+with bounds of their own that do not grow with the size of a score."""
+import numpy as np
+import pytest
+
+import steps_ref as R
+from test_gpu_kernels import mem  # noqa: F401 (fixture)
+from test_gpu_steps import Step, close, random_tree
+
+pytestmark = pytest.mark.gpu
+
+
+def exact_scores(s, slots):
+    """(n, heads, slots) of scale q.k in 64 bits, and sum |q k| scale."""
+    q = s.q[:, :s.nqh * s.hd].reshape(s.n, s.nqh, s.hd).astype(np.float64)
+    k = np.repeat(R.half(s.kc[s.layer, :slots]), s.nqh // s.nkh, 1)
+    return np.einsum("nhd,jhd->nhj", q, k) * s.scale, np.einsum("nhd,jhd->nhj", np.abs(q), np.abs(k)) * abs(s.scale)
+
+
+# ---- scores whose differences, but not whose sizes, an f32 exponent holds ------------------------------------------
+
+FAR_SHAPES = [(1, 300, 4, 2, 128), (2, 1500, 4, 1, 64), (3, 90, 6, 2, 80), (16, 700, 2, 2, 128), (70, 40, 2, 2, 64),
+              (40, 500, 4, 1, 128), (33, 200, 4, 2, 256), (20, 900, 3, 1, 40), (130, 5, 2, 1, 6)]
+
+
+@pytest.mark.parametrize("shape", FAR_SHAPES, ids=["-".join(map(str, s)) for s in FAR_SHAPES])
+@pytest.mark.parametrize("size", [1e3, 3e5])
+@pytest.mark.parametrize("sign", ["both", "below"])
+def test_one_slot_takes_the_whole_weight(dev, mem, shape, size, sign):
+    """Scores of `size`: where the greatest lies further above the second than f32 can be off, its V is the output, and 1
+    is its weight. A score is off by at most SPLIT + (2 hd + 8) F32 of sum |q k| scale (steps_ref.attend); 40 beyond
+    twice that the second's weight is below e^-40. The output is then V (f16) times a weight in two f16 parts over the same
+    weight in f32: 2^-22, and a division and a product. Every third row keeps scores of the usual size."""
+    n, past, nqh, nkh, hd = shape
+    rng = np.random.default_rng([n, int(np.log10(size)), sign == "below"])
+    s = Step(rng, mem, dev, *shape)
+    slots = past + n
+    if sign == "below":  # every score is negative
+        s.q, k = np.abs(s.q) + 0.1, s.kc.view(np.float16)
+        s.kc = (-np.abs(k) - np.float16(0.1)).astype(np.float16).view(np.uint16)
+        s.kc[:, slots:] = 0x7E00
+    usual = np.arange(n) % 3 == 2
+    s.q[~usual] *= np.float32(size)
+    score, total = exact_scores(s, slots)
+    see = R.sees_chunk(n, past)
+    score = np.where(see[:, None], score, -np.inf)
+    order = np.sort(score, -1)
+    off = (R.SPLIT + (2 * hd + 8) * R.F32) * np.where(see[:, None], total, 0).max(-1)
+    clear = (order[..., -1] - order[..., -2] > 2 * off + 40) & ~usual[:, None]
+    if n > 2:
+        assert clear[~usual].mean() > 0.5  # (most rows say something)
+    best = score.argmax(-1)
+    group = nqh // nkh
+    v = R.half(s.vc[s.layer, :slots])
+    mass0 = np.zeros((2, nkh, s.max_ctx), np.float32)
+    # a slot's weight of the rows that are not clear is anything from 0 to 1
+    want_out, w, tol, wtol = s.want(see)
+    want = np.stack([[v[best[i, h], h // group] for h in range(nqh)] for i in range(n)])
+    low, high = np.zeros((nkh, slots)), np.zeros((nkh, slots))
+    for i in range(n):
+        for h in range(nqh):
+            if usual[i]:
+                low[h // group] += w[i, h] - wtol[i, h]
+                high[h // group] += w[i, h] + wtol[i, h]
+            elif clear[i, h]:
+                low[h // group, best[i, h]] += 1 - 2.0 ** -20
+                high[h // group, best[i, h]] += 1 + 2.0 ** -20
+            else:
+                high[h // group] += np.where(see[i], 1 + 2.0 ** -20, 0)
+    for with_mass in (False, True):
+        got = s.chunk(**({"mass": mass0} if with_mass else {}))
+        assert np.isfinite(got).all()
+        close(got[clear], want[clear], np.abs(want[clear]) * 2.0 ** -20)
+        close(got[usual], want_out[usual], tol[usual])
+        if with_mass:
+            m = s.dev.download(s.pm, mass0.shape, np.float32)[1, :, :slots].astype(np.float64)
+            slack = (n * group + 2) * R.F32 * high + 2.0 ** -60
+            assert ((m >= low - slack) & (m <= high + slack)).all(), np.argwhere((m < low - slack) | (m > high + slack))[:4]
+            # each row hands out a weight of 1 in all
+            assert np.abs(m.sum(-1) - n * group).max() <= n * group * (2.0 ** -20 + slots * R.F32)
+    mask = random_tree(rng, n)
+    see = R.sees_tree(n, past, mask)
+    seen = np.where(see[:, None], score, -np.inf)
+    same = clear & (seen.argmax(-1) == best) & np.isfinite(seen.max(-1))
+    if past:
+        close(s.tree(mask)[same], want[same], np.abs(want[same]) * 2.0 ** -20)

@@ -68,6 +68,14 @@ __device__ __forceinline__ float row_score(const RowsArgs &a, float s, float slo
     return a.slopes ? row_far(s, slope, at, j) : s;
 }
 
+// The score from a product x of the matrix cores (x c1: scale q.k), in units of score_unit: by the operations of RowTile's
+// step one for one, so that the weights that k_mass adds are the numbers that l counted, at any size of a score.
+__device__ __forceinline__ float score_unit(const RowsArgs &a) { return a.cap > 0.f && !a.slopes ? a.cap : 1.f; }
+__device__ __forceinline__ float parts_score(const RowsArgs &a, float x, float c1, float slope, uint32_t at, uint32_t j) {
+    const float s = a.cap > 0.f ? tanh_any(x * (c1 * a.rcap)) : x * c1;
+    return a.slopes ? row_far(a.cap > 0.f ? s * a.cap : s, slope, at, j) : s;
+}
+
 __device__ __forceinline__ float row_dot(const float *q, const uint16_t *k, uint32_t hd) {
     float dot = 0.f;
     for (uint32_t d = 0; d < hd; d++) dot = fmaf(q[d], h2f(k[d]), dot);

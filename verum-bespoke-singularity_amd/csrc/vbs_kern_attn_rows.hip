@@ -407,13 +407,22 @@ struct RowTile {
                 }
             }
         }
-        if (scores && real)
-#pragma unroll
-            for (uint32_t i = 0; i < NS; i++) *reinterpret_cast<rf4 *>(scores + 16u * i + 4u * g) = S[i] * cm;
         float top = -INFINITY;
 #pragma unroll
         for (uint32_t i = 0; i < NS; i++) top = fmaxf(top, fmaxf(fmaxf(S[i][0], S[i][1]), fmaxf(S[i][2], S[i][3])));
         top *= cm;
+        if (scores) {
+            // (k_mass_few forms the weights from the rounded scores: from 2^10 on, where the rounding would show beside
+            // l, they are rounded here too)
+            if (__any(fabsf(top) > 1024.f && top > -INFINITY)) {
+#pragma unroll
+                for (uint32_t i = 0; i < NS; i++) S[i] *= cm;
+                cm = 1.f;
+            }
+            if (real)
+#pragma unroll
+                for (uint32_t i = 0; i < NS; i++) *reinterpret_cast<rf4 *>(scores + 16u * i + 4u * g) = S[i] * cm;
+        }
         if (__any(top > m + kLazy)) {
             top = fmaxf(top, lane_xor<16>(top));
             top = fmaxf(top, lane_xor<32>(top));
@@ -904,20 +913,22 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, RowsPart p
 #pragma unroll
                     for (uint32_t j = 0; j < NT; j++)
                         S[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[j][kk], v ? ql[kk] : qh[kk], S[j], 0, 0, 0);
+            float cm = c1 * kLog2e;
+            if (terms) {
+#pragma unroll
+                for (uint32_t j = 0; j < NT; j++)
+#pragma unroll
+                    for (uint32_t k = 0; k < 4u; k++)
+                        S[j][k] = parts_score(a, S[j][k], c1, slope, a.past + i, p0 + 16u * j + 4u * g + k);
+                cm = score_unit(a) * kLog2e;
+            }
 #pragma unroll
             for (uint32_t j = 0; j < NT; j++)
 #pragma unroll
                 for (uint32_t k = 0; k < 4u; k++) {
                     const uint32_t o = 16u * j + 4u * g + k;
-                    float y;
-                    if (full && !terms) {
-                        y = fmaf(S[j][k], c1 * kLog2e, -ms);
-                    } else {
-                        float s = S[j][k] * c1;
-                        if (terms) s = row_score(a, s, slope, a.past + i, p0 + o);
-                        const bool sees = (vis >> o & 1ull) & (ds[j][k] == doc);  // (0 == 0 without documents)
-                        y = sees ? fmaf(s, kLog2e, -ms) : -INFINITY;
-                    }
+                    float y = fmaf(S[j][k], cm, -ms);
+                    if (!full) y = (vis >> o & 1ull) & (ds[j][k] == doc) ? y : -INFINITY;  // (0 == 0 without documents)
                     sum[j][k] = fmaf(__builtin_amdgcn_exp2f(y), st.y, sum[j][k]);
                 }
         }
