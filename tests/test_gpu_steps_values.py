@@ -25,7 +25,7 @@ FAR_SHAPES = [(1, 300, 4, 2, 128), (2, 1500, 4, 1, 64), (3, 90, 6, 2, 80), (16, 
 
 
 @pytest.mark.parametrize("shape", FAR_SHAPES, ids=["-".join(map(str, s)) for s in FAR_SHAPES])
-@pytest.mark.parametrize("size", [1e3, 3e5])
+@pytest.mark.parametrize("size", [1e3, 3e5, 1.1e7, 3e8, 1e9, 1e12, 1e30])
 @pytest.mark.parametrize("sign", ["both", "below"])
 def test_one_slot_takes_the_whole_weight(dev, mem, shape, size, sign):
     """Scores of `size`: where the greatest lies further above the second than f32 can be off, its V is the output, and 1
@@ -85,3 +85,39 @@ def test_one_slot_takes_the_whole_weight(dev, mem, shape, size, sign):
     same = clear & (seen.argmax(-1) == best) & np.isfinite(seen.max(-1))
     if past:
         close(s.tree(mask)[same], want[same], np.abs(want[same]) * 2.0 ** -20)
+
+
+@pytest.mark.parametrize("shape", [(1, 2100, 4, 2, 64), (5, 300, 6, 3, 128), (150, 400, 4, 2, 80), (90, 30, 2, 1, 256)])
+@pytest.mark.parametrize("size", [1e5, 1e9])
+def test_far_scores_in_documents_with_a_bias(dev, mem, shape, size):
+    """As above with the slots of other documents unseen, a prefix, and a bias by distance, which adds 2 F32 of its size
+    and of the score's to the bound."""
+    n, past, nqh, nkh, hd = shape
+    rng = np.random.default_rng([n, int(size)])
+    s = Step(rng, mem, dev, *shape, size=2 * size)
+    slots, group = past + n, nqh // nkh
+    docs = rng.integers(0, 3, slots).astype(np.int32)
+    slopes = np.linspace(0.5, 20.0, nqh).astype(np.float32)
+    see = R.sees_chunk(n, past, past // 2, docs)
+    score, total = exact_scores(s, slots)
+    far = slopes[None, :, None] * np.abs(past + np.arange(n)[:, None] - np.arange(slots)[None])[:, None]
+    off = np.where(see[:, None], (R.SPLIT + (2 * hd + 10) * R.F32) * total + 4 * R.F32 * far, 0).max(-1)
+    score = np.where(see[:, None], score - far, -np.inf)
+    order = np.sort(score, -1)
+    clear = order[..., -1] - order[..., -2] > 2 * off + 40
+    assert clear.mean() > 0.5
+    best, v = score.argmax(-1), R.half(s.vc[s.layer, :slots])
+    mass0 = np.zeros((2, nkh, s.max_ctx), np.float32)
+    got = s.chunk(docs=docs, slopes=slopes, prefix=past // 2, mass=mass0)
+    want = np.stack([[v[best[i, h], h // group] for h in range(nqh)] for i in range(n)])
+    close(got[clear], want[clear], np.abs(want[clear]) * 2.0 ** -20)
+    m = s.dev.download(s.pm, mass0.shape, np.float32)[1, :, :slots].astype(np.float64)
+    low, high = np.zeros((nkh, slots)), np.zeros((nkh, slots))
+    for i, h in np.ndindex(n, nqh):
+        if clear[i, h]:
+            low[h // group, best[i, h]] += 1 - 2.0 ** -20
+            high[h // group, best[i, h]] += 1 + 2.0 ** -20
+        else:
+            high[h // group] += np.where(see[i], 1 + 2.0 ** -20, 0)
+    slack = (n * group + 2) * R.F32 * high + 2.0 ** -60
+    assert ((m >= low - slack) & (m <= high + slack)).all()

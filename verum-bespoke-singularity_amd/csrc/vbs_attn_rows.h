@@ -82,13 +82,24 @@ __device__ __forceinline__ float row_dot(const float *q, const uint16_t *k, uint
     return dot;
 }
 
+// A maximum (in units of log2) from which a row is taken in f32 products and rounded scores (row_whole). The matrix-core
+// path subtracts the rounded maximum from products that are not rounded: what that leaves, up to half a step of m, is
+// the same for every weight of the row and cancels as long as the weights hold it. From 2^24 on it reaches one and
+// more in log2 and the weights leave f16's range: such rows came out as 0 or not finite.
+constexpr float kFarScore = 0x1p24f;
+__device__ __forceinline__ bool far_row(float m) { return fabsf(m) > kFarScore && m > -INFINITY; }
+// Beyond this maximum a row that row_whole took is marked (its sum l goes on with its sign turned): its weights have to
+// come from the same f32 scores again, which differ from the matrix cores' by about 2^-22 of their size.
+constexpr float kMarkScore = 0x1p12f;
+
 // Row i, q head h over the slots [s0, s1), by one whole wave in f32 products: the
 // scores of 64 slots at a time, a slot per lane, a running maximum and sum, then
 // the lanes take the dims (lane + 64 c in acc[c]). For rows whose sums came out not
 // finite: an infinity in q or K meets the two f16 parts of the matrix-core path
 // as inf - inf or 0 * inf, and one in V the weight 0 of the rows that do not see
-// it. Here an unseen slot is never touched. m is in units of log2, as the scores of the
-// slots it sees, that go to scores[j] (if not NULL).
+// it. Here an unseen slot is never touched. And for rows of far scores: y is rounded
+// before the maximum is taken off, so that the greatest weighs exactly 1. m is in units of
+// log2, as the scores of the slots it sees, that go to scores[j] (if not NULL).
 template <uint32_t HD>
 __device__ __forceinline__ void row_whole(const RowsArgs &a, uint32_t i, uint32_t h, uint32_t s0, uint32_t s1,
                                           uint32_t lane, float &m_out, float &l_out, float (&acc)[(HD + 63) / 64],

@@ -489,9 +489,11 @@ struct RowsTo {
         stats = sp.n == 1u && pt.stats ? pt.stats + (uint64_t)kvh * rows + r : nullptr;
     }
     __device__ __forceinline__ float scale(float l) const { return ml ? 1.f : l == 0.f ? 0.f : __fdiv_rn(1.f, l); }
-    __device__ __forceinline__ void put_ml(float m, float l) const {
-        if (ml) *ml = make_float2(m, l);
-        if (stats) *stats = make_float2(m, l == 0.f ? 0.f : __fdiv_rn(1.f, l));
+    // `mark`: l or 1 / l with its sign turned
+    __device__ __forceinline__ void put_ml(float m, float l, bool mark = false) const {
+        const float sign = mark ? -1.f : 1.f;
+        if (ml) *ml = make_float2(m, sign * l);
+        if (stats) *stats = make_float2(m, l == 0.f ? 0.f : __fdiv_rn(sign, l));
     }
 };
 // The row again in f32 products, by a whole wave (row_whole), to the same place.
@@ -506,7 +508,7 @@ __device__ __forceinline__ void row_again(const RowsArgs &a, const RowsSplit &sp
 #pragma unroll
     for (uint32_t k = 0; k < (HD + 63u) / 64u; k++)
         if (64u * k + lane < a.hd) to.acc[64u * k + lane] = to.ml ? o[k] : l == 0.f ? 0.f : o[k] / l;
-    if (lane == 0) to.put_ml(m, l);
+    if (lane == 0) to.put_ml(m, l, m > -INFINITY && fabsf(m) > kMarkScore);
 }
 
 // ---- many rows: four waves with rows of their own, slots through two shared buffers ------
@@ -610,7 +612,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(RowsArgs a, RowsSplit sp, 
     for (uint32_t d = 0; d < DT; d++)
 #pragma unroll
         for (uint32_t k = 0; k < 4u; k++) nan = fmaf(R.acc[d][k], 0.f, nan);
-    const uint64_t bad = __ballot(R.real && nan != 0.f);  // (0 times anything finite is 0)
+    const uint64_t bad = __ballot(R.real && (nan != 0.f || far_row(R.m)));  // (0 times anything finite is 0)
     const uint32_t cols = (uint32_t)(bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xFFFFu;
     if (R.real && !(cols >> col & 1u)) {
         const RowsTo to(a, sp, pt, kvh, split, row0 + col);
@@ -628,7 +630,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(RowsArgs a, RowsSplit sp, 
         }
         if (g == 0) to.put_ml(R.m - kLift, R.l);
     }
-    // rows whose sums are not finite, one at a time
+    // rows whose sums are not finite or whose scores are far, one at a time
     for (uint32_t c = 0; cols >> c; c++)
         if (cols >> c & 1u) row_again<HD>(a, sp, pt, kvh, split, row0 + c, s0, s1, lane);
 }
@@ -733,7 +735,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_few(RowsArgs a, RowsSplit sp, R
         const RowsTo to(a, sp, pt, kvh, split, row0 + r);
         const float inv = to.scale(l);
         const float nan = fmaf(o[0], 0.f, fmaf(o[1], 0.f, fmaf(o[2], 0.f, fmaf(o[3], 0.f, l * 0.f))));
-        if (nan != 0.f) bad[r] = 1u;
+        if (nan != 0.f || far_row(M)) bad[r] = 1u;
         o *= inv;
         if (to.ml || wide_to) {
             *reinterpret_cast<rf4 *>(to.acc + d0) = o;
@@ -781,7 +783,8 @@ __global__ __launch_bounds__(256) void k_attn_rows_merge(RowsArgs a, RowsSplit s
     const float m0 = has(lane) ? y0.x : -INFINITY, m1 = has(lane + 64u) ? y1.x : -INFINITY;
     const float M = wave_max(fmaxf(m0, m1)), ref = M == -INFINITY ? 0.f : M;
     const float w0 = exp2f(m0 - ref), w1 = exp2f(m1 - ref);
-    const float L = wave_sum(fmaf(has(lane) ? y0.y : 0.f, w0, (has(lane + 64u) ? y1.y : 0.f) * w1));
+    const float L = wave_sum(fmaf(has(lane) ? fabsf(y0.y) : 0.f, w0, (has(lane + 64u) ? fabsf(y1.y) : 0.f) * w1));
+    const bool mark = __any((y0.y < 0.f && m0 == M) || (y1.y < 0.f && m1 == M));  // (the range of the maximum decides)
     rf4 o = {0.f, 0.f, 0.f, 0.f};
     for (uint32_t c0 = grp;;) {  // (the same rounds in every lane)
 #pragma unroll
@@ -810,14 +813,15 @@ __global__ __launch_bounds__(256) void k_attn_rows_merge(RowsArgs a, RowsSplit s
 #pragma unroll
     for (uint32_t k = 0; k < 4u; k++)
         if (4u * q + k < a.hd) to[k] = L == 0.f ? 0.f : o[k] * inv;
-    if (q == 0 && pt.stats) pt.stats[(uint64_t)kvh * rows + r] = make_float2(M, inv);
+    if (q == 0 && pt.stats) pt.stats[(uint64_t)kvh * rows + r] = make_float2(M, mark ? -inv : inv);
 }
 
 // ---- the weights that slots received ---------------------------------------------------
 // A workgroup takes 64 (32 for head_dim above 128) slots of a kv head, their K rows as A operands in registers;
 // its waves take the row tiles of 16 in turn (S^T as above) and each lane adds up
 // 2^(y - m) / l for its slots; the 16 columns, then the waves, are summed at the end
-// in a fixed order. A slot whose sum is not finite is taken again in f32 products.
+// in a fixed order. A slot whose sum is not finite is taken again in f32 products, and
+// marked rows (kMarkScore) and rows whose sum is no number are added in f32 products alone.
 // q's parts come from k_attn_rows, as the matrix cores take them: splitting q again for every 64 slots costs more
 // than the products (1024 tokens over 5120 slots, 32/8 heads of 128: 269 us under the tracer, 166 from the parts).
 // Where slots are few, the rows are split over `parts` workgroups and k_mass_add sums
@@ -834,6 +838,7 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, RowsPart p
                                                           bool wide_kv) {
     constexpr uint32_t KK = HD / 32u, NT = kMassTiles<HD>, NP = 16u * NT;  // tiles of 16 slots; slots
     __shared__ float sums[kMassWaves][NP];
+    __shared__ uint32_t apart[kMassWaves];  // whether the wave left rows out
     const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63u, col = lane & 15u, g = lane >> 4;
     const uint32_t waves = blockDim.x >> 6, kvh = blockIdx.x % a.nkh, rest = blockIdx.x / a.nkh;
     const uint32_t mine = rest % parts, p0 = rest / parts * NP;
@@ -853,6 +858,7 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, RowsPart p
             ds[i][r] = a.docs ? a.docs[min(p0 + 16u * i + 4u * g + r, slots - 1u)] : 0;
     }
     float sum[NT][4] = {};
+    bool left_out = false;
     const bool terms = a.cap > 0.f || a.slopes;
     int32_t lo = 0, hi = 0;  // the slots' documents
     if (a.docs) {
@@ -902,7 +908,11 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, RowsPart p
                               p0 + NP <= (a.mask ? a.past : row_end(a, row_token(a, 16u * rt)));
             const uint64_t vis = full ? ~0ull : real ? seen_bits(a, i, p0, slots) : 0ull;
             const int32_t doc = a.docs ? a.docs[a.past + i] : 0;
-            const float slope = a.slopes ? a.slopes[h] : 0.f, ms = st.x == -INFINITY ? 0.f : st.x;
+            // (a row that is left out: weights 2^-inf times 0)
+            const bool out = !(st.y >= 0.f);
+            left_out = left_out || out;
+            const float slope = a.slopes ? a.slopes[h] : 0.f, ms = out ? INFINITY : st.x == -INFINITY ? 0.f : st.x;
+            const float inv = out ? 0.f : st.y;
             rf4 S[NT];
 #pragma unroll
             for (uint32_t j = 0; j < NT; j++) S[j] = rf4{0.f, 0.f, 0.f, 0.f};
@@ -929,7 +939,7 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, RowsPart p
                     const uint32_t o = 16u * j + 4u * g + k;
                     float y = fmaf(S[j][k], cm, -ms);
                     if (!full) y = (vis >> o & 1ull) & (ds[j][k] == doc) ? y : -INFINITY;  // (0 == 0 without documents)
-                    sum[j][k] = fmaf(__builtin_amdgcn_exp2f(y), st.y, sum[j][k]);
+                    sum[j][k] = fmaf(__builtin_amdgcn_exp2f(y), inv, sum[j][k]);
                 }
         }
     }
@@ -945,28 +955,35 @@ __global__ __launch_bounds__(64 * kMassWaves) void k_mass(RowsArgs a, RowsPart p
             v += bfly_partner<1>(v, lane);
             if (col == 0) sums[wave][16u * j + 4u * g + k] = v;
         }
+    const uint32_t any_left_out = __any(left_out);
+    if (lane == 0) apart[wave] = any_left_out;
     __syncthreads();
     if (wave) return;
     const uint32_t j = p0 + lane;
     const bool in = lane < NP && j < slots;
     float v = 0.f;
-    for (uint32_t w = 0; w < waves; w++) v += sums[w][lane % NP];
+    uint32_t some = 0;
+    for (uint32_t w = 0; w < waves; w++) v += sums[w][lane % NP], some |= apart[w];
     const uint64_t bad = __ballot(in && v * 0.f != 0.f);
-    for (uint32_t c = 0; c < 64u && bad >> c; c++) {
-        if (!(bad >> c & 1ull)) continue;
+    const uint64_t again = some ? __ballot(in) : bad;
+    for (uint32_t c = 0; c < 64u && again >> c; c++) {
+        if (!(again >> c & 1ull)) continue;
+        const bool every = bad >> c & 1ull;  // (else the rows that were left out)
         const uint32_t jj = p0 + c;
         const uint16_t *k = a.kc + (uint64_t)jj * rstride + (uint64_t)kvh * a.hd;
         float whole = 0.f;
         for (uint32_t r = 16u * t0 + lane; r < min(16u * t1, rows); r += 64u) {
+            const float2 st = stats[r];
+            if (!every && st.y >= 0.f) continue;
             const uint32_t i = row_token(a, r), h = kvh * group + r - i * group;
             if (jj >= row_end(a, i) || !row_sees(a, i, jj)) continue;
             const float s = row_score(a, row_dot(a.q + (uint64_t)i * a.q_stride + (uint64_t)h * a.hd, k, a.hd) * a.scale,
                                       a.slopes ? a.slopes[h] : 0.f, a.past + i, jj);
-            const float2 st = stats[r];
-            whole += exp2f(fmaf(s, kLog2e, -(st.x == -INFINITY ? 0.f : st.x))) * st.y;
+            // (the product rounded, as row_whole's)
+            whole += exp2f(__fsub_rn(__fmul_rn(s, kLog2e), st.x == -INFINITY ? 0.f : st.x)) * fabsf(st.y);
         }
         whole = wave_sum(whole);
-        if (lane == c) v = whole;
+        if (lane == c) v = every ? whole : v + whole;
     }
     if (!in) return;
     if (parts > 1u)
@@ -986,7 +1003,7 @@ __global__ __launch_bounds__(256) void k_mass_few(RowsArgs a, RowsPart pt) {
         if (j >= row_end(a, i) || !row_sees(a, i, j)) continue;  // (its scores may not have been written)
         for (uint32_t r = i * group; r < (i + 1u) * group; r++) {
             const float2 st = stats[r];
-            v = fmaf(__builtin_amdgcn_exp2f(y[r * score_stride(slots)] - (st.x == -INFINITY ? 0.f : st.x)), st.y, v);
+            v = fmaf(__builtin_amdgcn_exp2f(y[r * score_stride(slots)] - (st.x == -INFINITY ? 0.f : st.x)), fabsf(st.y), v);
         }
     }
     a.mass[(uint64_t)kvh * a.max_ctx + j] += v;
