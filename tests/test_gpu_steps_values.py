@@ -121,3 +121,53 @@ def test_far_scores_in_documents_with_a_bias(dev, mem, shape, size):
             high[h // group] += np.where(see[i], 1 + 2.0 ** -20, 0)
     slack = (n * group + 2) * R.F32 * high + 2.0 ** -60
     assert ((m >= low - slack) & (m <= high + slack)).all()
+
+
+# ---- caps far above the scores ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("shape", [(1, 300, 4, 2, 128), (3, 700, 2, 2, 80), (40, 200, 4, 1, 64), (90, 100, 4, 2, 128),
+                                   (33, 70, 2, 1, 256)])
+@pytest.mark.parametrize("cap", [2e12, 1e20, 1e30, 3e36, 3e37, 1.7e38, 3e38, 3.4028234e38])
+@pytest.mark.parametrize("bias", [False, True])
+def test_a_cap_far_above_every_score_changes_nothing(dev, mem, shape, cap, bias):
+    """cap tanh(s / cap) is s to (s / cap)^2 / 3 of it, below F32 here. What may differ is a rounding of the score in
+    either call (F32 of its size, which is below 100) and, with it, each weight by 4 F32 times that size at most."""
+    n, past, nqh, nkh, hd = shape
+    rng = np.random.default_rng(n)
+    s = Step(rng, mem, dev, *shape, size=4.0)
+    score, _ = exact_scores(s, past + n)
+    assert np.abs(score).max() < 100
+    terms = {"mass": np.zeros((2, nkh, s.max_ctx), np.float32)}
+    if bias:
+        terms["slopes"] = np.linspace(0.02, 0.01, nqh).astype(np.float32)
+    plain, plain_mass = s.chunk(**terms), s.dev.download(s.pm, terms["mass"].shape, np.float32).astype(np.float64)
+    got = s.chunk(cap=float(np.float32(cap)), **terms)
+    rel = 4 * R.F32 * 100
+    v = np.abs(R.half(s.vc[1, :past + n])).max((0, 2)).repeat(nqh // nkh)[None, :, None]
+    assert (np.abs(got - plain) <= rel * v).all()
+    m = s.dev.download(s.pm, terms["mass"].shape, np.float32).astype(np.float64)
+    assert (np.abs(m - plain_mass) <= rel * plain_mass + 2.0 ** -80).all()
+
+
+@pytest.mark.parametrize("shape", [(2, 300, 4, 2, 128), (70, 60, 2, 1, 64)])
+@pytest.mark.parametrize("size,cap", [(1e12, 1e25), (1e12, 1e34), (1e25, 3.4e38)])
+def test_far_scores_below_a_farther_cap(dev, mem, shape, size, cap):
+    """Both calls take such rows in the same f32 products, and the cap leaves their scores as they are."""
+    s = Step(np.random.default_rng(3), mem, dev, *shape, size=size)
+    plain = s.chunk()
+    assert np.isfinite(plain).all() and np.array_equal(s.chunk(cap=cap), plain)
+
+
+@pytest.mark.parametrize("shape", [(2, 300, 4, 2, 128), (70, 60, 2, 1, 64)])
+@pytest.mark.parametrize("cap", [1e-30, 1e-20, 1e-6])
+@pytest.mark.parametrize("size", [1.0, 1e15, 1e30])
+def test_caps_far_below_the_scores(dev, mem, shape, cap, size):
+    """Every score lies within cap of 0: the weights are even, to e^(2 cap) and the rounding of the sums."""
+    n, past, nqh, nkh, hd = shape
+    s = Step(np.random.default_rng(4), mem, dev, *shape, size=size)
+    got, slots = s.chunk(cap=cap), past + n
+    v = R.half(s.vc[1, :slots])
+    even = R.sees_chunk(n, past) / (past + 1.0 + np.arange(n))[:, None]
+    want = np.einsum("nj,jhd->nhd", even, v).repeat(nqh // nkh, 1)
+    size_v = np.einsum("nj,jhd->nhd", even, np.abs(v)).repeat(nqh // nkh, 1)
+    close(got, want, size_v * (2 * cap + R.SPLIT + (2 * slots + 8) * R.F32))

@@ -63,17 +63,31 @@ __device__ __forceinline__ float tanh_any(float x) {
 __device__ __forceinline__ float row_far(float s, float slope, uint32_t at, uint32_t j) {
     return fmaf(-slope, fabsf((float)(int32_t)(at - j)), s);  // (slots are at most 2^31)
 }
+// The score capped. s / cap is a subnormal of few bits where the cap is far above s (and 1 / cap from 2^126 on): from
+// kFarCap on a score below 2^-13 of the cap is left as it is, of which the cap takes less than (s / cap)^2 / 3 < 2^-27.
+constexpr float kFarCap = 0x1p40f;
+__device__ __forceinline__ float capped(const RowsArgs &a, float s) {
+    const float t = a.cap * tanh_any(s * a.rcap);
+    return a.cap >= kFarCap && fabsf(s) < a.cap * 0x1p-13f ? s : t;
+}
 __device__ __forceinline__ float row_score(const RowsArgs &a, float s, float slope, uint32_t at, uint32_t j) {
-    if (a.cap > 0.f) s = a.cap * tanh_any(s * a.rcap);
+    if (a.cap > 0.f) s = capped(a, s);
     return a.slopes ? row_far(s, slope, at, j) : s;
 }
 
 // The score from a product x of the matrix cores (x c1: scale q.k), in units of score_unit: by the operations of RowTile's
 // step one for one, so that the weights that k_mass adds are the numbers that l counted, at any size of a score.
-__device__ __forceinline__ float score_unit(const RowsArgs &a) { return a.cap > 0.f && !a.slopes ? a.cap : 1.f; }
+__device__ __forceinline__ float score_unit(const RowsArgs &a) { return a.cap > 0.f && a.cap < kFarCap && !a.slopes ? a.cap : 1.f; }
 __device__ __forceinline__ float parts_score(const RowsArgs &a, float x, float c1, float slope, uint32_t at, uint32_t j) {
-    const float s = a.cap > 0.f ? tanh_any(x * (c1 * a.rcap)) : x * c1;
-    return a.slopes ? row_far(a.cap > 0.f ? s * a.cap : s, slope, at, j) : s;
+    if (a.cap >= kFarCap) {
+        x = capped(a, x * c1);
+    } else if (a.cap > 0.f) {
+        x = tanh_any(x * (c1 * a.rcap));
+        if (a.slopes) x *= a.cap;
+    } else {
+        x *= c1;
+    }
+    return a.slopes ? row_far(x, slope, at, j) : x;
 }
 
 __device__ __forceinline__ float row_dot(const float *q, const uint16_t *k, uint32_t hd) {

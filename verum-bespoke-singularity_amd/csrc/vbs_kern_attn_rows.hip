@@ -357,7 +357,12 @@ struct RowTile {
         float cm = c1 * kLog2e;
         if (a.cap > 0.f || a.slopes) {
             float unit = 1.f;
-            if (a.cap > 0.f) {
+            if (a.cap >= kFarCap) {
+#pragma unroll
+                for (uint32_t i = 0; i < NS; i++)
+#pragma unroll
+                    for (uint32_t k = 0; k < 4u; k++) S[i][k] = capped(a, S[i][k] * c1);
+            } else if (a.cap > 0.f) {
                 float far = 0.f;
 #pragma unroll
                 for (uint32_t i = 0; i < NS; i++) {
