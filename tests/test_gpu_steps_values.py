@@ -171,3 +171,26 @@ def test_caps_far_below_the_scores(dev, mem, shape, cap, size):
     want = np.einsum("nj,jhd->nhd", even, v).repeat(nqh // nkh, 1)
     size_v = np.einsum("nj,jhd->nhd", even, np.abs(v)).repeat(nqh // nkh, 1)
     close(got, want, size_v * (2 * cap + R.SPLIT + (2 * slots + 8) * R.F32))
+
+
+# ---- many small weights beside a great one --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("n,past,nqh,nkh", [(132, 65536, 128, 8), (1, 16384, 300, 300)])
+def test_many_small_weights(dev, mem, n, past, nqh, nkh):
+    """One slot of V = 0 and past - 1 of e^-22.875 = 2^-33 of its weight with V = 1, in one range of slots (more row tiles
+    than half the workgroups that share the work). A weight's low part is off by half of f16's least step, 2^-25,
+    where the greatest weighs 2^11: 2^-36 for each slot; the sums lose a rounding a slot at most."""
+    hd = 8
+    s = Step(np.random.default_rng(1), mem, dev, n, past, nqh, nkh, hd, layer=0)
+    s.q[:] = 0
+    s.q.reshape(n, nqh, hd)[..., 0] = 1
+    s.scale = 1.0
+    k, v = np.zeros(s.kc.shape, np.float16), np.ones(s.vc.shape, np.float16)
+    k[0, 0, :, 0], v[0, 0] = 22.875, 0
+    k[0, past:, :, 0] = -60000  # the tokens themselves weigh nothing
+    s.kc, s.vc = k.view(np.uint16), v.view(np.uint16)
+    rest = (past - 1) * np.exp(-22.875)
+    want = rest / (1 + rest)
+    tol = past * 2.0 ** -36 + want * (past + 200) * R.F32
+    assert want > 6 * tol
+    assert np.abs(s.chunk() - want).max() <= tol

@@ -20,9 +20,12 @@
 //   sums). A lane then holds the scores of one row (column lane & 15) at slots
 //   16 i + 4 (lane >> 4) + k, so the softmax needs no row-wise exchange but for the
 //   maximum.
-// * the running maximum moves only where a score passes it by more than 8 in
-//   log2: then the sums are rescaled. The weights are 2^(y - m + 7) <= 2^15, so that
-//   small ones keep their low part in f16.
+// * the running maximum moves only where a score passes it by more than 4 in
+//   log2: then the sums are rescaled. The weights are 2^(y - m + 11) <= 2^15, so that
+//   small ones keep their low part in f16: what lies 2^-36 below the greatest is in l
+//   but no longer in V's sum, 1e-6 of V over 65536 such slots in one range (8 and 2^7:
+//   2^-32 and 1.5e-5; 2 and 2^13: 2^-38). Moving it more often costs little: 2048 tokens over
+//   8192 slots, 32/8 heads of 128, 457 to 460 us, over 4096 of heads of 64 130 to 133.
 // * O^T += V^T P^T: B = P^T, the lane's own weights (hi, then lo), A = V^T with the
 //   k slots in the same order, by transposed LDS reads.
 // Each range of slots ends in m, l and acc per row; where a kv head's rows are few
@@ -46,7 +49,7 @@
 
 namespace vbs {
 
-constexpr float kLazy = 8.f, kLift = 7.f;  // log2: how far a score may pass m; the weights' scale
+constexpr float kLazy = 4.f, kLift = 11.f;  // log2: how far a score may pass m; the weights' scale
 
 // p - h[0] and p - h[1], the halves widened on the way (exact: h is p rounded).
 __device__ __forceinline__ float less_low(float p, rh2 h) {
