@@ -194,3 +194,31 @@ def test_many_small_weights(dev, mem, n, past, nqh, nkh):
     tol = past * 2.0 ** -36 + want * (past + 200) * R.F32
     assert want > 6 * tol
     assert np.abs(s.chunk() - want).max() <= tol
+
+
+# ---- a scale that is no number --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("shape", [(1, 200, 4, 2, 128), (3, 60, 2, 2, 80), (70, 30, 4, 1, 64), (5, 0, 2, 1, 256)])
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf")])
+def test_scales_that_are_no_numbers(dev, mem, shape, scale):
+    """A NaN scale makes every seen score, row and weight NaN; an infinite one every row that has a score of +inf (all
+    but by chance), and its weights. Rows that see nothing stay 0."""
+    n, past, nqh, nkh, hd = shape
+    rng = np.random.default_rng(n)
+    s = Step(rng, mem, dev, *shape)
+    s.scale = scale
+    s.q[:, :nqh * hd] = np.abs(s.q[:, :nqh * hd]) + 0.1
+    slots = past + n
+    s.kc[1, slots - 1 if n == 1 else past, :, :] = np.array([2.0 if scale > 0 else -2.0], np.float16).view(np.uint16)[0]
+    mass0 = np.zeros((2, nkh, s.max_ctx), np.float32)
+    got = s.chunk(mass=mass0)
+    assert np.isnan(got).all()
+    m = s.dev.download(s.pm, mass0.shape, np.float32)
+    assert (m[0] == 0).all() and (m[1, :, slots:] == 0).all()
+    if np.isnan(scale):
+        assert np.isnan(m[1, :, :slots]).all()
+    else:
+        assert np.isnan(m[1, :, past]).all()
+    mask = np.zeros((n, (n + 63) // 64), np.uint64)
+    got = s.tree(mask)
+    assert (got == 0).all() if past == 0 else np.isnan(got).all() or not np.isnan(scale)

@@ -117,7 +117,8 @@ struct RowQ {
         (void)frexpf(top, &e2);  // top < 2^e2
         // (a row below 2^-111 scores nothing that an f32 sum keeps; 2^-sq must stay a number)
         const int sq = top > 0.f && top < INFINITY ? (15 - e2 < 126 ? 15 - e2 : 126) : 0;
-        c = fmaxf(ldexpf(fabsf(scale), -sq), 0x1p-126f);  // (not 0: masked scores are -inf times it)
+        c = ldexpf(fabsf(scale), -sq);
+        if (c < 0x1p-126f) c = 0x1p-126f;  // (not 0: masked scores are -inf times it; a NaN stays)
         const float sign = scale < 0.f ? -1.f : 1.f;
 #pragma unroll
         for (uint32_t kk = 0; kk < KK; kk++)
