@@ -254,7 +254,8 @@ int vbs_gfx950_linear_batch_multi(int type, uint32_t n_mat, const void *const *w
  * slot + n - 1 of `layer` (k itself is left as it was). q may be NULL (k and v
  * alone), or k, v, kc and vc (q alone). Angles are formed in 64 bits, which far
  * positions need; vbs_gfx950_rope forms them in f32, as the reference does, and
- * differs by up to pos * 2^-23 rad: a loop takes one of the two throughout. */
+ * differs by up to pos * 2^-23 rad: a loop takes one of the two throughout.
+ * theta is at least 2^-21. */
 int vbs_gfx950_rope_axes(float *q, uint32_t q_stride, const float *k, const float *v,
                          uint32_t kv_stride, const int32_t *pos, uint32_t n, uint32_t n_axes,
                          const uint32_t *sections, uint16_t *kc, uint16_t *vc, uint32_t slot,

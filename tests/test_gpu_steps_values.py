@@ -222,3 +222,28 @@ def test_scales_that_are_no_numbers(dev, mem, shape, scale):
     mask = np.zeros((n, (n + 63) // 64), np.uint64)
     got = s.tree(mask)
     assert (got == 0).all() if past == 0 else np.isnan(got).all() or not np.isnan(scale)
+
+
+# ---- thetas below 1: the later pairs turn faster -------------------------------------------------------------------
+
+@pytest.mark.parametrize("theta,far", [(0.5, 1 << 20), (2.0 ** -21, 300), (1.0, 1 << 30), (2.0 ** -21, 1 << 31), (3e38, 1000)])
+def test_thetas_far_from_the_usual(dev, mem, theta, far):
+    """The rotated pairs' elements within 3 F32 of their length (cosine and sine, products, sum; 3 sqrt 2 for the length
+    itself) and the angle's own error: a position times a frequency that the
+    oracle and the library each have to 2^-49, so |angle| 2^-48; where that is more than a turn, only the length holds
+    (and the angle is that of the product in 64 bits, whatever its last bits)."""
+    rng = np.random.default_rng(5)
+    n, heads, hd, sec = 17, 4, 64, (8, 24)
+    q = rng.standard_normal((n, heads * hd)).astype(np.float32)
+    pos = rng.integers(-far // 2, far - 1, (2, n)).astype(np.int32)
+    p = mem.up(q)
+    dev.rope_axes(p, heads * hd, 0, 0, 0, mem.up(pos), n, sec, 0, 0, 0, 0, 0, heads, 1, hd, theta)
+    got = dev.download(p, (n, heads, hd), np.float32).astype(np.float64)
+    x = q.reshape(n, heads, hd).astype(np.float64)
+    length = np.hypot(x[..., 0::2], x[..., 1::2])
+    assert np.all(np.abs(np.hypot(got[..., 0::2], got[..., 1::2]) - length) <= 5 * R.F32 * length)
+    t = float(np.float32(theta))
+    freq = np.exp(-2.0 * np.arange(hd // 2) / hd * np.log(t))
+    angle = np.abs(pos[np.repeat([0, 1], sec)].T * freq)[:, None]  # (n, 1, pairs)
+    size = np.repeat(np.abs(x[..., 0::2]) + np.abs(x[..., 1::2]), 2, -1)
+    close(got, R.rope_axes(x, pos, sec, t), size * (4 * R.F32 + np.repeat(np.minimum(angle * 2.0 ** -48, 2.0), 2, -1)))

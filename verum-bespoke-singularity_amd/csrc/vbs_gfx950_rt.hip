@@ -842,6 +842,7 @@ int vbs_gfx950_rope_axes(float *q, uint32_t q_stride, const float *k, const floa
     if (!step_shape_ok("rope_axes", n, stored ? slot : 0u, stored ? max_ctx : n, nqh, nkh, hd)) return 0;
     if (n_axes == 0 || n_axes > kRopeAxes) return fail("rope_axes: %u axes (1-%u)", n_axes, kRopeAxes);
     if (!(theta > 0.f)) return fail("rope_axes: theta must be positive");
+    if (theta < kRopeLeastTheta) return fail("rope_axes: theta must be at least 2^-21");
     if ((q && q_stride < (uint64_t)nqh * hd) || (stored && kv_stride < (uint64_t)nkh * hd))
         return fail("rope_axes: stride smaller than a row");
     RopeAxesArgs a{q, q_stride, k, v, kv_stride, pos, n, {}, kc, vc, nqh, nkh, hd};

@@ -23,10 +23,11 @@ struct RopeFreqs {
     double f[kRopeMaxPairs];
 };
 
-// (cos a, sin a): a = k pi/2 + r with pi/2 in two parts (53 and 53 bits; |a| up to
-// 2^31 leaves r exact to about 2^-52 * |k| * 2^-53 beyond a's own rounding), then
-// the Taylor series of sine and cosine on |r| <= pi/4, whose first dropped terms
-// are r^15 / 15! < 2.1e-14 and r^16 / 16! < 1.1e-15.
+// (cos a, sin a): a = k pi/2 + r with pi/2 in two parts (53 and 53 bits). k times the first part and a are both multiples
+// of 2^-52 while |a| < 2^52, so the first difference is exact; what the parts lack of pi/2 is 2^-107 |k|. k is off by one
+// at most where |a| nears 2^52 (theta of 2^-21; for theta >= 1 |a| is 2^31 at most and |r| <= pi/4). Then the Taylor
+// series of sine and cosine, whose first dropped terms are r^15 / 15! < 2.1e-14 and r^16 / 16! < 1.1e-15 for
+// |r| <= pi/4 and below 1e-8 for the |r| < 1.9 of the farthest.
 __device__ __forceinline__ float2 cos_sin(double a) {
     const double k = rint(a * 0.63661977236758134308);  // 2 / pi
     double r = fma(k, -1.5707963267948965580, a);

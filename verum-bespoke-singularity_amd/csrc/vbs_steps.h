@@ -13,6 +13,7 @@ namespace vbs {
 
 constexpr uint32_t kRopeAxes = 4;       // position axes of one call
 constexpr uint32_t kRopeMaxPairs = 128;  // head_dim 256, as the attentions
+constexpr float kRopeLeastTheta = 0x1p-21f;  // positions of 31 bits then turn by less than 2^52, which the reduction holds
 
 struct RopeAxesArgs {
     float *q;  // NULL: k and v alone
