@@ -1071,7 +1071,8 @@ static RowsPlan rows_plan(const RowsArgs &a) {
     const uint32_t least = p.few || wgs < 128u ? 128u : p.hd <= 64u ? 1024u : 65536u / p.hd / 128u * 128u;
     const uint32_t most = (slots + least - 1u) / least;
     uint32_t n = 512u / wgs;
-    n = n < 1u ? 1u : n > most ? most : n > kMostRanges ? kMostRanges : n;
+    n = n < most ? n : most;
+    n = n < 1u ? 1u : n < kMostRanges ? n : kMostRanges;  // (what the merge adds up)
     p.sp.len = ((slots + n - 1u) / n + 127u) / 128u * 128u;
     p.sp.n = (slots + p.sp.len - 1u) / p.sp.len;
     const size_t all = (size_t)rows * a.nkh;
