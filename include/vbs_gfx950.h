@@ -268,7 +268,10 @@ int vbs_gfx950_rope_axes(float *q, uint32_t q_stride, const float *k, const floa
  * a token's ancestors and its own). out row i, per q head: sum_j w_j v_j with
  * w = softmax(scale q.k_j) over the slots it sees, in f32 as
  * vbs_gfx950_attention; a row that sees nothing, or whose scores are all -inf, gives
- * 0, and what a row does not see does not reach it, infinities and NaN included. out must not overlap q. */
+ * 0, and what a row does not see does not reach it, infinities and NaN included. out must not overlap q.
+ * Scores are held in f32 and in units of log2: up to 2e38 in size. A row with a score beyond 1.1e7, or with an infinity or
+ * a NaN in a K or V row among the slots its workgroup looks at, is right but slow: it is taken again by one wave (about
+ * 3 ms for the heads of one such token over 2048 slots, where a whole chunk takes 0.1). */
 int vbs_gfx950_attention_tree(const float *q, uint32_t q_stride, const uint16_t *kc,
                               const uint16_t *vc, float *out, uint32_t out_stride, uint32_t n,
                               uint32_t past, const uint64_t *mask, uint32_t layer,

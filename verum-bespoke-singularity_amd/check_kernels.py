@@ -15,7 +15,10 @@ for gfx950 with the ROCm LLVM tools):
   hand-counted waits off, and a copy of a destination register made before
   its wait would hold stale data). Scalar registers spilled into lanes of a
   vector register (v_writelane / v_readlane, no memory: the case whenever
-  .sgpr_spill_count is not 0 while the scratch size is) are allowed;
+  .sgpr_spill_count is not 0 while the scratch size is) are allowed. The LDS
+  DMA of k_attn_rows and k_attn_few is not among them: they wait for every
+  load at once (vmcnt(0)), which a spill's own load or store cannot throw off
+  (k_attn_rows<256> spills);
 * M0 is written only by the LDS-DMA sequence of csrc/vbs_lds_dma.h and
   csrc/vbs_kern_checksum.hip (s_mov_b32 m0, sN; s_nop 0; global_load_lds_*),
   and read by nothing else: those inline-assembly blocks set M0 without

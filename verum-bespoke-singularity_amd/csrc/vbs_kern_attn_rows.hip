@@ -42,6 +42,8 @@
 // Measured beside it: 32 rows a wave 614, 16 rows and four waves a SIMD 842 (registers
 // spill), three waves a SIMD 667, a ring of four tiles 581, V transposed by permutes
 // instead of by the LDS read 857.
+// A row that is taken again (row_whole) costs a wave of its own: 1024 tokens over 2048 slots, 32/8 heads of 128, of
+// which every row shares a tile with an unseen infinite V: 26.8 ms for 87 us; one token of far scores: 3.1 ms.
 // Short ones: launches and one round trip to memory each; 16 tokens over 2048 slots
 // 10.7 + 4.3 us under the tracer.
 #include "vbs_lds_dma.h"
@@ -321,7 +323,8 @@ struct RowTile {
     template <uint32_t NH, bool DOCS_LDS>
     __device__ __forceinline__ void step(const RowsArgs &a, const uint8_t *lds, uint32_t p0, uint64_t vis, bool full,
                                          const int32_t *docs, uint32_t lane, float *scores = nullptr) {
-        // 16-slot tiles; dim tiles at a time (two at head_dim 256, where four leave 37 registers in memory)
+        // 16-slot tiles; dim tiles at a time (two at head_dim 256, which leave 21 registers in memory; four
+        // 39)
         constexpr uint32_t NS = 2u * NH, ND = DT < 4u ? DT : DT % 4u || DT > 8u ? 2u : 4u;
         const uint32_t g = lane >> 4;
         // A product waits for the one before it into the same sums: the tiles are taken in turn, the high parts

@@ -269,7 +269,8 @@ hipError_t launch_evict(const EvictArgs &a, hipStream_t s) {
     const bool wide = a.hd % 8u == 0 && (((uintptr_t)a.kc | (uintptr_t)a.vc) & 15u) == 0;
     // Whole rows a workgroup where that gives a workgroup per CU (32 layers of 8 heads of 128, 8192
     // slots to 4096: 223 us, 4.8 TB/s read and written; half rows 253, quarters 303, eighths 335), else
-    // narrower slices, down to 32 bytes (one such layer, 2049 to 1024: 3.5 us; whole rows 11.2).
+    // narrower slices, down to 32 bytes (one such layer, 2049 to 1024, the move as a launch of its own: 3.5 us; whole
+    // rows 11.2).
     const uint32_t units = wide ? a.hd / 8u : a.hd, pairs = 2u * a.nkh * a.n_layers, least = wide ? 2u : 16u;
     uint32_t lanes = units;
     while (lanes > least && pairs * ((units + lanes - 1u) / lanes) < 256u) lanes = (lanes + 1u) / 2u;

@@ -103,7 +103,9 @@ __global__ __launch_bounds__(256) void k_rope_axes(RopeAxesArgs a, RopeFreqs fr)
 
 hipError_t launch_rope_axes(const RopeAxesArgs &a, float theta, hipStream_t s) {
     const uint32_t pairs = a.hd / 2u, heads = (a.q ? a.nqh : 0u) + (a.k ? a.nkh : 0u);
-    // (kept from one call to the next: 64 powers take about 2 us of a call's 10)
+    // A thread's last table, by its values: 64 powers anew are 0.4 us of a call's 5.4 (back to back; one token, 32/8 heads
+    // of 128), which two thetas in turn pay. One power and products in 64 bits of mantissa instead, with nothing kept:
+    // 5.3 back to back, but 9.7 for 8.6 between other work of the host.
     static thread_local RopeFreqs fr;
     static thread_local float fr_theta = 0.f;
     static thread_local uint32_t fr_hd = 0;
