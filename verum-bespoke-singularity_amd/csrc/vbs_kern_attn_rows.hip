@@ -36,16 +36,16 @@
 // bits 2.6e-7 to 1.1e-6 over scores of a few units, the same in f32 matrix products
 // 3.8e-7 to 2.1e-6.
 // Bound, long chunks: the matrix cores and the vector unit share a SIMD's issue; a
-// 64-slot tile of 16 rows is 64 products (1024 cycles) and about 350 vector
+// 64-slot tile of 16 rows is 64 products (1024 cycles) and about 335 vector
 // instructions with the cap. 2048 tokens over 8192 slots, 32/8 heads of 128, capped:
-// 540-570 us, 845-890 TFLOP/s of f16 products (a library product of 8192^3: 1120-1165).
+// 540-570 us, 840-890 TFLOP/s of f16 products (a library product of 8192^3: 1120-1165).
 // Measured beside it: 32 rows a wave 614, 16 rows and four waves a SIMD 842 (registers
 // spill), three waves a SIMD 667, a ring of four tiles 581, V transposed by permutes
 // instead of by the LDS read 857.
 // A row that is taken again (row_whole) costs a wave of its own: 1024 tokens over 2048 slots, 32/8 heads of 128, of
 // which every row shares a tile with an unseen infinite V: 26.8 ms for 87 us; one token of far scores: 3.1 ms.
 // Short ones: launches and one round trip to memory each; 16 tokens over 2048 slots
-// 10.7 + 4.3 us under the tracer.
+// 10.9 + 4.2 us under the tracer.
 #include "vbs_lds_dma.h"
 #include "vbs_attn_rows.h"
 
