@@ -835,7 +835,7 @@ __global__ __launch_bounds__(256) void k_attn_rows_merge(RowsArgs a, RowsSplit s
 // in a fixed order. A slot whose sum is not finite is taken again in f32 products, and
 // marked rows (kMarkScore) and rows whose sum is no number are added in f32 products alone.
 // q's parts come from k_attn_rows, as the matrix cores take them: splitting q again for every 64 slots costs more
-// than the products (1024 tokens over 5120 slots, 32/8 heads of 128: 269 us under the tracer, 166 from the parts).
+// than the products (1024 tokens over 5120 slots, 32/8 heads of 128: 269 us under the tracer, 144 from the parts).
 // Where slots are few, the rows are split over `parts` workgroups and k_mass_add sums
 // what they leave in `part`. At most 16 rows leave their scores on the way instead, and
 // k_mass_few adds up their weights without a second product (one token over 2047 slots,
