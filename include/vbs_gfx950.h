@@ -317,6 +317,91 @@ int vbs_gfx950_cache_evict(uint16_t *kc, uint16_t *vc, const float *mass, float 
                            uint32_t last, uint32_t layer, uint32_t n_layers, uint32_t max_ctx,
                            uint32_t n_kv_heads, uint32_t head_dim);
 
+/* ---- a paged cache (extension) ---------------------------------------------
+ * The reference's cache is one run of max_ctx rows per layer
+ * (src/vbs_host_math.h:150-159). These operators serve several sequences from one
+ * pool of pages: a page holds page_slots tokens of every kv head of one layer, a
+ * table gives each sequence's pages in order, and the same page may stand in
+ * several rows of it (a shared prefix). Values are held as F16, or as Q8_0: per
+ * token, kv head and 32 elements an f16 scale d and 32 int8 q, value q d.
+ *
+ * Layout of a page of K or V: [kv head][unit], a unit being 32 slots of one head,
+ * nb = ceil(head_dim / 32) blocks of 32 elements (those behind head_dim are 0):
+ *   F16  K [t 2][b nb][g 4][h 4][j 4][e 8]: slot 8 h + 4 t + j, element 32 b + 8 g + e
+ *        V [b nb][t 2][g 4][r 16][e 8]:     slot 8 g + e, element 32 b + 16 t + r
+ *   Q8_0 K int8 [b nb][g 4][h 4][j 4][t 2][e 8], then scales [b nb][slot 32]
+ *        V int8 [b nb][g 4][r 16][t 2][e 8],     then scales [b nb][slot 32]
+ * (the order in which the attention's matrix instructions take them: pages are
+ * read without LDS). 2048 nb bytes a unit for F16, 1088 nb for Q8_0. */
+typedef struct vbs_gfx950_pages {
+    void *k, *v;           /* device: [layer][n_pages] pages each, 16-byte aligned, apart */
+    int type;              /* F16 or Q8_0 */
+    uint32_t page_slots;   /* 32 to 1024, a power of two */
+    uint32_t n_pages;
+    uint32_t n_kv_heads, head_dim;  /* head_dim even and <= 256 */
+    const int32_t *table;  /* device: [n_seqs][table_stride] pages */
+    uint32_t n_seqs, table_stride;
+} vbs_gfx950_pages_t;
+
+/* Bytes of one page of K, and of one of V (0: not a shape that pages take). */
+uint64_t vbs_gfx950_page_bytes(int type, uint32_t page_slots, uint32_t n_kv_heads, uint32_t head_dim);
+
+/* Store k and v (f32 rows of n_kv_heads x head_dim, kv_stride floats apart) of n
+ * tokens (<= 65535) in `layer`: token i becomes slot at[i] of sequence seq[i] (seq
+ * NULL: of sequence i; device arrays). A negative slot stores nothing (padding), nor
+ * does a place that the table has no page for, or a page outside 0 .. n_pages - 1
+ * (no memory but the pool's is touched). Two tokens of a call must not have the same place. F16
+ * takes vbs_gfx950_cache_store's rounding. Q8_0: d = f16(max |x| / 127) and q the
+ * integer nearest x / d within 127, both rounded once from the exact quotient, ties to
+ * even; a block with a NaN or an infinity, or whose d passes f16's range, reads back as NaN. */
+int vbs_gfx950_page_store(const vbs_gfx950_pages_t *pages, uint32_t layer, const float *k,
+                          const float *v, uint32_t kv_stride, const int32_t *seq,
+                          const int32_t *at, uint32_t n);
+
+/* Read back the rows of n tokens, as F32 or F16 rows (out_type; k and v of that type,
+ * kv_stride elements apart), for instance into a cache of one sequence for the
+ * attention of several tokens. F16 pages come as they are; q d is rounded to f16 as
+ * vbs_gfx950_cache_store does. Rows of a negative slot are left as they were; a place without a
+ * page gives NaN. */
+int vbs_gfx950_page_load(const vbs_gfx950_pages_t *pages, uint32_t layer, int out_type, void *k,
+                         void *v, uint32_t kv_stride, const int32_t *seq, const int32_t *at,
+                         uint32_t n);
+
+/* Attention of `rows` single tokens (<= 65535, 0: nothing is done; at most 2^28 rows x q heads):
+ * row r sees the slots below lens[r] of sequence seq[r] (seq NULL: of sequence r),
+ * out = sum_j w_j v_j, w = softmax(scale q.k_j), per q head (at most 16 per kv head),
+ * in f32 as vbs_gfx950_attention. A decode step has one row per sequence; the drafted tokens of a
+ * sequence are several rows of it, each one slot longer. No lens[r] may pass max_len, by which the work is
+ * split (a captured call's is the most that its sequences will grow to). A row of length 0, or whose
+ * scores are all -inf, gives 0; a row whose length or sequence is out of range, or one of whose
+ * pages is, gives NaN. What lies behind a row's last slot does not reach it, infinities and
+ * NaN included. Scores are held in f32 in units of log2, up to 2e38 in size. Weights down to 2^-38 of a
+ * row's greatest count (Q8_0: of the greatest weight times the greatest of V's scales). Infinities and NaN in a row's
+ * own q, K or V are right but slow. out must not overlap q. No call waits for the device. */
+int vbs_gfx950_attention_paged(const vbs_gfx950_pages_t *pages, uint32_t layer, const float *q,
+                               uint32_t q_stride, float *out, uint32_t out_stride,
+                               const int32_t *seq, const int32_t *lens, uint32_t rows,
+                               uint32_t max_len, uint32_t n_q_heads, float scale);
+
+/* Drafted tokens (of vbs_gfx950_attention_tree's or several rows of
+ * vbs_gfx950_attention_paged's) accepted or refused so that what stays is distributed
+ * as the target's own tokens. Per sequence b < batch (<= 65535): n drafted tokens (<= 64), ids
+ * drafted[b n + i], of which the first id outside 0 .. vocab - 1 ends the draft; target logits in rows
+ * b (n + 1) + i (`stride` floats apart), row i the distribution of the token that drafted token i is
+ * compared with, and the last that of the token behind the draft; the draft's logits in rows b n + i, or NULL where drafted
+ * tokens were certain (looked up); random numbers u[b (n + 1) + i] in [0, 1), n for the drafted tokens and one to draw
+ * with. p_i, q_i = softmax(row / temperature). Token x_i stays while u_i q_i(x_i) < p_i(x_i);
+ * behind the last that stays comes the lowest x with sum_{y <= x} r(y) > u_n sum r, r = max(p_i - q_i, 0)
+ * at the first refusal (p_i where nothing is left of it), p_i at the draft's end. Temperature 0: the greatest
+ * logit (the lowest place among equals) is certain, the draft's logits are not read. accepted[b] receives how many stay, tokens[b (n + 1) ..] them,
+ * the token drawn, and -1s. A row with a NaN or +inf, or of -inf alone, has no distribution: the target's refuses and
+ * draws -1, the draft's refuses (at temperature 0 a NaN is the least of all; only a row of NaN draws -1).
+ * Probabilities and sums are held in 64 bits. vocab <= 2^24. No call waits for the device. */
+int vbs_gfx950_verify_draft(const float *logits, uint32_t stride, const float *draft,
+                            uint32_t draft_stride, const int32_t *drafted, const float *u,
+                            uint32_t batch, uint32_t n, uint32_t vocab, float temperature,
+                            int32_t *accepted, int32_t *tokens);
+
 /* XOR checksum of a device region, as partial words, for
  * i < vbs_gfx950_checksum_partials(bytes): the region is cut into consecutive
  * spans of up to 112 KB, one per workgroup of 16 waves, and partials[16 w + v]
@@ -352,7 +437,8 @@ int vbs_gfx950_checksum_variant(const void *p, size_t bytes, uint32_t *partials,
  * largest shape before capturing. Batched Q4_0, Q4_1, Q8_0 and F16 calls take
  * memory of the graph's own while captured, at any size, which is given back
  * with the graph and its executables: such graphs may run beside each other
- * and beside any call. So do vbs_gfx950_attention_tree and _chunk. */
+ * and beside any call. So do vbs_gfx950_attention_tree, _chunk and _paged, and
+ * vbs_gfx950_verify_draft. */
 void *vbs_gfx950_stream(void);
 
 /* ---- graph-replayed decode step (extension) -------------------------------

@@ -18,6 +18,7 @@
 #include "vbs_dev_common.h"
 #include "vbs_gfx950.h"
 #include "vbs_internal.h"
+#include "vbs_pages.h"
 #include "vbs_steps.h"
 
 // Partial results of vbs_gfx950_attention_noalloc: a fixed device array, so
@@ -920,6 +921,142 @@ int vbs_gfx950_cache_evict(uint16_t *kc, uint16_t *vc, const float *mass, float 
     if (!ready_or_fail()) return 0;
     const OnDevice on;
     return hip_ok(launch_evict(a, g_rt.stream), "cache_evict");
+}
+
+// ---- the paged cache -------------------------------------------------------------
+namespace {
+constexpr uint32_t kMaxVocab = 1u << 24;
+
+// The pages as the kernels take them, at `layer`; 0 with the reason set.
+int page_args(const char *who, const vbs_gfx950_pages_t *p, uint32_t layer, PageArgs &a) {
+    if (!p || !p->k || !p->v || !p->table) return fail("%s: null pointer", who);
+    if (p->type != kF16 && p->type != kQ8_0) return fail("%s: pages are F16 or Q8_0, not type %d", who, p->type);
+    if (p->page_slots < 32u || p->page_slots > 1024u || (p->page_slots & (p->page_slots - 1u)))
+        return fail("%s: %u slots a page (32 to 1024, a power of two)", who, p->page_slots);
+    if (p->n_pages == 0 || p->n_seqs == 0 || p->table_stride == 0 || p->n_kv_heads == 0 || p->head_dim == 0)
+        return fail("%s: empty shape", who);
+    if (p->n_pages > 0x7FFFFFFFu || p->n_seqs > 0x7FFFFFFFu) return fail("%s: more than 2^31 - 1 pages or sequences", who);
+    if (p->n_kv_heads > 65535u) return fail("%s: %u kv heads exceed 65535", who, p->n_kv_heads);
+    if (p->head_dim > 256u || (p->head_dim & 1u)) return fail("%s: head_dim %u must be even and <= 256", who, p->head_dim);
+    if (((uintptr_t)p->k | (uintptr_t)p->v) & 15u) return fail("%s: pages not 16-byte aligned", who);
+    a.q8 = p->type == kQ8_0;
+    a.n_pages = p->n_pages;
+    a.shift = 0;
+    while ((32u << a.shift) < p->page_slots) a.shift++;
+    a.nkh = p->n_kv_heads, a.hd = p->head_dim, a.nb = (p->head_dim + 31u) / 32u;
+    a.unit_bytes = page_unit_bytes(a.q8, a.hd);
+    a.page_bytes = (uint64_t)a.nkh * (p->page_slots / 32u) * a.unit_bytes;
+    if (a.page_bytes > (1ull << 48) / a.n_pages || a.page_bytes * a.n_pages > (1ull << 48) / (layer + 1ull))
+        return fail("%s: pages beyond 2^48 bytes", who);
+    const uint64_t pool = a.page_bytes * a.n_pages;
+    a.k = static_cast<uint8_t *>(p->k) + layer * pool;
+    a.v = static_cast<uint8_t *>(p->v) + layer * pool;
+    if (spans_overlap(a.k, pool, a.v, pool)) return fail("%s: the pages of k and v overlap", who);
+    a.table = p->table;
+    a.n_seqs = p->n_seqs, a.per_seq = p->table_stride;
+    return 1;
+}
+
+int page_rows(const char *who, const vbs_gfx950_pages_t *p, uint32_t layer, PageRowsArgs &a) {
+    if (!page_args(who, p, layer, a.p)) return 0;
+    if (!a.at) return fail("%s: null pointer", who);
+    if (a.n > kMaxStep) return fail("%s: at most %u tokens per call", who, kMaxStep);
+    if (a.stride < (uint64_t)a.p.nkh * a.p.hd) return fail("%s: stride smaller than a row", who);
+    return 1;
+}
+}  // namespace
+
+uint64_t vbs_gfx950_page_bytes(int type, uint32_t page_slots, uint32_t n_kv_heads, uint32_t head_dim) {
+    if ((type != kF16 && type != kQ8_0) || page_slots < 32u || page_slots > 1024u || (page_slots & (page_slots - 1u)) ||
+        n_kv_heads == 0 || n_kv_heads > 65535u || head_dim == 0 || head_dim > 256u || (head_dim & 1u))
+        return 0;
+    return (uint64_t)n_kv_heads * (page_slots / 32u) * page_unit_bytes(type == kQ8_0, head_dim);
+}
+
+int vbs_gfx950_page_store(const vbs_gfx950_pages_t *pages, uint32_t layer, const float *k, const float *v,
+                          uint32_t kv_stride, const int32_t *seq, const int32_t *at, uint32_t n) {
+    PageRowsArgs a{};
+    if (!k || !v) return fail("page_store: null pointer");
+    a.seq = seq, a.at = at, a.n = n, a.k = k, a.v = v, a.stride = kv_stride;
+    if (!page_rows("page_store", pages, layer, a)) return 0;
+    if (n == 0) return 1;
+    if (!ready_or_fail()) return 0;
+    const OnDevice on;
+    return hip_ok(launch_page_store(a, g_rt.stream), "page_store");
+}
+
+int vbs_gfx950_page_load(const vbs_gfx950_pages_t *pages, uint32_t layer, int out_type, void *k, void *v,
+                         uint32_t kv_stride, const int32_t *seq, const int32_t *at, uint32_t n) {
+    PageRowsArgs a{};
+    if (!k || !v) return fail("page_load: null pointer");
+    if (out_type != kF32 && out_type != kF16) return fail("page_load: rows are F32 or F16, not type %d", out_type);
+    a.seq = seq, a.at = at, a.n = n, a.out_k = k, a.out_v = v, a.out_f16 = out_type == kF16, a.stride = kv_stride;
+    if (!page_rows("page_load", pages, layer, a)) return 0;
+    if (n == 0) return 1;
+    if (!ready_or_fail()) return 0;
+    const OnDevice on;
+    return hip_ok(launch_page_load(a, g_rt.stream), "page_load");
+}
+
+int vbs_gfx950_attention_paged(const vbs_gfx950_pages_t *pages, uint32_t layer, const float *q, uint32_t q_stride,
+                               float *out, uint32_t out_stride, const int32_t *seq, const int32_t *lens,
+                               uint32_t rows, uint32_t max_len, uint32_t nqh, float scale) {
+    const char *who = "attention_paged";
+    PagedAttnArgs a{};
+    if (!q || !out || !lens) return fail("%s: null pointer", who);
+    if (!page_args(who, pages, layer, a.p)) return 0;
+    if (nqh == 0) return fail("%s: empty shape", who);
+    if (nqh % a.p.nkh) return fail("%s: %u q heads not a multiple of %u kv heads", who, nqh, a.p.nkh);
+    a.group = nqh / a.p.nkh;
+    if (a.group > 16u) return fail("%s: group size %u exceeds 16", who, a.group);
+    if (rows > kMaxStep) return fail("%s: at most %u rows per call", who, kMaxStep);
+    if ((uint64_t)rows * nqh > kMaxStepRows) return fail("%s: more than 2^28 rows x q heads", who);
+    if (max_len > (uint64_t)a.p.per_seq * pages->page_slots)
+        return fail("%s: max_len %u exceeds the table's %u pages of %u slots", who, max_len, a.p.per_seq, pages->page_slots);
+    if (max_len > kMaxSlots) return fail("%s: at most 2^31 slots", who);
+    const uint64_t row = (uint64_t)nqh * a.p.hd;
+    if (q_stride < row || out_stride < row) return fail("%s: stride smaller than a row", who);
+    if (rows == 0) return 1;
+    if (spans_overlap(q, 4u * ((uint64_t)(rows - 1u) * q_stride + row), out, 4u * ((uint64_t)(rows - 1u) * out_stride + row)))
+        return fail("%s: out overlaps q", who);
+    a.q = q, a.q_stride = q_stride, a.out = out, a.out_stride = out_stride, a.seq = seq, a.lens = lens;
+    a.rows = rows, a.max_len = max_len, a.nqh = nqh, a.scale = scale;
+    const size_t bytes = plan_attn_paged(a);
+    if (!ready_or_fail()) return 0;
+    const OnDevice on;
+    const std::lock_guard<std::mutex> together(g_scratch_mu);
+    void *scratch = nullptr;
+    if (bytes) {
+        hipError_t why = hipSuccess;
+        scratch = rt_scratch_or_captured(bytes, g_rt.stream, &why);
+        if (!scratch) return hip_ok(why, who);
+    }
+    return hip_ok(launch_attn_paged(a, scratch, g_rt.stream), who);
+}
+
+int vbs_gfx950_verify_draft(const float *logits, uint32_t stride, const float *draft, uint32_t draft_stride,
+                            const int32_t *drafted, const float *u, uint32_t batch, uint32_t n, uint32_t vocab,
+                            float temperature, int32_t *accepted, int32_t *tokens) {
+    const char *who = "verify_draft";
+    if (!logits || !u || !accepted || !tokens || (n && !drafted)) return fail("%s: null pointer", who);
+    if (vocab == 0) return fail("%s: empty shape", who);
+    if (vocab > kMaxVocab) return fail("%s: a vocabulary of more than 2^24", who);
+    if (n > kMaxDraft) return fail("%s: at most %u drafted tokens", who, kMaxDraft);
+    if (batch > kMaxStep) return fail("%s: at most %u sequences per call", who, kMaxStep);
+    if (stride < vocab || (draft && draft_stride < vocab)) return fail("%s: stride smaller than a row", who);
+    if (!(temperature >= 0.f) || isinf(temperature)) return fail("%s: temperature must be 0 or a positive number", who);
+    if (batch == 0) return 1;
+    VerifyArgs a{};
+    a.logits = logits, a.stride = stride, a.draft = draft, a.draft_stride = draft_stride, a.drafted = drafted, a.u = u;
+    a.batch = batch, a.n = n, a.vocab = vocab, a.temp = temperature, a.accepted = accepted, a.tokens = tokens;
+    const size_t bytes = plan_verify(a);
+    if (!ready_or_fail()) return 0;
+    const OnDevice on;
+    const std::lock_guard<std::mutex> together(g_scratch_mu);
+    hipError_t why = hipSuccess;
+    void *scratch = rt_scratch_or_captured(bytes, g_rt.stream, &why);
+    if (!scratch) return hip_ok(why, who);
+    return hip_ok(launch_verify(a, scratch, g_rt.stream), who);
 }
 
 uint32_t vbs_gfx950_checksum_partials(size_t bytes) { return checksum_partials(bytes); }

@@ -133,6 +133,13 @@ class AttnTerms(C.Structure):
     _fields_ = [("cap", _F), ("slopes", _P), ("docs", _P), ("prefix", _U32), ("mass", _P)]
 
 
+class Pages(C.Structure):
+    """vbs_gfx950_pages_t: a pool of pages and the table of its sequences."""
+    _fields_ = [("k", _P), ("v", _P), ("type", _I), ("page_slots", _U32), ("n_pages", _U32),
+                ("n_kv_heads", _U32), ("head_dim", _U32), ("table", _P), ("n_seqs", _U32),
+                ("table_stride", _U32)]
+
+
 _DEVICE_SIGS = {
     "abi_version": (_I, []),
     "init": (_I, []),
@@ -166,6 +173,11 @@ _DEVICE_SIGS = {
     "attention_chunk": (_I, [_P, _U32, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _U32, _U32, _F,
                              C.POINTER(AttnTerms)]),
     "cache_evict": (_I, [_P, _P, _P, _P, _P] + [_U32] * 9),
+    "page_bytes": (_U64, [_I, _U32, _U32, _U32]),
+    "page_store": (_I, [C.POINTER(Pages), _U32, _P, _P, _U32, _P, _P, _U32]),
+    "page_load": (_I, [C.POINTER(Pages), _U32, _I, _P, _P, _U32, _P, _P, _U32]),
+    "attention_paged": (_I, [C.POINTER(Pages), _U32, _P, _U32, _P, _U32, _P, _P, _U32, _U32, _U32, _F]),
+    "verify_draft": (_I, [_P, _U32, _P, _U32, _P, _P, _U32, _U32, _U32, _F, _P, _P]),
     "silu_mul": (_I, [_P, _P, _P, _U32]),
     "add": (_I, [_P, _P, _P, _U32]),
     "dequant_rows": (_I, [_I, _P, _P, _U32, _U32, _P]),
@@ -367,6 +379,32 @@ class DeviceLib:
         """Cut n_len slots to budget, per layer and kv head, by accumulated weight (mass_out may be 0)."""
         self.check(self._cache_evict(kc, vc, mass, mass_out or None, kept, n_len, budget, first, last, layer,
                                      n_layers, max_ctx, nkh, hd), "cache_evict")
+
+    def page_bytes(self, t, page_slots, nkh, hd) -> int:
+        """Bytes of one page of K (and of V); 0 for a shape that pages do not take."""
+        return int(self._page_bytes(t, page_slots, nkh, hd))
+
+    def page_store(self, pages, layer, k, v, kv_stride, seq, at, n):
+        """Store n tokens' k and v rows as slots at[i] of the sequences seq[i] (seq 0: token i of sequence i)."""
+        self.check(self._page_store(C.byref(pages), layer, k or None, v or None, kv_stride, seq or None, at or None, n),
+                   "page_store")
+
+    def page_load(self, pages, layer, out_type, k, v, kv_stride, seq, at, n):
+        """Read n tokens' rows back out of the pages, as F32 or F16 rows."""
+        self.check(self._page_load(C.byref(pages), layer, out_type, k or None, v or None, kv_stride, seq or None,
+                                   at or None, n), "page_load")
+
+    def attention_paged(self, pages, layer, q, q_stride, out, out_stride, seq, lens, rows, max_len, nqh, scale):
+        """Attention of single tokens: row r over the slots below lens[r] of sequence seq[r] (seq 0: of sequence r)."""
+        self.check(self._attention_paged(C.byref(pages), layer, q or None, q_stride, out or None, out_stride, seq or None,
+                                         lens or None, rows, max_len, nqh, scale), "attention_paged")
+
+    def verify_draft(self, logits, stride, draft, draft_stride, drafted, u, batch, n, vocab, temperature, accepted,
+                     tokens):
+        """Accept or refuse n drafted tokens of each sequence and draw the next (draft 0: the drafted tokens were
+        certain)."""
+        self.check(self._verify_draft(logits or None, stride, draft or None, draft_stride, drafted or None, u or None,
+                                      batch, n, vocab, temperature, accepted or None, tokens or None), "verify_draft")
 
     def silu_mul(self, g, u, out, n):
         self.check(self._silu_mul(g, u, out, n), "silu_mul")
