@@ -318,6 +318,46 @@ def test_attention(dev, mem, t, lens, nqh, nkh, hd, page):
 
 
 @TYPES
+@pytest.mark.parametrize("rows,longest,nqh,nkh,hd", [(70, 900, 8, 2, 64), (300, 600, 2, 1, 30), (64, 2000, 8, 8, 34), (70, 640, 16, 8, 64),
+                                                     (3, 3000, 2, 1, 128), (17, 1100, 12, 1, 256)])
+def test_attention_of_many_rows(dev, mem, t, rows, longest, nqh, nkh, hd):
+    """Shares that hold several rows and heads, begin and end anywhere in them, more rows than a wave has lanes, empty
+    rows and rows out of range among them."""
+    rng = np.random.default_rng(rows)
+    lens = rng.integers(1, longest + 1, rows)
+    lens[0] = longest
+    lens[1::7] = 0
+    r = Rows(rng, mem, dev, t, lens, nqh, nkh, hd, max_len=longest)
+    want, tol = r.want()
+    r.lens[2::9] = -5
+    r.lens[3::31] = longest + 1
+    got = r.run()
+    bad = (r.lens < 0) | (r.lens > longest)
+    assert np.isnan(got[bad]).all() and (got[r.lens == 0] == 0).all()
+    close(got[~bad], want[~bad], tol[~bad])
+
+
+def test_many_pieces_that_are_not_finite(dev, mem):
+    """Shares of more than 64 rows and heads, infinities in many of them: each is taken again by itself. A row of one slot
+    is that slot's V, exactly."""
+    rng = np.random.default_rng(33)
+    rows, nkh, hd, seqs = 1200, 64, 2, 6
+    lens = np.ones(rows, np.int64)
+    lens[5] = 600
+    r = Rows(rng, mem, dev, V.F16, lens, nkh, nkh, hd, q_size=0.1, seq=np.arange(rows) % seqs, junk=False)
+    for i in (0, 2, 4):
+        p, slot = r.c.place(i, 0)
+        for h in range(i, nkh, 5):
+            r.c.pool._values("v")[p, h, 0, R.place(V.F16, "v", hd, slot, 1)] = 0x7C00
+    want = np.array([r.c.pool.get("v", *r.c.place(i, 0)) for i in range(seqs)])[np.arange(rows) % seqs]
+    got = r.run()
+    k, v = (r.c.pool.rows(w, r.c.table[5], 600) for w in "kv")
+    close(got[5], *R.attend(r.q[5].reshape(nkh, hd).astype(np.float64), k, v, r.scale))
+    got[5] = want[5]
+    assert np.array_equal(got, want) and np.isposinf(got[0, 0, 1])
+
+
+@TYPES
 def test_attention_rows_of_a_sequence(dev, mem, t):
     """Drafted tokens: several rows of a sequence, each a slot longer, sequences in any order; a max_len far above."""
     rng = np.random.default_rng(5)

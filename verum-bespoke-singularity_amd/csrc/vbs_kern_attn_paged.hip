@@ -1,10 +1,10 @@
 // vbs_kern_attn_paged.hip — the attention of single tokens over the paged cache.
 //
 // Row r (one token; its q heads of one kv head are up to eight columns of a product):
-// out = sum_j w_j v_j, w = softmax(scale q.k_j) over the slots j < lens[r]. A row's units
-// of 32 slots are split over workgroups and over their four waves; each keeps the running
-// maximum m (in log2), the sum l and O of its own units, the four are joined through LDS and
-// the workgroups' by k_attn_paged_merge.
+// out = sum_j w_j v_j, w = softmax(scale q.k_j) over the slots j < lens[r]. The units of 32
+// slots of all rows and heads are shared out evenly over the workgroups that run at once, and
+// within one over its four waves; each keeps the running maximum m (in log2), the sum l and O of
+// its own units, the four are joined through LDS and the workgroups' by k_attn_paged_merge.
 //
 // Products: S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_16x16x32_f16, whose operands the
 // page's layout holds as they are (vbs_pages.h), so K and V go from memory to the registers
@@ -21,7 +21,11 @@
 // or whose sign differs) leave a sum that is not finite: the workgroup then takes its slots
 // again in plain f32 (slow_tile).
 //
-// Bound: HBM.
+// Bound: HBM where the caches are large (a workgroup reads its next unit while it computes, 64 KB or
+// more in flight a CU): 64 sequences of 4096 slots, 32/8 heads of 128, 5.7 TB/s of F16 (188 us) and 5.2 of
+// Q8_0 (111); launches and round trips where they are small: one sequence of 2048 slots 11.6 us, of which
+// the merge 4. Workgroups of fewer units each, in more than one round, cost 12 us of start each (lengths, table, first
+// unit, one after the other) under load: 264 us for 111 at four units a workgroup.
 #include <math.h>
 
 #include "vbs_dev_common.h"
@@ -33,6 +37,7 @@ namespace {
 
 typedef _Float16 ph8 __attribute__((ext_vector_type(8)));
 typedef _Float16 ph2 __attribute__((ext_vector_type(2)));
+typedef float pf2 __attribute__((ext_vector_type(2)));
 typedef float pf4 __attribute__((ext_vector_type(4)));
 typedef uint32_t pu4 __attribute__((ext_vector_type(4)));
 
@@ -56,90 +61,228 @@ __device__ __forceinline__ float over_groups_sum(float v) {
 __device__ __forceinline__ ph8 int8_to_f16(uint32_t lo, uint32_t hi) {
     lo ^= 0x80808080u, hi ^= 0x80808080u;
     const uint32_t e = 0x64646464u;
-    ph2 p[4];
-    p[0] = __builtin_bit_cast(ph2, __builtin_amdgcn_perm(e, lo, 0x04010400u));
-    p[1] = __builtin_bit_cast(ph2, __builtin_amdgcn_perm(e, lo, 0x04030402u));
-    p[2] = __builtin_bit_cast(ph2, __builtin_amdgcn_perm(e, hi, 0x04010400u));
-    p[3] = __builtin_bit_cast(ph2, __builtin_amdgcn_perm(e, hi, 0x04030402u));
     const ph2 off = {(_Float16)1152.f, (_Float16)1152.f};
-    ph8 r;
+    const ph2 p0 = __builtin_bit_cast(ph2, __builtin_amdgcn_perm(e, lo, 0x04010400u)) - off;
+    const ph2 p1 = __builtin_bit_cast(ph2, __builtin_amdgcn_perm(e, lo, 0x04030402u)) - off;
+    const ph2 p2 = __builtin_bit_cast(ph2, __builtin_amdgcn_perm(e, hi, 0x04010400u)) - off;
+    const ph2 p3 = __builtin_bit_cast(ph2, __builtin_amdgcn_perm(e, hi, 0x04030402u)) - off;
+    return ph8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+}
+
+// Of eight values the high f16 part where low is 0, and the low part, of what the high one leaves, where it is -1.
+__device__ __forceinline__ ph8 parts(const float x[8], float low) {
+    ph2 r[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        p[i] = p[i] - off;
-        r[2 * i] = p[i][0], r[2 * i + 1] = p[i][1];
+        const ph2 h = __builtin_convertvector((pf2{x[2 * i], x[2 * i + 1]}), ph2);
+        const float l0 = fmaf(low, (float)h[0], x[2 * i]), l1 = fmaf(low, (float)h[1], x[2 * i + 1]);
+        r[i] = __builtin_convertvector((pf2{l0, l1}), ph2);
     }
-    return r;
+    return ph8{r[0][0], r[0][1], r[1][0], r[1][1], r[2][0], r[2][1], r[3][0], r[3][1]};
 }
 
-// The high or the low f16 part of eight values.
-__device__ __forceinline__ ph8 parts(const float x[8], bool low) {
-    ph8 r;
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const _Float16 h = (_Float16)x[e];
-        const _Float16 l = (_Float16)(x[e] - (float)h);
-        r[e] = low ? l : h;
-    }
-    return r;
-}
-
-// What a workgroup is to do: the units [u0, u1) of a row.
-struct Span {
+// A row: its sequence, its slots (0 where one of the two is out of range: the row is NaN) and units.
+struct Row {
     int32_t seq;
-    uint32_t len, u0, u1;
-    bool bad;  // a length or sequence out of range: the row is NaN
+    uint32_t len, units;
+    bool bad;
 };
-__device__ __forceinline__ Span row_span(const PagedAttnArgs &a, uint32_t row) {
-    Span s;
-    s.seq = a.seq ? a.seq[row] : (int32_t)row;
+__device__ __forceinline__ Row row_at(const PagedAttnArgs &a, uint32_t row) {
+    Row r;
+    r.seq = a.seq ? a.seq[row] : (int32_t)row;
     const int32_t len = a.lens[row];
-    s.bad = len < 0 || (uint32_t)len > a.max_len || (uint32_t)s.seq >= a.p.n_seqs;
-    s.len = s.bad ? 0u : (uint32_t)len;
-    s.u0 = 0u;
-    s.u1 = (s.len + kUnit - 1u) / kUnit;
+    r.bad = len < 0 || (uint32_t)len > a.max_len || (uint32_t)r.seq >= a.p.n_seqs;
+    r.len = r.bad ? 0u : (uint32_t)len;
+    r.units = (r.len + kUnit - 1u) / kUnit;
+    return r;
+}
+
+// What every lane holds, told to the compiler.
+__device__ __forceinline__ uint64_t same(uint64_t v) {
+    return (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32 | __builtin_amdgcn_readfirstlane((uint32_t)v);
+}
+
+// How the units of all rows and heads are shared out. They lie in one line: row by row, within a row kv head (and tile of q
+// heads) by head, within that slot by slot, and a workgroup takes `share` of them, so all have the same work whatever the
+// lengths. Shares of few units (kAlignedShare) begin and end with their head, which `grain` pads in the line: a
+// second piece's start would take as long as the share. One workgroup a CU where the line is short: 8 heads
+// of one row of 8192 slots take 18.2 us with 256 workgroups (Q8_0, 128 elements) and 23.4 with 512, of 8 rows 44.6 and 38.5.
+constexpr uint32_t kAlignedShare = 16, kShortLine = 8192;
+
+struct Shares {
+    uint64_t share, grain;
+};
+__device__ __forceinline__ Shares shares(const PagedAttnArgs &a, uint64_t units, uint32_t line) {  // units: of a head, all rows
+    const uint64_t all = units * line;
+    const uint32_t workgroups = all < kShortLine ? min(a.workgroups, 256u) : a.workgroups;
+    Shares s;
+    s.share = (all + workgroups - 1u) / workgroups;
+    s.share = (s.share + kWaves - 1u) / kWaves * kWaves;
+    s.grain = a.aligned && s.share <= kAlignedShare ? s.share : 1u;
     return s;
 }
-__device__ __forceinline__ uint32_t row_splits(const PagedAttnArgs &a, const Span &s) {
-    return max(1u, (s.u1 + a.per_split - 1u) / a.per_split);
+__device__ __forceinline__ uint64_t padded(const Shares &s, uint32_t units) {
+    return s.grain == 1u ? units : (units + s.grain - 1u) / s.grain * s.grain;
+}
+// The sum of v over a workgroup of 256 threads; w: 4 words.
+__device__ __forceinline__ uint64_t sum_of_256(uint64_t v, uint64_t *w) {
+    for (uint32_t o = 32; o; o >>= 1) v += __shfl_xor((unsigned long long)v, (int)o, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63u) == 0u) w[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return same((w[0] + w[1]) + (w[2] + w[3]));
+}
+__device__ __forceinline__ uint64_t wave_total(uint64_t v) {
+    for (uint32_t o = 32; o; o >>= 1) v += __shfl_xor((unsigned long long)v, (int)o, 64);
+    return same(v);
+}
+// v summed over the lanes up to each.
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v, uint32_t lane) {
+    for (uint32_t o = 1; o < 64u; o <<= 1) {
+        const uint64_t t = __shfl_up((unsigned long long)v, (int)o, 64);
+        if (lane >= o) v += t;
+    }
+    return v;
 }
 
-template <uint32_t NB, bool Q8>
-struct Unit {
-    pu4 k[Q8 ? NB : 2 * NB], v[Q8 ? NB : 2 * NB];
-    pu4 ks[Q8 ? NB : 1], vs[Q8 ? NB : 1];
+// The row that unit `at` of the line lies in, and where the row begins (padded units of a head before it); false where
+// the line ends before. Up to 64 rows every wave looks by itself, a row a lane; beyond, the workgroup's
+// 256 threads, thread t the rows t R .. t R + R - 1.
+struct Found {
+    uint32_t row;
+    uint64_t before;
+};
+__device__ __forceinline__ bool find_row(const PagedAttnArgs &a, uint32_t line, uint32_t workgroup, Shares &sh, uint64_t &at, uint64_t &end,
+                                         Found &f, uint64_t *sums) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    if (a.rows <= 64u) {
+        const uint32_t units = lane < a.rows ? row_at(a, lane).units : 0u;
+        if (a.rows == 1u) {
+            const uint32_t n = __builtin_amdgcn_readfirstlane(units);
+            sh = shares(a, n, line);
+            at = workgroup * sh.share, end = padded(sh, n) * line;
+            end = min(end, at + sh.share);
+            f.row = 0u, f.before = 0u;
+            return at < end;
+        }
+        sh = shares(a, wave_total(units), line);
+        const uint64_t mine = padded(sh, units), to = wave_scan(mine, lane);
+        at = workgroup * sh.share;
+        const uint64_t here = __ballot(at < to * line);
+        if (here == 0u) return false;
+        const uint64_t all = __shfl((unsigned long long)to, 63, 64), before = __shfl((unsigned long long)(to - mine), __ffsll((unsigned long long)here) - 1, 64);
+        end = min(at + sh.share, same(all) * line);
+        f.row = (uint32_t)__ffsll((unsigned long long)here) - 1u, f.before = same(before);
+        return true;
+    }
+    __shared__ Found found;
+    const uint32_t each = (a.rows + 255u) / 256u, r0 = min(tid * each, a.rows), r1 = min(r0 + each, a.rows);
+    uint64_t mine = 0;
+    for (uint32_t r = r0; r < r1; r++) mine += row_at(a, r).units;
+    sh = shares(a, sum_of_256(mine, sums), line);
+    if (sh.grain != 1u) {
+        mine = 0;
+        for (uint32_t r = r0; r < r1; r++) mine += padded(sh, row_at(a, r).units);
+    }
+    uint64_t to = wave_scan(mine, lane), all = 0;
+    __syncthreads();
+    if (lane == 63u) sums[wave] = to;
+    __syncthreads();
+    for (uint32_t w = 0; w < kWaves; w++) {
+        if (w < wave) to += sums[w];
+        all += sums[w];
+    }
+    at = workgroup * sh.share;
+    end = min(at + sh.share, same(all) * line);
+    if (at >= end) return false;
+    uint64_t before = to - mine;
+    if (before * line <= at && at < to * line) {
+        uint32_t r = r0;
+        for (;; r++) {
+            const uint64_t n = padded(sh, row_at(a, r).units);
+            if ((before + n) * line > at) break;
+            before += n;
+        }
+        found = Found{r, before};
+    }
+    __syncthreads();
+    f.row = __builtin_amdgcn_readfirstlane(found.row), f.before = same(found.before);
+    return true;
+}
+// The other way: where `row` begins.
+__device__ __forceinline__ uint64_t row_begins(const PagedAttnArgs &a, uint32_t line, uint32_t row, Shares &sh, uint64_t *sums) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
+    if (a.rows <= 64u) {
+        const uint32_t units = lane < a.rows ? row_at(a, lane).units : 0u;
+        sh = shares(a, a.rows == 1u ? __builtin_amdgcn_readfirstlane(units) : wave_total(units), line);
+        return row ? wave_total(lane < row ? padded(sh, units) : 0u) : 0u;
+    }
+    uint64_t all = 0, before = 0;
+    for (uint32_t k = tid; k < a.rows; k += 256u) {
+        const uint32_t u = row_at(a, k).units;
+        all += u;
+        if (k < row) before += u;
+    }
+    sh = shares(a, sum_of_256(all, sums), line);
+    if (sh.grain != 1u) {
+        before = 0;
+        for (uint32_t k = tid; k < row; k += 256u) before += padded(sh, row_at(a, k).units);
+    }
+    return sum_of_256(before, sums);
+}
 
-    __device__ __forceinline__ void load_k(const uint8_t *p, uint32_t lane) {
+// Workgroups of a CU, by the registers of a unit in flight (64 sequences of 4096 slots, 8 kv heads, Q8_0: heads of 32
+// take 43 us with four and 53 with two, of 128 111 with two and 121 with three, of 192 162 with two and 193 with one, of
+// 256, which spill with two, 249 with one and 338 with two).
+constexpr uint32_t per_cu(uint32_t nb) { return nb == 1u ? 4u : nb <= 7u ? 2u : 1u; }
+
+// A unit of K or of V on its way: its values as an operand takes them, and (Q8_0) its 32 NB scales, two in a dword, dword
+// 64 i + lane in ds[i].
+template <uint32_t NB, bool Q8>
+struct Half {
+    static constexpr uint32_t kValues = Q8 ? NB : 2 * NB, kScales = Q8 ? (NB + 3u) / 4u : 1u;
+    pu4 x[kValues];
+    uint32_t ds[kScales];
+
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (uint32_t i = 0; i < (Q8 ? NB : 2 * NB); i++) k[i] = *reinterpret_cast<const pu4 *>(p + i * 1024u + lane * 16u);
+        for (uint32_t i = 0; i < kValues; i++) x[i] = pu4{0u, 0u, 0u, 0u};
+#pragma unroll
+        for (uint32_t i = 0; i < kScales; i++) ds[i] = 0u;
+    }
+    __device__ __forceinline__ void load(const uint8_t *p, uint32_t lane) {
+#pragma unroll
+        for (uint32_t i = 0; i < kValues; i++) x[i] = *reinterpret_cast<const pu4 *>(p + i * 1024u + lane * 16u);
         if constexpr (Q8) {
 #pragma unroll
-            for (uint32_t b = 0; b < NB; b++) ks[b] = *reinterpret_cast<const pu4 *>(p + NB * 1024u + b * 64u + (lane >> 4) * 16u);
+            for (uint32_t i = 0; i < kScales; i++)
+                if (64u * i + lane < NB * 16u) ds[i] = *reinterpret_cast<const uint32_t *>(p + NB * 1024u + i * 256u + lane * 4u);
         }
     }
-    __device__ __forceinline__ void load_v(const uint8_t *p, uint32_t lane) {
+    // The scales through LDS (a wave's own words): every lane reads the eight of its slots, block by block.
+    __device__ __forceinline__ void spread(uint32_t *w, uint32_t lane) const {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-        for (uint32_t i = 0; i < (Q8 ? NB : 2 * NB); i++) v[i] = *reinterpret_cast<const pu4 *>(p + i * 1024u + lane * 16u);
-        if constexpr (Q8) {
-#pragma unroll
-            for (uint32_t b = 0; b < NB; b++) vs[b] = *reinterpret_cast<const pu4 *>(p + NB * 1024u + b * 64u + (lane >> 4) * 16u);
-        }
+        for (uint32_t i = 0; i < kScales; i++)
+            if (64u * i + lane < NB * 16u) w[64u * i + lane] = ds[i];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 };
 
 }  // namespace
 
-// The workgroup's slots [32 u0, min(32 u1, len)) again for one q head, in f32 products and sums: m, l and O (thread d
+// The slots [32 u0, min(32 u1, len)) of a sequence again for one q head, in f32 products and sums: m, l and O (thread d
 // holds element d). `w` holds 256 floats.
 template <bool Q8>
-__device__ __noinline__ void slow_tile(const PagedAttnArgs &a, const Span &sp, uint32_t kvh, const float *q, float *w, float &m,
-                                       float &l, float &o) {
-    const uint32_t tid = threadIdx.x, hd = a.p.hd, nb = a.p.nb, end = min(sp.u1 * kUnit, sp.len);
+__device__ __forceinline__ void slow_tile(const PagedAttnArgs &a, int32_t seq, uint32_t u0, uint32_t u1, uint32_t len, uint32_t kvh,
+                                       const float *q, float *w, float &m, float &l, float &o) {
+    const uint32_t tid = threadIdx.x, hd = a.p.hd, nb = a.p.nb, end = min(u1 * kUnit, len);
     m = -INFINITY, l = 0.f, o = 0.f;
-    for (uint32_t j0 = sp.u0 * kUnit; j0 < end; j0 += 256u) {
+    for (uint32_t j0 = u0 * kUnit; j0 < end; j0 += 256u) {
         const uint32_t j = j0 + tid, count = min(256u, end - j0);
         float s = 0.f;
         if (j < end) {
-            const int32_t page = page_at(a.p, sp.seq, j / kUnit);
+            const int32_t page = page_at(a.p, seq, j / kUnit);
             if (page < 0) {
                 s = NAN;
             } else {
@@ -172,7 +315,7 @@ __device__ __noinline__ void slow_tile(const PagedAttnArgs &a, const Span &sp, u
             const float p = w[i];
             l += p;
             const uint32_t jj = j0 + i;
-            const int32_t page = page_at(a.p, sp.seq, jj / kUnit);
+            const int32_t page = page_at(a.p, seq, jj / kUnit);
             if (tid >= hd || page < 0) continue;
             const uint8_t *unit = a.p.v + unit_offset(a.p, page, jj / kUnit, kvh);
             const uint32_t slot = jj & (kUnit - 1u);
@@ -188,45 +331,79 @@ __device__ __noinline__ void slow_tile(const PagedAttnArgs &a, const Span &sp, u
     }
 }
 
-// grid (splits x kv heads x tiles of eight q heads, rows)
+template <uint32_t NB>
+struct Shared {
+    float o[kWaves][kHeads][NB * 32u + 4u];
+    float m[kWaves][kHeads], l[kWaves][kHeads];
+    uint32_t scales[kWaves][2][NB * 16u];
+    uint32_t odd;
+};
+
+// Units [u0, u1) of a row and a kv head (and tile of eight of its q heads), by a workgroup: to out, or as a partial
+// result if part is given. False, and nothing written, where sums are not finite (slow_units then does it).
 template <uint32_t NB, bool Q8>
-__global__ __launch_bounds__(256, 2) void k_attn_paged(PagedAttnArgs a) {
-    __shared__ float so[kWaves][kHeads][NB * 32u + 4u];
-    __shared__ float sm[kWaves][kHeads], sl[kWaves][kHeads];
-    __shared__ uint32_t odd;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15u;
-    const uint32_t tiles = (a.group + kHeads - 1u) / kHeads, split = blockIdx.x % a.splits, hx = blockIdx.x / a.splits;
-    const uint32_t kvh = hx / tiles, tile = hx % tiles, row = blockIdx.y, hd = a.p.hd;
-    Span sp = row_span(a, row);
-    if (split >= row_splits(a, sp)) return;
-    const uint32_t nsplit = row_splits(a, sp);
-    sp.u0 = split * a.per_split;
-    sp.u1 = min(sp.u0 + a.per_split, sp.u1);
+__device__ __forceinline__ bool attend_units(const PagedAttnArgs &a, Shared<NB> &sh, uint32_t row, uint32_t hx, int32_t seq, uint32_t len,
+                                             uint32_t u0, uint32_t u1, float *part, float2 *ml) {
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    uint32_t lane = tid & 63u;
+    asm volatile("" : "+v"(lane));  // (else what depends on the lane alone is kept from piece to piece: 60 registers more, and spills)
+    const uint32_t g = lane >> 4, c = lane & 15u;
+    const uint32_t tiles = (a.group + kHeads - 1u) / kHeads, kvh = hx / tiles, tile = hx % tiles, hd = a.p.hd;
     const uint32_t head0 = kvh * a.group + tile * kHeads, heads = min(kHeads, a.group - tile * kHeads);
     const float *q0 = a.q + (uint64_t)row * a.q_stride + (uint64_t)head0 * hd;
-    if (tid == 0) odd = 0u;
+    if (tid == 0) sh.odd = 0u;
+
+    uint32_t u = u0 + wave;
+    int32_t page = u < u1 ? page_at(a.p, seq, u) : 0;
+    bool lost = page < 0;
+    Half<NB, Q8> k, v;
+    k.clear(), v.clear();  // (so that nothing of them lives from one piece to the next)
+    uint32_t *ks = sh.scales[wave][0], *vs = sh.scales[wave][1];
+    if (u < u1 && !lost) {
+        const uint64_t at = unit_offset(a.p, page, u, kvh);
+        k.load(a.p.k + at, lane);
+        v.load(a.p.v + at, lane);
+    }
 
     // q's parts: column c the head c & 7, its elements 32 b + 8 g ..
+    const float low = c < 8u ? 0.f : -1.f;
     ph8 qf[NB];
     float unscale;
     {
         const uint32_t h = c & 7u;
         float x[NB][8], top = 0.f;
+        if (a.q_vec) {
+#pragma unroll
+            for (uint32_t b = 0; b < NB; b++) {
+                const uint32_t d = b * 32u + g * 8u;
+                pf4 y0 = {0.f, 0.f, 0.f, 0.f}, y1 = y0;
+                if (h < heads && d < hd) {
+                    const pf4 *from = reinterpret_cast<const pf4 *>(q0 + h * hd + d);
+                    y0 = from[0], y1 = from[1];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[b][e] = y0[e], x[b][4 + e] = y1[e];
+            }
+        } else {
+#pragma unroll
+            for (uint32_t b = 0; b < NB; b++)
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e++) {
+                    const uint32_t d = b * 32u + g * 8u + e;
+                    x[b][e] = h < heads && d < hd ? q0[h * hd + d] : 0.f;
+                }
+        }
 #pragma unroll
         for (uint32_t b = 0; b < NB; b++)
 #pragma unroll
-            for (uint32_t e = 0; e < 8; e++) {
-                const uint32_t d = b * 32u + g * 8u + e;
-                x[b][e] = h < heads && d < hd ? q0[(uint64_t)h * hd + d] : 0.f;
-                top = fmaxf(top, fabsf(x[b][e]));
-            }
+            for (uint32_t e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[b][e]));
         top = over_groups_max(top);
         const int up = 13 + 127 - (int)max(vbs_float_to_bits(top) >> 23, 1u);  // (an infinity stays one)
 #pragma unroll
         for (uint32_t b = 0; b < NB; b++) {
 #pragma unroll
             for (uint32_t e = 0; e < 8; e++) x[b][e] = __builtin_ldexpf(x[b][e], up);
-            qf[b] = parts(x[b], c >= 8u);
+            qf[b] = parts(x[b], low);
         }
         unscale = __builtin_ldexpf(a.scale * kPagedLog2e, -up);
     }
@@ -236,28 +413,21 @@ __global__ __launch_bounds__(256, 2) void k_attn_paged(PagedAttnArgs a) {
     for (uint32_t i = 0; i < 2 * NB; i++) o[i] = pf4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
     int top_e = -60;  // Q8_0: V's scales are below 2^top_e
-    bool lost = false;
-    for (uint32_t u = sp.u0 + wave; u < sp.u1; u += kWaves) {
-        const int32_t page = __builtin_amdgcn_readfirstlane(page_at(a.p, sp.seq, u));
-        if (page < 0) {
-            lost = true;
-            break;
-        }
-        const uint64_t at = unit_offset(a.p, page, u, kvh);
-        Unit<NB, Q8> f;
-        f.load_k(a.p.k + at, lane);
-        f.load_v(a.p.v + at, lane);
+    while (u < u1 && !lost) {
+        const uint32_t next = u + kWaves;
+        page = next < u1 ? page_at(a.p, seq, next) : 0;
         // scores: lane (g, c) holds slots 8 g + e of column c
         float s[8];
         if constexpr (Q8) {
 #pragma unroll
             for (int e = 0; e < 8; e++) s[e] = 0.f;
+            k.spread(ks, lane);
 #pragma unroll
             for (uint32_t b = 0; b < NB; b++) {
-                const ph8 d = __builtin_bit_cast(ph8, f.ks[b]);
+                const ph8 d = *reinterpret_cast<const ph8 *>(ks + b * 16u + g * 4u);
                 const pf4 zero = {0.f, 0.f, 0.f, 0.f};
-                const pf4 s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(int8_to_f16(f.k[b][0], f.k[b][1]), qf[b], zero, 0, 0, 0);
-                const pf4 s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(int8_to_f16(f.k[b][2], f.k[b][3]), qf[b], zero, 0, 0, 0);
+                const pf4 s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(int8_to_f16(k.x[b][0], k.x[b][1]), qf[b], zero, 0, 0, 0);
+                const pf4 s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(int8_to_f16(k.x[b][2], k.x[b][3]), qf[b], zero, 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     s[i] = fmaf(s0[i], (float)d[i], s[i]);
@@ -268,39 +438,43 @@ __global__ __launch_bounds__(256, 2) void k_attn_paged(PagedAttnArgs a) {
             pf4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll
             for (uint32_t b = 0; b < NB; b++) {
-                s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, f.k[b]), qf[b], s0, 0, 0, 0);
-                s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, f.k[NB + b]), qf[b], s1, 0, 0, 0);
+                s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, k.x[b]), qf[b], s0, 0, 0, 0);
+                s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, k.x[NB + b]), qf[b], s1, 0, 0, 0);
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) s[i] = s0[i], s[4 + i] = s1[i];
         }
+        // the next unit's K is on its way during the softmax and the second product, its V during the next scores
+        lost = page < 0;
+        const uint64_t at = lost ? 0u : unit_offset(a.p, page, next, kvh);
+        const bool more = next < u1 && !lost;
+        if (more) k.load(a.p.k + at, lane);
         const uint32_t mine = u * kUnit + g * 8u;  // the lane's first slot
-        const bool tail = (u + 1u) * kUnit > sp.len;
+        const bool tail = (u + 1u) * kUnit > len;
         float top = m;
 #pragma unroll
-        for (uint32_t e = 0; e < 8; e++) {
-            s[e] = (s[e] + row_ror8(s[e])) * unscale;
-            if (tail && mine + e >= sp.len) s[e] = -INFINITY;
-            top = fmaxf(top, s[e]);
-        }
-        top = over_groups_max(top);
-        const float ref = top == -INFINITY ? 0.f : top;
+        for (uint32_t e = 0; e < 8; e++) s[e] = (s[e] + row_ror8(s[e])) * unscale;
         if (tail) {  // what lies behind the last slot may be anything
 #pragma unroll
-            for (uint32_t i = 0; i < (Q8 ? 0u : 2 * NB); i++)
+            for (uint32_t e = 0; e < 8; e++)
+                if (mine + e >= len) s[e] = -INFINITY;
+            auto kept = [&](uint32_t j) { return (j < len ? 0xFFFFu : 0u) | (j + 1u < len ? 0xFFFF0000u : 0u); };
+            if constexpr (Q8) {
+#pragma unroll
+                for (uint32_t &d : v.ds) d &= kept(u * kUnit + 2u * (lane & 15u));
+            } else {
 #pragma unroll
                 for (uint32_t w = 0; w < 4; w++) {
-                    const uint32_t j = mine + 2u * w;
-                    f.v[i][w] &= (j < sp.len ? 0xFFFFu : 0u) | (j + 1u < sp.len ? 0xFFFF0000u : 0u);
-                }
+                    const uint32_t keep = kept(mine + 2u * w);
 #pragma unroll
-            for (uint32_t i = 0; i < (Q8 ? NB : 0u); i++)
-#pragma unroll
-                for (uint32_t w = 0; w < 4; w++) {
-                    const uint32_t j = mine + 2u * w;
-                    f.vs[i][w] &= (j < sp.len ? 0xFFFFu : 0u) | (j + 1u < sp.len ? 0xFFFF0000u : 0u);
+                    for (pu4 &x : v.x) x[w] &= keep;
                 }
+            }
         }
+#pragma unroll
+        for (uint32_t e = 0; e < 8; e++) top = fmaxf(top, s[e]);
+        top = over_groups_max(top);
+        const float ref = top == -INFINITY ? 0.f : top;
         float p[8], sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
@@ -308,17 +482,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_paged(PagedAttnArgs a) {
             sum += p[e];
         }
         float keep = __builtin_amdgcn_exp2f(m - ref);
-        l = l * keep + sum;
+        l = fmaf(l, keep, sum);
         m = top;
         if constexpr (Q8) {
-            uint32_t big = 0u;
+            uint32_t e5 = 0u;
 #pragma unroll
-            for (uint32_t b = 0; b < NB; b++)
-#pragma unroll
-                for (int w = 0; w < 4; w++) big = max(big, max(f.vs[b][w] & 0x7FFFu, (f.vs[b][w] >> 16) & 0x7FFFu));
-            big = max(big, lane_xor<16>(big));
-            big = max(big, lane_xor<32>(big));
-            const int e = __builtin_amdgcn_readfirstlane((int)min(big >> 10, 30u)) - 14;
+            for (uint32_t d : v.ds) e5 = max(e5, max(d & 0x7FFFu, (d >> 16) & 0x7FFFu));
+            e5 = wave_butterfly(e5, [](uint32_t x, uint32_t y) { return max(x, y); });
+            const int e = __builtin_amdgcn_readfirstlane((int)min(e5 >> 10, 30u)) - 14;
             if (e > top_e) {
                 keep = __builtin_ldexpf(keep, top_e - e);
                 top_e = e;
@@ -331,26 +502,30 @@ __global__ __launch_bounds__(256, 2) void k_attn_paged(PagedAttnArgs a) {
                 for (int r = 0; r < 4; r++) o[i][r] *= keep;
         }
         if constexpr (Q8) {
+            v.spread(vs, lane);
+            const float raise = __builtin_ldexpf(1.f, kWeightBits - top_e);
 #pragma unroll
-            for (int e = 0; e < 8; e++) p[e] = __builtin_ldexpf(p[e], kWeightBits - top_e);
+            for (int e = 0; e < 8; e++) p[e] *= raise;
 #pragma unroll
             for (uint32_t b = 0; b < NB; b++) {
-                const ph8 d = __builtin_bit_cast(ph8, f.vs[b]);
+                const ph8 d = *reinterpret_cast<const ph8 *>(vs + b * 16u + g * 4u);
                 float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = p[e] * (float)d[e];
-                const ph8 w = parts(x, c >= 8u);
-                o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(int8_to_f16(f.v[b][0], f.v[b][1]), w, o[2 * b], 0, 0, 0);
-                o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(int8_to_f16(f.v[b][2], f.v[b][3]), w, o[2 * b + 1], 0, 0, 0);
+                for (int e = 0; e < 8; e++) x[e] = fmaf(p[e], (float)d[e], 0.f);
+                const ph8 w = parts(x, low);
+                o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(int8_to_f16(v.x[b][0], v.x[b][1]), w, o[2 * b], 0, 0, 0);
+                o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(int8_to_f16(v.x[b][2], v.x[b][3]), w, o[2 * b + 1], 0, 0, 0);
             }
         } else {
 #pragma unroll
             for (int e = 0; e < 8; e++) p[e] *= (float)(1 << kWeightBits);
-            const ph8 w = parts(p, c >= 8u);
+            const ph8 w = parts(p, low);
 #pragma unroll
             for (uint32_t i = 0; i < 2 * NB; i++)
-                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, f.v[i]), w, o[i], 0, 0, 0);
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, v.x[i]), w, o[i], 0, 0, 0);
         }
+        if (more) v.load(a.p.v + at, lane);
+        u = next;
     }
     l = over_groups_sum(l);
     const float down = __builtin_ldexpf(1.f, (Q8 ? top_e : 0) - kWeightBits);
@@ -362,98 +537,231 @@ __global__ __launch_bounds__(256, 2) void k_attn_paged(PagedAttnArgs a) {
             o[i][r] = (o[i][r] + row_ror8(o[i][r])) * down;
             fine = fine && fabsf(o[i][r]) < INFINITY;
         }
-        if (c < 8u) *reinterpret_cast<pf4 *>(&so[wave][c][i * 16u + g * 4u]) = o[i];
+        if (c < 8u) *reinterpret_cast<pf4 *>(&sh.o[wave][c][i * 16u + g * 4u]) = o[i];
     }
-    if (g == 0u && c < 8u) sm[wave][c] = m, sl[wave][c] = l;
+    if (g == 0u && c < 8u) sh.m[wave][c] = m, sh.l[wave][c] = l;
     fine = fine || (c & 7u) >= heads;
     __syncthreads();  // (odd is 0)
-    if ((lost || __any(!fine)) && lane == 0u) odd = 1u;
+    if ((lost || __any(!fine)) && lane == 0u) sh.odd = 1u;
     __syncthreads();
-    const bool again = odd != 0u, direct = nsplit == 1u && a.splits == 1u;
+    if (__builtin_amdgcn_readfirstlane(sh.odd)) return false;
+    float *out = a.out + (uint64_t)row * a.out_stride + (uint64_t)head0 * hd;
+    for (uint32_t i = tid; i < heads * NB * 32u; i += 256u) {
+        const uint32_t h = i / (NB * 32u), d = i % (NB * 32u);
+        const float mm = fmaxf(fmaxf(sh.m[0][h], sh.m[1][h]), fmaxf(sh.m[2][h], sh.m[3][h])), ref = mm == -INFINITY ? 0.f : mm;
+        float ll = 0.f, oo = 0.f;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; w++) {
+            const float k = __builtin_amdgcn_exp2f(sh.m[w][h] - ref);
+            ll = fmaf(k, sh.l[w][h], ll);
+            oo = fmaf(k, sh.o[w][h][d], oo);
+        }
+        if (!part) {
+            if (d < hd) out[h * hd + d] = ll == 0.f ? 0.f : oo / ll;
+        } else {
+            if (d < hd) part[h * hd + d] = oo;
+            if (d == 0u) ml[h] = make_float2(mm, ll);
+        }
+    }
+    return true;
+}
+
+// The same in plain f32.
+template <uint32_t NB, bool Q8>
+__device__ __forceinline__ void slow_units(const PagedAttnArgs &a, Shared<NB> &sh, uint32_t row, uint32_t hx, int32_t seq, uint32_t len,
+                                           uint32_t u0, uint32_t u1, float *part, float2 *ml) {
+    const uint32_t tiles = (a.group + kHeads - 1u) / kHeads, kvh = hx / tiles, tile = hx % tiles, hd = a.p.hd, tid = threadIdx.x;
+    const uint32_t head0 = kvh * a.group + tile * kHeads, heads = min(kHeads, a.group - tile * kHeads);
+    const float *q0 = a.q + (uint64_t)row * a.q_stride + (uint64_t)head0 * hd;
+    float *out = a.out + (uint64_t)row * a.out_stride + (uint64_t)head0 * hd;
     for (uint32_t h = 0; h < heads; h++) {
         float mm, ll, oo;
-        if (again) {
-            __syncthreads();
-            slow_tile<Q8>(a, sp, kvh, q0 + (uint64_t)h * hd, &so[0][0][0], mm, ll, oo);
+        __syncthreads();
+        slow_tile<Q8>(a, seq, u0, u1, len, kvh, q0 + h * hd, &sh.o[0][0][0], mm, ll, oo);
+        if (!part) {
+            if (tid < hd) out[h * hd + tid] = ll == 0.f ? 0.f : oo / ll;
         } else {
-            mm = fmaxf(fmaxf(sm[0][h], sm[1][h]), fmaxf(sm[2][h], sm[3][h]));
-            ll = 0.f, oo = 0.f;
-            const float ref = mm == -INFINITY ? 0.f : mm;
-#pragma unroll
-            for (uint32_t w = 0; w < kWaves; w++) {
-                const float f = __builtin_amdgcn_exp2f(sm[w][h] - ref);
-                ll = fmaf(f, sl[w][h], ll);
-                if (tid < hd) oo = fmaf(f, so[w][h][tid], oo);
-            }
-        }
-        if (sp.bad) ll = NAN;
-        const uint32_t head = head0 + h;
-        if (direct) {
-            if (tid < hd) a.out[(uint64_t)row * a.out_stride + (uint64_t)head * hd + tid] = ll == 0.f ? 0.f : oo / ll;
-        } else {
-            const uint64_t at = ((uint64_t)row * a.nqh + head) * a.splits + split;
-            if (tid < hd) a.part[at * hd + tid] = oo;
-            if (tid == 0u) a.ml[at] = make_float2(mm, ll);
+            if (tid < hd) part[h * hd + tid] = oo;
+            if (tid == 0u) ml[h] = make_float2(mm, ll);
         }
     }
 }
 
-// The splits of a row joined: grid (q heads, rows).
-__global__ __launch_bounds__(256) void k_attn_paged_merge(PagedAttnArgs a) {
-    const uint32_t head = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, hd = a.p.hd;
-    const Span sp = row_span(a, row);
-    const uint32_t n = row_splits(a, sp);
-    const uint64_t at = ((uint64_t)row * a.nqh + head) * a.splits;
-    float m = -INFINITY;
-    for (uint32_t i = 0; i < n; i++) m = fmaxf(m, a.ml[at + i].x);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o = 0.f;
-    for (uint32_t i = 0; i < n; i++) {
-        const float2 x = a.ml[at + i];
-        const float f = __builtin_amdgcn_exp2f(x.x - ref);
-        l = fmaf(f, x.y, l);
-        if (tid < hd) o = fmaf(f, a.part[(at + i) * hd + tid], o);
+// Rows of few units: a workgroup for each row and head, nothing to join. grid (kv heads x tiles of eight q heads, rows)
+template <uint32_t NB, bool Q8>
+__global__ __launch_bounds__(256, per_cu(NB)) void k_attn_paged_whole(PagedAttnArgs a) {
+    __shared__ Shared<NB> sh;
+    const uint32_t row = blockIdx.y, hd = a.p.hd;
+    const Row r = row_at(a, row);
+    if (r.units) {
+        if (!attend_units<NB, Q8>(a, sh, row, blockIdx.x, r.seq, r.len, 0u, r.units, nullptr, nullptr))
+            slow_units<NB, Q8>(a, sh, row, blockIdx.x, r.seq, r.len, 0u, r.units, nullptr, nullptr);
+        return;
     }
-    if (tid < hd) a.out[(uint64_t)row * a.out_stride + (uint64_t)head * hd + tid] = l == 0.f ? 0.f : o / l;
+    const uint32_t tiles = (a.group + kHeads - 1u) / kHeads, kvh = blockIdx.x / tiles, tile = blockIdx.x % tiles;
+    const uint32_t n = min(kHeads, a.group - tile * kHeads) * hd;
+    float *out = a.out + (uint64_t)row * a.out_stride + (uint64_t)(kvh * a.group + tile * kHeads) * hd;
+    for (uint32_t i = threadIdx.x; i < n; i += 256u) out[i] = r.bad ? NAN : 0.f;
 }
+
+// All rows' units in equal shares, one a workgroup. What lies whole in a share is done with it; the piece of a row and head
+// that goes on in the next share is the workgroup's second partial result, one that began in an earlier share its first.
+template <uint32_t NB, bool Q8>
+__global__ __launch_bounds__(256, per_cu(NB)) void k_attn_paged(PagedAttnArgs a) {
+    __shared__ Shared<NB> sh;
+    __shared__ uint64_t sums[kWaves];
+    const uint32_t line = a.p.nkh * ((a.group + kHeads - 1u) / kHeads);  // heads (tiles) of a row
+    Shares sh_;
+    uint64_t at, end;
+    Found f;
+    if (!find_row(a, line, blockIdx.x, sh_, at, end, f, sums)) return;
+    const uint32_t row0 = f.row;
+    const Row first = row_at(a, row0);
+    const uint64_t in = at - f.before * line, long0 = padded(sh_, first.units);
+    const uint32_t hx0 = (uint32_t)(in / long0), u00 = (uint32_t)(in % long0);
+    // the share's pieces one after the other; in the second round, if there is one, those that were not finite (the 64th
+    // and all behind it together)
+    uint64_t odd = 0;
+    for (uint32_t round = 0; round < 2u; round++) {
+        Row r = first;
+        uint32_t row = row0, hx = hx0, u0 = u00, n = 0;
+        uint64_t left = end - at;
+        while (true) {
+            const uint32_t u1 = r.units - u0 < left ? r.units : u0 + (uint32_t)left;
+            const bool begun = u0 != 0u, whole = !begun && u1 == r.units;
+            const uint64_t slot = ((uint64_t)blockIdx.x * 2u + (begun ? 0u : 1u)) * kHeads;
+            float *part = whole ? nullptr : a.part + slot * a.p.hd;
+            const uint64_t bit = 1ull << min(n, 63u);
+            if (round == 0u) {
+                if (!attend_units<NB, Q8>(a, sh, row, hx, r.seq, r.len, u0, u1, part, a.ml + slot)) odd |= bit;
+            } else if (odd & bit) {
+                slow_units<NB, Q8>(a, sh, row, hx, r.seq, r.len, u0, u1, part, a.ml + slot);
+            }
+            left -= u1 - u0;
+            if (left == 0u || sh_.grain != 1u) break;
+            n++;
+            u0 = 0u;
+            if (++hx == line) {
+                hx = 0u;
+                do r = row_at(a, ++row);
+                while (r.units == 0u);
+            }
+            __syncthreads();
+        }
+        if (!odd) break;
+    }
+}
+
+// The pieces of the rows and heads that lie in several shares, joined, and the rows without units: grid (q heads, rows).
+// Threads of 256 / W groups (W: hd in whole waves) take every so many pieces of an element each; their first values are
+// on their way while the weights are formed.
+constexpr uint32_t kAhead = 8;
+
+__global__ __launch_bounds__(256) void k_attn_paged_merge(PagedAttnArgs a) {
+    __shared__ float w[256], so[256], sx[8];
+    __shared__ uint64_t sums[4];
+    const uint32_t head = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, hd = a.p.hd;
+    const uint32_t tiles = (a.group + kHeads - 1u) / kHeads, line = a.p.nkh * tiles, kvh = head / a.group, in = head % a.group;
+    const Row r = row_at(a, row);
+    float *out = a.out + (uint64_t)row * a.out_stride + (uint64_t)head * hd;
+    if (r.units == 0u) {
+        if (tid < hd) out[tid] = r.bad ? NAN : 0.f;
+        return;
+    }
+    Shares sh;
+    const uint64_t before = row_begins(a, line, row, sh, sums);
+    const uint64_t s0 = before * line + (kvh * tiles + in / kHeads) * padded(sh, r.units);
+    const uint32_t w0 = (uint32_t)(s0 / sh.share), n = (uint32_t)((s0 + r.units - 1u) / sh.share) - w0 + 1u;
+    if (n == 1u) return;
+    // piece k: workgroup w0 + k's first partial result, for k = 0 its second
+    auto piece = [&](uint32_t k) { return ((uint64_t)(w0 + k) * 2u + (k ? 0u : 1u)) * kHeads + in % kHeads; };
+    const uint32_t width = (hd + 63u) & ~63u, groups = 256u / width, d = tid % width, grp = tid / width;
+    const bool mine = d < hd && grp < groups;
+    float x[kAhead];
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; i++) {
+        const uint32_t k = grp + i * groups;
+        x[i] = mine && k < n ? a.part[piece(k) * hd + d] : 0.f;
+    }
+    float m = -INFINITY, l = 0.f, o = 0.f;
+    for (uint32_t k0 = 0; k0 < n; k0 += 256u) {  // (once, but for more than 256 pieces)
+        const float2 ml = k0 + tid < n ? a.ml[piece(k0 + tid)] : make_float2(-INFINITY, 0.f);
+        float top = wave_max(ml.x);
+        __syncthreads();
+        if (lane == 0u) sx[wave] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(fmaxf(sx[0], sx[1]), fmaxf(sx[2], sx[3])), m);
+        const float ref = top == -INFINITY ? 0.f : top, keep = __builtin_amdgcn_exp2f(m - ref), f = __builtin_amdgcn_exp2f(ml.x - ref);
+        w[tid] = f;
+        const float sum = wave_sum(k0 + tid < n ? f * ml.y : 0.f);
+        if (lane == 0u) sx[4u + wave] = sum;
+        __syncthreads();
+        l = fmaf(l, keep, (sx[4] + sx[5]) + (sx[6] + sx[7]));
+        o *= keep;
+        m = top;
+        const uint32_t k1 = min(n, k0 + 256u);
+        if (k0 == 0u) {
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead; i++) {
+                const uint32_t k = grp + i * groups;
+                if (k < k1) o = fmaf(w[k], x[i], o);
+            }
+        }
+        if (mine)
+            for (uint32_t k = k0 ? k0 + grp : grp + kAhead * groups; k < k1; k += groups)
+                o = fmaf(w[k - k0], a.part[piece(k) * hd + d], o);
+    }
+    so[tid] = o;
+    __syncthreads();
+    if (tid >= hd) return;
+    for (uint32_t k = 1; k < groups; k++) o += so[tid + k * width];
+    out[tid] = l == 0.f ? 0.f : o / l;
+}
+
+// Rows of at most so many units are not split: one of 512 slots takes 9.7 us (8 heads of 128, Q8_0), in shares 11.2.
+constexpr uint32_t kWholeUnits = 16;
 
 size_t plan_attn_paged(PagedAttnArgs &a) {
     const uint32_t units = (a.max_len + kUnit - 1u) / kUnit, tiles = (a.group + kHeads - 1u) / kHeads;
-    const uint64_t all = (uint64_t)units * a.rows * a.p.nkh * tiles;
-    uint64_t per = (all + 1023u) / 1024u;
-    per = (per + kWaves - 1u) / kWaves * kWaves;
-    if (per < kWaves) per = kWaves;
-    if ((uint64_t)units > per * 256u) per = ((uint64_t)units + 255u) / 256u;
-    a.per_split = (uint32_t)per;
-    a.splits = units ? (uint32_t)((units + per - 1u) / per) : 1u;
-    if (a.splits == 1u) return 0;
-    return (uint64_t)a.rows * a.nqh * a.splits * (sizeof(float2) + 4ull * a.p.hd);
+    a.workgroups = 0;
+    const uint32_t most = 256u * per_cu(a.p.nb);
+    if (units <= kWholeUnits) return 0;
+    const uint64_t heads = (uint64_t)a.rows * a.p.nkh * tiles, each = (units * heads + kWaves - 1u) / kWaves;
+    a.workgroups = each < most ? (uint32_t)each : most;
+    a.aligned = heads <= most;
+    a.grid = a.workgroups + (a.aligned ? (uint32_t)heads : 0u);  // (each head's last share may be short)
+    return (uint64_t)a.grid * 2u * kHeads * (sizeof(float2) + 4ull * a.p.hd);
 }
 
+template <uint32_t NB, bool Q8>
+static void launch_one(const PagedAttnArgs &a, hipStream_t s) {
+    const uint32_t tiles = (a.group + kHeads - 1u) / kHeads;
+    if (a.workgroups) k_attn_paged<NB, Q8><<<a.grid, 256, 0, s>>>(a);
+    else k_attn_paged_whole<NB, Q8><<<dim3(a.p.nkh * tiles, a.rows), 256, 0, s>>>(a);
+}
 template <bool Q8>
-static void launch_nb(const PagedAttnArgs &a, dim3 grid, hipStream_t s) {
+static void launch_nb(const PagedAttnArgs &a, hipStream_t s) {
     switch (a.p.nb) {
-        case 1: k_attn_paged<1, Q8><<<grid, 256, 0, s>>>(a); break;
-        case 2: k_attn_paged<2, Q8><<<grid, 256, 0, s>>>(a); break;
-        case 3: k_attn_paged<3, Q8><<<grid, 256, 0, s>>>(a); break;
-        case 4: k_attn_paged<4, Q8><<<grid, 256, 0, s>>>(a); break;
-        case 5: k_attn_paged<5, Q8><<<grid, 256, 0, s>>>(a); break;
-        case 6: k_attn_paged<6, Q8><<<grid, 256, 0, s>>>(a); break;
-        case 7: k_attn_paged<7, Q8><<<grid, 256, 0, s>>>(a); break;
-        default: k_attn_paged<8, Q8><<<grid, 256, 0, s>>>(a); break;
+        case 1: launch_one<1, Q8>(a, s); break;
+        case 2: launch_one<2, Q8>(a, s); break;
+        case 3: launch_one<3, Q8>(a, s); break;
+        case 4: launch_one<4, Q8>(a, s); break;
+        case 5: launch_one<5, Q8>(a, s); break;
+        case 6: launch_one<6, Q8>(a, s); break;
+        case 7: launch_one<7, Q8>(a, s); break;
+        default: launch_one<8, Q8>(a, s); break;
     }
 }
 
 hipError_t launch_attn_paged(PagedAttnArgs a, void *scratch, hipStream_t s) {
-    const uint32_t tiles = (a.group + kHeads - 1u) / kHeads;
+    a.q_vec = !(((uintptr_t)a.q & 15u) | (a.q_stride & 3u) | (a.p.hd & 7u));
     a.ml = static_cast<float2 *>(scratch);
-    a.part = reinterpret_cast<float *>(a.ml + (uint64_t)a.rows * a.nqh * a.splits);
-    const dim3 grid(a.splits * a.p.nkh * tiles, a.rows);
-    if (a.p.q8) launch_nb<true>(a, grid, s);
-    else launch_nb<false>(a, grid, s);
+    a.part = reinterpret_cast<float *>(a.ml + (uint64_t)a.grid * 2u * kHeads);
+    if (a.p.q8) launch_nb<true>(a, s);
+    else launch_nb<false>(a, s);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.splits == 1u) return e;
-    k_attn_paged_merge<<<dim3(a.nqh, a.rows), (a.p.hd + 63u) / 64u * 64u, 0, s>>>(a);
+    if (e != hipSuccess || a.workgroups == 0u) return e;
+    k_attn_paged_merge<<<dim3(a.nqh, a.rows), 256, 0, s>>>(a);
     return hipGetLastError();
 }
 

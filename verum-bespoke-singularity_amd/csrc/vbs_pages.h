@@ -87,11 +87,14 @@ struct PagedAttnArgs {
     const int32_t *seq, *lens;
     uint32_t rows, max_len, nqh, group;
     float scale;
-    uint32_t per_split, splits;  // units of a split, splits of the longest row
-    float2 *ml;                  // [rows][nqh][splits]: maximum (log2) and sum
-    float *part;                 // [rows][nqh][splits][hd]
+    int q_vec;  // q's rows can be read 16 bytes at a time, eight elements of a head together
+    uint32_t workgroups;  // that share all rows' units; 0: one for each row and head
+    uint32_t grid;        // of the launch: some more where shares may end with their head (`aligned`)
+    int aligned;
+    float2 *ml;   // [grid][2][8]: maximum (log2) and sum of partial results
+    float *part;  // [grid][2][8][hd]
 };
-// Sets per_split and splits; the bytes of ml and part together (0: none needed).
+// Sets workgroups, grid and aligned; the bytes of ml and part together (0: none needed).
 size_t plan_attn_paged(PagedAttnArgs &a);
 hipError_t launch_attn_paged(PagedAttnArgs a, void *scratch, hipStream_t s);
 
