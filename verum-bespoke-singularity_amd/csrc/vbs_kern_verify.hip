@@ -11,8 +11,10 @@
 // number lies, there are `vocab` borders, and a sum in f32 would move them by as much as small
 // probabilities are wide. T = 0: the greatest logit (lowest place) has p = 1.
 //
-// Three launches: every row's maximum and sum by chunks; acceptance, from those, and what is
-// left in each chunk of the row to draw from; the chunk, and the place in it.
+// Three launches: every row's maximum and sum by chunks of 4096; acceptance, from those, and what
+// is left in each chunk of 1024 of the row to draw from; the chunk, and the place in it.
+// Bound: HBM and, beside it, the 64-bit vector unit (about 19 operations a logit) where the rows
+// are many and long; the three launches and their round trips where they are few.
 #include <math.h>
 
 #include "vbs_dev_common.h"
@@ -22,273 +24,364 @@ namespace vbs {
 
 namespace {
 
-constexpr uint32_t kChunk = 4096, kThreads = 256, kEach = kChunk / kThreads;
+constexpr uint32_t kThreads = 256, kWaves = 4, kGroups = 4;  // a lane takes kGroups times four neighbours
+constexpr uint32_t kChunk = 256 * kGroups;       // of a wave: what is left is summed by these
+constexpr uint32_t kRowChunk = kWaves * kChunk;  // of a workgroup: rows are summed by these
 
-// e^x for x <= 0 (and 0 for -inf, NaN for NaN).
-__device__ __forceinline__ double exp_neg(double x) { return exp(x); }
+typedef float vf4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ double block_sum(double v, double *w) {
-    v = wave_sum_d(v);
-    __syncthreads();
-    if ((threadIdx.x & 63u) == 0u) w[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (w[0] + w[1]) + (w[2] + w[3]);
+// 2^t for t <= 0 (0 far below, NaN for NaN): t = n + f, |f| <= 1/2, a polynomial that interpolates 2^f at the 12 Chebyshev
+// nodes (off by 2e-17 of the value, beside the roundings'), times 2^n.
+__device__ __forceinline__ double exp2_neg(double t) {
+    t = t < -1100.0 ? -1100.0 : t;
+    const double r = t + 0x1.8p52;
+    const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, r);
+    const double f = t - (r - 0x1.8p52);
+    double p = 0x1.e9ec1fcb69a7fp-32;
+    p = fma(p, f, 0x1.e6228acd1c6e5p-28);
+    p = fma(p, f, 0x1.b524ebd13a55fp-24);
+    p = fma(p, f, 0x1.62bfc2c86d700p-20);
+    p = fma(p, f, 0x1.ffcbfc6da6ed1p-17);
+    p = fma(p, f, 0x1.430913112c61bp-13);
+    p = fma(p, f, 0x1.5d87fe78a3f9cp-10);
+    p = fma(p, f, 0x1.3b2ab6fb9f1a5p-7);
+    p = fma(p, f, 0x1.c6b08d704a0c6p-5);
+    p = fma(p, f, 0x1.ebfbdff82c5aep-3);
+    p = fma(p, f, 0x1.62e42fefa39efp-1);
+    p = fma(p, f, 1.0);
+    return __builtin_ldexp(p, n);
 }
 
-// The drafted tokens before the first that is none (an id outside the vocabulary).
+// The drafted tokens before the first that is none (an id outside the vocabulary); n is at most 64.
 __device__ __forceinline__ uint32_t draft_length(const VerifyArgs &a, uint32_t b) {
-    uint32_t n = 0;
-    while (n < a.n && (uint32_t)a.drafted[(uint64_t)b * a.n + n] < a.vocab) n++;
-    return n;
+    const uint32_t lane = threadIdx.x & 63u;
+    const bool none = lane >= a.n || (uint32_t)a.drafted[(uint64_t)b * a.n + lane] >= a.vocab;
+    const uint64_t at = __ballot(none);
+    return at ? (uint32_t)__ffsll((unsigned long long)at) - 1u : 64u;
 }
 __device__ __forceinline__ const float *row_of(const VerifyArgs &a, uint32_t b, uint32_t r) {
     return r <= a.n ? a.logits + ((uint64_t)b * (a.n + 1u) + r) * a.stride
                     : a.draft + ((uint64_t)b * a.n + (r - a.n - 1u)) * a.draft_stride;
 }
+// Four neighbouring logits from e on; -inf behind the last.
+__device__ __forceinline__ vf4 four(const VerifyArgs &a, const float *x, uint32_t e) {
+    if (a.vec && e + 4u <= a.vocab) return *reinterpret_cast<const vf4 *>(x + e);
+    vf4 v;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) v[j] = x[min(e + j, a.vocab - 1u)];
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) v[j] = e + j < a.vocab ? v[j] : -INFINITY;
+    return v;
+}
 
 }  // namespace
 
-// grid (chunks, rows of a sequence, sequences)
+// grid (chunks of 4096, rows of a sequence, sequences)
+template <bool GREEDY>
 __global__ __launch_bounds__(kThreads) void k_verify_sum(VerifyArgs a) {
-    __shared__ double w[4];
-    __shared__ float top_w[4];
-    __shared__ int32_t at_w[4];
-    const uint32_t b = blockIdx.z, r = blockIdx.y, tid = threadIdx.x, c0 = blockIdx.x * kChunk;
-    const uint32_t n = draft_length(a, b);
-    if (r <= a.n ? r > n : r - a.n - 1u >= n) return;
+    __shared__ float tops[kWaves];
+    __shared__ uint32_t places[kWaves];
+    __shared__ double sums[kWaves];
+    const uint32_t b = blockIdx.z, r = blockIdx.y, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    const uint32_t c0 = blockIdx.x * kRowChunk + wave * kChunk;
     const float *x = row_of(a, b, r);
-    float v[kEach], top = -INFINITY;
-    int32_t at = 0x7FFFFFFF;
+    vf4 v[kGroups];
 #pragma unroll
-    for (uint32_t i = 0; i < kEach; i++) {
-        const uint32_t e = c0 + i * kThreads + tid;
-        v[i] = e < a.vocab ? x[e] : -INFINITY;
-        if (v[i] > top || (v[i] == top && (int32_t)e < at && e < a.vocab)) top = v[i], at = (int32_t)e;
-    }
-    for (uint32_t o = 32; o; o >>= 1) {
-        const float t = __shfl_xor(top, (int)o, 64);
-        const int32_t p = __shfl_xor(at, (int)o, 64);
-        if (t > top || (t == top && p < at)) top = t, at = p;
-    }
-    if ((tid & 63u) == 0u) top_w[tid >> 6] = top, at_w[tid >> 6] = at;
-    __syncthreads();
-    top = top_w[0], at = at_w[0];
-    for (uint32_t i = 1; i < 4; i++)
-        if (top_w[i] > top || (top_w[i] == top && at_w[i] < at)) top = top_w[i], at = at_w[i];
+    for (uint32_t i = 0; i < kGroups; i++) v[i] = four(a, x, c0 + i * 256u + lane * 4u);
+    const uint32_t n = draft_length(a, b);
+    if (r <= a.n ? r > n : r - a.n - 1u >= n) return;  // (a row behind the draft's end)
     const uint64_t to = ((uint64_t)b * (2u * a.n + 1u) + r) * a.chunks + blockIdx.x;
-    double sum = 0.0;
-    if (a.temp > 0.f) {
-        const double rt = 1.0 / (double)a.temp, ref = top == -INFINITY ? 0.0 : (double)top;
+    float top = -INFINITY;
+    if constexpr (GREEDY) {
+        uint32_t at = 0xFFFFFFFFu;
 #pragma unroll
-        for (uint32_t i = 0; i < kEach; i++) sum += exp_neg(((double)v[i] - ref) * rt);
-        sum = block_sum(sum, w);
+        for (uint32_t i = 0; i < kGroups; i++)
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const uint32_t e = c0 + i * 256u + lane * 4u + j;
+                if (e < a.vocab && (v[i][j] > top || (v[i][j] == top && e < at))) top = v[i][j], at = e;
+            }
+        for (uint32_t o = 32; o; o >>= 1) {
+            const float t = __shfl_xor(top, (int)o, 64);
+            const uint32_t p = __shfl_xor(at, (int)o, 64);
+            if (t > top || (t == top && p < at)) top = t, at = p;
+        }
+        if (lane == 0u) tops[wave] = top, places[wave] = at;
+        __syncthreads();
+        if (tid) return;
+        for (uint32_t w = 1; w < kWaves; w++)
+            if (tops[w] > top || (tops[w] == top && places[w] < at)) top = tops[w], at = places[w];
+        a.tops[to] = top, a.arg[to] = (int32_t)at;
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < kGroups; i++)
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) top = fmaxf(top, v[i][j]);
+        top = wave_max(top);
+        if (lane == 0u) tops[wave] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        const double ref = top == -INFINITY ? 0.0 : (double)top;
+        double s[2] = {0.0, 0.0};
+#pragma unroll
+        for (uint32_t i = 0; i < kGroups; i++)
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) s[j & 1u] += exp2_neg(((double)v[i][j] - ref) * a.rate);
+        const double sum = wave_sum_d(s[0] + s[1]);
+        if (lane == 0u) sums[wave] = sum;
+        __syncthreads();
+        if (tid == 0u) a.tops[to] = top, a.sums[to] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     }
-    if (tid == 0u) a.tops[to] = top, a.arg[to] = at, a.sums[to] = sum;
 }
 
-// What row r of a sequence sums to, by a wave: its maximum, its sum relative to it, the maximum's place.
+// What a row sums to: its maximum, its sum relative to it, the maximum's place (temperature 0).
 struct RowSum {
     float top;
-    double sum;
     int32_t at;
+    double sum;
 };
-__device__ __forceinline__ RowSum row_sum(const VerifyArgs &a, uint32_t b, uint32_t r, uint32_t lane) {
+// Of row r by `width` neighbouring lanes (a power of two, up to 64), `i` the lane among them.
+__device__ __forceinline__ RowSum row_sum(const VerifyArgs &a, uint32_t b, uint32_t r, uint32_t i, uint32_t width) {
     const uint64_t from = ((uint64_t)b * (2u * a.n + 1u) + r) * a.chunks;
-    RowSum s{-INFINITY, 0.0, 0x7FFFFFFF};
-    for (uint32_t i = lane; i < a.chunks; i += 64u) {
-        const float t = a.tops[from + i];
-        const int32_t p = a.arg[from + i];
-        if (t > s.top || (t == s.top && p < s.at)) s.top = t, s.at = p;
-    }
-    for (uint32_t o = 32; o; o >>= 1) {
-        const float t = __shfl_xor(s.top, (int)o, 64);
-        const int32_t p = __shfl_xor(s.at, (int)o, 64);
-        if (t > s.top || (t == s.top && p < s.at)) s.top = t, s.at = p;
-    }
-    if (a.temp > 0.f) {
-        const double rt = 1.0 / (double)a.temp, ref = s.top == -INFINITY ? 0.0 : (double)s.top;
-        for (uint32_t i = lane; i < a.chunks; i += 64u) {
-            const float t = a.tops[from + i];
-            s.sum += a.sums[from + i] * exp_neg(((t == -INFINITY ? ref : (double)t) - ref) * rt);
+    RowSum s{-INFINITY, -1, 0.0};
+    if (a.temp == 0.f) {
+        uint32_t at = 0xFFFFFFFFu;
+        for (uint32_t k = i; k < a.chunks; k += width) {
+            const float t = a.tops[from + k];
+            const uint32_t p = (uint32_t)a.arg[from + k];
+            if (t > s.top || (t == s.top && p < at)) s.top = t, at = p;
         }
-        s.sum = wave_sum_d(s.sum);
+        for (uint32_t o = width >> 1; o; o >>= 1) {
+            const float t = __shfl_xor(s.top, (int)o, 64);
+            const uint32_t p = __shfl_xor(at, (int)o, 64);
+            if (t > s.top || (t == s.top && p < at)) s.top = t, at = p;
+        }
+        s.at = (int32_t)at;
+        return s;
     }
+    // (the sums of up to two chunks a lane are on their way with the maxima)
+    double first = 0.0, second = 0.0;
+    float t0 = -INFINITY, t1 = -INFINITY;
+    if (i < a.chunks) t0 = a.tops[from + i], first = a.sums[from + i];
+    if (i + width < a.chunks) t1 = a.tops[from + i + width], second = a.sums[from + i + width];
+    s.top = fmaxf(t0, t1);
+    for (uint32_t k = i + 2u * width; k < a.chunks; k += width) s.top = fmaxf(s.top, a.tops[from + k]);
+    for (uint32_t o = width >> 1; o; o >>= 1) s.top = fmaxf(s.top, __shfl_xor(s.top, (int)o, 64));
+    const double ref = s.top == -INFINITY ? 0.0 : (double)s.top;
+    auto part = [&](float t, double v) { return t == -INFINITY && !(v != v) ? 0.0 : v * exp2_neg(((double)t - ref) * a.rate); };
+    s.sum = part(t0, first) + part(t1, second);
+    for (uint32_t k = i + 2u * width; k < a.chunks; k += width) s.sum += part(a.tops[from + k], a.sums[from + k]);
+    for (uint32_t o = width >> 1; o; o >>= 1) s.sum += __shfl_xor(s.sum, (int)o, 64);
     return s;
 }
 
 // What is left to draw from: r(x) of the row the draft stopped at.
 struct Left {
     const float *x, *y;  // the target's row; the draft's, or NULL
-    double rt, top, rsum, ytop, yrsum;
+    double top, rsum, ytop, yrsum;
     int32_t without;  // the token of a certain draft that was refused, or -1
-    __device__ __forceinline__ void at(uint32_t e, double &p, double &less) const {
-        p = exp_neg(((double)x[e] - top) * rt) * rsum;
+    __device__ __forceinline__ void at(const VerifyArgs &a, uint32_t e, float lx, float ly, double &p, double &less) const {
+        p = exp2_neg(((double)lx - top) * a.rate) * rsum;
         less = p;
-        if (y) less = fmax(p - exp_neg(((double)y[e] - ytop) * rt) * yrsum, 0.0);
+        if (y) less = fmax(p - exp2_neg(((double)ly - ytop) * a.rate) * yrsum, 0.0);
         if ((int32_t)e == without) less = 0.0;
     }
 };
 
-// grid (chunks, sequences)
+// grid (chunks of 1024 / 4, sequences)
 __global__ __launch_bounds__(kThreads) void k_verify_accept(VerifyArgs a) {
-    __shared__ double w[4];
     __shared__ RowSum rows[2 * kMaxDraft + 1];
     __shared__ uint32_t stop_w;
-    const uint32_t b = blockIdx.y, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, c0 = blockIdx.x * kChunk;
-    const uint32_t n = draft_length(a, b), with = a.draft ? n : 0u;
-    for (uint32_t i = wave; i < n + 1u + with; i += 4u) {
-        const uint32_t r = i <= n ? i : a.n + 1u + (i - n - 1u);
-        const RowSum s = row_sum(a, b, r, lane);
-        if (lane == 0u) rows[i] = s;
-    }
-    if (tid == 0u) stop_w = n;
-    __syncthreads();
-    const double rt = a.temp > 0.f ? 1.0 / (double)a.temp : 0.0;
+    const uint32_t b = blockIdx.y, tid = threadIdx.x, lane = tid & 63u;
+    const uint32_t n = draft_length(a, b), count = n + 1u + (a.draft ? n : 0u);
+    uint32_t width = 4u;
+    while (width < 64u && width < a.chunks) width *= 2u;
+    int32_t token = 0;
+    float u = 0.f, lx = 0.f, ly = 0.f;
     if (tid < n) {
-        const uint32_t x = (uint32_t)a.drafted[(uint64_t)b * a.n + tid];
-        bool yes;
-        if (a.temp > 0.f) {
-            const double p = exp_neg(((double)row_of(a, b, tid)[x] - (double)rows[tid].top) * rt) / rows[tid].sum;
-            double q = 1.0;
-            if (a.draft) q = exp_neg(((double)row_of(a, b, a.n + 1u + tid)[x] - (double)rows[n + 1u + tid].top) * rt) / rows[n + 1u + tid].sum;
-            yes = (double)a.u[(uint64_t)b * (a.n + 1u) + tid] * q < p;
+        token = a.drafted[(uint64_t)b * a.n + tid];
+        u = a.u[(uint64_t)b * (a.n + 1u) + tid];
+        lx = row_of(a, b, tid)[token];
+        if (a.draft) ly = row_of(a, b, a.n + 1u + tid)[token];
+    }
+    for (uint32_t i0 = 0; i0 < count; i0 += kThreads / width) {
+        const uint32_t i = i0 + tid / width, in = min(i, count - 1u);  // (all lanes work together)
+        const RowSum s = row_sum(a, b, in <= n ? in : a.n + in - n, tid & (width - 1u), width);
+        if ((tid & (width - 1u)) == 0u && i < count) rows[i] = s;
+    }
+    __syncthreads();
+    if (tid < 64u) {
+        bool yes = tid >= n;
+        if (yes) {
+        } else if (a.temp > 0.f) {
+            // u q < p, both sides times the two sums
+            const RowSum p = rows[tid], q = a.draft ? rows[n + 1u + tid] : RowSum{0.f, 0, 1.0};
+            const double qx = a.draft ? exp2_neg(((double)ly - (double)q.top) * a.rate) : 1.0;
+            yes = (double)u * qx * p.sum < exp2_neg(((double)lx - (double)p.top) * a.rate) * q.sum;
         } else {
-            yes = rows[tid].at == (int32_t)x && a.u[(uint64_t)b * (a.n + 1u) + tid] < 1.f;
+            yes = rows[tid].at == token && u < 1.f;
         }
-        if (!yes) atomicMin(&stop_w, tid);
+        const uint64_t no = __ballot(!yes);
+        if (tid == 0u) stop_w = no ? (uint32_t)__ffsll((unsigned long long)no) - 1u : n;
     }
     __syncthreads();
     const uint32_t stop = stop_w;
     const bool refused = stop < n;
     if (a.temp == 0.f) {
-        if (blockIdx.x == 0u) {
-            int32_t *out = a.tokens + (uint64_t)b * (a.n + 1u);
-            const int32_t at = rows[stop].at;
-            for (uint32_t i = tid; i <= a.n; i += kThreads)
-                out[i] = i < stop ? a.drafted[(uint64_t)b * a.n + i] : i == stop && (uint32_t)at < a.vocab ? at : -1;
-            if (tid == 0u) a.accepted[b] = (int32_t)stop;
-        }
+        const int32_t at = rows[stop].at;
+        for (uint32_t i = tid; i <= a.n; i += kThreads)
+            a.tokens[(uint64_t)b * (a.n + 1u) + i] = i < stop ? a.drafted[(uint64_t)b * a.n + i] : i == stop && (uint32_t)at < a.vocab ? at : -1;
+        if (tid == 0u) a.accepted[b] = (int32_t)stop;
         return;
     }
     Left left;
     left.x = row_of(a, b, stop);
     left.y = refused && a.draft ? row_of(a, b, a.n + 1u + stop) : nullptr;
-    left.rt = rt;
     left.top = (double)rows[stop].top;
     left.rsum = 1.0 / rows[stop].sum;
     left.ytop = left.y ? (double)rows[n + 1u + stop].top : 0.0;
     left.yrsum = left.y ? 1.0 / rows[n + 1u + stop].sum : 0.0;
     left.without = refused && !a.draft ? a.drafted[(uint64_t)b * a.n + stop] : -1;
-    double all = 0.0, less = 0.0;
-    for (uint32_t i = 0; i < kEach; i++) {
-        const uint32_t e = c0 + i * kThreads + tid;
-        if (e >= a.vocab) break;
-        double p, l;
-        left.at(e, p, l);
-        all += p, less += l;
+    if (blockIdx.x == 0u && tid == 0u) {
+        a.stop[b] = (int32_t)(stop | (refused ? 1u << 16 : 0u));
+        double *st = a.stats + (uint64_t)b * 4u;
+        st[0] = left.top, st[1] = left.rsum, st[2] = left.ytop, st[3] = left.yrsum;
     }
-    all = block_sum(all, w);
-    less = block_sum(less, w);
-    if (tid == 0u) {
-        a.left[((uint64_t)b * 2u) * a.chunks + blockIdx.x] = less;
-        a.left[((uint64_t)b * 2u + 1u) * a.chunks + blockIdx.x] = all;
-        if (blockIdx.x == 0u) {
-            a.stop[b] = (int32_t)(stop | (refused ? 1u << 16 : 0u));
-            double *st = a.stats + (uint64_t)b * 4u;
-            st[0] = left.top, st[1] = left.rsum, st[2] = left.ytop, st[3] = left.yrsum;
+    const uint32_t chunk = blockIdx.x * kWaves + (tid >> 6);
+    if (chunk >= a.small) return;
+    vf4 x[kGroups], y[kGroups];
+#pragma unroll
+    for (uint32_t i = 0; i < kGroups; i++) x[i] = four(a, left.x, chunk * kChunk + i * 256u + lane * 4u);
+#pragma unroll
+    for (uint32_t i = 0; i < kGroups; i++) y[i] = left.y ? four(a, left.y, chunk * kChunk + i * 256u + lane * 4u) : vf4{0.f, 0.f, 0.f, 0.f};
+    double all = 0.0, less = 0.0;  // (behind the last, logits of -inf add 0)
+#pragma unroll
+    for (uint32_t i = 0; i < kGroups; i++)
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+            double p, l;
+            left.at(a, chunk * kChunk + i * 256u + lane * 4u + j, x[i][j], y[i][j], p, l);
+            all += p, less += l;
         }
+    all = wave_sum_d(all);
+    less = wave_sum_d(less);
+    if (lane == 0u) {
+        a.left[((uint64_t)b * 2u) * a.small + chunk] = less;
+        a.left[((uint64_t)b * 2u + 1u) * a.small + chunk] = all;
     }
 }
 
-// grid (sequences)
+__device__ __forceinline__ double scan_64(double v, uint32_t lane) {
+    for (uint32_t o = 1; o < 64u; o <<= 1) {
+        const double t = __shfl_up(v, (int)o, 64);
+        if (lane >= o) v += t;
+    }
+    return v;
+}
+
+// grid (sequences): every wave finds the chunk; a thread then takes four neighbours of it.
 __global__ __launch_bounds__(kThreads) void k_verify_pick(VerifyArgs a) {
-    __shared__ double scan[kThreads];
-    __shared__ uint32_t found, last;
-    const uint32_t b = blockIdx.x, tid = threadIdx.x;
+    __shared__ double ends[kWaves];
+    __shared__ uint32_t found[kWaves], last[kWaves];
+    const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     const uint32_t stop = (uint32_t)a.stop[b] & 0xFFFFu;
     const bool refused = (uint32_t)a.stop[b] >> 16;
     const double *st = a.stats + (uint64_t)b * 4u;
     Left left;
     left.x = row_of(a, b, stop);
     left.y = refused && a.draft ? row_of(a, b, a.n + 1u + stop) : nullptr;
-    left.rt = 1.0 / (double)a.temp;
     left.top = st[0], left.rsum = st[1], left.ytop = st[2], left.yrsum = st[3];
     left.without = refused && !a.draft ? a.drafted[(uint64_t)b * a.n + stop] : -1;
-    const double *sums = a.left + (uint64_t)b * 2u * a.chunks;
-    double total = 0.0;
-    for (uint32_t i = 0; i < a.chunks; i++) total += sums[i];
-    const bool whole = !(total > 0.0) && !(total != total);  // nothing left: the target's own
-    if (whole) {
-        sums += a.chunks;
-        total = 0.0;
-        for (uint32_t i = 0; i < a.chunks; i++) total += sums[i];
-    }
+    const double *sums = a.left + (uint64_t)b * 2u * a.small;
+    const float u = a.u[(uint64_t)b * (a.n + 1u) + a.n];
+    double less = 0.0, all = 0.0;
+    for (uint32_t k = lane; k < a.small; k += 64u) less += sums[k], all += sums[a.small + k];
+    less = wave_sum_d(less);
+    const bool whole = !(less > 0.0) && !(less != less);  // nothing left: the target's own
+    const double total = whole ? wave_sum_d(all) : less;
+    if (whole) sums += a.small;
     int32_t next = -1;
     if (total > 0.0) {
-        const double want = fmax((double)a.u[(uint64_t)b * (a.n + 1u) + a.n], 0.0) * total;
-        double before = 0.0, run = 0.0;
+        const double want = fmax((double)u, 0.0) * total;
+        // the first chunk that passes `want`, or the last that holds anything
+        double run = 0.0, before = 0.0;
         uint32_t chunk = 0;
-        bool in = false;
-        for (uint32_t i = 0; i < a.chunks && !in; i++) {
-            const double to = run + sums[i];
-            if (sums[i] > 0.0) chunk = i, before = run;
-            in = to > want;
-            run = to;
+        for (uint32_t k0 = 0; k0 < a.small; k0 += 64u) {
+            const double s = k0 + lane < a.small ? sums[k0 + lane] : 0.0, to = run + scan_64(s, lane);
+            const uint64_t some = __ballot(s > 0.0), past = __ballot(to > want && s > 0.0);
+            if (some) {
+                const uint32_t at = past ? (uint32_t)__ffsll((unsigned long long)past) - 1u : 63u - (uint32_t)__clzll((unsigned long long)some);
+                chunk = k0 + at;
+                before = __shfl(to - s, (int)at, 64);
+            }
+            if (past) break;
+            run = __shfl(to, 63, 64);
         }
-        if (tid == 0u) found = 0xFFFFFFFFu, last = 0u;
-        // each thread takes kEach neighbouring elements
-        const uint32_t e0 = chunk * kChunk + tid * kEach;
-        double mine = 0.0;
-        for (uint32_t i = 0; i < kEach; i++) {
-            if (e0 + i >= a.vocab) break;
+        const uint32_t e = chunk * kChunk + tid * 4u;
+        const vf4 x = four(a, left.x, e), y = left.y ? four(a, left.y, e) : vf4{0.f, 0.f, 0.f, 0.f};
+        double r[4], mine = 0.0;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
             double p, l;
-            left.at(e0 + i, p, l);
-            mine += whole ? p : l;
+            left.at(a, e + j, x[j], y[j], p, l);
+            mine += r[j] = whole ? p : l;
         }
-        scan[tid] = mine;
+        double at = scan_64(mine, lane);
+        if (lane == 63u) ends[wave] = at;
         __syncthreads();
-        double at = before;
-        for (uint32_t i = 0; i < tid; i++) at += scan[i];
-        for (uint32_t i = 0; i < kEach; i++) {
-            if (e0 + i >= a.vocab) break;
-            double p, l;
-            left.at(e0 + i, p, l);
-            const double r = whole ? p : l;
-            at += r;
-            if (r > 0.0) atomicMax(&last, e0 + i);
-            if (at > want) {
-                atomicMin(&found, e0 + i);
-                break;
+        at += before - mine;
+        for (uint32_t k = 0; k < wave; k++) at += ends[k];
+        constexpr uint32_t none = 0xFFFFFFFFu;
+        uint32_t here = none, some = none;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+            at += r[j];
+            if (r[j] > 0.0) {
+                some = e + j;
+                if (at > want && here == none) here = e + j;
             }
         }
+        const uint64_t past = __ballot(here != none), any = __ballot(some != none);
+        here = __shfl(here, past ? __ffsll((unsigned long long)past) - 1 : 0, 64);
+        some = __shfl(some, any ? 63 - __clzll((unsigned long long)any) : 0, 64);
+        if (lane == 0u) found[wave] = past ? here : none, last[wave] = any ? some : none;
         __syncthreads();
-        next = (int32_t)(found != 0xFFFFFFFFu ? found : last);
+        uint32_t pick = none;
+        for (uint32_t k = 0; k < kWaves; k++) pick = min(pick, found[k]);
+        if (pick == none)  // (the sums' roundings: the last that holds anything)
+            for (uint32_t k = 0; k < kWaves; k++)
+                if (last[k] != none) pick = last[k];
+        next = (int32_t)pick;
     }
-    int32_t *out = a.tokens + (uint64_t)b * (a.n + 1u);
     for (uint32_t i = tid; i <= a.n; i += kThreads)
-        out[i] = i < stop ? a.drafted[(uint64_t)b * a.n + i] : i == stop ? next : -1;
+        a.tokens[(uint64_t)b * (a.n + 1u) + i] = i < stop ? a.drafted[(uint64_t)b * a.n + i] : i == stop ? next : -1;
     if (tid == 0u) a.accepted[b] = (int32_t)stop;
 }
 
 size_t plan_verify(VerifyArgs &a) {
-    a.chunks = (a.vocab + kChunk - 1u) / kChunk;
+    a.chunks = (a.vocab + kRowChunk - 1u) / kRowChunk;
+    a.small = (a.vocab + kChunk - 1u) / kChunk;
     const uint64_t parts = (uint64_t)a.batch * (2u * a.n + 1u) * a.chunks;
-    return parts * 16u + (uint64_t)a.batch * (a.chunks * 16u + 40u);
+    return parts * 16u + (uint64_t)a.batch * (a.small * 16u + 40u);
 }
 
 hipError_t launch_verify(VerifyArgs a, void *scratch, hipStream_t s) {
     const uint64_t parts = (uint64_t)a.batch * (2u * a.n + 1u) * a.chunks;
     a.sums = static_cast<double *>(scratch);
     a.left = a.sums + parts;
-    a.stats = a.left + 2u * (uint64_t)a.batch * a.chunks;
+    a.stats = a.left + 2u * (uint64_t)a.batch * a.small;
     a.tops = reinterpret_cast<float *>(a.stats + 4u * (uint64_t)a.batch);
     a.arg = reinterpret_cast<int32_t *>(a.tops + parts);
     a.stop = a.arg + parts;
     if (a.temp == 0.f) a.draft = nullptr;
-    k_verify_sum<<<dim3(a.chunks, a.n + 1u + (a.draft ? a.n : 0u), a.batch), kThreads, 0, s>>>(a);
+    a.rate = a.temp > 0.f ? 1.4426950408889634074 / (double)a.temp : 0.0;  // log2 e / T
+    a.vec = !(((uintptr_t)a.logits & 15u) | (a.stride & 3u) | ((uintptr_t)a.draft & 15u) | (a.draft ? a.draft_stride & 3u : 0u));
+    const dim3 grid(a.chunks, a.n + 1u + (a.draft ? a.n : 0u), a.batch);
+    if (a.temp == 0.f) k_verify_sum<true><<<grid, kThreads, 0, s>>>(a);
+    else k_verify_sum<false><<<grid, kThreads, 0, s>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    k_verify_accept<<<dim3(a.chunks, a.batch), kThreads, 0, s>>>(a);
+    k_verify_accept<<<dim3(a.temp == 0.f ? 1u : a.chunks, a.batch), kThreads, 0, s>>>(a);
     e = hipGetLastError();
     if (e != hipSuccess || a.temp == 0.f) return e;
     k_verify_pick<<<a.batch, kThreads, 0, s>>>(a);

@@ -108,12 +108,14 @@ struct VerifyArgs {
     uint32_t batch, n, vocab;
     float temp;
     int32_t *accepted, *tokens;
-    uint32_t chunks;
+    double rate;      // log2 e / T
+    int vec;          // rows can be read 16 bytes at a time
+    uint32_t chunks, small;  // of a row, and of what is left of one
     double *sums;   // [batch][2 n + 1][chunks]: target rows, then draft rows
     float *tops;    // the same, the maxima
     int32_t *arg;   // the same, their places (temperature 0)
-    double *left;   // [batch][2][chunks]: what is left to draw from, and the target alone
-    double *stats;  // [batch][4]: log-space maximum and sum of the row drawn from, of the target and of the draft
+    double *left;   // [batch][2][small]: what is left to draw from, and the target alone
+    double *stats;  // [batch][4]: maximum and reciprocal sum of the row to draw from, of the target and of the draft
     int32_t *stop;  // [batch]: the row drawn from | refused << 16
 };
 size_t plan_verify(VerifyArgs &a);
