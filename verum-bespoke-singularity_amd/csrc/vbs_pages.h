@@ -73,10 +73,11 @@ struct PageRowsArgs {
     const float *k, *v;  // rows to store
     void *out_k, *out_v;  // rows to fill
     int out_f16;
+    int vec;  // eight elements of a row can be read or written 16 bytes at a time
     uint32_t stride;
 };
-hipError_t launch_page_store(const PageRowsArgs &a, hipStream_t s);
-hipError_t launch_page_load(const PageRowsArgs &a, hipStream_t s);
+hipError_t launch_page_store(PageRowsArgs a, hipStream_t s);
+hipError_t launch_page_load(PageRowsArgs a, hipStream_t s);
 
 struct PagedAttnArgs {
     PageArgs p;
