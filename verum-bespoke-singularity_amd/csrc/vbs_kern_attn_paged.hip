@@ -42,7 +42,7 @@ typedef float pf4 __attribute__((ext_vector_type(4)));
 typedef uint32_t pu4 __attribute__((ext_vector_type(4)));
 
 constexpr float kPagedLog2e = 1.44269504088896341f;
-constexpr uint32_t kHeads = 8, kWaves = 4;
+constexpr uint32_t kWaves = 4;
 constexpr int kWeightBits = 14;  // weights stand 2^14 high
 
 __device__ __forceinline__ float row_ror8(float v) {
@@ -233,8 +233,8 @@ __device__ __forceinline__ uint64_t row_begins(const PagedAttnArgs &a, uint32_t 
 
 // Workgroups of a CU, by the registers of a unit in flight (64 sequences of 4096 slots, 8 kv heads, Q8_0: heads of 32
 // take 43 us with four and 53 with two, of 128 111 with two and 121 with three, of 192 162 with two and 193 with one, of
-// 256, which spill with two, 249 with one and 338 with two).
-constexpr uint32_t per_cu(uint32_t nb) { return nb == 1u ? 4u : nb <= 7u ? 2u : 1u; }
+// 224 and 256, which spill with two, 220 and 249 with one, 230 and 338 with two).
+constexpr uint32_t per_cu(uint32_t nb) { return nb == 1u ? 4u : nb <= 6u ? 2u : 1u; }
 
 // A unit of K or of V on its way: its values as an operand takes them, and (Q8_0) its 32 NB scales, two in a dword, dword
 // 64 i + lane in ds[i].
@@ -331,25 +331,25 @@ __device__ __forceinline__ void slow_tile(const PagedAttnArgs &a, int32_t seq, u
     }
 }
 
-template <uint32_t NB>
+template <uint32_t NB, uint32_t CT>
 struct Shared {
-    float o[kWaves][kHeads][NB * 32u + 4u];
-    float m[kWaves][kHeads], l[kWaves][kHeads];
+    float o[kWaves][8u * CT][NB * 32u + 4u];
+    float m[kWaves][8u * CT], l[kWaves][8u * CT];
     uint32_t scales[kWaves][2][NB * 16u];
     uint32_t odd;
 };
 
-// Units [u0, u1) of a row and a kv head (and tile of eight of its q heads), by a workgroup: to out, or as a partial
+// Units [u0, u1) of a row and a kv head (and tile of its q heads), by a workgroup: to out, or as a partial
 // result if part is given. False, and nothing written, where sums are not finite (slow_units then does it).
-template <uint32_t NB, bool Q8>
-__device__ __forceinline__ bool attend_units(const PagedAttnArgs &a, Shared<NB> &sh, uint32_t row, uint32_t hx, int32_t seq, uint32_t len,
+template <uint32_t NB, bool Q8, uint32_t CT>
+__device__ __forceinline__ bool attend_units(const PagedAttnArgs &a, Shared<NB, CT> &sh, uint32_t row, uint32_t hx, int32_t seq, uint32_t len,
                                              uint32_t u0, uint32_t u1, float *part, float2 *ml) {
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     uint32_t lane = tid & 63u;
     asm volatile("" : "+v"(lane));  // (else what depends on the lane alone is kept from piece to piece: 60 registers more, and spills)
     const uint32_t g = lane >> 4, c = lane & 15u;
-    const uint32_t tiles = (a.group + kHeads - 1u) / kHeads, kvh = hx / tiles, tile = hx % tiles, hd = a.p.hd;
-    const uint32_t head0 = kvh * a.group + tile * kHeads, heads = min(kHeads, a.group - tile * kHeads);
+    const uint32_t tiles = (a.group + a.tile - 1u) / a.tile, kvh = hx / tiles, tile = hx % tiles, hd = a.p.hd;
+    const uint32_t head0 = kvh * a.group + tile * a.tile, heads = min(a.tile, a.group - tile * a.tile);
     const float *q0 = a.q + (uint64_t)row * a.q_stride + (uint64_t)head0 * hd;
     if (tid == 0) sh.odd = 0u;
 
@@ -367,10 +367,11 @@ __device__ __forceinline__ bool attend_units(const PagedAttnArgs &a, Shared<NB> 
 
     // q's parts: column c the head c & 7, its elements 32 b + 8 g ..
     const float low = c < 8u ? 0.f : -1.f;
-    ph8 qf[NB];
-    float unscale;
-    {
-        const uint32_t h = c & 7u;
+    ph8 qf[CT][NB];
+    float unscale[CT];
+#pragma unroll
+    for (uint32_t ct = 0; ct < CT; ct++) {
+        const uint32_t h = ct * 8u + (c & 7u);
         float x[NB][8], top = 0.f;
         if (a.q_vec) {
 #pragma unroll
@@ -403,46 +404,59 @@ __device__ __forceinline__ bool attend_units(const PagedAttnArgs &a, Shared<NB> 
         for (uint32_t b = 0; b < NB; b++) {
 #pragma unroll
             for (uint32_t e = 0; e < 8; e++) x[b][e] = __builtin_ldexpf(x[b][e], up);
-            qf[b] = parts(x[b], low);
+            qf[ct][b] = parts(x[b], low);
         }
-        unscale = __builtin_ldexpf(a.scale * kPagedLog2e, -up);
+        unscale[ct] = __builtin_ldexpf(a.scale * kPagedLog2e, -up);
     }
 
-    pf4 o[2 * NB];
+    pf4 o[CT][2 * NB];
+    float m[CT], l[CT];
 #pragma unroll
-    for (uint32_t i = 0; i < 2 * NB; i++) o[i] = pf4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
+    for (uint32_t t = 0; t < CT; t++) {
+#pragma unroll
+        for (uint32_t i = 0; i < 2 * NB; i++) o[t][i] = pf4{0.f, 0.f, 0.f, 0.f};
+        m[t] = -INFINITY, l[t] = 0.f;
+    }
     int top_e = -60;  // Q8_0: V's scales are below 2^top_e
     while (u < u1 && !lost) {
         const uint32_t next = u + kWaves;
         page = next < u1 ? page_at(a.p, seq, next) : 0;
         // scores: lane (g, c) holds slots 8 g + e of column c
-        float s[8];
+        float s[CT][8];
         if constexpr (Q8) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) s[e] = 0.f;
+            for (uint32_t t = 0; t < CT; t++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) s[t][e] = 0.f;
             k.spread(ks, lane);
 #pragma unroll
             for (uint32_t b = 0; b < NB; b++) {
                 const ph8 d = *reinterpret_cast<const ph8 *>(ks + b * 16u + g * 4u);
+                const ph8 k0 = int8_to_f16(k.x[b][0], k.x[b][1]), k1 = int8_to_f16(k.x[b][2], k.x[b][3]);
                 const pf4 zero = {0.f, 0.f, 0.f, 0.f};
-                const pf4 s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(int8_to_f16(k.x[b][0], k.x[b][1]), qf[b], zero, 0, 0, 0);
-                const pf4 s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(int8_to_f16(k.x[b][2], k.x[b][3]), qf[b], zero, 0, 0, 0);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    s[i] = fmaf(s0[i], (float)d[i], s[i]);
-                    s[4 + i] = fmaf(s1[i], (float)d[4 + i], s[4 + i]);
+                for (uint32_t t = 0; t < CT; t++) {
+                    const pf4 s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qf[t][b], zero, 0, 0, 0);
+                    const pf4 s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qf[t][b], zero, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        s[t][i] = fmaf(s0[i], (float)d[i], s[t][i]);
+                        s[t][4 + i] = fmaf(s1[i], (float)d[4 + i], s[t][4 + i]);
+                    }
                 }
             }
         } else {
-            pf4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll
-            for (uint32_t b = 0; b < NB; b++) {
-                s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, k.x[b]), qf[b], s0, 0, 0, 0);
-                s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, k.x[NB + b]), qf[b], s1, 0, 0, 0);
+            for (uint32_t t = 0; t < CT; t++) {
+                pf4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+#pragma unroll
+                for (uint32_t b = 0; b < NB; b++) {
+                    s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, k.x[b]), qf[t][b], s0, 0, 0, 0);
+                    s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, k.x[NB + b]), qf[t][b], s1, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[t][i] = s0[i], s[t][4 + i] = s1[i];
             }
-#pragma unroll
-            for (int i = 0; i < 4; i++) s[i] = s0[i], s[4 + i] = s1[i];
         }
         // the next unit's K is on its way during the softmax and the second product, its V during the next scores
         lost = page < 0;
@@ -451,13 +465,16 @@ __device__ __forceinline__ bool attend_units(const PagedAttnArgs &a, Shared<NB> 
         if (more) k.load(a.p.k + at, lane);
         const uint32_t mine = u * kUnit + g * 8u;  // the lane's first slot
         const bool tail = (u + 1u) * kUnit > len;
-        float top = m;
 #pragma unroll
-        for (uint32_t e = 0; e < 8; e++) s[e] = (s[e] + row_ror8(s[e])) * unscale;
+        for (uint32_t t = 0; t < CT; t++)
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) s[t][e] = (s[t][e] + row_ror8(s[t][e])) * unscale[t];
         if (tail) {  // what lies behind the last slot may be anything
 #pragma unroll
-            for (uint32_t e = 0; e < 8; e++)
-                if (mine + e >= len) s[e] = -INFINITY;
+            for (uint32_t t = 0; t < CT; t++)
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e++)
+                    if (mine + e >= len) s[t][e] = -INFINITY;
             auto kept = [&](uint32_t j) { return (j < len ? 0xFFFFu : 0u) | (j + 1u < len ? 0xFFFF0000u : 0u); };
             if constexpr (Q8) {
 #pragma unroll
@@ -471,19 +488,24 @@ __device__ __forceinline__ bool attend_units(const PagedAttnArgs &a, Shared<NB> 
                 }
             }
         }
+        // weights, in place of the scores
+        float keep[CT];
 #pragma unroll
-        for (uint32_t e = 0; e < 8; e++) top = fmaxf(top, s[e]);
-        top = over_groups_max(top);
-        const float ref = top == -INFINITY ? 0.f : top;
-        float p[8], sum = 0.f;
+        for (uint32_t t = 0; t < CT; t++) {
+            float top = m[t], sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            p[e] = __builtin_amdgcn_exp2f(s[e] - ref);
-            sum += p[e];
+            for (uint32_t e = 0; e < 8; e++) top = fmaxf(top, s[t][e]);
+            top = over_groups_max(top);
+            const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                s[t][e] = __builtin_amdgcn_exp2f(s[t][e] - ref);
+                sum += s[t][e];
+            }
+            keep[t] = __builtin_amdgcn_exp2f(m[t] - ref);
+            l[t] = fmaf(l[t], keep[t], sum);
+            m[t] = top;
         }
-        float keep = __builtin_amdgcn_exp2f(m - ref);
-        l = fmaf(l, keep, sum);
-        m = top;
         if constexpr (Q8) {
             uint32_t e5 = 0u;
 #pragma unroll
@@ -491,56 +513,70 @@ __device__ __forceinline__ bool attend_units(const PagedAttnArgs &a, Shared<NB> 
             e5 = wave_butterfly(e5, [](uint32_t x, uint32_t y) { return max(x, y); });
             const int e = __builtin_amdgcn_readfirstlane((int)min(e5 >> 10, 30u)) - 14;
             if (e > top_e) {
-                keep = __builtin_ldexpf(keep, top_e - e);
+#pragma unroll
+                for (uint32_t t = 0; t < CT; t++) keep[t] = __builtin_ldexpf(keep[t], top_e - e);
                 top_e = e;
             }
         }
-        if (__any(keep != 1.f)) {
+        // 2^14 high (Q8_0: less what V's scales may add)
+        const float raise = __builtin_ldexpf(1.f, kWeightBits - (Q8 ? top_e : 0));
 #pragma unroll
-            for (uint32_t i = 0; i < 2 * NB; i++)
+        for (uint32_t t = 0; t < CT; t++) {
+            if (__any(keep[t] != 1.f)) {
 #pragma unroll
-                for (int r = 0; r < 4; r++) o[i][r] *= keep;
+                for (uint32_t i = 0; i < 2 * NB; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) o[t][i][r] *= keep[t];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) s[t][e] *= raise;
         }
         if constexpr (Q8) {
             v.spread(vs, lane);
-            const float raise = __builtin_ldexpf(1.f, kWeightBits - top_e);
-#pragma unroll
-            for (int e = 0; e < 8; e++) p[e] *= raise;
 #pragma unroll
             for (uint32_t b = 0; b < NB; b++) {
                 const ph8 d = *reinterpret_cast<const ph8 *>(vs + b * 16u + g * 4u);
-                float x[8];
+                const ph8 v0 = int8_to_f16(v.x[b][0], v.x[b][1]), v1 = int8_to_f16(v.x[b][2], v.x[b][3]);
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = fmaf(p[e], (float)d[e], 0.f);
-                const ph8 w = parts(x, low);
-                o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(int8_to_f16(v.x[b][0], v.x[b][1]), w, o[2 * b], 0, 0, 0);
-                o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(int8_to_f16(v.x[b][2], v.x[b][3]), w, o[2 * b + 1], 0, 0, 0);
+                for (uint32_t t = 0; t < CT; t++) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = fmaf(s[t][e], (float)d[e], 0.f);
+                    const ph8 w = parts(x, low);
+                    o[t][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, w, o[t][2 * b], 0, 0, 0);
+                    o[t][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, w, o[t][2 * b + 1], 0, 0, 0);
+                }
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) p[e] *= (float)(1 << kWeightBits);
-            const ph8 w = parts(p, low);
+            for (uint32_t t = 0; t < CT; t++) {
+                const ph8 w = parts(s[t], low);
 #pragma unroll
-            for (uint32_t i = 0; i < 2 * NB; i++)
-                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, v.x[i]), w, o[i], 0, 0, 0);
+                for (uint32_t i = 0; i < 2 * NB; i++)
+                    o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, v.x[i]), w, o[t][i], 0, 0, 0);
+            }
         }
         if (more) v.load(a.p.v + at, lane);
         u = next;
     }
-    l = over_groups_sum(l);
     const float down = __builtin_ldexpf(1.f, (Q8 ? top_e : 0) - kWeightBits);
-    bool fine = fabsf(l) < INFINITY;
+    bool fine = true;
 #pragma unroll
-    for (uint32_t i = 0; i < 2 * NB; i++) {
+    for (uint32_t t = 0; t < CT; t++) {
+        const float sum = over_groups_sum(l[t]);
+        bool good = fabsf(sum) < INFINITY;
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            o[i][r] = (o[i][r] + row_ror8(o[i][r])) * down;
-            fine = fine && fabsf(o[i][r]) < INFINITY;
+        for (uint32_t i = 0; i < 2 * NB; i++) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                o[t][i][r] = (o[t][i][r] + row_ror8(o[t][i][r])) * down;
+                good = good && fabsf(o[t][i][r]) < INFINITY;
+            }
+            if (c < 8u) *reinterpret_cast<pf4 *>(&sh.o[wave][t * 8u + c][i * 16u + g * 4u]) = o[t][i];
         }
-        if (c < 8u) *reinterpret_cast<pf4 *>(&sh.o[wave][c][i * 16u + g * 4u]) = o[i];
+        if (g == 0u && c < 8u) sh.m[wave][t * 8u + c] = m[t], sh.l[wave][t * 8u + c] = sum;
+        fine = fine && (good || t * 8u + (c & 7u) >= heads);
     }
-    if (g == 0u && c < 8u) sh.m[wave][c] = m, sh.l[wave][c] = l;
-    fine = fine || (c & 7u) >= heads;
     __syncthreads();  // (odd is 0)
     if ((lost || __any(!fine)) && lane == 0u) sh.odd = 1u;
     __syncthreads();
@@ -567,11 +603,11 @@ __device__ __forceinline__ bool attend_units(const PagedAttnArgs &a, Shared<NB> 
 }
 
 // The same in plain f32.
-template <uint32_t NB, bool Q8>
-__device__ __forceinline__ void slow_units(const PagedAttnArgs &a, Shared<NB> &sh, uint32_t row, uint32_t hx, int32_t seq, uint32_t len,
+template <uint32_t NB, bool Q8, uint32_t CT>
+__device__ __forceinline__ void slow_units(const PagedAttnArgs &a, Shared<NB, CT> &sh, uint32_t row, uint32_t hx, int32_t seq, uint32_t len,
                                            uint32_t u0, uint32_t u1, float *part, float2 *ml) {
-    const uint32_t tiles = (a.group + kHeads - 1u) / kHeads, kvh = hx / tiles, tile = hx % tiles, hd = a.p.hd, tid = threadIdx.x;
-    const uint32_t head0 = kvh * a.group + tile * kHeads, heads = min(kHeads, a.group - tile * kHeads);
+    const uint32_t tiles = (a.group + a.tile - 1u) / a.tile, kvh = hx / tiles, tile = hx % tiles, hd = a.p.hd, tid = threadIdx.x;
+    const uint32_t head0 = kvh * a.group + tile * a.tile, heads = min(a.tile, a.group - tile * a.tile);
     const float *q0 = a.q + (uint64_t)row * a.q_stride + (uint64_t)head0 * hd;
     float *out = a.out + (uint64_t)row * a.out_stride + (uint64_t)head0 * hd;
     for (uint32_t h = 0; h < heads; h++) {
@@ -587,30 +623,30 @@ __device__ __forceinline__ void slow_units(const PagedAttnArgs &a, Shared<NB> &s
     }
 }
 
-// Rows of few units: a workgroup for each row and head, nothing to join. grid (kv heads x tiles of eight q heads, rows)
-template <uint32_t NB, bool Q8>
+// Rows of few units: a workgroup for each row and head, nothing to join. grid (kv heads x tiles of its q heads, rows)
+template <uint32_t NB, bool Q8, uint32_t CT>
 __global__ __launch_bounds__(256, per_cu(NB)) void k_attn_paged_whole(PagedAttnArgs a) {
-    __shared__ Shared<NB> sh;
+    __shared__ Shared<NB, CT> sh;
     const uint32_t row = blockIdx.y, hd = a.p.hd;
     const Row r = row_at(a, row);
     if (r.units) {
-        if (!attend_units<NB, Q8>(a, sh, row, blockIdx.x, r.seq, r.len, 0u, r.units, nullptr, nullptr))
-            slow_units<NB, Q8>(a, sh, row, blockIdx.x, r.seq, r.len, 0u, r.units, nullptr, nullptr);
+        if (!attend_units<NB, Q8, CT>(a, sh, row, blockIdx.x, r.seq, r.len, 0u, r.units, nullptr, nullptr))
+            slow_units<NB, Q8, CT>(a, sh, row, blockIdx.x, r.seq, r.len, 0u, r.units, nullptr, nullptr);
         return;
     }
-    const uint32_t tiles = (a.group + kHeads - 1u) / kHeads, kvh = blockIdx.x / tiles, tile = blockIdx.x % tiles;
-    const uint32_t n = min(kHeads, a.group - tile * kHeads) * hd;
-    float *out = a.out + (uint64_t)row * a.out_stride + (uint64_t)(kvh * a.group + tile * kHeads) * hd;
+    const uint32_t tiles = (a.group + a.tile - 1u) / a.tile, kvh = blockIdx.x / tiles, tile = blockIdx.x % tiles;
+    const uint32_t n = min(a.tile, a.group - tile * a.tile) * hd;
+    float *out = a.out + (uint64_t)row * a.out_stride + (uint64_t)(kvh * a.group + tile * a.tile) * hd;
     for (uint32_t i = threadIdx.x; i < n; i += 256u) out[i] = r.bad ? NAN : 0.f;
 }
 
 // All rows' units in equal shares, one a workgroup. What lies whole in a share is done with it; the piece of a row and head
 // that goes on in the next share is the workgroup's second partial result, one that began in an earlier share its first.
-template <uint32_t NB, bool Q8>
+template <uint32_t NB, bool Q8, uint32_t CT>
 __global__ __launch_bounds__(256, per_cu(NB)) void k_attn_paged(PagedAttnArgs a) {
-    __shared__ Shared<NB> sh;
+    __shared__ Shared<NB, CT> sh;
     __shared__ uint64_t sums[kWaves];
-    const uint32_t line = a.p.nkh * ((a.group + kHeads - 1u) / kHeads);  // heads (tiles) of a row
+    const uint32_t line = a.p.nkh * ((a.group + a.tile - 1u) / a.tile);  // heads (tiles) of a row
     Shares sh_;
     uint64_t at, end;
     Found f;
@@ -629,13 +665,13 @@ __global__ __launch_bounds__(256, per_cu(NB)) void k_attn_paged(PagedAttnArgs a)
         while (true) {
             const uint32_t u1 = r.units - u0 < left ? r.units : u0 + (uint32_t)left;
             const bool begun = u0 != 0u, whole = !begun && u1 == r.units;
-            const uint64_t slot = ((uint64_t)blockIdx.x * 2u + (begun ? 0u : 1u)) * kHeads;
+            const uint64_t slot = ((uint64_t)blockIdx.x * 2u + (begun ? 0u : 1u)) * a.tile;
             float *part = whole ? nullptr : a.part + slot * a.p.hd;
             const uint64_t bit = 1ull << min(n, 63u);
             if (round == 0u) {
-                if (!attend_units<NB, Q8>(a, sh, row, hx, r.seq, r.len, u0, u1, part, a.ml + slot)) odd |= bit;
+                if (!attend_units<NB, Q8, CT>(a, sh, row, hx, r.seq, r.len, u0, u1, part, a.ml + slot)) odd |= bit;
             } else if (odd & bit) {
-                slow_units<NB, Q8>(a, sh, row, hx, r.seq, r.len, u0, u1, part, a.ml + slot);
+                slow_units<NB, Q8, CT>(a, sh, row, hx, r.seq, r.len, u0, u1, part, a.ml + slot);
             }
             left -= u1 - u0;
             if (left == 0u || sh_.grain != 1u) break;
@@ -661,7 +697,7 @@ __global__ __launch_bounds__(256) void k_attn_paged_merge(PagedAttnArgs a) {
     __shared__ float w[256], so[256], sx[8];
     __shared__ uint64_t sums[4];
     const uint32_t head = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, hd = a.p.hd;
-    const uint32_t tiles = (a.group + kHeads - 1u) / kHeads, line = a.p.nkh * tiles, kvh = head / a.group, in = head % a.group;
+    const uint32_t tiles = (a.group + a.tile - 1u) / a.tile, line = a.p.nkh * tiles, kvh = head / a.group, in = head % a.group;
     const Row r = row_at(a, row);
     float *out = a.out + (uint64_t)row * a.out_stride + (uint64_t)head * hd;
     if (r.units == 0u) {
@@ -670,11 +706,11 @@ __global__ __launch_bounds__(256) void k_attn_paged_merge(PagedAttnArgs a) {
     }
     Shares sh;
     const uint64_t before = row_begins(a, line, row, sh, sums);
-    const uint64_t s0 = before * line + (kvh * tiles + in / kHeads) * padded(sh, r.units);
+    const uint64_t s0 = before * line + (kvh * tiles + in / a.tile) * padded(sh, r.units);
     const uint32_t w0 = (uint32_t)(s0 / sh.share), n = (uint32_t)((s0 + r.units - 1u) / sh.share) - w0 + 1u;
     if (n == 1u) return;
     // piece k: workgroup w0 + k's first partial result, for k = 0 its second
-    auto piece = [&](uint32_t k) { return ((uint64_t)(w0 + k) * 2u + (k ? 0u : 1u)) * kHeads + in % kHeads; };
+    auto piece = [&](uint32_t k) { return ((uint64_t)(w0 + k) * 2u + (k ? 0u : 1u)) * a.tile + in % a.tile; };
     const uint32_t width = (hd + 63u) & ~63u, groups = 256u / width, d = tid % width, grp = tid / width;
     const bool mine = d < hd && grp < groups;
     float x[kAhead];
@@ -718,11 +754,16 @@ __global__ __launch_bounds__(256) void k_attn_paged_merge(PagedAttnArgs a) {
     out[tid] = l == 0.f ? 0.f : o / l;
 }
 
+// Heads of up to so many blocks have 9 to 16 q heads of a kv head in one pass over its slots (two tiles of columns), whose
+// sums the registers of more do not hold: 64 sequences of 4096 slots, 96/8 heads of 128, 202 us for 373 in two passes
+// (F16), 143 for 217 (Q8_0).
+constexpr uint32_t kTwoTiles = 4;
 // Rows of at most so many units are not split: one of 512 slots takes 9.7 us (8 heads of 128, Q8_0), in shares 11.2.
 constexpr uint32_t kWholeUnits = 16;
 
 size_t plan_attn_paged(PagedAttnArgs &a) {
-    const uint32_t units = (a.max_len + kUnit - 1u) / kUnit, tiles = (a.group + kHeads - 1u) / kHeads;
+    a.tile = a.group > 8u && a.p.nb <= kTwoTiles ? 16u : 8u;
+    const uint32_t units = (a.max_len + kUnit - 1u) / kUnit, tiles = (a.group + a.tile - 1u) / a.tile;
     a.workgroups = 0;
     const uint32_t most = 256u * per_cu(a.p.nb);
     if (units <= kWholeUnits) return 0;
@@ -730,33 +771,40 @@ size_t plan_attn_paged(PagedAttnArgs &a) {
     a.workgroups = each < most ? (uint32_t)each : most;
     a.aligned = heads <= most;
     a.grid = a.workgroups + (a.aligned ? (uint32_t)heads : 0u);  // (each head's last share may be short)
-    return (uint64_t)a.grid * 2u * kHeads * (sizeof(float2) + 4ull * a.p.hd);
+    return (uint64_t)a.grid * 2u * a.tile * (sizeof(float2) + 4ull * a.p.hd);
 }
 
-template <uint32_t NB, bool Q8>
+template <uint32_t NB, bool Q8, uint32_t CT>
 static void launch_one(const PagedAttnArgs &a, hipStream_t s) {
-    const uint32_t tiles = (a.group + kHeads - 1u) / kHeads;
-    if (a.workgroups) k_attn_paged<NB, Q8><<<a.grid, 256, 0, s>>>(a);
-    else k_attn_paged_whole<NB, Q8><<<dim3(a.p.nkh * tiles, a.rows), 256, 0, s>>>(a);
+    const uint32_t tiles = (a.group + a.tile - 1u) / a.tile;
+    if (a.workgroups) k_attn_paged<NB, Q8, CT><<<a.grid, 256, 0, s>>>(a);
+    else k_attn_paged_whole<NB, Q8, CT><<<dim3(a.p.nkh * tiles, a.rows), 256, 0, s>>>(a);
+}
+template <uint32_t NB, bool Q8>
+static void launch_tile(const PagedAttnArgs &a, hipStream_t s) {
+    if constexpr (NB <= kTwoTiles) {
+        if (a.tile == 16u) return launch_one<NB, Q8, 2>(a, s);
+    }
+    launch_one<NB, Q8, 1>(a, s);
 }
 template <bool Q8>
 static void launch_nb(const PagedAttnArgs &a, hipStream_t s) {
     switch (a.p.nb) {
-        case 1: launch_one<1, Q8>(a, s); break;
-        case 2: launch_one<2, Q8>(a, s); break;
-        case 3: launch_one<3, Q8>(a, s); break;
-        case 4: launch_one<4, Q8>(a, s); break;
-        case 5: launch_one<5, Q8>(a, s); break;
-        case 6: launch_one<6, Q8>(a, s); break;
-        case 7: launch_one<7, Q8>(a, s); break;
-        default: launch_one<8, Q8>(a, s); break;
+        case 1: launch_tile<1, Q8>(a, s); break;
+        case 2: launch_tile<2, Q8>(a, s); break;
+        case 3: launch_tile<3, Q8>(a, s); break;
+        case 4: launch_tile<4, Q8>(a, s); break;
+        case 5: launch_tile<5, Q8>(a, s); break;
+        case 6: launch_tile<6, Q8>(a, s); break;
+        case 7: launch_tile<7, Q8>(a, s); break;
+        default: launch_tile<8, Q8>(a, s); break;
     }
 }
 
 hipError_t launch_attn_paged(PagedAttnArgs a, void *scratch, hipStream_t s) {
     a.q_vec = !(((uintptr_t)a.q & 15u) | (a.q_stride & 3u) | (a.p.hd & 7u));
     a.ml = static_cast<float2 *>(scratch);
-    a.part = reinterpret_cast<float *>(a.ml + (uint64_t)a.grid * 2u * kHeads);
+    a.part = reinterpret_cast<float *>(a.ml + (uint64_t)a.grid * 2u * a.tile);
     if (a.p.q8) launch_nb<true>(a, s);
     else launch_nb<false>(a, s);
     const hipError_t e = hipGetLastError();
