@@ -559,7 +559,7 @@ class Draft:
 
 
 @pytest.mark.parametrize("batch,n,vocab,pad", [(1, 1, 2, 0), (3, 4, 1000, 3), (2, 7, 32000, 0), (5, 0, 4096, 0), (4, 64, 257, 1),
-                                               (2, 3, 4097, 0), (1, 2, 131072, 0), (9, 5, 1, 0), (200, 3, 64, 2)])
+                                               (2, 3, 4097, 0), (1, 2, 131072, 0), (9, 5, 1, 0), (200, 3, 64, 2), (2, 2, 600001, 3)])
 @pytest.mark.parametrize("temp", [0.0, 0.7, 1.5])
 @pytest.mark.parametrize("draft", [True, False])
 def test_verify(dev, mem, batch, n, vocab, pad, temp, draft):

@@ -13,7 +13,7 @@
 //
 // Three launches: every row's maximum and sum by chunks of 4096; acceptance, from those, and what
 // is left in each chunk of 1024 of the row to draw from; the chunk, and the place in it.
-// Bound: HBM and, beside it, the 64-bit vector unit (about 19 operations a logit) where the rows
+// Bound: HBM and, beside it, the 64-bit vector unit (about 16 operations a logit) where the rows
 // are many and long; the three launches and their round trips where they are few.
 #include <math.h>
 
@@ -30,26 +30,47 @@ constexpr uint32_t kRowChunk = kWaves * kChunk;  // of a workgroup: rows are sum
 
 typedef float vf4 __attribute__((ext_vector_type(4)));
 
-// 2^t for t <= 0 (0 far below, NaN for NaN): t = n + f, |f| <= 1/2, a polynomial that interpolates 2^f at the 12 Chebyshev
-// nodes (off by 2e-17 of the value, beside the roundings'), times 2^n.
-__device__ __forceinline__ double exp2_neg(double t) {
-    t = t < -1100.0 ? -1100.0 : t;
+// 2^(j / 32); in LDS, where the 32 entries lie in banks of their own, less j 2^15 in their upper words (see power_of).
+__constant__ double kTwo[32] = {
+    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0, 0x1.172b83c7d517bp+0,
+    0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0, 0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0,
+    0x1.3dea64c123422p+0, 0x1.44e086061892dp+0, 0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0,
+    0x1.6247eb03a5585p+0, 0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0, 0x1.ae89f995ad3adp+0,
+    0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0, 0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0,
+    0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
+__device__ __forceinline__ void load_two(double *two) {
+    if (threadIdx.x < 32u)
+        two[threadIdx.x] = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, kTwo[threadIdx.x]) - ((uint64_t)threadIdx.x << 47));
+}
+
+// 2^(t / 32) for t <= 0 as two factors, from t = 32 n + j + f, |f| <= 1/2: w = 2^(n + j / 32) from the table, and the polynomial
+// that interpolates 2^(f / 32) at the six Chebyshev nodes, its first coefficient 1 (off by 1.4e-16 of the value,
+// beside the roundings'). From t = kFar down, and for NaN, 2^(kFar / 32). 13 operations in 64 bits with the sum, where a
+// polynomial for the whole octave took 22.
+constexpr double kFar = -32000.0;
+struct Power {
+    double w, p;
+};
+__device__ __forceinline__ Power power_of(double t, const double *two) {
+    t = fmax(t, kFar);
     const double r = t + 0x1.8p52;
-    const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, r);
+    const int32_t n = (int32_t)(uint32_t)__builtin_bit_cast(uint64_t, r);
     const double f = t - (r - 0x1.8p52);
-    double p = 0x1.e9ec1fcb69a7fp-32;
-    p = fma(p, f, 0x1.e6228acd1c6e5p-28);
-    p = fma(p, f, 0x1.b524ebd13a55fp-24);
-    p = fma(p, f, 0x1.62bfc2c86d700p-20);
-    p = fma(p, f, 0x1.ffcbfc6da6ed1p-17);
-    p = fma(p, f, 0x1.430913112c61bp-13);
-    p = fma(p, f, 0x1.5d87fe78a3f9cp-10);
-    p = fma(p, f, 0x1.3b2ab6fb9f1a5p-7);
-    p = fma(p, f, 0x1.c6b08d704a0c6p-5);
-    p = fma(p, f, 0x1.ebfbdff82c5aep-3);
-    p = fma(p, f, 0x1.62e42fefa39efp-1);
+    double p = 0x1.5d885e6ef14a6p-35;
+    p = fma(p, f, 0x1.3b2b301f1eb9cp-27);
+    p = fma(p, f, 0x1.c6b08d70380ddp-20);
+    p = fma(p, f, 0x1.ebfbdff7feebap-13);
+    p = fma(p, f, 0x1.62e42fefa39efp-6);
     p = fma(p, f, 1.0);
-    return __builtin_ldexp(p, n);
+    const uint64_t w = __builtin_bit_cast(uint64_t, two[n & 31]);  // (n = 32 m + j adds m to the exponent and j 2^15 beside it)
+    const uint32_t high = (uint32_t)(w >> 32) + ((uint32_t)n << 15);
+    return Power{__builtin_bit_cast(double, (uint64_t)high << 32 | (uint32_t)w), p};
+}
+// The product, and 0 from kFar down.
+__device__ __forceinline__ double exp2_neg(double t, const double *two) {
+    const Power x = power_of(t, two);
+    return t <= kFar ? 0.0 : x.w * x.p;
 }
 
 // The drafted tokens before the first that is none (an id outside the vocabulary); n is at most 64.
@@ -81,7 +102,7 @@ template <bool GREEDY>
 __global__ __launch_bounds__(kThreads) void k_verify_sum(VerifyArgs a) {
     __shared__ float tops[kWaves];
     __shared__ uint32_t places[kWaves];
-    __shared__ double sums[kWaves];
+    __shared__ double sums[kWaves], two[32];
     const uint32_t b = blockIdx.z, r = blockIdx.y, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     const uint32_t c0 = blockIdx.x * kRowChunk + wave * kChunk;
     const float *x = row_of(a, b, r);
@@ -119,6 +140,7 @@ __global__ __launch_bounds__(kThreads) void k_verify_sum(VerifyArgs a) {
             for (uint32_t j = 0; j < 4; j++) top = fmaxf(top, v[i][j]);
         top = wave_max(top);
         if (lane == 0u) tops[wave] = top;
+        load_two(two);
         __syncthreads();
         top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         const double ref = top == -INFINITY ? 0.0 : (double)top;
@@ -126,8 +148,18 @@ __global__ __launch_bounds__(kThreads) void k_verify_sum(VerifyArgs a) {
 #pragma unroll
         for (uint32_t i = 0; i < kGroups; i++)
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++) s[j & 1u] += exp2_neg(((double)v[i][j] - ref) * a.rate);
-        const double sum = wave_sum_d(s[0] + s[1]);
+            for (uint32_t j = 0; j < 4; j++) {
+                const Power x = power_of(((double)v[i][j] - ref) * a.rate, two);
+                s[j & 1u] = fma(x.w, x.p, s[j & 1u]);
+            }
+        bool nan = false;
+#pragma unroll
+        for (uint32_t i = 0; i < kGroups; i++)
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) nan = nan || v[i][j] != v[i][j];
+        double sum = wave_sum_d(s[0] + s[1]);
+        if (__any(nan) || top == INFINITY) sum = NAN;  // (no distribution)
+        else if (top == -INFINITY) sum = 0.0;
         if (lane == 0u) sums[wave] = sum;
         __syncthreads();
         if (tid == 0u) a.tops[to] = top, a.sums[to] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
@@ -141,7 +173,7 @@ struct RowSum {
     double sum;
 };
 // Of row r by `width` neighbouring lanes (a power of two, up to 64), `i` the lane among them.
-__device__ __forceinline__ RowSum row_sum(const VerifyArgs &a, uint32_t b, uint32_t r, uint32_t i, uint32_t width) {
+__device__ __forceinline__ RowSum row_sum(const VerifyArgs &a, uint32_t b, uint32_t r, uint32_t i, uint32_t width, const double *two) {
     const uint64_t from = ((uint64_t)b * (2u * a.n + 1u) + r) * a.chunks;
     RowSum s{-INFINITY, -1, 0.0};
     if (a.temp == 0.f) {
@@ -168,10 +200,11 @@ __device__ __forceinline__ RowSum row_sum(const VerifyArgs &a, uint32_t b, uint3
     for (uint32_t k = i + 2u * width; k < a.chunks; k += width) s.top = fmaxf(s.top, a.tops[from + k]);
     for (uint32_t o = width >> 1; o; o >>= 1) s.top = fmaxf(s.top, __shfl_xor(s.top, (int)o, 64));
     const double ref = s.top == -INFINITY ? 0.0 : (double)s.top;
-    auto part = [&](float t, double v) { return t == -INFINITY && !(v != v) ? 0.0 : v * exp2_neg(((double)t - ref) * a.rate); };
+    auto part = [&](float t, double v) { return t == -INFINITY && !(v != v) ? 0.0 : v * exp2_neg(((double)t - ref) * a.rate, two); };
     s.sum = part(t0, first) + part(t1, second);
     for (uint32_t k = i + 2u * width; k < a.chunks; k += width) s.sum += part(a.tops[from + k], a.sums[from + k]);
     for (uint32_t o = width >> 1; o; o >>= 1) s.sum += __shfl_xor(s.sum, (int)o, 64);
+    if (s.top == -INFINITY) s.sum = NAN;  // (no distribution)
     return s;
 }
 
@@ -180,10 +213,11 @@ struct Left {
     const float *x, *y;  // the target's row; the draft's, or NULL
     double top, rsum, ytop, yrsum;
     int32_t without;  // the token of a certain draft that was refused, or -1
+    const double *two;
     __device__ __forceinline__ void at(const VerifyArgs &a, uint32_t e, float lx, float ly, double &p, double &less) const {
-        p = exp2_neg(((double)lx - top) * a.rate) * rsum;
+        p = exp2_neg(((double)lx - top) * a.rate, two) * rsum;
         less = p;
-        if (y) less = fmax(p - exp2_neg(((double)ly - ytop) * a.rate) * yrsum, 0.0);
+        if (y) less = fmax(p - exp2_neg(((double)ly - ytop) * a.rate, two) * yrsum, 0.0);
         if ((int32_t)e == without) less = 0.0;
     }
 };
@@ -192,10 +226,13 @@ struct Left {
 __global__ __launch_bounds__(kThreads) void k_verify_accept(VerifyArgs a) {
     __shared__ RowSum rows[2 * kMaxDraft + 1];
     __shared__ uint32_t stop_w;
+    __shared__ double two[32];
     const uint32_t b = blockIdx.y, tid = threadIdx.x, lane = tid & 63u;
     const uint32_t n = draft_length(a, b), count = n + 1u + (a.draft ? n : 0u);
     uint32_t width = 4u;
     while (width < 64u && width < a.chunks) width *= 2u;
+    load_two(two);
+    __syncthreads();
     int32_t token = 0;
     float u = 0.f, lx = 0.f, ly = 0.f;
     if (tid < n) {
@@ -206,7 +243,7 @@ __global__ __launch_bounds__(kThreads) void k_verify_accept(VerifyArgs a) {
     }
     for (uint32_t i0 = 0; i0 < count; i0 += kThreads / width) {
         const uint32_t i = i0 + tid / width, in = min(i, count - 1u);  // (all lanes work together)
-        const RowSum s = row_sum(a, b, in <= n ? in : a.n + in - n, tid & (width - 1u), width);
+        const RowSum s = row_sum(a, b, in <= n ? in : a.n + in - n, tid & (width - 1u), width, two);
         if ((tid & (width - 1u)) == 0u && i < count) rows[i] = s;
     }
     __syncthreads();
@@ -216,8 +253,8 @@ __global__ __launch_bounds__(kThreads) void k_verify_accept(VerifyArgs a) {
         } else if (a.temp > 0.f) {
             // u q < p, both sides times the two sums
             const RowSum p = rows[tid], q = a.draft ? rows[n + 1u + tid] : RowSum{0.f, 0, 1.0};
-            const double qx = a.draft ? exp2_neg(((double)ly - (double)q.top) * a.rate) : 1.0;
-            yes = (double)u * qx * p.sum < exp2_neg(((double)lx - (double)p.top) * a.rate) * q.sum;
+            const double qx = a.draft ? exp2_neg(((double)ly - (double)q.top) * a.rate, two) : 1.0;
+            yes = (double)u * qx * p.sum < exp2_neg(((double)lx - (double)p.top) * a.rate, two) * q.sum;
         } else {
             yes = rows[tid].at == token && u < 1.f;
         }
@@ -242,6 +279,7 @@ __global__ __launch_bounds__(kThreads) void k_verify_accept(VerifyArgs a) {
     left.ytop = left.y ? (double)rows[n + 1u + stop].top : 0.0;
     left.yrsum = left.y ? 1.0 / rows[n + 1u + stop].sum : 0.0;
     left.without = refused && !a.draft ? a.drafted[(uint64_t)b * a.n + stop] : -1;
+    left.two = two;
     if (blockIdx.x == 0u && tid == 0u) {
         a.stop[b] = (int32_t)(stop | (refused ? 1u << 16 : 0u));
         double *st = a.stats + (uint64_t)b * 4u;
@@ -281,7 +319,7 @@ __device__ __forceinline__ double scan_64(double v, uint32_t lane) {
 
 // grid (sequences): every wave finds the chunk; a thread then takes four neighbours of it.
 __global__ __launch_bounds__(kThreads) void k_verify_pick(VerifyArgs a) {
-    __shared__ double ends[kWaves];
+    __shared__ double ends[kWaves], two[32];
     __shared__ uint32_t found[kWaves], last[kWaves];
     const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     const uint32_t stop = (uint32_t)a.stop[b] & 0xFFFFu;
@@ -292,6 +330,9 @@ __global__ __launch_bounds__(kThreads) void k_verify_pick(VerifyArgs a) {
     left.y = refused && a.draft ? row_of(a, b, a.n + 1u + stop) : nullptr;
     left.top = st[0], left.rsum = st[1], left.ytop = st[2], left.yrsum = st[3];
     left.without = refused && !a.draft ? a.drafted[(uint64_t)b * a.n + stop] : -1;
+    left.two = two;
+    load_two(two);
+    __syncthreads();
     const double *sums = a.left + (uint64_t)b * 2u * a.small;
     const float u = a.u[(uint64_t)b * (a.n + 1u) + a.n];
     double less = 0.0, all = 0.0;
@@ -374,7 +415,7 @@ hipError_t launch_verify(VerifyArgs a, void *scratch, hipStream_t s) {
     a.arg = reinterpret_cast<int32_t *>(a.tops + parts);
     a.stop = a.arg + parts;
     if (a.temp == 0.f) a.draft = nullptr;
-    a.rate = a.temp > 0.f ? 1.4426950408889634074 / (double)a.temp : 0.0;  // log2 e / T
+    a.rate = a.temp > 0.f ? 32.0 * 1.4426950408889634074 / (double)a.temp : 0.0;  // 32 log2 e / T
     a.vec = !(((uintptr_t)a.logits & 15u) | (a.stride & 3u) | ((uintptr_t)a.draft & 15u) | (a.draft ? a.draft_stride & 3u : 0u));
     const dim3 grid(a.chunks, a.n + 1u + (a.draft ? a.n : 0u), a.batch);
     if (a.temp == 0.f) k_verify_sum<true><<<grid, kThreads, 0, s>>>(a);

@@ -110,7 +110,7 @@ struct VerifyArgs {
     uint32_t batch, n, vocab;
     float temp;
     int32_t *accepted, *tokens;
-    double rate;      // log2 e / T
+    double rate;      // 32 log2 e / T
     int vec;          // rows can be read 16 bytes at a time
     uint32_t chunks, small;  // of a row, and of what is left of one
     double *sums;   // [batch][2 n + 1][chunks]: target rows, then draft rows
