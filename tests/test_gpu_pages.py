@@ -337,6 +337,51 @@ def test_attention_of_many_rows(dev, mem, t, rows, longest, nqh, nkh, hd):
     close(got[~bad], want[~bad], tol[~bad])
 
 
+@TYPES
+def test_a_row_in_many_pieces(dev, mem, t):
+    """One row and head over more shares than a merging workgroup has threads; every slot the same but for the last, so
+    the oracle is a formula."""
+    rng = np.random.default_rng(40)
+    n, hd = 262144 + 5, 32
+    r = Rows(rng, mem, dev, t, [64], 1, 1, hd, page=1024, junk=False)
+    r.c.table = np.full((1, n // 1024 + 1), int(r.c.table[0, 0]), np.int32)  # one page again and again
+    page = r.c.table[0, 0]
+    for j in range(1024):
+        r.c.pool.put("k", page, j, np.zeros((1, hd), np.float32))
+        r.c.pool.put("v", page, j, np.full((1, hd), 2.0 if j == (n - 1) % 1024 else 1.0, np.float32))
+    r.c.per_seq, r.lens, r.max_len = n // 1024 + 1, np.array([n], np.int32), n
+    k, v = (r.c.pool.get(w, page, (n - 1) % 1024) for w in "kv")
+    assert (k == 0).all()
+    got = r.run()
+    one = r.c.pool.get("v", page, 0)
+    hits = (n - 1) // 1024 + 1  # the slot comes once in every round of the page
+    want = (one * (n - hits) + v * hits) / n
+    # weights are equal and exact (2^0); n additions of a sum that ends at n, in f32, however they are grouped
+    close(got[0], want, 2 * n * S.F32 * np.abs(want) / 64)
+
+
+@TYPES
+def test_many_short_rows(dev, mem, t):
+    """Thousands of rows of few sequences, with empty ones and rows out of range, in one call."""
+    rng = np.random.default_rng(41)
+    rows, seqs, nkh, hd = 3000, 4, 2, 32
+    seq = rng.integers(0, seqs, rows)
+    lens = rng.integers(0, 3, rows)
+    lens[7], seq[7] = 700, 2
+    r = Rows(rng, mem, dev, t, lens, 2, nkh, hd, seq=seq, max_len=704, junk=False)
+    r.lens[11::50] = -1
+    r.lens[7] = 700
+    r.seq[13::50] = seqs
+    got = r.run()
+    bad = (r.lens < 0) | (r.seq >= seqs)
+    assert np.isnan(got[bad]).all() and (got[~bad & (r.lens == 0)] == 0).all()
+    kv = [[r.c.pool.rows(w, r.c.table[i], 700 if i == 2 else 2) for w in "kv"] for i in range(seqs)]
+    for i in np.flatnonzero(~bad & (r.lens > 0)):
+        k, v = kv[r.seq[i]]
+        n = r.lens[i]
+        close(got[i], *R.attend(r.q[i].reshape(2, hd).astype(np.float64), k[:n], v[:n], r.scale, 127 * 0.2 if t == V.Q8_0 else None))
+
+
 def test_many_pieces_that_are_not_finite(dev, mem):
     """Shares of more than 64 rows and heads, infinities in many of them: each is taken again by itself. A row of one slot
     is that slot's V, exactly."""

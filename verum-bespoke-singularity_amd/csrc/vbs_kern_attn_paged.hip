@@ -209,28 +209,6 @@ __device__ __forceinline__ bool find_row(const PagedAttnArgs &a, uint32_t line, 
     f.row = __builtin_amdgcn_readfirstlane(found.row), f.before = same(found.before);
     return true;
 }
-// The other way: where `row` begins.
-__device__ __forceinline__ uint64_t row_begins(const PagedAttnArgs &a, uint32_t line, uint32_t row, Shares &sh, uint64_t *sums) {
-    const uint32_t tid = threadIdx.x, lane = tid & 63u;
-    if (a.rows <= 64u) {
-        const uint32_t units = lane < a.rows ? row_at(a, lane).units : 0u;
-        sh = shares(a, a.rows == 1u ? __builtin_amdgcn_readfirstlane(units) : wave_total(units), line);
-        return row ? wave_total(lane < row ? padded(sh, units) : 0u) : 0u;
-    }
-    uint64_t all = 0, before = 0;
-    for (uint32_t k = tid; k < a.rows; k += 256u) {
-        const uint32_t u = row_at(a, k).units;
-        all += u;
-        if (k < row) before += u;
-    }
-    sh = shares(a, sum_of_256(all, sums), line);
-    if (sh.grain != 1u) {
-        before = 0;
-        for (uint32_t k = tid; k < row; k += 256u) before += padded(sh, row_at(a, k).units);
-    }
-    return sum_of_256(before, sums);
-}
-
 // Workgroups of a CU, by the registers of a unit in flight (64 sequences of 4096 slots, 8 kv heads, Q8_0: heads of 32
 // take 43 us with four and 53 with two, of 128 111 with two and 121 with three, of 192 162 with two and 193 with one, of
 // 224 and 256, which spill with two, 220 and 249 with one, 230 and 338 with two).
@@ -641,7 +619,8 @@ __global__ __launch_bounds__(256, per_cu(NB)) void k_attn_paged_whole(PagedAttnA
 }
 
 // All rows' units in equal shares, one a workgroup. What lies whole in a share is done with it; the piece of a row and head
-// that goes on in the next share is the workgroup's second partial result, one that began in an earlier share its first.
+// that goes on in the next share is the workgroup's second partial result, one that began in an earlier share its first. Of
+// the first kind there is one at most, which `joins` names, with the number of its pieces, for the merge.
 template <uint32_t NB, bool Q8, uint32_t CT>
 __global__ __launch_bounds__(256, per_cu(NB)) void k_attn_paged(PagedAttnArgs a) {
     __shared__ Shared<NB, CT> sh;
@@ -650,67 +629,80 @@ __global__ __launch_bounds__(256, per_cu(NB)) void k_attn_paged(PagedAttnArgs a)
     Shares sh_;
     uint64_t at, end;
     Found f;
-    if (!find_row(a, line, blockIdx.x, sh_, at, end, f, sums)) return;
-    const uint32_t row0 = f.row;
-    const Row first = row_at(a, row0);
-    const uint64_t in = at - f.before * line, long0 = padded(sh_, first.units);
-    const uint32_t hx0 = (uint32_t)(in / long0), u00 = (uint32_t)(in % long0);
-    // the share's pieces one after the other; in the second round, if there is one, those that were not finite (the 64th
-    // and all behind it together)
-    uint64_t odd = 0;
-    for (uint32_t round = 0; round < 2u; round++) {
-        Row r = first;
-        uint32_t row = row0, hx = hx0, u0 = u00, n = 0;
-        uint64_t left = end - at;
-        while (true) {
-            const uint32_t u1 = r.units - u0 < left ? r.units : u0 + (uint32_t)left;
-            const bool begun = u0 != 0u, whole = !begun && u1 == r.units;
-            const uint64_t slot = ((uint64_t)blockIdx.x * 2u + (begun ? 0u : 1u)) * a.tile;
-            float *part = whole ? nullptr : a.part + slot * a.p.hd;
-            const uint64_t bit = 1ull << min(n, 63u);
-            if (round == 0u) {
-                if (!attend_units<NB, Q8, CT>(a, sh, row, hx, r.seq, r.len, u0, u1, part, a.ml + slot)) odd |= bit;
-            } else if (odd & bit) {
-                slow_units<NB, Q8, CT>(a, sh, row, hx, r.seq, r.len, u0, u1, part, a.ml + slot);
+    uint32_t open_row = 0u, open_hx = 0u, pieces = 0u;
+    if (find_row(a, line, blockIdx.x, sh_, at, end, f, sums)) {
+        const uint32_t row0 = f.row;
+        const Row first = row_at(a, row0);
+        const uint64_t in = at - f.before * line, long0 = padded(sh_, first.units);
+        const uint32_t hx0 = (uint32_t)(in / long0), u00 = (uint32_t)(in % long0);
+        // the share's pieces one after the other; in the second round, if there is one, those that were not finite (the
+        // 64th and all behind it together)
+        uint64_t odd = 0;
+        for (uint32_t round = 0; round < 2u; round++) {
+            Row r = first;
+            uint32_t row = row0, hx = hx0, u0 = u00, n = 0;
+            uint64_t left = end - at;
+            while (true) {
+                const uint32_t u1 = r.units - u0 < left ? r.units : u0 + (uint32_t)left;
+                const bool begun = u0 != 0u, whole = !begun && u1 == r.units;
+                const uint64_t slot = ((uint64_t)blockIdx.x * 2u + (begun ? 0u : 1u)) * a.tile;
+                float *part = whole ? nullptr : a.part + slot * a.p.hd;
+                const uint64_t bit = 1ull << min(n, 63u);
+                if (!begun && !whole)
+                    open_row = row, open_hx = hx, pieces = 1u + (uint32_t)((r.units - u1 + sh_.share - 1u) / sh_.share);
+                if (round == 0u) {
+                    if (!attend_units<NB, Q8, CT>(a, sh, row, hx, r.seq, r.len, u0, u1, part, a.ml + slot)) odd |= bit;
+                } else if (odd & bit) {
+                    slow_units<NB, Q8, CT>(a, sh, row, hx, r.seq, r.len, u0, u1, part, a.ml + slot);
+                }
+                left -= u1 - u0;
+                if (left == 0u || sh_.grain != 1u) break;
+                n++;
+                u0 = 0u;
+                if (++hx == line) {
+                    hx = 0u;
+                    do r = row_at(a, ++row);
+                    while (r.units == 0u);
+                }
+                __syncthreads();
             }
-            left -= u1 - u0;
-            if (left == 0u || sh_.grain != 1u) break;
-            n++;
-            u0 = 0u;
-            if (++hx == line) {
-                hx = 0u;
-                do r = row_at(a, ++row);
-                while (r.units == 0u);
-            }
-            __syncthreads();
+            if (!odd) break;
         }
-        if (!odd) break;
+    }
+    const uint32_t tid = threadIdx.x;
+    if (tid == 0u) a.joins[blockIdx.x] = make_uint4(open_row, open_hx, pieces, 0u);
+    // rows without units: row w + gridDim t is thread t's of workgroup w to look at
+    if (blockIdx.x >= a.rows) return;
+    __syncthreads();
+    uint32_t *empty = reinterpret_cast<uint32_t *>(&sh.o[0][0][0]), &count = sh.odd;
+    if (tid == 0u) count = 0u;
+    __syncthreads();
+    const uint64_t mine = blockIdx.x + (uint64_t)gridDim.x * tid;
+    if (mine < a.rows) {
+        const Row r = row_at(a, (uint32_t)mine);
+        if (r.units == 0u) empty[atomicAdd(&count, 1u)] = (uint32_t)mine * 2u + r.bad;
+    }
+    __syncthreads();
+    for (uint32_t k = 0; k < count; k++) {
+        float *out = a.out + (uint64_t)(empty[k] >> 1) * a.out_stride;
+        for (uint32_t i = tid; i < a.nqh * a.p.hd; i += 256u) out[i] = empty[k] & 1u ? NAN : 0.f;
     }
 }
 
-// The pieces of the rows and heads that lie in several shares, joined, and the rows without units: grid (q heads, rows).
+// The pieces of a row and head that lie in several shares, joined: grid (the workgroups they begin in, q heads of a tile).
 // Threads of 256 / W groups (W: hd in whole waves) take every so many pieces of an element each; their first values are
 // on their way while the weights are formed.
 constexpr uint32_t kAhead = 8;
 
 __global__ __launch_bounds__(256) void k_attn_paged_merge(PagedAttnArgs a) {
     __shared__ float w[256], so[256], sx[8];
-    __shared__ uint64_t sums[4];
-    const uint32_t head = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, hd = a.p.hd;
-    const uint32_t tiles = (a.group + a.tile - 1u) / a.tile, line = a.p.nkh * tiles, kvh = head / a.group, in = head % a.group;
-    const Row r = row_at(a, row);
-    float *out = a.out + (uint64_t)row * a.out_stride + (uint64_t)head * hd;
-    if (r.units == 0u) {
-        if (tid < hd) out[tid] = r.bad ? NAN : 0.f;
-        return;
-    }
-    Shares sh;
-    const uint64_t before = row_begins(a, line, row, sh, sums);
-    const uint64_t s0 = before * line + (kvh * tiles + in / a.tile) * padded(sh, r.units);
-    const uint32_t w0 = (uint32_t)(s0 / sh.share), n = (uint32_t)((s0 + r.units - 1u) / sh.share) - w0 + 1u;
-    if (n == 1u) return;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, hd = a.p.hd, w0 = blockIdx.x, in = blockIdx.y;
+    const uint4 join = a.joins[w0];
+    const uint32_t n = join.z, tiles = (a.group + a.tile - 1u) / a.tile, kvh = join.y / tiles, h = join.y % tiles * a.tile + in;
+    if (n == 0u || h >= a.group) return;
+    float *out = a.out + (uint64_t)join.x * a.out_stride + (uint64_t)(kvh * a.group + h) * hd;
     // piece k: workgroup w0 + k's first partial result, for k = 0 its second
-    auto piece = [&](uint32_t k) { return ((uint64_t)(w0 + k) * 2u + (k ? 0u : 1u)) * a.tile + in % a.tile; };
+    auto piece = [&](uint32_t k) { return ((uint64_t)(w0 + k) * 2u + (k ? 0u : 1u)) * a.tile + in; };
     const uint32_t width = (hd + 63u) & ~63u, groups = 256u / width, d = tid % width, grp = tid / width;
     const bool mine = d < hd && grp < groups;
     float x[kAhead];
@@ -771,7 +763,7 @@ size_t plan_attn_paged(PagedAttnArgs &a) {
     a.workgroups = each < most ? (uint32_t)each : most;
     a.aligned = heads <= most;
     a.grid = a.workgroups + (a.aligned ? (uint32_t)heads : 0u);  // (each head's last share may be short)
-    return (uint64_t)a.grid * 2u * a.tile * (sizeof(float2) + 4ull * a.p.hd);
+    return (uint64_t)a.grid * (sizeof(uint4) + 2u * a.tile * (sizeof(float2) + 4ull * a.p.hd));
 }
 
 template <uint32_t NB, bool Q8, uint32_t CT>
@@ -803,13 +795,14 @@ static void launch_nb(const PagedAttnArgs &a, hipStream_t s) {
 
 hipError_t launch_attn_paged(PagedAttnArgs a, void *scratch, hipStream_t s) {
     a.q_vec = !(((uintptr_t)a.q & 15u) | (a.q_stride & 3u) | (a.p.hd & 7u));
-    a.ml = static_cast<float2 *>(scratch);
+    a.joins = static_cast<uint4 *>(scratch);
+    a.ml = reinterpret_cast<float2 *>(a.joins + a.grid);
     a.part = reinterpret_cast<float *>(a.ml + (uint64_t)a.grid * 2u * a.tile);
     if (a.p.q8) launch_nb<true>(a, s);
     else launch_nb<false>(a, s);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.workgroups == 0u) return e;
-    k_attn_paged_merge<<<dim3(a.nqh, a.rows), 256, 0, s>>>(a);
+    k_attn_paged_merge<<<dim3(a.grid, a.group < a.tile ? a.group : a.tile), 256, 0, s>>>(a);
     return hipGetLastError();
 }
 

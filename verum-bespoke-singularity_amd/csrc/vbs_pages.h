@@ -93,10 +93,11 @@ struct PagedAttnArgs {
     uint32_t grid;        // of the launch: some more where shares may end with their head (`aligned`)
     int aligned;
     uint32_t tile;  // q heads of a kv head that are taken together, 8 or 16
+    uint4 *joins;   // [grid]: row and head (tile) that begin in the share and go on, and their pieces (0: none)
     float2 *ml;     // [grid][2][tile]: maximum (log2) and sum of partial results
     float *part;    // [grid][2][tile][hd]
 };
-// Sets workgroups, grid, aligned and tile; the bytes of ml and part together (0: none needed).
+// Sets workgroups, grid, aligned and tile; the bytes of joins, ml and part together (0: none needed).
 size_t plan_attn_paged(PagedAttnArgs &a);
 hipError_t launch_attn_paged(PagedAttnArgs a, void *scratch, hipStream_t s);
 
