@@ -293,7 +293,7 @@ class Rows:
             if self.c.t == V.Q8_0 and n:
                 d = [self.c.pool.scales("v")[self.c.table[s, j // self.c.page], :, j % self.c.page // 32].reshape(self.nkh, -1, 32)[..., j % 32]
                      for j in range(n)]
-                vmax = 127.0 * float(np.max(np.array(d).view(np.float16).astype(np.float64)))
+                vmax = 127.0 * float(np.max(np.abs(np.array(d).view(np.float16).astype(np.float64))))
             o, e = R.attend(q[:self.nqh * self.hd].reshape(self.nqh, self.hd).astype(np.float64), k, v, self.scale, vmax)
             out.append(o)
             tol.append(e)
@@ -449,8 +449,9 @@ def test_scores_of_all_sizes(dev, mem, t, lens, nqh, nkh, hd):
     for f in (2.0 ** -90, 2.0 ** 90):
         r.q, r.scale = q * np.float32(f), float(np.float32(0.02 / f))
         close(r.run(), *r.want())
-    r.q, r.scale = q, 0.0
-    close(r.run(), *r.want())
+    for scale in (0.0, -0.03, 1e-30):
+        r.q, r.scale = q, float(np.float32(scale))
+        close(r.run(), *r.want())
 
 
 @TYPES
@@ -467,6 +468,32 @@ def test_small_weights_beside_a_great_one(dev, mem, t):
     r.q[:] = 0
     r.q[:, ::hd] = 1.0
     r.scale = 1.0
+    close(r.run(), *r.want())
+
+
+@TYPES
+def test_subnormal_values(dev, mem, t):
+    """K and V whose f16 (or whose scales) are subnormal, beside a q that makes scores of ordinary size of them."""
+    rng = np.random.default_rng(16)
+    hd = 64
+    r = Rows(rng, mem, dev, t, [300], 4, 1, hd, junk=False)
+    for j in range(300):
+        for w in "kv":
+            r.c.pool.put(w, *r.c.place(0, j), (rng.standard_normal((1, hd)) * 2e-5).astype(np.float32))
+    r.q = (rng.standard_normal(r.q.shape) * 1e4).astype(np.float32)
+    got = r.run()
+    want, tol = r.want()
+    assert np.abs(want).max() > 1e-7 and (tol < np.abs(want).max() / 100).all()
+    close(got, want, tol)
+
+
+def test_scales_of_both_signs(dev, mem):
+    """Pages that callers build themselves may hold negative scales."""
+    rng = np.random.default_rng(17)
+    r = Rows(rng, mem, dev, V.Q8_0, [200, 33], 8, 2, 64, junk=False)
+    for w in "kv":
+        d = r.c.pool.scales(w)
+        d ^= (rng.integers(0, 2, d.shape) << 15).astype(np.uint16)
     close(r.run(), *r.want())
 
 
@@ -666,8 +693,8 @@ def test_verify_far_logits(dev, mem):
 
 @TYPES
 def test_a_serving_step(dev, mem, t):
-    """A prompt into pages, read back for the attention of several tokens, drafted tokens stored and attended as rows
-    of their sequence, verified, the next step written over what was refused."""
+    """q and k rotated, a prompt into pages, read back for the attention of several tokens, drafted tokens stored and
+    attended as rows of their sequence, verified, the next step written over what was refused."""
     rng = np.random.default_rng(30)
     nqh, nkh, hd, page, past, n, vocab = 8, 2, 64, 32, 75, 4, 512
     kvd, qd = nkh * hd, nqh * hd
@@ -676,11 +703,15 @@ def test_a_serving_step(dev, mem, t):
     x = {w: rng.standard_normal((total, kvd)).astype(np.float32) for w in "kv"}
     px = {w: mem.up(x[w]) for w in "kv"}
     seq, at = mem.up(np.ones(total, np.int32)), mem.up(np.arange(total, dtype=np.int32))
+    dev.rope_axes(px["k"], kvd, 0, 0, 0, at, total, (hd // 2,), 0, 0, 0, 0, 0, nkh, nkh, hd, 10000.0)
+    x["k"] = dev.download(px["k"], (total, kvd), np.float32)
     dev.page_store(c.pages, 0, px["k"], px["v"], kvd, seq, at, past)                                     # the prompt
     off = 4 * past
     dev.page_store(c.pages, 0, px["k"] + off * kvd, px["v"] + off * kvd, kvd, seq + off, at + off, n)    # the draft
     q = (2 * rng.standard_normal((n, qd))).astype(np.float32)
     pq, out = mem.up(q), mem.zeros(n * qd)
+    dev.rope_axes(pq, qd, 0, 0, 0, at + off, n, (hd // 2,), 0, 0, 0, 0, 0, nqh, nkh, hd, 10000.0)
+    q = dev.download(pq, (n, qd), np.float32)
     lens = mem.up(np.arange(past + 1, total + 1, dtype=np.int32))
     dev.attention_paged(c.pages, 0, pq, qd, out, qd, seq, lens, n, 128, nqh, 0.125)
     got = dev.download(out, (n, nqh, hd), np.float32).astype(np.float64)
