@@ -706,11 +706,14 @@ __global__ __launch_bounds__(256) void k_attn_paged_merge(PagedAttnArgs a) {
     const uint32_t width = (hd + 63u) & ~63u, groups = 256u / width, d = tid % width, grp = tid / width;
     const bool mine = d < hd && grp < groups;
     float x[kAhead];
+    auto eight = [&](uint32_t from, uint32_t to) {
 #pragma unroll
-    for (uint32_t i = 0; i < kAhead; i++) {
-        const uint32_t k = grp + i * groups;
-        x[i] = mine && k < n ? a.part[piece(k) * hd + d] : 0.f;
-    }
+        for (uint32_t i = 0; i < kAhead; i++) {
+            const uint32_t k = from + i * groups;
+            x[i] = mine && k < to ? a.part[piece(k) * hd + d] : 0.f;
+        }
+    };
+    eight(grp, min(n, 256u));
     float m = -INFINITY, l = 0.f, o = 0.f;
     for (uint32_t k0 = 0; k0 < n; k0 += 256u) {  // (once, but for more than 256 pieces)
         const float2 ml = k0 + tid < n ? a.ml[piece(k0 + tid)] : make_float2(-INFINITY, 0.f);
@@ -728,16 +731,12 @@ __global__ __launch_bounds__(256) void k_attn_paged_merge(PagedAttnArgs a) {
         o *= keep;
         m = top;
         const uint32_t k1 = min(n, k0 + 256u);
-        if (k0 == 0u) {
+        for (uint32_t k = k0 + grp; k < k1; k += kAhead * groups) {
+            if (k != grp) eight(k, k1);
 #pragma unroll
-            for (uint32_t i = 0; i < kAhead; i++) {
-                const uint32_t k = grp + i * groups;
-                if (k < k1) o = fmaf(w[k], x[i], o);
-            }
+            for (uint32_t i = 0; i < kAhead; i++)
+                if (k + i * groups < k1) o = fmaf(w[k - k0 + i * groups], x[i], o);
         }
-        if (mine)
-            for (uint32_t k = k0 ? k0 + grp : grp + kAhead * groups; k < k1; k += groups)
-                o = fmaf(w[k - k0], a.part[piece(k) * hd + d], o);
     }
     so[tid] = o;
     __syncthreads();
