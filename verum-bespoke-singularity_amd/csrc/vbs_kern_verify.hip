@@ -14,9 +14,9 @@
 // Three launches: every row's maximum and sum by chunks of 4096; acceptance, from those, and what
 // is left in each chunk of 1024 of the row to draw from; the chunk, and the place in it.
 // Bound: HBM and, close behind, the vector units (about 27 instructions a logit, 13 of them in 64 bits) where the
-// rows are many and long: 32 sequences of 7 drafted tokens of 131072 take 75 us, 53 of them the rows' sums at 4.5 TB/s
+// rows are many and long: 32 sequences of 7 drafted tokens of 131072 take 77 us, 53 of them the rows' sums at 4.5 TB/s
 // (two chunks a workgroup, with half the joins of lanes: the same). The three launches and their round trips
-// where they are few: one sequence of 4 of 32000 takes 14 us.
+// where they are few: one sequence of 4 of 32000 takes 15 us.
 #include <math.h>
 
 #include "vbs_dev_common.h"
@@ -86,31 +86,45 @@ __device__ __forceinline__ const float *row_of(const VerifyArgs &a, uint32_t b, 
     return r <= a.n ? a.logits + ((uint64_t)b * (a.n + 1u) + r) * a.stride
                     : a.draft + ((uint64_t)b * a.n + (r - a.n - 1u)) * a.draft_stride;
 }
-// Four neighbouring logits from e on; -inf behind the last.
-__device__ __forceinline__ vf4 four(const VerifyArgs &a, const float *x, uint32_t e) {
-    if (a.vec && e + 4u <= a.vocab) return *reinterpret_cast<const vf4 *>(x + e);
+// Four logits from e on, `step` apart; -inf behind the last. Rows that can be read 16 bytes at a time give a lane four
+// neighbours (step 1); others, where the order does not matter, every 64th, so that a wave's words are neighbours (32
+// sequences of 7 of 131071: 99 -> 83 us).
+template <bool VEC>
+__device__ __forceinline__ vf4 four(const VerifyArgs &a, const float *x, uint32_t e, uint32_t step = VEC ? 1u : 64u) {
+    if (VEC && e + 4u <= a.vocab) return *reinterpret_cast<const vf4 *>(x + e);
     vf4 v;
 #pragma unroll
-    for (uint32_t j = 0; j < 4; j++) v[j] = x[min(e + j, a.vocab - 1u)];
+    for (uint32_t j = 0; j < 4; j++) v[j] = x[min(e + j * step, a.vocab - 1u)];
 #pragma unroll
-    for (uint32_t j = 0; j < 4; j++) v[j] = e + j < a.vocab ? v[j] : -INFINITY;
+    for (uint32_t j = 0; j < 4; j++) v[j] = e + j * step < a.vocab ? v[j] : -INFINITY;
     return v;
+}
+
+// A wave's chunk from c0 on: of group i lane l has the four from c0 + 256 i + 4 l (VEC; else c0 + 256 i + l) on.
+template <bool VEC>
+__device__ __forceinline__ void whole_chunk(const VerifyArgs &a, const float *x, uint32_t c0, uint32_t lane, vf4 v[kGroups]) {
+    if (VEC && c0 + kChunk <= a.vocab) {
+#pragma unroll
+        for (uint32_t i = 0; i < kGroups; i++) v[i] = *reinterpret_cast<const vf4 *>(x + c0 + i * 256u + lane * 4u);
+        return;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kGroups; i++) v[i] = four<VEC>(a, x, c0 + i * 256u + (VEC ? lane * 4u : lane));
 }
 
 }  // namespace
 
 // grid (chunks of 4096, rows of a sequence, sequences)
-template <bool GREEDY>
+template <bool GREEDY, bool VEC>
 __global__ __launch_bounds__(kThreads) void k_verify_sum(VerifyArgs a) {
     __shared__ float tops[kWaves];
     __shared__ uint32_t places[kWaves];
     __shared__ double sums[kWaves], two[32];
     const uint32_t b = blockIdx.z, r = blockIdx.y, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-    const uint32_t c0 = blockIdx.x * kRowChunk + wave * kChunk;
+    const uint32_t c0 = __builtin_amdgcn_readfirstlane(blockIdx.x * kRowChunk + wave * kChunk);
     const float *x = row_of(a, b, r);
     vf4 v[kGroups];
-#pragma unroll
-    for (uint32_t i = 0; i < kGroups; i++) v[i] = four(a, x, c0 + i * 256u + lane * 4u);
+    whole_chunk<VEC>(a, x, c0, lane, v);
     const uint32_t n = draft_length(a, b);
     if (r <= a.n ? r > n : r - a.n - 1u >= n) return;  // (a row behind the draft's end)
     const uint64_t to = ((uint64_t)b * (2u * a.n + 1u) + r) * a.chunks + blockIdx.x;
@@ -121,7 +135,7 @@ __global__ __launch_bounds__(kThreads) void k_verify_sum(VerifyArgs a) {
         for (uint32_t i = 0; i < kGroups; i++)
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++) {
-                const uint32_t e = c0 + i * 256u + lane * 4u + j;
+                const uint32_t e = c0 + i * 256u + (VEC ? lane * 4u + j : j * 64u + lane);
                 if (e < a.vocab && (v[i][j] > top || (v[i][j] == top && e < at))) top = v[i][j], at = e;
             }
         for (uint32_t o = 32; o; o >>= 1) {
@@ -225,6 +239,7 @@ struct Left {
 };
 
 // grid (chunks of 1024 / 4, sequences)
+template <bool VEC>
 __global__ __launch_bounds__(kThreads) void k_verify_accept(VerifyArgs a) {
     __shared__ RowSum rows[2 * kMaxDraft + 1];
     __shared__ uint32_t stop_w;
@@ -289,18 +304,22 @@ __global__ __launch_bounds__(kThreads) void k_verify_accept(VerifyArgs a) {
     }
     const uint32_t chunk = blockIdx.x * kWaves + (tid >> 6);
     if (chunk >= a.small) return;
+    const uint32_t c0 = __builtin_amdgcn_readfirstlane(chunk * kChunk);
     vf4 x[kGroups], y[kGroups];
+    whole_chunk<VEC>(a, left.x, c0, lane, x);
+    if (left.y) {
+        whole_chunk<VEC>(a, left.y, c0, lane, y);
+    } else {
 #pragma unroll
-    for (uint32_t i = 0; i < kGroups; i++) x[i] = four(a, left.x, chunk * kChunk + i * 256u + lane * 4u);
-#pragma unroll
-    for (uint32_t i = 0; i < kGroups; i++) y[i] = left.y ? four(a, left.y, chunk * kChunk + i * 256u + lane * 4u) : vf4{0.f, 0.f, 0.f, 0.f};
+        for (uint32_t i = 0; i < kGroups; i++) y[i] = vf4{0.f, 0.f, 0.f, 0.f};
+    }
     double all = 0.0, less = 0.0;  // (behind the last, logits of -inf add 0)
 #pragma unroll
     for (uint32_t i = 0; i < kGroups; i++)
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) {
             double p, l;
-            left.at(a, chunk * kChunk + i * 256u + lane * 4u + j, x[i][j], y[i][j], p, l);
+            left.at(a, c0 + i * 256u + (VEC ? lane * 4u + j : j * 64u + lane), x[i][j], y[i][j], p, l);
             all += p, less += l;
         }
     all = wave_sum_d(all);
@@ -320,6 +339,7 @@ __device__ __forceinline__ double scan_64(double v, uint32_t lane) {
 }
 
 // grid (sequences): every wave finds the chunk; a thread then takes four neighbours of it.
+template <bool VEC>
 __global__ __launch_bounds__(kThreads) void k_verify_pick(VerifyArgs a) {
     __shared__ double ends[kWaves], two[32];
     __shared__ uint32_t found[kWaves], last[kWaves];
@@ -361,7 +381,7 @@ __global__ __launch_bounds__(kThreads) void k_verify_pick(VerifyArgs a) {
             run = __shfl(to, 63, 64);
         }
         const uint32_t e = chunk * kChunk + tid * 4u;
-        const vf4 x = four(a, left.x, e), y = left.y ? four(a, left.y, e) : vf4{0.f, 0.f, 0.f, 0.f};
+        const vf4 x = four<VEC>(a, left.x, e, 1u), y = left.y ? four<VEC>(a, left.y, e, 1u) : vf4{0.f, 0.f, 0.f, 0.f};
         double r[4], mine = 0.0;
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) {
@@ -418,16 +438,16 @@ hipError_t launch_verify(VerifyArgs a, void *scratch, hipStream_t s) {
     a.stop = a.arg + parts;
     if (a.temp == 0.f) a.draft = nullptr;
     a.rate = a.temp > 0.f ? 32.0 * 1.4426950408889634074 / (double)a.temp : 0.0;  // 32 log2 e / T
-    a.vec = !(((uintptr_t)a.logits & 15u) | (a.stride & 3u) | ((uintptr_t)a.draft & 15u) | (a.draft ? a.draft_stride & 3u : 0u));
+    const bool vec = !(((uintptr_t)a.logits & 15u) | (a.stride & 3u) | ((uintptr_t)a.draft & 15u) | (a.draft ? a.draft_stride & 3u : 0u));
     const dim3 grid(a.chunks, a.n + 1u + (a.draft ? a.n : 0u), a.batch);
-    if (a.temp == 0.f) k_verify_sum<true><<<grid, kThreads, 0, s>>>(a);
-    else k_verify_sum<false><<<grid, kThreads, 0, s>>>(a);
+    if (a.temp == 0.f) (vec ? k_verify_sum<true, true> : k_verify_sum<true, false>)<<<grid, kThreads, 0, s>>>(a);
+    else (vec ? k_verify_sum<false, true> : k_verify_sum<false, false>)<<<grid, kThreads, 0, s>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    k_verify_accept<<<dim3(a.temp == 0.f ? 1u : a.chunks, a.batch), kThreads, 0, s>>>(a);
+    (vec ? k_verify_accept<true> : k_verify_accept<false>)<<<dim3(a.temp == 0.f ? 1u : a.chunks, a.batch), kThreads, 0, s>>>(a);
     e = hipGetLastError();
     if (e != hipSuccess || a.temp == 0.f) return e;
-    k_verify_pick<<<a.batch, kThreads, 0, s>>>(a);
+    (vec ? k_verify_pick<true> : k_verify_pick<false>)<<<a.batch, kThreads, 0, s>>>(a);
     return hipGetLastError();
 }
 

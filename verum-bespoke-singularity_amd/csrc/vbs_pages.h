@@ -112,7 +112,6 @@ struct VerifyArgs {
     float temp;
     int32_t *accepted, *tokens;
     double rate;      // 32 log2 e / T
-    int vec;          // rows can be read 16 bytes at a time
     uint32_t chunks, small;  // of a row, and of what is left of one
     double *sums;   // [batch][2 n + 1][chunks]: target rows, then draft rows
     float *tops;    // the same, the maxima
