@@ -105,8 +105,11 @@ __device__ __forceinline__ uint64_t same(uint64_t v) {
 // How the units of all rows and heads are shared out. They lie in one line: row by row, within a row kv head (and tile of q
 // heads) by head, within that slot by slot, and a workgroup takes `share` of them, so all have the same work whatever the
 // lengths. Shares of few units (kAlignedShare) begin and end with their head, which `grain` pads in the line: a
-// second piece's start would take as long as the share. One workgroup a CU where the line is short: 8 heads
-// of one row of 8192 slots take 18.2 us with 256 workgroups (Q8_0, 128 elements) and 23.4 with 512, of 8 rows 44.6 and 38.5.
+// second piece's start would take as long as the share: one row of 600 slots takes 11.9 us and without 15.6, 4 of 1500
+// 14.6 and 18.9. Up to 64 units instead of 16, 40 rows of 1500 take 53.2 for 42.0 and 20 of up to 3000 take 35.6 for 30.9,
+// while few rows of one length gain (4 of 9000: 24.8 for 29.0; Q8_0, 32 q and 8 kv heads of 128). One workgroup
+// a CU where the line is short: 8 heads of one row of 8192 slots take 18.2 us with 256 workgroups (Q8_0, 128 elements) and
+// 23.4 with 512, of 8 rows 44.6 and 38.5.
 constexpr uint32_t kAlignedShare = 16, kShortLine = 8192;
 
 struct Shares {
