@@ -1,0 +1,62 @@
+"""vbs_gfx950_attention_paged where the units of the rows are shared out over workgroups (more than 512 slots by max_len)
+against its definition in 64 bits: no row with a slot, rows in many pieces, pieces that are not finite, every head size.
+No counterpart in the reference (src/vbs_host_math.h:150-209 has one cache and one token): parity unpinned."""
+import numpy as np
+import pytest
+
+import vbs_gfx950 as V
+from test_gpu_kernels import mem  # noqa: F401 (fixture)
+from test_gpu_pages import TYPES, Rows
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- no row with a slot -------------------------------------------------------------------------
+
+# one row, rows that a wave looks up, more of them; the last with more rows x kv heads than workgroups
+EMPTY = [(1, 1, 32), (1, 8, 128), (3, 2, 64), (64, 2, 32), (100, 1, 32), (300, 8, 32)]
+
+
+@TYPES
+@pytest.mark.parametrize("rows,nkh,hd", EMPTY)
+def test_no_row_has_a_slot(dev, mem, t, rows, nkh, hd):
+    """Every row empty (zeros), every row out of range (NaN), and both in one call: a step whose sequences are all
+    padding. Pages hold NaN."""
+    rng = np.random.default_rng(rows + nkh)
+    r = Rows(rng, mem, dev, t, [0] * rows, nkh, nkh, hd, seq=np.arange(rows) % 4, max_len=2048)
+    assert (r.run() == 0).all()
+    for lens, seq in ((-1, 0), (2049, 0), (2**31 - 1, 3), (0, 4), (64, -1)):
+        dev.write(r.pl, np.full(rows, lens, np.int32))
+        dev.write(r.ps, np.full(rows, seq, np.int32))
+        dev.write(r.po, r.out0)
+        r.call()
+        assert np.isnan(r.got()).all(), (lens, seq)
+    lens = np.where(np.arange(rows) % 3 == 1, -7, 0).astype(np.int32)
+    dev.write(r.pl, lens)
+    dev.write(r.ps, r.seq)
+    r.call()
+    got = r.got()
+    assert np.isnan(got[lens < 0]).all() and (got[lens == 0] == 0).all()
+
+
+@TYPES
+def test_a_captured_step_whose_rows_become_empty(dev, mem, t):
+    """A graph replayed with lengths, without any, and with the lengths again: as the eager calls."""
+    rng = np.random.default_rng(3)
+    r = Rows(rng, mem, dev, t, [700, 33, 1025], 8, 2, 64, max_len=2048, junk=False)
+    first = r.run()
+    graph = V.Hip().capture(dev.stream(), r.call)
+    try:
+        for lens in ([0, 0, 0], r.lens, [0, -1, 5000], [0, 0, 0], r.lens):
+            lens = np.asarray(lens, np.int32)
+            dev.write(r.pl, lens)
+            dev.write(r.po, r.out0)
+            V.Hip().launch(graph, dev.stream())
+            dev.sync()
+            got = r.got()
+            bad = (lens < 0) | (lens > 2048)
+            assert np.isnan(got[bad]).all() and (got[lens == 0] == 0).all()
+            if lens[2] == r.lens[2]:
+                assert np.array_equal(got, first)
+    finally:
+        V.Hip().destroy(graph)

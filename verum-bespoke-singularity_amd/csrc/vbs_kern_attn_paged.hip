@@ -120,7 +120,7 @@ __device__ __forceinline__ Shares shares(const PagedAttnArgs &a, uint64_t units,
     const uint32_t workgroups = all < kShortLine ? min(a.workgroups, 256u) : a.workgroups;
     Shares s;
     s.share = (all + workgroups - 1u) / workgroups;
-    s.share = (s.share + kWaves - 1u) / kWaves * kWaves;
+    s.share = max((s.share + kWaves - 1u) / kWaves, (uint64_t)1) * kWaves;  // (not 0 where no row has a unit: `grain` divides)
     s.grain = a.aligned && s.share <= kAlignedShare ? s.share : 1u;
     return s;
 }
