@@ -312,12 +312,14 @@ __device__ __forceinline__ void slow_tile(const PagedAttnArgs &a, int32_t seq, u
     }
 }
 
+// o is written and the scales are read 16 bytes at a time.
 template <uint32_t NB, uint32_t CT>
 struct Shared {
-    float o[kWaves][8u * CT][NB * 32u + 4u];
+    alignas(16) float o[kWaves][8u * CT][NB * 32u + 4u];
     float m[kWaves][8u * CT], l[kWaves][8u * CT];
-    uint32_t scales[kWaves][2][NB * 16u];
+    alignas(16) uint32_t scales[kWaves][2][NB * 16u];
     uint32_t odd;
+    static_assert((NB * 32u + 4u) % 4u == 0u && NB * 16u % 4u == 0u, "rows of 16 bytes");
 };
 
 // Units [u0, u1) of a row and a kv head (and tile of its q heads), by a workgroup: to out, or as a partial
