@@ -4,9 +4,11 @@ No counterpart in the reference (src/vbs_host_math.h:150-209 has one cache and o
 import numpy as np
 import pytest
 
+import pages_long as L
 import vbs_gfx950 as V
 from test_gpu_kernels import mem  # noqa: F401 (fixture)
 from test_gpu_pages import TYPES, Rows
+from test_gpu_steps import close
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +62,25 @@ def test_a_captured_step_whose_rows_become_empty(dev, mem, t):
                 assert np.array_equal(got, first)
     finally:
         V.Hip().destroy(graph)
+
+
+# ---- rows in many pieces ------------------------------------------------------------------------
+
+@TYPES
+@pytest.mark.parametrize("hd", [32, 160])
+def test_batches_of_pieces_that_differ(dev, mem, t, hd):
+    """One row in 683 (heads of 32) or 410 pieces, more than the merge takes at once: every piece's values and every
+    batch's maximum differ, and a lost, repeated, moved or unscaled piece is seen (test_pages_long.py)."""
+    row = L.LongRow(np.random.default_rng(hd), t, hd)
+    order = np.random.default_rng(1).permutation(row.pages)
+    pool = {}
+    for w in "kv":
+        x = np.empty_like(row.bytes[w])
+        x[order] = row.bytes[w]
+        pool[w] = mem.up(x)
+    pages = V.Pages(pool["k"], pool["v"], t, L.PAGE, row.pages, 1, hd, mem.up(order.astype(np.int32)), 1, row.pages)
+    out = mem.up(np.full(3 * hd, 7.5, np.float32))
+    dev.attention_paged(pages, 0, mem.up(row.q), 2 * hd, out, 2 * hd, 0, mem.up(np.int32([L.SLOTS])), 1, L.SLOTS, 2, 1.0)
+    got = dev.download(out, (3, hd), np.float32)
+    assert (got[2] == 7.5).all()
+    close(got[:2].astype(np.float64), *row.want(*row.parts()))
