@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 import pages_long as L
+import pages_ref as R
 import vbs_gfx950 as V
 from test_gpu_kernels import mem  # noqa: F401 (fixture)
 from test_gpu_pages import TYPES, Rows
@@ -84,3 +85,55 @@ def test_batches_of_pieces_that_differ(dev, mem, t, hd):
     got = dev.download(out, (3, hd), np.float32)
     assert (got[2] == 7.5).all()
     close(got[:2].astype(np.float64), *row.want(*row.parts()))
+
+
+# ---- every head size and group ------------------------------------------------------------------
+
+class Want:
+    """The rows of a call by the formula, a sequence's slots read once."""
+
+    def __init__(self, r):
+        self.r, c = r, r.c
+        long = {int(s): int(max(r.lens[r.seq == s].max(), 0)) for s in np.unique(r.seq)}
+        self.kv = {s: [c.pool.rows(w, c.table[s], n) for w in "kv"] for s, n in long.items()}
+        self.vmax = {}
+        for s, n in long.items():
+            self.vmax[s] = None
+            if c.t == V.Q8_0 and n:
+                d = c.pool.scales("v")[c.table[s, :-(-n // c.page)]].view(np.float16).astype(np.float64)
+                self.vmax[s] = 127.0 * float(np.abs(d[np.isfinite(d)]).max())
+
+    def __call__(self):
+        out, tol = zip(*(self.row(i) for i in range(len(self.r.lens))))
+        return np.array(out), np.array(tol)
+
+    def row(self, i):
+        r, s, n = self.r, int(self.r.seq[i]), int(self.r.lens[i])
+        q = r.q[i, :r.nqh * r.hd].reshape(r.nqh, r.hd).astype(np.float64)
+        return R.attend(q, self.kv[s][0][:n], self.kv[s][1][:n], r.scale, self.vmax[s])
+
+
+SIZES = [(8, 2, 80, 0), (6, 2, 96, 0), (12, 4, 96, 2), (9, 1, 96, 0), (24, 2, 96, 0), (16, 1, 80, 0), (9, 1, 128, 0), (24, 2, 128, 0),
+         (32, 2, 128, 6), (4, 1, 160, 0), (10, 1, 160, 0), (3, 3, 192, 0), (16, 1, 192, 2), (4, 2, 224, 0), (12, 1, 256, 0)]
+
+
+@TYPES
+@pytest.mark.parametrize("nqh,nkh,hd,pad", SIZES)
+def test_long_rows_of_every_head_size(dev, mem, t, nqh, nkh, hd, pad):
+    """Ragged rows in several pieces each, empty and short ones among them, shares that end with their head."""
+    rng = np.random.default_rng(nqh + hd)
+    r = Rows(rng, mem, dev, t, [1500, 0, 700, 33, 1101], nqh, nkh, hd, pad=pad, max_len=1536)
+    got = r.run()
+    close(got, *Want(r)())
+    assert (got[1] == 0).all()
+
+
+@TYPES
+@pytest.mark.parametrize("rows,nqh,nkh,hd", [(130, 48, 4, 96), (70, 8, 8, 192), (40, 16, 16, 80), (100, 9, 3, 224), (130, 36, 4, 128)])
+def test_shares_across_rows_of_every_head_size(dev, mem, t, rows, nqh, nkh, hd):
+    """More rows x kv heads than workgroups: shares go on from head to head and row to row."""
+    rng = np.random.default_rng(rows + hd)
+    lens = rng.integers(0, 601, rows)
+    lens[::17] = 600
+    r = Rows(rng, mem, dev, t, lens, nqh, nkh, hd, seq=np.arange(rows) % 5, max_len=608)
+    close(r.run(), *Want(r)())
