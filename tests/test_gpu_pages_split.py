@@ -137,3 +137,94 @@ def test_shares_across_rows_of_every_head_size(dev, mem, t, rows, nqh, nkh, hd):
     lens[::17] = 600
     r = Rows(rng, mem, dev, t, lens, nqh, nkh, hd, seq=np.arange(rows) % 5, max_len=608)
     close(r.run(), *Want(r)())
+
+
+# ---- pieces that are not finite -----------------------------------------------------------------
+
+# A score of -inf or +inf for a q that is positive throughout, in kv head h: an element of K, or (Q8_0) the 32 of a block
+# at 1 or -1 and their scale.
+def infinite_k(c, seq, slots, h, sign):
+    for j in slots:
+        page, slot = c.place(seq, j)
+        if c.t == V.F16:
+            c.pool._values("k")[page, h, slot // 32, R.place(V.F16, "k", c.hd, slot % 32, 1)] = 0x7C00 if sign > 0 else 0xFC00
+            continue
+        c.pool._values("k")[page, h, slot // 32, R.place(V.Q8_0, "k", c.hd, slot % 32, np.arange(32))] = sign
+        c.pool.scales("k")[page, h, slot // 32, slot % 32] = 0x7C00
+
+
+# V's element 2 of kv head h; Q8_0: its block of 32, all of one sign.
+def odd_v(c, seq, j, h, bits):
+    page, slot = c.place(seq, j)
+    if c.t == V.F16:
+        c.pool._values("v")[page, h, slot // 32, R.place(V.F16, "v", c.hd, slot % 32, 2)] = bits
+        return
+    c.pool._values("v")[page, h, slot // 32, R.place(V.Q8_0, "v", c.hd, slot % 32, np.arange(32))] = 5
+    c.pool.scales("v")[page, h, slot // 32, slot % 32] = bits
+
+
+# rows, nqh, nkh, hd: six long rows alone (shares of four units, which end with their head), with one q head per kv head
+# and with nine; and among 64 short rows of their sequences, in shares of 20 units that go on across rows
+ODD = [(6, 4, 2, 64), (6, 18, 2, 64), (70, 8, 8, 64), (6, 10, 1, 160)]
+
+
+@TYPES
+@pytest.mark.parametrize("rows,nqh,nkh,hd", ODD)
+def test_pieces_that_are_not_finite(dev, mem, t, rows, nqh, nkh, hd):
+    """Infinities and NaN in the first, a middle and the last piece of long rows, joined with pieces that are finite."""
+    rng = np.random.default_rng(rows + hd)
+    lens = np.full(rows, 300)
+    lens[::12 if rows > 6 else 1] = [2100, 2300, 2000, 2047, 2200, 1999]
+    r = Rows(rng, mem, dev, t, lens, nqh, nkh, hd, seq=np.arange(rows) % 6 if rows == 6 else (np.arange(rows) + np.arange(rows) // 12) % 6,
+             q_size=0.5, max_len=2304)
+    long = {int(s): int(n) for s, n in zip(r.seq, r.lens) if n > 300}
+    assert len(long) == 6
+    r.q = np.abs(r.q) + np.float32(0.01)
+    c, last = r.c, nkh - 1
+    odd_v(c, 0, 3, 0, 0x7C00)                               # +inf in the first piece and in the last, -inf in the middle
+    odd_v(c, 0, long[0] - 1, last, 0x7C00)
+    odd_v(c, 1, 1100, 0, 0xFC00)
+    infinite_k(c, 1, (0, 64, 1000, long[1] - 1), last, -1)  # weights 0
+    infinite_k(c, 2, range(380, 1800), 0, -1)               # whole pieces of them, at either share
+    odd_v(c, 3, long[3] - 1, 0, 0x7E00)                     # NaN
+    infinite_k(c, 4, (1024,), 0, 1)                         # a score of +inf: the kv head's rows are NaN
+    infinite_k(c, 5, range(long[5]), last, -1)              # nothing but -inf: 0
+    nan_row = int(np.flatnonzero(r.seq == 3)[0])
+    r.q[nan_row, hd - 1] = np.nan                           # one head
+    got = r.run()
+    want, tol = Want(r)()
+    group = nqh // nkh
+    reached = (r.seq == 4) & (r.lens > 1024)
+    want[reached, :group] = np.nan
+    want[nan_row, 0] = np.nan
+    for i in np.flatnonzero(r.lens > 300):  # the inputs are what they are meant to be
+        s = r.seq[i]
+        assert np.isposinf(want[i, :group, 2]).all() if s == 0 else True
+        assert np.isneginf(want[i, :group, 2]).all() if s == 1 else True
+        assert np.isnan(want[i, (0 if i != nan_row else 1):group, 2]).all() if s == 3 else True
+        assert (want[i, -group:] == 0).all() if s == 5 else True
+        assert np.isfinite(want[i]).all() if s in (2, 5) else True
+    # (where the bound itself is none, the value is an infinity or NaN, which `close` wants to be the same)
+    close(got, want, np.where(np.isfinite(tol), tol, 0.0))
+
+
+@TYPES
+@pytest.mark.parametrize("rows,nqh,nkh,hd", ODD)
+def test_pages_that_are_none_in_long_rows(dev, mem, t, rows, nqh, nkh, hd):
+    """A table entry that is no page makes the rows that reach it NaN, in whichever piece it lies, and no others."""
+    rng = np.random.default_rng(rows + hd + 1)
+    lens = np.full(rows, 300)
+    lens[::12 if rows > 6 else 1] = [2100, 2300, 2000, 2048, 2200, 1999]
+    r = Rows(rng, mem, dev, t, lens, nqh, nkh, hd, seq=np.arange(rows) % 6 if rows == 6 else (np.arange(rows) + np.arange(rows) // 12) % 6,
+             max_len=2304)
+    want, tol = Want(r)()
+    c = r.c
+    lost = np.full(6, 1 << 30)  # the first slot without a page
+    for s, entry, page in ((0, 0, -1), (1, 35, c.n_pages), (2, 2000 // 32, -2**31), (3, 2048 // 32, -1), (4, 70, 2**31 - 1)):
+        c.table[s, entry] = page
+        lost[s] = entry * 32
+    got = r.run()
+    bad = r.lens > lost[r.seq]
+    assert bad.any() and not bad.all() and not bad[(r.seq == 3) | (r.seq == 4)].any()
+    assert np.isnan(got[bad]).all()
+    close(got[~bad], want[~bad], tol[~bad])
