@@ -350,7 +350,8 @@ uint64_t vbs_gfx950_page_bytes(int type, uint32_t page_slots, uint32_t n_kv_head
  * tokens (<= 65535) in `layer`: token i becomes slot at[i] of sequence seq[i] (seq
  * NULL: of sequence i; device arrays). A negative slot stores nothing (padding), nor
  * does a place that the table has no page for, or a page outside 0 .. n_pages - 1
- * (no memory but the pool's is touched). Two tokens of a call must not have the same place. F16
+ * (no memory but the pool's is touched). Two tokens of a call must not have the same place, nor
+ * may the rows overlap the layer's pages. F16
  * takes vbs_gfx950_cache_store's rounding. Q8_0: d = f16(max |x| / 127) and q the
  * integer nearest x / d within 127, both rounded once from the exact quotient, ties to
  * even; a block with a NaN or an infinity, or whose d passes f16's range, reads back as NaN. */
@@ -362,7 +363,8 @@ int vbs_gfx950_page_store(const vbs_gfx950_pages_t *pages, uint32_t layer, const
  * kv_stride elements apart), for instance into a cache of one sequence for the
  * attention of several tokens. F16 pages come as they are; q d is rounded to f16 as
  * vbs_gfx950_cache_store does. Rows of a negative slot are left as they were; a place without a
- * page gives NaN. */
+ * page gives NaN. The rows of k and v must not share elements with each other (they may lie
+ * between each other's) or overlap the layer's pages. */
 int vbs_gfx950_page_load(const vbs_gfx950_pages_t *pages, uint32_t layer, int out_type, void *k,
                          void *v, uint32_t kv_stride, const int32_t *seq, const int32_t *at,
                          uint32_t n);
@@ -377,7 +379,7 @@ int vbs_gfx950_page_load(const vbs_gfx950_pages_t *pages, uint32_t layer, int ou
  * pages is, gives NaN. What lies behind a row's last slot does not reach it, infinities and
  * NaN included. Scores are held in f32 in units of log2, up to 2e38 in size. Weights down to 2^-38 of a
  * row's greatest count (Q8_0: of the greatest weight times the greatest of V's scales). Infinities and NaN in a row's
- * own q, K or V are right but slow. out must not overlap q. No call waits for the device. */
+ * own q, K or V are right but slow. out must not overlap q or the layer's pages. No call waits for the device. */
 int vbs_gfx950_attention_paged(const vbs_gfx950_pages_t *pages, uint32_t layer, const float *q,
                                uint32_t q_stride, float *out, uint32_t out_stride,
                                const int32_t *seq, const int32_t *lens, uint32_t rows,
@@ -396,7 +398,8 @@ int vbs_gfx950_attention_paged(const vbs_gfx950_pages_t *pages, uint32_t layer, 
  * logit (the lowest place among equals) is certain, the draft's logits are not read. accepted[b] receives how many stay, tokens[b (n + 1) ..] them,
  * the token drawn, and -1s. A row with a NaN or +inf, or of -inf alone, has no distribution: the target's refuses and
  * draws -1, the draft's refuses (at temperature 0 a NaN is the least of all; only a row of NaN draws -1).
- * Probabilities and sums are held in 64 bits. vocab <= 2^24. No call waits for the device. */
+ * Probabilities and sums are held in 64 bits. vocab <= 2^24. accepted and tokens must not overlap each other or what is
+ * read (nor drafted: a sequence's tokens are one more than its drafted ones). No call waits for the device. */
 int vbs_gfx950_verify_draft(const float *logits, uint32_t stride, const float *draft,
                             uint32_t draft_stride, const int32_t *drafted, const float *u,
                             uint32_t batch, uint32_t n, uint32_t vocab, float temperature,

@@ -957,11 +957,30 @@ int page_args(const char *who, const vbs_gfx950_pages_t *p, uint32_t layer, Page
     return 1;
 }
 
+// Whether [p, p + bytes) reaches the layer's pages.
+bool meets_pages(const PageArgs &a, const void *p, uint64_t bytes) {
+    const uint64_t pool = a.page_bytes * a.n_pages;
+    return spans_overlap(p, bytes, a.k, pool) || spans_overlap(p, bytes, a.v, pool);
+}
+// Whether two sets of n rows of `row` bytes, `stride` apart in both, share a byte (they may lie between each other).
+bool rows_meet(const void *a, const void *b, uint64_t stride, uint64_t row, uint64_t n) {
+    const uint64_t x = (uint64_t)(uintptr_t)a, y = (uint64_t)(uintptr_t)b, apart = x < y ? y - x : x - y;
+    const uint64_t rows = apart / stride, rest = apart % stride;
+    return (rest < row && rows < n) || (stride - rest < row && rows + 1u < n);
+}
+
 int page_rows(const char *who, const vbs_gfx950_pages_t *p, uint32_t layer, PageRowsArgs &a) {
     if (!page_args(who, p, layer, a.p)) return 0;
     if (!a.at) return fail("%s: null pointer", who);
     if (a.n > kMaxStep) return fail("%s: at most %u tokens per call", who, kMaxStep);
-    if (a.stride < (uint64_t)a.p.nkh * a.p.hd) return fail("%s: stride smaller than a row", who);
+    const uint64_t row = (uint64_t)a.p.nkh * a.p.hd;
+    if (a.stride < row) return fail("%s: stride smaller than a row", who);
+    if (a.n == 0) return 1;
+    const bool load = a.out_k != nullptr;
+    const uint64_t size = load && a.out_f16 ? 2u : 4u, span = size * ((a.n - 1u) * (uint64_t)a.stride + row);
+    const void *k = load ? a.out_k : a.k, *v = load ? a.out_v : a.v;
+    if (meets_pages(a.p, k, span) || meets_pages(a.p, v, span)) return fail("%s: the rows overlap the pages", who);
+    if (load && rows_meet(k, v, size * a.stride, size * row, a.n)) return fail("%s: the rows of k and v overlap", who);
     return 1;
 }
 }  // namespace
@@ -1017,8 +1036,9 @@ int vbs_gfx950_attention_paged(const vbs_gfx950_pages_t *pages, uint32_t layer, 
     const uint64_t row = (uint64_t)nqh * a.p.hd;
     if (q_stride < row || out_stride < row) return fail("%s: stride smaller than a row", who);
     if (rows == 0) return 1;
-    if (spans_overlap(q, 4u * ((uint64_t)(rows - 1u) * q_stride + row), out, 4u * ((uint64_t)(rows - 1u) * out_stride + row)))
-        return fail("%s: out overlaps q", who);
+    const uint64_t out_bytes = 4u * ((uint64_t)(rows - 1u) * out_stride + row);
+    if (spans_overlap(q, 4u * ((uint64_t)(rows - 1u) * q_stride + row), out, out_bytes)) return fail("%s: out overlaps q", who);
+    if (meets_pages(a.p, out, out_bytes)) return fail("%s: out overlaps the pages", who);
     a.q = q, a.q_stride = q_stride, a.out = out, a.out_stride = out_stride, a.seq = seq, a.lens = lens;
     a.rows = rows, a.max_len = max_len, a.nqh = nqh, a.scale = scale;
     const size_t bytes = plan_attn_paged(a);
@@ -1046,6 +1066,15 @@ int vbs_gfx950_verify_draft(const float *logits, uint32_t stride, const float *d
     if (stride < vocab || (draft && draft_stride < vocab)) return fail("%s: stride smaller than a row", who);
     if (!(temperature >= 0.f) || isinf(temperature)) return fail("%s: temperature must be 0 or a positive number", who);
     if (batch == 0) return 1;
+    const uint64_t rows = (uint64_t)batch * (n + 1u), drafts = (uint64_t)batch * n;
+    const struct { const void *p; uint64_t bytes; } reads[] = {
+        {logits, 4u * ((rows - 1u) * stride + vocab)},
+        {draft, draft && drafts && temperature > 0.f ? 4u * ((drafts - 1u) * draft_stride + vocab) : 0u},
+        {drafted, 4u * drafts}, {u, 4u * rows}};
+    bool apart = !spans_overlap(accepted, 4u * (uint64_t)batch, tokens, 4u * rows);
+    for (const auto &r : reads)
+        if (r.bytes) apart = apart && !spans_overlap(accepted, 4u * (uint64_t)batch, r.p, r.bytes) && !spans_overlap(tokens, 4u * rows, r.p, r.bytes);
+    if (!apart) return fail("%s: the results overlap each other or the arguments", who);
     VerifyArgs a{};
     a.logits = logits, a.stride = stride, a.draft = draft, a.draft_stride = draft_stride, a.drafted = drafted, a.u = u;
     a.batch = batch, a.n = n, a.vocab = vocab, a.temp = temperature, a.accepted = accepted, a.tokens = tokens;
