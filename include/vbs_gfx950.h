@@ -378,7 +378,8 @@ int vbs_gfx950_page_load(const vbs_gfx950_pages_t *pages, uint32_t layer, int ou
  * scores are all -inf, gives 0; a row whose length or sequence is out of range, or one of whose
  * pages is, gives NaN. What lies behind a row's last slot does not reach it, infinities and
  * NaN included. Scores are held in f32 in units of log2, up to 2e38 in size. Weights down to 2^-38 of a
- * row's greatest count (Q8_0: of the greatest weight times the greatest of V's scales). Infinities and NaN in a row's
+ * row's greatest count (Q8_0: of the greatest weight times the greatest of V's scales); q's elements are
+ * held to 2^-22 of themselves or 2^-38 of their head's greatest, whichever is more. Infinities and NaN in a row's
  * own q, K or V are right but slow. out must not overlap q or the layer's pages. No call waits for the device. */
 int vbs_gfx950_attention_paged(const vbs_gfx950_pages_t *pages, uint32_t layer, const float *q,
                                uint32_t q_stride, float *out, uint32_t out_stride,

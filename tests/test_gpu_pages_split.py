@@ -228,3 +228,39 @@ def test_pages_that_are_none_in_long_rows(dev, mem, t, rows, nqh, nkh, hd):
     assert bad.any() and not bad.all() and not bad[(r.seq == 3) | (r.seq == 4)].any()
     assert np.isnan(got[bad]).all()
     close(got[~bad], want[~bad], tol[~bad])
+
+
+# ---- q of far sizes within a head ---------------------------------------------------------------
+
+@TYPES
+@pytest.mark.parametrize("lens", [[300], [1500, 64]], ids=["whole", "split"])
+def test_small_elements_of_q_beside_great_ones(dev, mem, t, lens):
+    """Elements 2^-24 of their head's greatest, that meet all of K (the great ones meet zeros), make scores of ordinary
+    size. As two f16 parts with the greatest between 2^13 and 2^14 an element is off by half of the last step, 2^-25, so by
+    2^-38 of the greatest: a score by that times scale sum |k|, a weight by twice the largest of these."""
+    rng = np.random.default_rng(18)
+    hd, nqh = 64, 4
+    r = Rows(rng, mem, dev, t, lens, nqh, 1, hd, junk=False)
+    for s, n in enumerate(lens):
+        for j in range(n):
+            x = rng.standard_normal((1, hd)).astype(np.float32)
+            x[:, :32] = 0
+            r.c.pool.put("k", *r.c.place(s, j), x)
+    r.q = rng.standard_normal(r.q.shape).astype(np.float32).reshape(-1, nqh, hd)
+    r.q[..., :32] *= 2.0 ** 10
+    r.q[..., 32:] *= 2.0 ** -14
+    r.q, r.scale = r.q.reshape(len(lens), -1), 2.0 ** 12
+    got, want = r.run(), Want(r)
+    got, want = r.run(), Want(r)
+    plain, tol = want()
+    for i, n in enumerate(lens):
+        k, v = (x[:n, 0] for x in want.kv[i])
+        for h in range(nqh):
+            q = r.q[i].reshape(nqh, hd)[h].astype(np.float64)
+            s = r.scale * (k @ q)
+            assert s.std() > 0.5
+            w = np.exp(s - s.max())
+            off = 2.0 ** -38 * np.abs(q).max() * r.scale * np.abs(k).sum(1).max()
+            tol[i, h] += 2 * off * ((w / w.sum()) @ np.abs(v))
+            assert (tol[i, h] < 0.05 * np.abs(plain[i, h]).max()).all()
+    close(got, plain, tol)
