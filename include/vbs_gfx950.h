@@ -386,9 +386,9 @@ int vbs_gfx950_attention_paged(const vbs_gfx950_pages_t *pages, uint32_t layer, 
                                const int32_t *seq, const int32_t *lens, uint32_t rows,
                                uint32_t max_len, uint32_t n_q_heads, float scale);
 
-/* Drafted tokens (of vbs_gfx950_attention_tree's or several rows of
- * vbs_gfx950_attention_paged's) accepted or refused so that what stays is distributed
- * as the target's own tokens. Per sequence b < batch (<= 65535): n drafted tokens (<= 64), ids
+/* Drafted tokens (each behind the one before: several rows of vbs_gfx950_attention_paged, a chunk, or one
+ * path through vbs_gfx950_attention_tree's; the branches of a tree are not compared) accepted or refused so that
+ * what stays is distributed as the target's own tokens, at one temperature for all sequences of a call. Per sequence b < batch (<= 65535): n drafted tokens (<= 64), ids
  * drafted[b n + i], of which the first id outside 0 .. vocab - 1 ends the draft; target logits in rows
  * b (n + 1) + i (`stride` floats apart), row i the distribution of the token that drafted token i is
  * compared with, and the last that of the token behind the draft; the draft's logits in rows b n + i, or NULL where drafted

@@ -1,6 +1,6 @@
 // vbs_kern_attn_paged.hip — the attention of single tokens over the paged cache.
 //
-// Row r (one token; its q heads of one kv head are up to eight columns of a product):
+// Row r (one token; up to eight of its q heads of one kv head are the columns of a product, 9 to 16 those of two):
 // out = sum_j w_j v_j, w = softmax(scale q.k_j) over the slots j < lens[r]. The units of 32
 // slots of all rows and heads are shared out evenly over the workgroups that run at once, and
 // within one over its four waves; each keeps the running maximum m (in log2), the sum l and O of
@@ -106,8 +106,10 @@ __device__ __forceinline__ uint64_t same(uint64_t v) {
 // heads) by head, within that slot by slot, and a workgroup takes `share` of them, so all have the same work whatever the
 // lengths. Shares of few units (kAlignedShare) begin and end with their head, which `grain` pads in the line: a
 // second piece's start would take as long as the share: one row of 600 slots takes 11.9 us and without 15.6, 4 of 1500
-// 14.6 and 18.9. Up to 64 units instead of 16, 40 rows of 1500 take 53.2 for 42.0 and 20 of up to 3000 take 35.6 for 30.9,
-// while few rows of one length gain (4 of 9000: 24.8 for 29.0; Q8_0, 32 q and 8 kv heads of 128). One workgroup
+// 14.6 and 18.9 (Q8_0, 32 q and 8 kv heads of 128). With up to 64 units instead of 16, 40 rows of 1500 take 53.2 for 42.0 and 20
+// of up to 3000 take 35.6 for 30.9, but 4 of 9000 take 24.8 for 29.0, 40 of 600 22.6 for 29.6 and one of 20000 20.7 for 25.0:
+// those whose padded shares are still one round of the workgroups that run at once (480, 320 and 256 of 512), where 40
+// of 1500 have 640. 16 keeps the first two from their loss and leaves the others' gain. One workgroup
 // a CU where the line is short: 8 heads of one row of 8192 slots take 18.2 us with 256 workgroups (Q8_0, 128 elements) and
 // 23.4 with 512, of 8 rows 44.6 and 38.5.
 constexpr uint32_t kAlignedShare = 16, kShortLine = 8192;
@@ -750,8 +752,8 @@ __global__ __launch_bounds__(256) void k_attn_paged_merge(PagedAttnArgs a) {
     out[tid] = l == 0.f ? 0.f : o / l;
 }
 
-// Heads of up to so many blocks have 9 to 16 q heads of a kv head in one pass over its slots (two tiles of columns), whose
-// sums the registers of more do not hold: 64 sequences of 4096 slots, 96/8 heads of 128, 202 us for 373 in two passes
+// Heads of up to so many blocks have 9 to 16 q heads of a kv head in one pass over its slots (two tiles of columns); larger
+// ones in two passes (two tiles of them were not tried): 64 sequences of 4096 slots, 96/8 heads of 128, 202 us for 373 in two passes
 // (F16), 143 for 217 (Q8_0).
 constexpr uint32_t kTwoTiles = 4;
 // Rows of at most so many units are not split: one of 512 slots takes 9.7 us (8 heads of 128, Q8_0), in shares 11.2.
